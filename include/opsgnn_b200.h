@@ -47,6 +47,7 @@ extern "C" {
 #define OPSGNN_U8 6
 #define OPSGNN_I16 7
 #define OPSGNN_F64 8
+#define OPSGNN_F8E4M3 9 /* operands of opsgnn_segment_matmul_fp8 only */
 
 /* ---- reductions of the CSR engine -------------------------------------- */
 #define OPSGNN_REDUCE_SUM 0
@@ -412,6 +413,76 @@ OPSGNN_API int opsgnn_grouped_forward_permuted(const OpsgnnGroupedDesc* desc, co
 OPSGNN_API int opsgnn_grouped_backward(const OpsgnnGroupedDesc* desc, const void* src, const void* out, const void* grad_out,
                             const void* index, void* grad_src, void* workspace, int64_t workspace_bytes,
                             void* stream);
+
+/* ======================================================================== */
+/* routed experts: choice, dispatch structure, segment products              */
+/* (no counterpart in the reference)                                         */
+/* ======================================================================== */
+#define OPSGNN_ROUTE_SOFTMAX 0
+#define OPSGNN_ROUTE_SIGMOID 1
+
+typedef struct OpsgnnRouteDesc {
+    int64_t rows;        /* T                                                            */
+    int64_t experts;     /* E <= 1024                                                    */
+    int64_t k;           /* experts per row, <= 32 and <= kept_groups * E / groups       */
+    int64_t groups;      /* <= 32, divides E; 1: no groups                               */
+    int64_t kept_groups; /* groups a row may choose from                                 */
+    float scale;         /* factor of the weights                                        */
+    int32_t group_top;   /* 1 or 2: scores of a group that are added up to rank it       */
+    int32_t score;       /* OPSGNN_ROUTE_*                                               */
+    int32_t renormalize; /* weights of a row add up to scale                             */
+    int32_t dtype;       /* of logits, weight and their gradients: F32 / F16 / BF16      */
+} OpsgnnRouteDesc;
+
+/* weight[T, k], index[T, k] <- the k best experts of each row of logits[T, E], best first, ties to the lower index.  bias[E]
+ * (fp32, may be NULL) is added to the scores for the choice only.  Experts with a logit of -inf come last and weigh 0. */
+OPSGNN_API int opsgnn_topk_route(const OpsgnnRouteDesc* desc, const void* logits, const float* bias, void* weight, int64_t* index,
+                                 void* stream);
+/* grad_logits[T, E] of the weights; the choice itself has no gradient.  Indices outside [0, E) are left out. */
+OPSGNN_API int opsgnn_topk_route_backward(const OpsgnnRouteDesc* desc, const void* logits, const int64_t* index,
+                                          const void* grad_weight, void* grad_logits, void* stream);
+
+/* The CSR structure of `count` labels: indptr[experts + 1], perm[count] (the labels' positions in stable order of their
+ * experts) and position[count] (perm's inverse).  Labels outside [0, experts) come last, behind indptr[experts].
+ * experts <= 4096, count < 2^31. */
+OPSGNN_API int opsgnn_route_csr_workspace_bytes(int64_t count, int64_t experts, int64_t* bytes);
+OPSGNN_API int opsgnn_route_csr(const void* index, int index_type, int64_t count, int64_t experts, int64_t* indptr, int64_t* perm,
+                                int64_t* position, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Segment e holds rows [indptr[e], indptr[e + 1]) of a matrix of `rows` rows.  The kernels clamp every pointer to
+ * [0, rows] and a segment's end to its start, so no pointer content leads out of bounds; where segments overlap, the rows
+ * they share hold one segment's result. */
+typedef struct OpsgnnSegmentMatmulDesc {
+    int64_t rows;                  /* of src and out                                        */
+    int64_t segments;              /* indptr has segments + 1 entries                       */
+    int64_t width;                 /* columns of src: the reduced dimension                 */
+    int64_t out;                   /* columns of out                                        */
+    int64_t src_stride;            /* elements between rows of src                          */
+    int64_t weight_segment_stride; /* strides of weight[e, width, out] in elements          */
+    int64_t weight_width_stride;
+    int64_t weight_out_stride;
+    int32_t index_type;            /* I32 / I64                                             */
+    int32_t in_type;               /* of src and weight                                     */
+    int32_t out_type;              /* = in_type; fp8: F32 / F16 / BF16                      */
+} OpsgnnSegmentMatmulDesc;
+
+/* out[r, :] = src[r, :] @ weight[e] for the rows of segment e; 0 in rows of no segment.  out is contiguous. */
+OPSGNN_API int opsgnn_segment_matmul(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src, const void* weight,
+                                     void* out, void* stream);
+/* grad_weight[e] = src[rows of e]^T @ grad[rows of e], contiguous [segments, width, out]; the weight strides of desc are not
+ * used.  grad_stride: elements between rows of grad. */
+OPSGNN_API int opsgnn_segment_matmul_weight_grad(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src,
+                                                 const void* grad, int64_t grad_stride, void* grad_weight, void* stream);
+/* The same product on float8_e4m3 values: src[rows, width] with src_scale[rows, ceil(width / 128)], weight[e, out, width]
+ * (its strides in desc as above) with weight_scale[e, ceil(out / 128), ceil(width / 128)], all scales contiguous fp32.
+ * indptr NULL (with segments = 1): one dense product. */
+OPSGNN_API int opsgnn_segment_matmul_fp8(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src,
+                                         const float* src_scale, const void* weight, const float* weight_scale, void* out,
+                                         void* stream);
+/* values (float8_e4m3, layout of src[batch, rows, width]) and scales: block_rows 1: [batch, rows, ceil(width / 128)],
+ * block_rows 128: [batch, ceil(rows / 128), ceil(width / 128)].  Scales are powers of two. */
+OPSGNN_API int opsgnn_quantize_fp8(const void* src, int dtype, int64_t batch, int64_t rows, int64_t width, int block_rows,
+                                   void* values, float* scales, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,713 @@
+// Routing rows to experts: scores, choice of the best k and their weights (forward and backward), and the CSR structure
+// of the chosen (row, expert) pairs.
+//
+// topk_route, one row per warp.  With l the row's logits and b the bias (fp32, choice only, no gradient):
+//     s = softmax(l) or sigmoid(l)        c = s + b        c = -inf where l = -inf (a masked expert) or c is NaN
+//     a group's score = sum of its group_top (1 or 2) largest c; the kept_groups best groups stay open
+//     index = the k largest c of the open groups, descending, ties to the lowest index (groups likewise)
+//     weight = scale * s[index] / (renormalize ? sum s[index] : 1), 0 where that sum is 0
+// The choice must not hang on how exp rounds.  Without bias, and with groups ranked by one score, c orders as l does and the
+// choice compares the logits themselves, exactly.  Otherwise c is formed in 64 bits.
+//
+// Backward (u = grad * scale, sums over the chosen i):
+//     softmax, renormalized:  dl_i = w_i (u_i - sum u w)                     with w the softmax over the chosen logits
+//     softmax:                dl_j = s_j ([j chosen] u_j - sum u s)          for every expert j
+//     sigmoid:                dl_i = v_i s_i (1 - s_i),  v = u or (u - sum u w) / sum s when renormalized
+// and 0 for every expert that has no term.
+//
+// route_csr is a stable counting sort of the pairs by expert; see there.
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace opsgnn {
+namespace route {
+
+constexpr int kWarps = 4;
+constexpr unsigned kFull = 0xffffffffu;
+
+struct RouteParams {
+    int64_t rows;
+    int32_t experts, k, groups, kept_groups, group_top;
+    int32_t softmax, renormalize;
+    float scale;
+};
+
+// Order-preserving keys; 0 is below every number and marks what cannot be chosen any more.  NaN ranks with -inf.
+__device__ __forceinline__ uint32_t KeyOf(float v)
+{
+    v = (v != v) ? -INFINITY : v + 0.0f;  // -0 and +0 are one value
+    const uint32_t u = __float_as_uint(v);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t KeyOf(double v)
+{
+    v = (v != v) ? -static_cast<double>(INFINITY) : v + 0.0;
+    const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
+    return (u >> 63) ? ~u : (u | 0x8000000000000000ULL);
+}
+
+__device__ __forceinline__ uint32_t WarpMax(uint32_t v) { return __reduce_max_sync(kFull, v); }
+__device__ __forceinline__ uint64_t WarpMax(uint64_t v)
+{
+    const uint32_t hi = static_cast<uint32_t>(v >> 32);
+    const uint32_t top = __reduce_max_sync(kFull, hi);
+    const uint32_t lo = __reduce_max_sync(kFull, hi == top ? static_cast<uint32_t>(v) : 0u);
+    return (static_cast<uint64_t>(top) << 32) | lo;
+}
+__device__ __forceinline__ float WarpMax(float v)
+{
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        v = fmaxf(v, __shfl_xor_sync(kFull, v, d));
+    }
+    return v;
+}
+template <class T> __device__ __forceinline__ T WarpSum(T v)
+{
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        v += __shfl_xor_sync(kFull, v, d);
+    }
+    return v;
+}
+
+// Lane l holds experts l * VPL + j, j < VPL, of its warp's row: a row of whole vectors is read with wide loads.
+template <class T, int VPL> __device__ __forceinline__ void LoadRow(const T* row, int experts, bool wide, int lane, float (&out)[VPL])
+{
+    constexpr int VEC = VPL * sizeof(T) >= 16 ? 16 / sizeof(T) : VPL;
+    if (wide) {
+#pragma unroll
+        for (int j = 0; j < VPL; j += VEC) {
+            const int at = lane * VPL + j;
+            if (at < experts) {
+                const Pack<T, VEC> p = *reinterpret_cast<const Pack<T, VEC>*>(row + at);
+                float f[VEC];
+                Unpack<float, T, VEC>(p, f);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    out[j + i] = f[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    out[j + i] = -INFINITY;
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            const int at = lane * VPL + j;
+            out[j] = at < experts ? Widen<float, T>(LoadNc(row + at)) : -INFINITY;
+        }
+    }
+}
+
+template <class Key, class T, int VPL>
+__global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T* __restrict__ logits, const float* __restrict__ bias,
+                                                          T* __restrict__ weight, int64_t* __restrict__ index, bool wide)
+{
+    // The keys of a warp's row, needed across lanes only where groups are ranked.
+    extern __shared__ __align__(16) unsigned char shared[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Key* row_keys = reinterpret_cast<Key*>(shared) + static_cast<size_t>(warp) * p.experts;
+    constexpr bool kFine = sizeof(Key) == 8;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWarps + warp; r < p.rows; r += static_cast<int64_t>(gridDim.x) * kWarps) {
+        float l[VPL];
+        LoadRow<T, VPL>(logits + r * p.experts, p.experts, wide, lane, l);
+        float top = -INFINITY;
+        bool nan = false;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            top = fmaxf(top, l[j]);
+            nan |= l[j] != l[j];
+        }
+        if (p.softmax) {
+            top = WarpMax(top);
+            nan = __any_sync(kFull, nan);
+        }
+        // A softmax over NaN or +inf has no finite value: the whole row is NaN, as torch.softmax has it.
+        const float base = p.softmax ? ((nan || top == INFINITY) ? NAN : top) : 0.0f;
+
+        Key key[VPL];
+        if constexpr (kFine) {
+            double c[VPL];
+            double total = 1.0;
+            if (p.softmax) {
+                double part = 0.0;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) {
+                    const bool real = lane * VPL + j < p.experts && l[j] != -INFINITY;
+                    c[j] = real ? exp(static_cast<double>(l[j]) - static_cast<double>(base)) : 0.0;
+                    part += c[j];
+                }
+                total = WarpSum(part);
+            }
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                const int at = lane * VPL + j;
+                double v = p.softmax ? c[j] / total : 1.0 / (1.0 + exp(-static_cast<double>(l[j])));
+                if (bias != nullptr && at < p.experts) {
+                    v += static_cast<double>(__ldg(bias + at));
+                }
+                v = l[j] == -INFINITY ? -static_cast<double>(INFINITY) : v;
+                key[j] = at < p.experts ? KeyOf(v) : 0;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                key[j] = lane * VPL + j < p.experts ? KeyOf(p.softmax && base != base ? NAN : l[j]) : 0;
+            }
+        }
+
+        if (p.groups > 1) {
+            const int size = p.experts / p.groups;
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                if (lane * VPL + j < p.experts) {
+                    row_keys[lane * VPL + j] = key[j];
+                }
+            }
+            __syncwarp();
+            // Lane g ranks group g (at most 32 groups).
+            Key mine = 0;
+            if (lane < p.groups) {
+                Key first = 0, second = 0;
+                for (int i = 0; i < size; ++i) {
+                    const Key v = row_keys[lane * size + i];
+                    second = v > first ? first : (v > second ? v : second);
+                    first = v > first ? v : first;
+                }
+                mine = first;
+                if constexpr (kFine) {
+                    if (p.group_top == 2) {
+                        // back from keys to values; both are numbers or -inf
+                        const uint64_t a = (first >> 63) ? (first & 0x7fffffffffffffffULL) : ~static_cast<uint64_t>(first);
+                        const uint64_t b = (second >> 63) ? (second & 0x7fffffffffffffffULL) : ~static_cast<uint64_t>(second);
+                        mine = KeyOf(__longlong_as_double(static_cast<long long>(a)) + __longlong_as_double(static_cast<long long>(b)));
+                    }
+                }
+            }
+            int ahead = 0;
+            for (int g = 0; g < p.groups; ++g) {
+                const Key other = __shfl_sync(kFull, mine, g);
+                ahead += (other > mine || (other == mine && g < lane)) ? 1 : 0;
+            }
+            const unsigned open = __ballot_sync(kFull, lane < p.groups && ahead < p.kept_groups);
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                const int at = lane * VPL + j;
+                if (at < p.experts && !((open >> (at / size)) & 1u)) {
+                    key[j] = 0;
+                }
+            }
+        }
+
+        // k times: the largest key, at the lowest lane that has it (lanes hold ascending ranges of experts).
+        Key best = 0;
+        int where = 0;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            where = key[j] > best ? j : where;
+            best = key[j] > best ? key[j] : best;
+        }
+        int chosen = 0;
+        float chosen_logit = -INFINITY;
+        for (int i = 0; i < p.k; ++i) {
+            const Key winner = WarpMax(best);
+            const int owner = __ffs(__ballot_sync(kFull, best == winner)) - 1;
+            float value = 0.0f;
+            int at = 0;
+            if (lane == owner) {
+                at = lane * VPL + where;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) {
+                    if (j == where) {
+                        value = l[j];
+                        key[j] = 0;
+                    }
+                }
+                best = 0;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) {
+                    where = key[j] > best ? j : where;
+                    best = key[j] > best ? key[j] : best;
+                }
+            }
+            at = __shfl_sync(kFull, at, owner);
+            value = __shfl_sync(kFull, value, owner);
+            if (lane == i) {
+                chosen = at;
+                chosen_logit = value;
+            }
+        }
+
+        float s = 0.0f;
+        if (lane < p.k) {
+            if (p.softmax) {
+                s = chosen_logit == -INFINITY && base == base ? 0.0f : expf(chosen_logit - base);
+            } else {
+                s = 1.0f / (1.0f + expf(-chosen_logit));
+            }
+        }
+        float total = 1.0f;
+        if (p.renormalize) {
+            total = WarpSum(s);
+        } else if (p.softmax) {
+            float part = 0.0f;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                part += l[j] == -INFINITY && base == base ? 0.0f : expf(l[j] - base);
+            }
+            total = WarpSum(part);
+        }
+        if (lane < p.k) {
+            weight[r * p.k + lane] = Narrow<T, float>(total == 0.0f ? 0.0f : s / total * p.scale);
+            index[r * p.k + lane] = chosen;
+        }
+    }
+}
+
+template <class T, int VPL>
+__global__ void __launch_bounds__(kWarps * 32) TopkBackwardKernel(RouteParams p, const T* __restrict__ logits,
+                                                                  const int64_t* __restrict__ index, const T* __restrict__ grad,
+                                                                  T* __restrict__ grad_logits, bool wide)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int VEC = VPL * sizeof(T) >= 16 ? 16 / sizeof(T) : VPL;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWarps + warp; r < p.rows; r += static_cast<int64_t>(gridDim.x) * kWarps) {
+        const T* row = logits + r * p.experts;
+        T* out = grad_logits + r * p.experts;
+        int64_t at = -1;
+        float u = 0.0f, x = -INFINITY;
+        if (lane < p.k) {
+            at = index[r * p.k + lane];
+            if (at >= 0 && at < p.experts) {
+                u = Widen<float, T>(grad[r * p.k + lane]) * p.scale;
+                x = Widen<float, T>(row[at]);
+            } else {
+                at = -1;
+            }
+        }
+        float value = 0.0f;   // gradient of the lane's chosen expert
+        float spread = 0.0f;  // every other expert j gets -s_j * spread (softmax without renormalisation)
+        float top = 0.0f, total = 1.0f;
+        float l[VPL];
+        if (p.softmax) {
+            if (p.renormalize) {
+                top = WarpMax(at >= 0 ? x : -INFINITY);
+                float e = at < 0 || (x == -INFINITY && top == -INFINITY) ? 0.0f : expf(x - top);
+                const float sum = WarpSum(e);
+                const float w = sum == 0.0f ? 0.0f : e / sum;
+                value = w * (u - WarpSum(u * w));
+            } else {
+                LoadRow<T, VPL>(row, p.experts, wide, lane, l);
+                top = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) {
+                    top = fmaxf(top, l[j]);
+                }
+                top = WarpMax(top);
+                float part = 0.0f;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) {
+                    part += l[j] == -INFINITY ? 0.0f : expf(l[j] - top);
+                }
+                total = WarpSum(part);
+                const float s = at < 0 || x == -INFINITY ? 0.0f : expf(x - top) / total;
+                spread = WarpSum(u * s);
+                value = s * (u - spread);
+            }
+        } else {
+            const float s = at < 0 ? 0.0f : 1.0f / (1.0f + expf(-x));
+            float v = u;
+            if (p.renormalize) {
+                const float sum = WarpSum(s);
+                const float w = sum == 0.0f ? 0.0f : s / sum;
+                v = sum == 0.0f ? 0.0f : (u - WarpSum(u * w)) / sum;
+            }
+            value = v * s * (1.0f - s);
+        }
+        // The whole row first, the chosen experts over it: same warp, ordered by the barrier.
+        const bool dense = p.softmax && !p.renormalize;
+        if (wide) {
+#pragma unroll
+            for (int j = 0; j < VPL; j += VEC) {
+                if (lane * VPL + j < p.experts) {
+                    float f[VEC];
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        f[i] = dense && l[j + i] != -INFINITY ? -expf(l[j + i] - top) / total * spread : 0.0f;
+                    }
+                    *reinterpret_cast<Pack<T, VEC>*>(out + lane * VPL + j) = Repack<T, float, VEC>(f);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                if (lane * VPL + j < p.experts) {
+                    out[lane * VPL + j] = Narrow<T, float>(dense && l[j] != -INFINITY ? -expf(l[j] - top) / total * spread : 0.0f);
+                }
+            }
+        }
+        __syncwarp();
+        if (at >= 0) {
+            out[at] = Narrow<T, float>(value);
+        }
+    }
+}
+
+// ---- route_csr -----------------------------------------------------------------------------------------------------------
+// Pairs (in the order they come) sorted by expert, stable: a counting sort in tiles of kTile consecutive pairs.  A label
+// outside [0, experts) is a dropped pair and counts in one more bin behind the last expert.
+//   CountKernel  per tile: how many pairs of each bin                                  -> counts[bin][tile]
+//   ScanKernel   per bin: exclusive prefix of its counts over the tiles, and its total -> counts, totals[bin]
+//   PlaceKernel  per tile: where every bin starts (prefix of the totals), then every pair's place: bin start + pairs of the
+//                bin in earlier tiles, in earlier warps of the tile, in earlier rounds of the warp, in lower lanes
+// One tile needs the last kernel only.  No atomics on global memory; shared counters are per warp and commute.
+constexpr int kSortWarps = 8;
+constexpr int kRounds = 8;
+constexpr int kTile = kSortWarps * 32 * kRounds;
+
+template <class I> __device__ __forceinline__ int BinOf(const I* index, int64_t at, int64_t count, int experts)
+{
+    if (at >= count) {
+        return -1;
+    }
+    const int64_t v = static_cast<int64_t>(index[at]);
+    return v >= 0 && v < experts ? static_cast<int>(v) : experts;
+}
+
+template <class I>
+__global__ void __launch_bounds__(kSortWarps * 32) CountKernel(const I* __restrict__ index, int64_t count, int experts, int64_t tiles,
+                                                               int32_t* __restrict__ counts)
+{
+    extern __shared__ int32_t bins[];
+    for (int b = threadIdx.x; b <= experts; b += blockDim.x) {
+        bins[b] = 0;
+    }
+    __syncthreads();
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kTile;
+    for (int i = threadIdx.x; i < kTile; i += blockDim.x) {
+        const int b = BinOf(index, first + i, count, experts);
+        if (b >= 0) {
+            atomicAdd(&bins[b], 1);
+        }
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b <= experts; b += blockDim.x) {
+        counts[b * tiles + blockIdx.x] = bins[b];
+    }
+}
+
+__device__ __forceinline__ int64_t BlockExclusive(int64_t v, int64_t* scratch, int64_t& total)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t inclusive = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t up = __shfl_up_sync(kFull, inclusive, d);
+        inclusive += lane >= d ? up : 0;
+    }
+    if (lane == 31) {
+        scratch[warp] = inclusive;
+    }
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) {
+        before += w < warp ? scratch[w] : 0;
+        total += scratch[w];
+    }
+    __syncthreads();
+    return before + inclusive - v;
+}
+
+__global__ void __launch_bounds__(kSortWarps * 32) ScanKernel(int32_t* __restrict__ counts, int64_t tiles, int64_t* __restrict__ totals)
+{
+    __shared__ int64_t scratch[kSortWarps];
+    int32_t* mine = counts + static_cast<int64_t>(blockIdx.x) * tiles;
+    int64_t before = 0;
+    for (int64_t from = 0; from < tiles; from += blockDim.x) {
+        const int64_t t = from + threadIdx.x;
+        const int64_t v = t < tiles ? mine[t] : 0;
+        int64_t total;
+        const int64_t exclusive = BlockExclusive(v, scratch, total);
+        if (t < tiles) {
+            mine[t] = static_cast<int32_t>(before + exclusive);  // at most `count` < 2^31 pairs (checked on the host)
+        }
+        before += total;
+    }
+    if (threadIdx.x == 0) {
+        totals[blockIdx.x] = before;
+    }
+}
+
+template <class I>
+__global__ void __launch_bounds__(kSortWarps * 32)
+    PlaceKernel(const I* __restrict__ index, int64_t count, int experts, int64_t tiles, const int32_t* __restrict__ counts,
+                const int64_t* __restrict__ totals, int64_t* __restrict__ indptr, int64_t* __restrict__ perm,
+                int64_t* __restrict__ position)
+{
+    extern __shared__ int32_t place[];  // [kSortWarps][experts + 1]: where the warp's next pair of a bin goes
+    __shared__ int64_t scratch[kSortWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int bins = experts + 1;
+    int32_t* mine = place + warp * bins;
+    for (int b = threadIdx.x; b < bins * kSortWarps; b += blockDim.x) {
+        place[b] = 0;
+    }
+    __syncthreads();
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kTile + warp * (32 * kRounds);
+    int bin[kRounds];
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+        bin[i] = BinOf(index, first + i * 32 + lane, count, experts);
+        if (bin[i] >= 0) {
+            atomicAdd(&mine[bin[i]], 1);
+        }
+    }
+    __syncthreads();
+    int64_t before = 0;
+    for (int from = 0; from < bins; from += blockDim.x) {
+        const int b = from + threadIdx.x;
+        int64_t in_tile = 0;
+        if (b < bins) {
+            for (int w = 0; w < kSortWarps; ++w) {
+                in_tile += place[w * bins + b];
+            }
+        }
+        const int64_t v = b < bins ? (totals != nullptr ? totals[b] : in_tile) : 0;
+        int64_t total;
+        const int64_t start = before + BlockExclusive(v, scratch, total);
+        before += total;
+        if (b < bins) {
+            if (blockIdx.x == 0) {
+                indptr[b] = start;  // bin `experts` starts where the last expert ends
+            }
+            int64_t next = start + (counts != nullptr ? counts[b * tiles + blockIdx.x] : 0);
+            for (int w = 0; w < kSortWarps; ++w) {
+                const int32_t here = place[w * bins + b];
+                place[w * bins + b] = static_cast<int32_t>(next);
+                next += here;
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+        const unsigned peers = __match_any_sync(kFull, bin[i]);
+        if (bin[i] >= 0) {
+            const int lower = __popc(peers & ((1u << lane) - 1u));
+            const int32_t to = mine[bin[i]] + lower;
+            const int64_t at = first + i * 32 + lane;
+            perm[to] = at;
+            position[at] = to;
+        }
+        __syncwarp();
+        if (bin[i] >= 0 && lane == __ffs(peers) - 1) {
+            mine[bin[i]] += __popc(peers);
+        }
+        __syncwarp();
+    }
+}
+
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxChosen = 32;
+constexpr int kMaxGroups = 32;
+constexpr int kMaxBins = 4096;
+
+int CheckRoute(const OpsgnnRouteDesc* d)
+{
+    if (d == nullptr || d->rows < 0 || d->experts < 1 || d->k < 1 || d->groups < 1 || d->kept_groups < 1 ||
+        d->kept_groups > d->groups || d->experts % d->groups != 0 || (d->group_top != 1 && d->group_top != 2) ||
+        (d->score != OPSGNN_ROUTE_SOFTMAX && d->score != OPSGNN_ROUTE_SIGMOID)) {
+        return OPSGNN_ERR_INVALID;
+    }
+    const int64_t size = d->experts / d->groups;
+    if (d->k > size * d->kept_groups || (d->groups > 1 && d->group_top > size)) {
+        return OPSGNN_ERR_INVALID;
+    }
+    if (d->experts > kMaxExperts || d->k > kMaxChosen || d->groups > kMaxGroups) {
+        return OPSGNN_ERR_LIMIT;
+    }
+    if (d->dtype != OPSGNN_F32 && d->dtype != OPSGNN_F16 && d->dtype != OPSGNN_BF16) {
+        return OPSGNN_ERR_UNSUPPORTED;
+    }
+    return OPSGNN_OK;
+}
+
+RouteParams ParamsOf(const OpsgnnRouteDesc& d)
+{
+    RouteParams p;
+    p.rows = d.rows;
+    p.experts = static_cast<int32_t>(d.experts);
+    p.k = static_cast<int32_t>(d.k);
+    p.groups = static_cast<int32_t>(d.groups);
+    p.kept_groups = static_cast<int32_t>(d.kept_groups);
+    p.group_top = d.group_top;
+    p.softmax = d.score == OPSGNN_ROUTE_SOFTMAX;
+    p.renormalize = d.renormalize;
+    p.scale = d.scale;
+    return p;
+}
+
+int Grid(int64_t rows) { return static_cast<int>(std::min<int64_t>(CeilDiv(rows, kWarps), static_cast<int64_t>(SmCount()) * 16)); }
+
+// Whole vectors: a lane's VPL values start on a vector boundary in every row.
+template <class T, int VPL> bool Wide(int64_t experts, const void* a, const void* b)
+{
+    constexpr int VEC = VPL * sizeof(T) >= 16 ? 16 / sizeof(T) : VPL;
+    return experts % VEC == 0 && Aligned(a, VEC * sizeof(T)) && Aligned(b, VEC * sizeof(T));
+}
+
+template <class T, int VPL>
+int RunTopk(const OpsgnnRouteDesc& d, const void* logits, const float* bias, void* weight, int64_t* index, cudaStream_t stream)
+{
+    const RouteParams p = ParamsOf(d);
+    const bool fine = bias != nullptr || (d.groups > 1 && d.group_top == 2);
+    const bool wide = Wide<T, VPL>(d.experts, logits, logits);
+    const size_t shared = d.groups > 1 ? static_cast<size_t>(kWarps) * d.experts * (fine ? 8 : 4) : 0;
+    const T* in = static_cast<const T*>(logits);
+    T* out = static_cast<T*>(weight);
+    if (fine) {
+        TopkKernel<uint64_t, T, VPL><<<Grid(d.rows), kWarps * 32, shared, stream>>>(p, in, bias, out, index, wide);
+    } else {
+        TopkKernel<uint32_t, T, VPL><<<Grid(d.rows), kWarps * 32, shared, stream>>>(p, in, bias, out, index, wide);
+    }
+    return LaunchStatus();
+}
+
+template <class T, int VPL>
+int RunTopkBackward(const OpsgnnRouteDesc& d, const void* logits, const int64_t* index, const void* grad, void* grad_logits,
+                    cudaStream_t stream)
+{
+    const bool wide = Wide<T, VPL>(d.experts, logits, grad_logits);
+    TopkBackwardKernel<T, VPL><<<Grid(d.rows), kWarps * 32, 0, stream>>>(ParamsOf(d), static_cast<const T*>(logits), index,
+                                                                        static_cast<const T*>(grad), static_cast<T*>(grad_logits),
+                                                                        wide);
+    return LaunchStatus();
+}
+
+// f(type tag, integral constant VPL): experts a lane holds, a power of two.
+template <class F> int Dispatch(const OpsgnnRouteDesc& d, F&& f)
+{
+    auto by_width = [&](auto tag) {
+        using std::integral_constant;
+        if (d.experts <= 32) {
+            return f(tag, integral_constant<int, 1>());
+        }
+        if (d.experts <= 64) {
+            return f(tag, integral_constant<int, 2>());
+        }
+        if (d.experts <= 128) {
+            return f(tag, integral_constant<int, 4>());
+        }
+        if (d.experts <= 256) {
+            return f(tag, integral_constant<int, 8>());
+        }
+        if (d.experts <= 512) {
+            return f(tag, integral_constant<int, 16>());
+        }
+        return f(tag, integral_constant<int, 32>());
+    };
+    switch (d.dtype) {
+        case OPSGNN_F32:
+            return by_width(float());
+        case OPSGNN_F16:
+            return by_width(__half());
+        default:
+            return by_width(__nv_bfloat16());
+    }
+}
+
+}  // namespace route
+}  // namespace opsgnn
+
+using namespace opsgnn;
+
+extern "C" int opsgnn_topk_route(const OpsgnnRouteDesc* desc, const void* logits, const float* bias, void* weight, int64_t* index,
+                                 void* stream)
+{
+    const int status = route::CheckRoute(desc);
+    if (status != OPSGNN_OK || desc->rows == 0) {
+        return status;
+    }
+    if (logits == nullptr || weight == nullptr || index == nullptr) {
+        return OPSGNN_ERR_INVALID;
+    }
+    return route::Dispatch(*desc, [&](auto tag, auto vpl) {
+        return route::RunTopk<decltype(tag), decltype(vpl)::value>(*desc, logits, bias, weight, index, AsStream(stream));
+    });
+}
+
+extern "C" int opsgnn_topk_route_backward(const OpsgnnRouteDesc* desc, const void* logits, const int64_t* index, const void* grad_weight,
+                                          void* grad_logits, void* stream)
+{
+    const int status = route::CheckRoute(desc);
+    if (status != OPSGNN_OK || desc->rows == 0) {
+        return status;
+    }
+    if (logits == nullptr || index == nullptr || grad_weight == nullptr || grad_logits == nullptr) {
+        return OPSGNN_ERR_INVALID;
+    }
+    return route::Dispatch(*desc, [&](auto tag, auto vpl) {
+        return route::RunTopkBackward<decltype(tag), decltype(vpl)::value>(*desc, logits, index, grad_weight, grad_logits,
+                                                                           AsStream(stream));
+    });
+}
+
+extern "C" int opsgnn_route_csr_workspace_bytes(int64_t count, int64_t experts, int64_t* bytes)
+{
+    if (bytes == nullptr || count < 0 || experts < 1) {
+        return OPSGNN_ERR_INVALID;
+    }
+    if (experts > route::kMaxBins || count >= (INT64_C(1) << 31)) {
+        return OPSGNN_ERR_LIMIT;
+    }
+    const int64_t tiles = CeilDiv(count, route::kTile);
+    *bytes = tiles > 1 ? AlignUp((experts + 1) * 8, 256) + (experts + 1) * tiles * 4 : 0;
+    return OPSGNN_OK;
+}
+
+extern "C" int opsgnn_route_csr(const void* index, int index_type, int64_t count, int64_t experts, int64_t* indptr, int64_t* perm,
+                                int64_t* position, void* workspace, int64_t workspace_bytes, void* stream)
+{
+    int64_t need = 0;
+    const int status = opsgnn_route_csr_workspace_bytes(count, experts, &need);
+    if (status != OPSGNN_OK) {
+        return status;
+    }
+    if (indptr == nullptr || (count > 0 && (index == nullptr || perm == nullptr || position == nullptr)) ||
+        (index_type != OPSGNN_I32 && index_type != OPSGNN_I64)) {
+        return OPSGNN_ERR_INVALID;
+    }
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !Aligned(workspace, 8))) {
+        return OPSGNN_ERR_WORKSPACE;
+    }
+    const int64_t tiles = std::max<int64_t>(1, CeilDiv(count, route::kTile));
+    const int bins = static_cast<int>(experts) + 1;
+    int64_t* totals = tiles > 1 ? static_cast<int64_t*>(workspace) : nullptr;
+    int32_t* counts =
+        tiles > 1 ? reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + AlignUp(static_cast<int64_t>(bins) * 8, 256)) : nullptr;
+    const size_t shared = static_cast<size_t>(route::kSortWarps) * bins * 4;
+    auto run = [&](auto tag) {
+        using I = decltype(tag);
+        const I* in = static_cast<const I*>(index);
+        const int threads = route::kSortWarps * 32;
+        OPSGNN_CUDA_TRY(cudaFuncSetAttribute(route::PlaceKernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(route::kSortWarps * (route::kMaxBins + 1) * 4)));
+        if (tiles > 1) {
+            route::CountKernel<I><<<static_cast<unsigned>(tiles), threads, bins * 4, AsStream(stream)>>>(
+                in, count, static_cast<int>(experts), tiles, counts);
+            route::ScanKernel<<<bins, threads, 0, AsStream(stream)>>>(counts, tiles, totals);
+        }
+        route::PlaceKernel<I><<<static_cast<unsigned>(tiles), threads, shared, AsStream(stream)>>>(
+            in, count, static_cast<int>(experts), tiles, counts, totals, indptr, perm, position);
+        return LaunchStatus();
+    };
+    return index_type == OPSGNN_I32 ? run(int32_t()) : run(int64_t());
+}

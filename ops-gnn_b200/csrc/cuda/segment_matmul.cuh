@@ -1,0 +1,40 @@
+// Shared declarations of the segment products: launch parameters, and the entry points of their kernels.
+#pragma once
+
+#include "common.cuh"
+#include "segment_walk.cuh"
+
+namespace opsgnn {
+namespace segmm {
+
+// out[r, n] = sum_k a[r, k] * b[e, k, n] for the rows r of segment e; rows of no segment are 0.
+struct RowsProblem {
+    SegmentPointers ptr;
+    const void* a;
+    const void* b;
+    void* out;
+    const float* a_scale;             // 8-bit operands only: [rows, ceil(k / 128)]
+    const float* b_scale;             // [segments, ceil(n / 128), ceil(k / 128)]
+    int64_t k, n;
+    int64_t lda, ldo;                 // row strides, elements
+    int64_t b_segment, b_k, b_n;      // strides of b, elements
+    int32_t in_type, out_type;
+};
+
+// out[e, k, n] = sum over the rows r of segment e of a[r, k] * b[r, n]; 0 for an empty segment.
+struct OuterProblem {
+    SegmentPointers ptr;
+    const void* a;
+    const void* b;
+    void* out;
+    int64_t k, n;
+    int64_t lda, ldb;
+    int32_t type;
+};
+
+// Any type, size, stride and alignment (segment_matmul_simple.cu).
+int RunRowsSimple(const RowsProblem& p, cudaStream_t stream);
+int RunOuterSimple(const OuterProblem& p, cudaStream_t stream);
+
+}  // namespace segmm
+}  // namespace opsgnn

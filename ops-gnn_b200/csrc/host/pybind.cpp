@@ -120,6 +120,8 @@ void BindScatter(py::module_& m);
 void BindGrouped(py::module_& m);
 void BindGather(py::module_& m);
 void BindAttention(py::module_& m);
+void BindRoute(py::module_& m);
+void BindSegmentMatmul(py::module_& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
 {
@@ -162,4 +164,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     BindGrouped(m);
     BindGather(m);
     BindAttention(m);
+    BindRoute(m);
+    BindSegmentMatmul(m);
 }

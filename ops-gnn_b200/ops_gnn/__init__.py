@@ -52,6 +52,11 @@ from .scatter import (
 from .scatter_softmax import scatter_softmax
 from .scatter_log_softmax import scatter_log_softmax
 from .scatter_logsumexp import scatter_logsumexp
+from .topk_route import topk_route
+from .route_csr import route_csr
+from .segment_matmul import segment_matmul
+from .quantize_fp8 import quantize_fp8
+from .segment_matmul_fp8 import segment_matmul_fp8
 from . import torch_sparse_spmm
 
 
@@ -85,6 +90,7 @@ __all__ = [
     "scatter", "scatter_sum", "scatter_add", "scatter_mul", "scatter_mean", "scatter_min", "scatter_max",
     "native_available",
     "scatter_softmax", "scatter_log_softmax", "scatter_logsumexp",
+    "topk_route", "route_csr", "segment_matmul", "quantize_fp8", "segment_matmul_fp8",
     "torch_sparse_spmm",
     "Tensor",
     "OptTensor",

@@ -14,7 +14,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIBRARY_PATH = os.path.join(_HERE, "sm100", "libopsgnn_b200.so")
 
 # dtype ids (include/opsgnn_b200.h)
-F32, F16, BF16, I8, I32, I64, U8, I16, F64 = range(9)
+F32, F16, BF16, I8, I32, I64, U8, I16, F64, F8E4M3 = range(10)
 REDUCE_SUM, REDUCE_MEAN, REDUCE_MIN, REDUCE_MAX, REDUCE_LOGSUMEXP = range(5)
 EXTREMUM_IGNORE_NAN, EXTREMUM_PROPAGATE_NAN, EXTREMUM_SEEDED, EXTREMUM_SEEDED_LAST = range(4)
 SDDMM_OPS = {"dot": 0, "add": 1, "sub": 2, "mul": 3, "div": 4, "copy_lhs": 5, "copy_rhs": 6}
@@ -35,6 +35,8 @@ EXPORTS = (
     "opsgnn_index_longest_run",
     "opsgnn_scatter_workspace_bytes", "opsgnn_scatter",
     "opsgnn_grouped_workspace_bytes", "opsgnn_grouped_forward", "opsgnn_grouped_forward_permuted", "opsgnn_grouped_backward",
+    "opsgnn_topk_route", "opsgnn_topk_route_backward", "opsgnn_route_csr_workspace_bytes", "opsgnn_route_csr",
+    "opsgnn_segment_matmul", "opsgnn_segment_matmul_weight_grad", "opsgnn_segment_matmul_fp8", "opsgnn_quantize_fp8",
 )
 
 
@@ -73,6 +75,21 @@ class GroupedDesc(Structure):
     _fields_ = [
         ("batch", c_int64), ("dim_len", c_int64), ("after", c_int64), ("groups", c_int64),
         ("mode", c_int32), ("dtype", c_int32), ("sorted", c_int32), ("index_type", c_int32),
+    ]
+
+
+class RouteDesc(Structure):
+    _fields_ = [
+        ("rows", c_int64), ("experts", c_int64), ("k", c_int64), ("groups", c_int64), ("kept_groups", c_int64),
+        ("scale", ctypes.c_float), ("group_top", c_int32), ("score", c_int32), ("renormalize", c_int32), ("dtype", c_int32),
+    ]
+
+
+class SegmentMatmulDesc(Structure):
+    _fields_ = [
+        ("rows", c_int64), ("segments", c_int64), ("width", c_int64), ("out", c_int64), ("src_stride", c_int64),
+        ("weight_segment_stride", c_int64), ("weight_width_stride", c_int64), ("weight_out_stride", c_int64),
+        ("index_type", c_int32), ("in_type", c_int32), ("out_type", c_int32),
     ]
 
 
@@ -123,6 +140,16 @@ _PROTOTYPES = {
                                                 c_int64, c_void_p]),
     "opsgnn_grouped_backward": (c_int, [POINTER(GroupedDesc), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                         c_void_p, c_int64, c_void_p]),
+    "opsgnn_topk_route": (c_int, [POINTER(RouteDesc), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "opsgnn_topk_route_backward": (c_int, [POINTER(RouteDesc), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "opsgnn_route_csr_workspace_bytes": (c_int, [c_int64, c_int64, POINTER(c_int64)]),
+    "opsgnn_route_csr": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "opsgnn_segment_matmul": (c_int, [POINTER(SegmentMatmulDesc), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "opsgnn_segment_matmul_weight_grad": (c_int, [POINTER(SegmentMatmulDesc), c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
+                                                  c_void_p]),
+    "opsgnn_segment_matmul_fp8": (c_int, [POINTER(SegmentMatmulDesc), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                          c_void_p, c_void_p]),
+    "opsgnn_quantize_fp8": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
 }
 
 _LIB = None

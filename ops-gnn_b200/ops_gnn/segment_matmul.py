@@ -1,0 +1,81 @@
+"""One matrix product per CSR segment.  An addition: the reference has no counterpart; its segment operators reduce rows,
+this one multiplies them (typed linear layers of relational graphs, experts of a routed layer)."""
+import torch
+
+from . import _pybind
+
+_SUPPORTED_DTYPES = (torch.float16, torch.float32, torch.bfloat16)
+_SUPPORTED_PTR_DTYPES = (torch.int32, torch.int64)
+
+
+class _SegmentMatmul(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, src, indptr, weight):
+        ctx.save_for_backward(src, indptr, weight)
+        return _pybind.segment_matmul_forward(src, indptr, weight)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        src, indptr, weight = ctx.saved_tensors
+        grad_src = grad_weight = None
+        if ctx.needs_input_grad[0]:
+            grad_src = _pybind.segment_matmul_forward(grad, indptr, weight.transpose(1, 2))
+        if ctx.needs_input_grad[2]:
+            if weight.stride(1) == 1 and weight.stride(2) != 1:  # the gradient in the layout of the weight
+                grad_weight = _pybind.segment_matmul_weight_grad(grad, indptr, src).transpose(1, 2)
+            else:
+                grad_weight = _pybind.segment_matmul_weight_grad(src, indptr, grad)
+        return grad_src, None, grad_weight
+
+
+def check_segments(src: torch.Tensor, indptr: torch.Tensor, segments: int) -> torch.Tensor:
+    if not isinstance(indptr, torch.Tensor):
+        raise TypeError(f"indptr must be a torch.Tensor, got {type(indptr).__name__}")
+    if indptr.dtype not in _SUPPORTED_PTR_DTYPES:
+        raise TypeError(f"indptr dtype must be int32 or int64, got {indptr.dtype}")
+    if indptr.dim() != 1:
+        raise ValueError(f"indptr must be 1-D, got {indptr.dim()}-D")
+    if indptr.numel() != segments + 1:
+        raise ValueError(f"indptr must hold one pointer more than weight has matrices ({segments}), got {indptr.numel()}")
+    if indptr.device != src.device:
+        raise ValueError(f"src and indptr must be on the same device, got {src.device} and {indptr.device}")
+    return indptr.contiguous()
+
+
+def segment_matmul(src: torch.Tensor, indptr: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    """``out[r] = src[r] @ weight[e]`` for the rows ``indptr[e] <= r < indptr[e + 1]`` of each segment ``e``.
+
+    ``src`` is ``[M, K]``, ``weight`` ``[E, K, N]`` of the same dtype (float16, float32 or bfloat16), ``indptr`` ``[E + 1]``
+    (int32 / int64, non-decreasing); the result is ``[M, N]``.  Segments may be empty; rows before ``indptr[0]`` and from
+    ``indptr[E]`` on belong to none and give 0, and have gradient 0.  Sums are held in fp32 and rounded once.  Any strides:
+    rows of ``src`` and either layout of ``weight`` (``weight.transpose(1, 2)`` of ``[E, N, K]``) are read in place, other
+    layouts are copied first.  Differentiable in ``src`` and ``weight`` (second derivatives are not built).
+
+    The pointers stay on the device: nothing is read back, so the call can be captured into a graph and replayed with other
+    pointers.  Their order is not checked; a pointer outside ``[0, M]`` counts as the nearer end and a segment that would
+    end before it starts is empty.  Raises ``TypeError`` / ``ValueError`` for bad arguments and ``RuntimeError`` for tensors
+    that are not on a CUDA device.
+    """
+    if not isinstance(src, torch.Tensor):
+        raise TypeError(f"src must be a torch.Tensor, got {type(src).__name__}")
+    if not isinstance(weight, torch.Tensor):
+        raise TypeError(f"weight must be a torch.Tensor, got {type(weight).__name__}")
+    if src.dtype not in _SUPPORTED_DTYPES:
+        raise TypeError(f"src dtype must be one of float16, float32, bfloat16; got {src.dtype}")
+    if weight.dtype != src.dtype:
+        raise TypeError(f"weight dtype must match src ({src.dtype}), got {weight.dtype}")
+    if src.dim() != 2:
+        raise ValueError(f"src must be 2-D, got {src.dim()}-D")
+    if weight.dim() != 3:
+        raise ValueError(f"weight must be 3-D, got {weight.dim()}-D")
+    if weight.size(1) != src.size(1):
+        raise ValueError(f"weight.size(1) ({weight.size(1)}) must match src.size(1) ({src.size(1)})")
+    if weight.device != src.device:
+        raise ValueError(f"src and weight must be on the same device, got {src.device} and {weight.device}")
+    indptr = check_segments(src, indptr, weight.size(0))
+    if src.device.type != "cuda":
+        raise RuntimeError("segment_matmul requires CUDA tensors")
+    if torch.is_grad_enabled() and (src.requires_grad or weight.requires_grad):
+        return _SegmentMatmul.apply(src, indptr, weight)
+    return _pybind.segment_matmul_forward(src, indptr, weight)

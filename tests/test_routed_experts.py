@@ -1,0 +1,944 @@
+"""Routed experts: topk_route, route_csr, segment_matmul, quantize_fp8, segment_matmul_fp8 and a layer made of them, against
+plain float64 restatements on the CPU.
+
+Bounds.  A result of 16 or 32 bits is rounded once, by at most eps / 2 of its value.  A sum of n products held in fp32 is off
+by at most n * 2^-23 of the sum of their magnitudes, whatever its order and whether an addition rounds or cuts off (2^-23 is a
+whole step of fp32).  Scores: exp and the division are good to a few steps of fp32, their sum over E experts to E half steps.
+"""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from conftest import requires_gpu
+
+STEP = 2.0 ** -23
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---- plain restatements --------------------------------------------------------------------------------------------------
+
+def _plain_scores(logits, score):
+    x = logits.double()
+    if score == "sigmoid":
+        return torch.sigmoid(x)
+    top = x.max(1, keepdim=True).values
+    top = torch.where(top == -math.inf, torch.zeros_like(top), top)
+    z = torch.exp(x - top)
+    total = z.sum(1, keepdim=True)
+    return torch.where(total == 0, torch.zeros_like(z), z / total)
+
+
+def _plain_choice(logits, k, score, bias, groups, kept, group_top):
+    """Row by row, as the definition says it; returns a list of k experts per row."""
+    s = _plain_scores(logits, score)
+    experts = logits.size(1)
+    size = experts // groups
+    chosen = []
+    for r in range(logits.size(0)):
+        row = [float(v) for v in s[r]]
+        if bias is None and (groups == 1 or group_top == 1):
+            row = [float(v) if not math.isnan(row[j]) else math.nan for j, v in enumerate(logits[r].double())]
+        if bias is not None:
+            row = [v + float(b) for v, b in zip(row, bias.double())]
+        row = [-math.inf if float(l) == -math.inf or math.isnan(v) else v for v, l in zip(row, logits[r])]
+        rank = sorted(range(groups), key=lambda g: (-sum(sorted(row[g * size:(g + 1) * size], reverse=True)[:group_top]), g))
+        open_groups = set(rank[:kept])
+        order = sorted((j for j in range(experts) if j // size in open_groups), key=lambda j: (-row[j], j))
+        chosen.append(order[:k])
+    return torch.tensor(chosen, dtype=torch.int64).reshape(logits.size(0), k)
+
+
+def _plain_weight(logits, index, score, renormalize, scale):
+    if score == "softmax" and renormalize:
+        # the sum over all experts cancels; leaving it out keeps float64 rounding off the experts not chosen
+        return _plain_scores(logits.gather(1, index), score) * scale
+    s = _plain_scores(logits, score).gather(1, index)
+    if renormalize:
+        total = s.sum(1, keepdim=True)
+        s = torch.where(total == 0, torch.zeros_like(s), s / total)
+    return s * scale
+
+
+def _plain_matmul(src, ptr, weight):
+    out = torch.zeros(src.size(0), weight.size(2), dtype=torch.float64)
+    for e in range(weight.size(0)):
+        out[ptr[e]:ptr[e + 1]] = src[ptr[e]:ptr[e + 1]].double() @ weight[e].double()
+    return out
+
+
+def _plain_weight_grad(src, ptr, grad):
+    return torch.stack([src[ptr[e]:ptr[e + 1]].double().t() @ grad[ptr[e]:ptr[e + 1]].double() for e in range(len(ptr) - 1)]) \
+        if len(ptr) > 1 else torch.zeros(0, src.size(1), grad.size(1), dtype=torch.float64)
+
+
+def _within(actual, expected, magnitude, terms, what):
+    """|actual - expected| <= eps / 2 * |expected| + terms * 2^-23 * magnitude, plus half the smallest subnormal step."""
+    assert actual.shape == expected.shape, what
+    info = torch.finfo(actual.dtype)
+    got, want = actual.detach().cpu().double(), expected.double()
+    assert torch.isfinite(got).all(), what + ": unexpected NaN or infinity"
+    slack = info.eps / 2 * want.abs() + terms * STEP * magnitude.double() * (1 + info.eps) + info.smallest_normal * info.eps
+    over = ((got - want).abs() / slack.clamp(min=1e-300)).max().item() if got.numel() else 0.0
+    assert over <= 1.0, f"{what}: {over:.2f} times the bound"
+
+
+def _pointers(lengths, first=0):
+    return torch.tensor([first] + list(first + torch.tensor(lengths, dtype=torch.int64).cumsum(0))) if len(lengths) \
+        else torch.tensor([first])
+
+
+# ---- refusals (no GPU) ---------------------------------------------------------------------------------------------------
+
+def test_topk_route_refuses():
+    from ops_gnn import topk_route
+
+    x = torch.zeros(4, 16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        topk_route(x, 2)
+    with pytest.raises(TypeError, match="torch.Tensor"):
+        topk_route([1.0], 1)
+    with pytest.raises(TypeError, match="float16"):
+        topk_route(x.double(), 2)
+    with pytest.raises(ValueError, match="dimension"):
+        topk_route(torch.tensor(1.0), 1)
+    with pytest.raises(ValueError, match="softmax"):
+        topk_route(x, 2, score="tanh")
+    for bad in (0, 17):
+        with pytest.raises(ValueError, match="k must be"):
+            topk_route(x, bad)
+    with pytest.raises(TypeError, match="k must be an int"):
+        topk_route(x, True)
+    with pytest.raises(ValueError, match="divide"):
+        topk_route(x, 2, groups=3)
+    with pytest.raises(ValueError, match="kept_groups"):
+        topk_route(x, 2, groups=4, kept_groups=5)
+    with pytest.raises(ValueError, match="k must be"):
+        topk_route(x, 5, groups=4, kept_groups=1)
+    with pytest.raises(ValueError, match="group_top"):
+        topk_route(x, 2, groups=16, group_top=2)
+    with pytest.raises(ValueError, match="group_top"):
+        topk_route(x, 2, groups=4, group_top=3)
+    with pytest.raises(ValueError, match="experts"):
+        topk_route(torch.zeros(1, 1025), 1)
+    with pytest.raises(ValueError, match="k must be"):
+        topk_route(torch.zeros(1, 64), 33)
+    with pytest.raises(TypeError, match="bias"):
+        topk_route(x, 2, bias=torch.zeros(16, dtype=torch.float64))
+    with pytest.raises(ValueError, match="bias"):
+        topk_route(x, 2, bias=torch.zeros(15))
+
+
+def test_route_csr_refuses():
+    from ops_gnn import route_csr
+
+    x = torch.zeros(4, 2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        route_csr(x, 4)
+    with pytest.raises(TypeError, match="int32"):
+        route_csr(x.float(), 4)
+    with pytest.raises(TypeError, match="torch.Tensor"):
+        route_csr([1], 4)
+    with pytest.raises(TypeError, match="num_experts"):
+        route_csr(x, 4.0)
+    for bad in (0, 4097):
+        with pytest.raises(ValueError, match="num_experts"):
+            route_csr(x, bad)
+
+
+def test_segment_matmul_refuses():
+    from ops_gnn import segment_matmul
+
+    src, ptr, weight = torch.zeros(4, 8), torch.tensor([0, 4]), torch.zeros(1, 8, 3)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        segment_matmul(src, ptr, weight)
+    with pytest.raises(TypeError, match="src"):
+        segment_matmul([1], ptr, weight)
+    with pytest.raises(TypeError, match="weight"):
+        segment_matmul(src, ptr, None)
+    with pytest.raises(TypeError, match="dtype"):
+        segment_matmul(src.double(), ptr, weight.double())
+    with pytest.raises(TypeError, match="match"):
+        segment_matmul(src, ptr, weight.half())
+    with pytest.raises(TypeError, match="indptr"):
+        segment_matmul(src, ptr.float(), weight)
+    with pytest.raises(ValueError, match="2-D"):
+        segment_matmul(src[0], ptr, weight)
+    with pytest.raises(ValueError, match="3-D"):
+        segment_matmul(src, ptr, weight[0])
+    with pytest.raises(ValueError, match="size"):
+        segment_matmul(src, ptr, weight[:, :7])
+    with pytest.raises(ValueError, match="pointer"):
+        segment_matmul(src, torch.tensor([0, 2, 4]), weight)
+    with pytest.raises(ValueError, match="1-D"):
+        segment_matmul(src, ptr.view(1, 2), weight)
+
+
+def test_fp8_refuses():
+    from ops_gnn import quantize_fp8, segment_matmul_fp8
+
+    src = torch.zeros(4, 160)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        quantize_fp8(src)
+    with pytest.raises(TypeError, match="dtype"):
+        quantize_fp8(src.double())
+    with pytest.raises(ValueError, match="two dimensions"):
+        quantize_fp8(src[0])
+    with pytest.raises(ValueError, match="block_rows"):
+        quantize_fp8(src, block_rows=64)
+    with pytest.raises(TypeError, match="block_rows"):
+        quantize_fp8(src, block_rows=True)
+    f8 = torch.float8_e4m3fn
+    args = [src.to(f8), torch.ones(4, 2), torch.zeros(3, 8, 160).to(f8), torch.ones(3, 1, 2)]
+    ptr = torch.tensor([0, 1, 2, 4])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        segment_matmul_fp8(*args, ptr)
+    with pytest.raises(TypeError, match="src dtype"):
+        segment_matmul_fp8(src, *args[1:], ptr)
+    with pytest.raises(TypeError, match="weight_scale dtype"):
+        segment_matmul_fp8(*args[:3], args[3].double(), ptr)
+    with pytest.raises(TypeError, match="out_dtype"):
+        segment_matmul_fp8(*args, ptr, out_dtype=torch.float64)
+    with pytest.raises(ValueError, match="2-D"):
+        segment_matmul_fp8(*args)  # three weights and no pointers
+    with pytest.raises(ValueError, match="src_scale"):
+        segment_matmul_fp8(args[0], torch.ones(4, 1), *args[2:], ptr)
+    with pytest.raises(ValueError, match="weight_scale"):
+        segment_matmul_fp8(*args[:3], torch.ones(3, 2, 2), ptr)
+    with pytest.raises(ValueError, match="pointer"):
+        segment_matmul_fp8(*args, ptr[:3])
+
+
+def test_c_abi_refuses():
+    """Bad descriptors and null pointers come back as status codes before anything is launched."""
+    from ops_gnn import _cabi
+
+    lib = _cabi.load()
+    size = ctypes.c_int64()
+    ref = ctypes.byref
+
+    def route(**kw):
+        fields = dict(rows=4, experts=16, k=2, groups=1, kept_groups=1, scale=1.0, group_top=1, score=0, renormalize=1,
+                      dtype=_cabi.F32)
+        fields.update(kw)
+        return lib.opsgnn_topk_route(ref(_cabi.RouteDesc(*fields.values())), None, None, None, None, None)
+
+    assert route() == -1 and route(rows=0) == 0
+    assert route(groups=3) == -1 and route(k=17) == -1 and route(kept_groups=2) == -1 and route(group_top=3) == -1
+    assert route(experts=2048) == -4 and route(experts=64, k=33) == -4 and route(dtype=_cabi.F64) == -2
+    assert lib.opsgnn_route_csr_workspace_bytes(10, 4097, ref(size)) == -4
+    assert lib.opsgnn_route_csr_workspace_bytes(2 ** 31, 16, ref(size)) == -4
+    assert lib.opsgnn_route_csr_workspace_bytes(-1, 16, ref(size)) == -1
+    assert lib.opsgnn_route_csr_workspace_bytes(100000, 16, ref(size)) == 0 and size.value > 0
+    assert lib.opsgnn_route_csr(1, _cabi.I64, 100000, 16, 1, 1, 1, None, 0, None) == -3
+
+    def matmul(call, *pointers, **kw):
+        fields = dict(rows=4, segments=2, width=8, out=8, src_stride=8, weight_segment_stride=64, weight_width_stride=8,
+                      weight_out_stride=1, index_type=_cabi.I64, in_type=_cabi.BF16, out_type=_cabi.BF16)
+        fields.update(kw)
+        return call(ref(_cabi.SegmentMatmulDesc(*fields.values())), *pointers)
+
+    rows, outer, fp8 = lib.opsgnn_segment_matmul, lib.opsgnn_segment_matmul_weight_grad, lib.opsgnn_segment_matmul_fp8
+    assert matmul(rows, None, None, None, None, None) == -1
+    assert matmul(rows, None, None, None, None, None, rows=0) == 0
+    assert matmul(rows, None, None, None, None, None, src_stride=7) == -1
+    assert matmul(rows, None, None, None, None, None, out_type=_cabi.F32) == -2
+    assert matmul(rows, None, None, None, None, None, in_type=_cabi.F64, out_type=_cabi.F64) == -2
+    assert matmul(rows, None, None, None, None, None, index_type=_cabi.F32) == -1
+    assert matmul(outer, None, None, None, 8, None, None) == -1
+    assert matmul(outer, None, None, None, 8, None, None, segments=0) == 0
+    assert matmul(fp8, None, None, None, None, None, None, None) == -2
+    assert matmul(fp8, None, None, None, None, None, None, None, in_type=_cabi.F8E4M3) == -1
+    assert lib.opsgnn_quantize_fp8(None, _cabi.BF16, 1, 4, 4, 1, None, None, None) == -1
+    assert lib.opsgnn_quantize_fp8(None, _cabi.BF16, 1, 0, 4, 1, None, None, None) == 0
+    assert lib.opsgnn_quantize_fp8(None, _cabi.BF16, 1, 4, 4, 64, None, None, None) == -1
+    assert lib.opsgnn_quantize_fp8(1, _cabi.F64, 1, 4, 4, 1, 1, 1, None) == -2
+
+
+# ---- topk_route ----------------------------------------------------------------------------------------------------------
+
+ROUTES = [
+    # rows, experts, k, score, bias, groups, kept, group_top, renormalize, dtype
+    (1, 1, 1, "softmax", False, 1, 1, 2, True, torch.float32),
+    (1, 64, 2, "softmax", False, 1, 1, 2, True, torch.bfloat16),
+    (37, 7, 3, "sigmoid", False, 1, 1, 2, False, torch.float16),
+    (65, 33, 4, "softmax", True, 1, 1, 2, False, torch.float32),
+    (129, 100, 8, "softmax", False, 1, 1, 2, False, torch.bfloat16),
+    (70, 96, 6, "sigmoid", True, 6, 2, 2, True, torch.float32),
+    (70, 96, 6, "softmax", True, 8, 3, 1, True, torch.bfloat16),
+    (33, 256, 8, "sigmoid", True, 8, 4, 2, True, torch.float32),
+    (33, 256, 8, "sigmoid", False, 8, 4, 1, True, torch.float16),
+    (33, 160, 6, "softmax", False, 8, 3, 2, False, torch.float32),
+    (9, 384, 8, "sigmoid", True, 1, 1, 2, True, torch.bfloat16),
+    (9, 513, 32, "softmax", False, 1, 1, 2, True, torch.float32),
+    (5, 1024, 32, "sigmoid", True, 32, 32, 2, True, torch.float32),
+    (5, 1024, 9, "softmax", False, 32, 5, 2, True, torch.bfloat16),
+    (3, 32, 32, "softmax", False, 1, 1, 2, False, torch.float32),
+]
+
+
+def _route_inputs(case, seed=3):
+    rows, experts, k, score, with_bias, groups, kept, top, renormalize, dtype = case
+    gen = _gen(seed)
+    logits = (torch.randn(rows, experts, generator=gen) * 2).to(dtype)
+    bias = torch.randn(experts, generator=gen) * 0.1 if with_bias else None
+    return logits, bias
+
+
+def _check_route(logits, bias, case, weight, index, what):
+    rows, experts, k, score, _, groups, kept, top, renormalize, dtype = case
+    want_index = _plain_choice(logits, k, score, bias, groups, kept, 1 if groups == 1 else top)
+    assert torch.equal(index.cpu(), want_index), what + ": index"
+    want = _plain_weight(logits, want_index, score, renormalize, 1.0)
+    _within(weight, want, want, experts + 16, what + ": weight")
+
+
+@requires_gpu
+@pytest.mark.parametrize("case", ROUTES, ids=str)
+def test_topk_route_forward(cuda_device, case):
+    from ops_gnn import topk_route
+
+    logits, bias = _route_inputs(case)
+    _, _, k, score, _, groups, kept, top, renormalize, _ = case
+    weight, index = topk_route(logits.to(cuda_device), k, score, None if bias is None else bias.to(cuda_device), groups, kept, top,
+                               renormalize)
+    _check_route(logits, bias, case, weight, index, str(case))
+
+
+@requires_gpu
+@pytest.mark.parametrize("case", [c for c in ROUTES if c[1] >= 32], ids=str)
+def test_topk_route_ties_and_masks(cuda_device, case):
+    """Whole-number logits (many ties), masked experts, a row with one expert left and a row with none."""
+    from ops_gnn import topk_route
+
+    rows, experts, k, score, _, groups, kept, top, renormalize, dtype = case
+    logits, bias = _route_inputs(case, 5)
+    logits = logits.round()
+    logits[torch.rand(logits.shape, generator=_gen(6)) < 0.3] = -math.inf
+    logits[0] = -math.inf
+    if rows > 2:
+        logits[2] = -math.inf
+        logits[2, experts // 2] = 1.0
+    if rows > 3:
+        logits[3] = torch.finfo(dtype).min
+    weight, index = topk_route(logits.to(cuda_device), k, score, None if bias is None else bias.to(cuda_device), groups, kept, top,
+                               renormalize)
+    _check_route(logits, bias, case, weight, index, str(case))
+    assert (weight[0] == 0).all()
+
+
+@requires_gpu
+def test_topk_route_nan_and_infinity(cuda_device):
+    from ops_gnn import topk_route
+
+    x = torch.randn(6, 40, generator=_gen(1))
+    x[1, 3] = math.nan
+    x[2, 5] = math.inf
+    weight, index = topk_route(x.to(cuda_device), 4)
+    plain, plain_index = topk_route(torch.randn(6, 40, generator=_gen(1)).to(cuda_device), 4)
+    for r in (0, 3, 4, 5):  # the other rows do not change
+        assert torch.equal(weight[r], plain[r]) and torch.equal(index[r], plain_index[r])
+    assert torch.isnan(weight[1]).all() and torch.isnan(weight[2]).all()
+    assert index[1].tolist() == [0, 1, 2, 3] and index[2].tolist() == [0, 1, 2, 3]
+    weight, index = topk_route(x.to(cuda_device), 4, score="sigmoid", renormalize=False)
+    assert 3 not in index[1].tolist() and index[2, 0] == 5 and weight[2, 0] == 1 and not torch.isnan(weight).any()
+
+
+@requires_gpu
+def test_topk_route_close_scores(cuda_device):
+    """Scores that differ by less than fp32 tells apart: the bias is the only difference, in its last bits."""
+    from ops_gnn import topk_route
+
+    experts = 128
+    bias = torch.full((experts,), 1.0)
+    bias[77] = torch.nextafter(torch.tensor(1.0), torch.tensor(2.0))
+    logits = torch.full((3, experts), -20.0)  # sigmoid(-20) = 2e-9: lost beside 1 in fp32
+    logits[1, 9] = -19.999
+    weight, index = topk_route(logits.to(cuda_device), 3, score="sigmoid", bias=bias.to(cuda_device))
+    assert index.tolist() == [[77, 0, 1], [77, 9, 0], [77, 0, 1]]
+
+
+@requires_gpu
+@pytest.mark.parametrize("case", ROUTES, ids=str)
+def test_topk_route_gradient(cuda_device, case):
+    """Against the formula by float64 autograd of the restated weights, and against central differences of them."""
+    from ops_gnn import topk_route
+
+    rows, experts, k, score, _, groups, kept, top, renormalize, dtype = case
+    logits, bias = _route_inputs(case)
+    if experts > 4:
+        logits[rows // 2, 1] = -math.inf
+    leaf = logits.to(cuda_device).requires_grad_()
+    weight, index = topk_route(leaf, k, score, None if bias is None else bias.to(cuda_device), groups, kept, top, renormalize, 2.5)
+    grad = torch.randn(rows, k, generator=_gen(8)).to(dtype)
+    got, = torch.autograd.grad(weight, leaf, grad.to(cuda_device))
+    assert got.dtype == dtype
+
+    chosen = index.cpu()
+    x = logits.double().requires_grad_()
+    w = _plain_weight(x, chosen, score, renormalize, 2.5)
+    want, = torch.autograd.grad(w, x, grad.double())
+    want = torch.nan_to_num(want)  # exp(-inf) in float64 autograd
+    s = _plain_scores(logits, score)
+    u = 2.5 * grad.double().abs()
+    magnitude = torch.zeros_like(s).scatter_add_(1, chosen, u) + (u * s.gather(1, chosen)).sum(1, keepdim=True)
+    if renormalize:
+        picked = s.gather(1, chosen)
+        total = picked.sum(1, keepdim=True)
+        mean = (u * picked).sum(1, keepdim=True) / total
+        magnitude = torch.zeros_like(s).scatter_add_(1, chosen, (u + mean) / total)
+    _within(got, want, magnitude * s, 4 * experts + 64, str(case))
+
+    # Central differences of the restated sum at a few places, step 1e-5: truncation 1e-10, cancellation 1e-11.
+    for r, j in ((0, int(chosen[0, 0])), (rows - 1, int(chosen[rows - 1, -1])), (rows // 2, 0)):
+        if logits[r, j] == -math.inf:
+            continue
+        low, high = logits.double(), logits.double()
+        low[r, j] -= 1e-5
+        high[r, j] += 1e-5
+        slope = ((_plain_weight(high, chosen, score, renormalize, 2.5) - _plain_weight(low, chosen, score, renormalize, 2.5))[r]
+                 * grad[r].double()).sum() / 2e-5
+        bound = 1e-6 + torch.finfo(dtype).eps * abs(float(slope)) + (4 * experts + 64) * STEP * float((magnitude * s)[r, j])
+        assert abs(float(slope) - float(got[r, j])) <= bound
+
+
+@requires_gpu
+def test_topk_route_shapes_and_layouts(cuda_device):
+    from ops_gnn import topk_route
+
+    x = torch.randn(2, 3, 24, generator=_gen(2)).to(cuda_device)
+    weight, index = topk_route(x, 4)
+    assert weight.shape == (2, 3, 4) and index.shape == (2, 3, 4) and index.dtype == torch.int64
+    flat_weight, flat_index = topk_route(x.view(6, 24), 4)
+    assert torch.equal(weight.view(6, 4), flat_weight) and torch.equal(index.view(6, 4), flat_index)
+    turned = x.view(6, 24).t().contiguous().t()
+    assert torch.equal(topk_route(turned, 4)[1], flat_index)
+    shifted = torch.empty(6 * 24 + 1, device=cuda_device)[1:].view(6, 24).copy_(x.view(6, 24))  # 4-byte aligned only
+    assert torch.equal(topk_route(shifted, 4)[0], flat_weight)
+    one = topk_route(x[0, 0], 4)
+    assert torch.equal(one[0], weight[0, 0]) and one[0].shape == (4,)
+    empty_weight, empty_index = topk_route(x.new_zeros(0, 24), 4)
+    assert empty_weight.shape == (0, 4) and empty_index.shape == (0, 4)
+    leaf = x.view(6, 24).clone().requires_grad_()
+    weight, index = topk_route(leaf, 4)
+    assert weight.requires_grad and not index.requires_grad
+    again, = torch.autograd.grad(weight.sum(), leaf)  # weights add up to 1: the gradient of their sum is 0
+    assert float(again.abs().max()) <= 8 * STEP
+
+
+# ---- route_csr -----------------------------------------------------------------------------------------------------------
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
+@pytest.mark.parametrize("count,experts", [(0, 1), (1, 1), (31, 3), (512, 64), (2048, 300), (2049, 8), (5000, 4096), (70001, 257),
+                                           (300000, 17)])
+def test_route_csr(cuda_device, count, experts, dtype):
+    from ops_gnn import route_csr
+
+    gen = _gen(count + experts)
+    index = torch.randint(0, experts, (count,), generator=gen, dtype=dtype)
+    if count > 40:
+        index[torch.rand(count, generator=gen) < 0.1] = experts - 1     # a popular expert
+        index[torch.rand(count, generator=gen) < 0.05] = -1             # dropped
+        index[7], index[11] = experts, torch.iinfo(dtype).min           # outside the range
+    indptr, perm, position = route_csr(index.to(cuda_device), experts)
+    label = torch.where((index >= 0) & (index < experts), index, experts).long()
+    want = torch.sort(label, stable=True).indices
+    assert torch.equal(perm.cpu(), want)
+    counts = torch.bincount(label, minlength=experts + 1)[:experts]
+    assert torch.equal(indptr.cpu(), torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)]))
+    back = torch.empty_like(want)
+    back[want] = torch.arange(count)
+    assert torch.equal(position.cpu(), back)
+
+
+@requires_gpu
+def test_route_csr_shape_and_strides(cuda_device):
+    from ops_gnn import route_csr
+
+    index = torch.randint(0, 9, (50, 4), generator=_gen(1)).to(cuda_device)
+    indptr, perm, position = route_csr(index, 9)
+    assert position.shape == (50, 4) and perm.shape == (200,)
+    other = route_csr(index.t().contiguous().t(), 9)
+    assert all(torch.equal(a, b) for a, b in zip((indptr, perm, position), other))
+    assert torch.equal(index.view(-1)[perm], torch.sort(index.view(-1)).values)
+
+
+# ---- segment_matmul ------------------------------------------------------------------------------------------------------
+
+MATMULS = [
+    # lengths, rows before, rows behind, K, N
+    ([5], 0, 0, 16, 24),
+    ([1], 0, 0, 8, 8),
+    ([3, 0, 1, 130, 0, 64], 0, 0, 64, 96),
+    ([0, 0, 0], 0, 7, 32, 16),
+    ([127, 128, 129, 1, 0, 255], 3, 5, 136, 264),
+    ([40, 30], 2, 0, 7, 5),          # nothing is a whole vector
+    ([33, 65, 2], 0, 1, 65, 130),
+    ([200, 57], 0, 0, 256, 8),
+    ([300], 0, 0, 8, 520),
+    ([2] * 70, 0, 0, 72, 40),        # more segments than a warp has lanes
+    ([1, 700, 0, 450], 0, 0, 520, 264),
+    ([513], 10, 10, 1, 1),
+]
+KINDS = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _matmul_inputs(case, dtype, seed=11):
+    lengths, before, behind, k, n = case
+    gen = _gen(seed)
+    rows = before + sum(lengths) + behind
+    src = torch.randn(rows, k, generator=gen).to(dtype)
+    weight = torch.randn(len(lengths), k, n, generator=gen).to(dtype)
+    grad = torch.randn(rows, n, generator=gen).to(dtype)
+    return src, _pointers(lengths, before), weight, grad
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", KINDS, ids=str)
+@pytest.mark.parametrize("case", MATMULS, ids=str)
+def test_segment_matmul(cuda_device, case, dtype):
+    """Forward and both gradients, both layouts of the weight, both pointer widths."""
+    from ops_gnn import segment_matmul
+
+    src, ptr, weight, grad = _matmul_inputs(case, dtype)
+    want = _plain_matmul(src, ptr, weight)
+    want_src = _plain_matmul(grad, ptr, weight.transpose(1, 2))
+    want_weight = _plain_weight_grad(src, ptr, grad)
+    size = _plain_matmul(src.abs(), ptr, weight.abs())
+    size_src = _plain_matmul(grad.abs(), ptr, weight.abs().transpose(1, 2))
+    size_weight = _plain_weight_grad(src.abs(), ptr, grad.abs())
+    longest = max(case[0])
+    for turned in (False, True):
+        x = src.to(cuda_device).requires_grad_()
+        w = (weight.transpose(1, 2).contiguous() if turned else weight).to(cuda_device).requires_grad_()
+        pointers = ptr.to(cuda_device).to(torch.int32 if turned else torch.int64)
+        out = segment_matmul(x, pointers, w.transpose(1, 2) if turned else w)
+        grad_src, grad_weight = torch.autograd.grad(out, (x, w), grad.to(cuda_device))
+        if turned:
+            grad_weight = grad_weight.transpose(1, 2)
+        _within(out, want, size, case[3] + 2, "out")
+        _within(grad_src, want_src, size_src, case[4] + 2, "grad_src")
+        _within(grad_weight, want_weight, size_weight, longest + 2, "grad_weight")
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", KINDS, ids=str)
+def test_segment_matmul_layouts(cuda_device, dtype):
+    """Rows of a wider matrix, rows at an odd offset, turned rows, a weight of another stride, one weight for all segments."""
+    from ops_gnn import segment_matmul
+
+    src, ptr, weight, _ = _matmul_inputs(([30, 0, 140, 9], 1, 2, 64, 72), dtype)
+    d_src, d_ptr, d_weight = src.to(cuda_device), ptr.to(cuda_device), weight.to(cuda_device)
+    size = _plain_matmul(src.abs(), ptr, weight.abs())
+    want = _plain_matmul(src, ptr, weight)
+    wide = torch.full((src.size(0), 100), math.nan, dtype=dtype, device=cuda_device)
+    for offset in (0, 8, 3):
+        view = wide[:, offset:offset + 64]
+        view.copy_(d_src)
+        _within(segment_matmul(view, d_ptr, d_weight), want, size, 66, f"offset {offset}")
+        view.fill_(math.nan)
+    _within(segment_matmul(d_src.t().contiguous().t(), d_ptr, d_weight), want, size, 66, "turned rows")
+    padded = torch.full((4, 80, 100), math.nan, dtype=dtype, device=cuda_device)
+    for k0, n0 in ((0, 0), (8, 16), (1, 3)):
+        view = padded[:, k0:k0 + 64, n0:n0 + 72]
+        view.copy_(d_weight)
+        _within(segment_matmul(d_src, d_ptr, view), want, size, 66, f"weight at {k0}, {n0}")
+        view.fill_(math.nan)
+    shared = weight[:1].expand(4, -1, -1)
+    leaf = weight[:1].to(cuda_device).requires_grad_()
+    out = segment_matmul(d_src, d_ptr, leaf.expand(4, -1, -1))
+    _within(out, _plain_matmul(src, ptr, shared), _plain_matmul(src.abs(), ptr, shared.abs()), 66, "one weight")
+    total, = torch.autograd.grad(out.float().sum(), leaf)
+    inside = src[1:180].double()
+    # the four segments' gradients are rounded to the dtype each and added in it: four more roundings of the magnitude
+    bound = (200 * STEP + 4 * torch.finfo(dtype).eps) * inside.abs().sum(0)
+    assert ((total[0].cpu().double() - inside.sum(0).unsqueeze(1)).abs() <= bound.unsqueeze(1)).all()
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", KINDS, ids=str)
+def test_segment_matmul_empty(cuda_device, dtype):
+    from ops_gnn import segment_matmul
+
+    def run(rows, lengths, k, n):
+        x = torch.ones(rows, k, dtype=dtype, device=cuda_device, requires_grad=True)
+        w = torch.ones(len(lengths), k, n, dtype=dtype, device=cuda_device, requires_grad=True)
+        out = segment_matmul(x, _pointers(lengths).to(cuda_device), w)
+        return (out,) + torch.autograd.grad(out.sum(), (x, w))
+
+    out, gx, gw = run(5, [], 16, 8)                  # no segments: zeros
+    assert out.shape == (5, 8) and not out.any() and not gx.any() and gw.shape == (0, 16, 8)
+    out, gx, gw = run(0, [0, 0], 16, 8)              # no rows
+    assert out.shape == (0, 8) and gx.shape == (0, 16) and gw.shape == (2, 16, 8) and not gw.any()
+    out, gx, gw = run(6, [2, 4], 0, 8)               # empty sums
+    assert out.shape == (6, 8) and not out.any() and gx.shape == (6, 0) and gw.shape == (2, 0, 8)
+    out, gx, gw = run(6, [2, 4], 16, 0)
+    assert out.shape == (6, 0) and not gx.any() and gw.shape == (2, 16, 0)
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", KINDS, ids=str)
+@pytest.mark.parametrize("k,n", [(64, 128), (200, 72), (33, 5)])
+def test_segment_matmul_special_values_stay_in_their_segment(cuda_device, dtype, k, n):
+    """NaN and infinities of one segment, and in rows of no segment, reach nothing outside that segment's results."""
+    from ops_gnn import segment_matmul
+
+    lengths = [10, 130, 1, 70]
+    src, ptr, weight, grad = _matmul_inputs((lengths, 4, 6, k, n), dtype)
+    clean = [t.to(cuda_device) for t in (src, ptr, weight, grad)]
+    dirty = [t.clone() for t in clean]
+    low, high = int(ptr[1]), int(ptr[2])
+    for t in (dirty[0], dirty[3]):
+        t[low:high] = math.nan
+        t[:4] = math.inf
+        t[-6:] = -math.inf
+    dirty[2][1] = math.inf
+
+    def run(x, p, w, g):
+        x, w = x.requires_grad_(), w.requires_grad_()
+        out = segment_matmul(x, p, w)
+        return (out.detach(),) + torch.autograd.grad(out, (x, w), g)
+
+    plain, other = run(*clean), run(*dirty)
+    keep = torch.ones(src.size(0), dtype=torch.bool, device=cuda_device)
+    keep[low:high] = False
+    for a, b in zip(plain[:2], other[:2]):
+        assert torch.equal(a[keep], b[keep]) and torch.isnan(b[low:high]).all()
+    for e in (0, 2, 3):
+        assert torch.equal(plain[2][e], other[2][e])
+    assert torch.isnan(other[2][1]).all()
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", KINDS, ids=str)
+def test_segment_matmul_infinities_as_the_formula_has_them(cuda_device, dtype):
+    from ops_gnn import segment_matmul
+
+    src = torch.ones(140, 64, dtype=dtype)
+    weight = torch.ones(1, 64, 72, dtype=dtype) * 0.5
+    src[3, 5] = math.inf
+    src[4, 5], src[4, 6] = math.inf, -math.inf
+    src[139, 0] = -math.inf
+    weight[0, 9, 7] = math.inf
+    weight[0, :, 8] = 0
+    out = segment_matmul(src.to(cuda_device), torch.tensor([0, 140], device=cuda_device), weight.to(cuda_device)).cpu()
+    want = src.double() @ weight[0].double()
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out[~torch.isnan(out)].double(), want[~torch.isnan(want)])
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", KINDS, ids=str)
+def test_segment_matmul_pointers_out_of_range(cuda_device, dtype):
+    """Pointers outside the rows count as the nearer end, a segment that ends before it starts is empty."""
+    from ops_gnn import segment_matmul
+
+    src, _, weight, grad = _matmul_inputs(([100, 100, 100], 0, 0, 64, 64), dtype)
+    ptr = torch.tensor([-5, 40, 2 ** 40, 2 ** 62])
+    x, w = src.to(cuda_device).requires_grad_(), weight.to(cuda_device).requires_grad_()
+    out = segment_matmul(x, ptr.to(cuda_device), w)
+    grad_src, grad_weight = torch.autograd.grad(out, (x, w), grad.to(cuda_device))
+    sane = torch.tensor([0, 40, 300, 300])
+    _within(out, _plain_matmul(src, sane, weight), _plain_matmul(src.abs(), sane, weight.abs()), 66, "out")
+    _within(grad_weight, _plain_weight_grad(src, sane, grad), _plain_weight_grad(src.abs(), sane, grad.abs()), 302, "grad_weight")
+    back = segment_matmul(src.to(cuda_device), torch.tensor([0, 200, 100, 300], device=cuda_device), weight.to(cuda_device))
+    _within(back[:100], _plain_matmul(src, torch.tensor([0, 200, 200, 300]), weight)[:100],
+            _plain_matmul(src.abs(), torch.tensor([0, 200, 200, 300]), weight.abs())[:100], 66, "before the overlap")
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", KINDS, ids=str)
+def test_segment_matmul_gradients_against_differences(cuda_device, dtype):
+    """The sum of out * grad is linear in src and in weight, so differences with a step of 1 are exact up to rounding."""
+    from ops_gnn import segment_matmul
+
+    src, ptr, weight, grad = _matmul_inputs(([20, 0, 45], 0, 3, 40, 24), dtype)
+    x, w = src.to(cuda_device).requires_grad_(), weight.to(cuda_device).requires_grad_()
+    grads = torch.autograd.grad(segment_matmul(x, ptr.to(cuda_device), w), (x, w), grad.to(cuda_device))
+
+    def total(a, b):
+        return (_plain_matmul(a, ptr, b) * grad.double()).sum()
+
+    base = total(src, weight)
+    for at in ((0, 0), (19, 39), (20, 7), (64, 1), (66, 2)):
+        moved = src.double()
+        moved[at] += 1
+        slope = float(total(moved, weight) - base)
+        size = float((grad[at[0]].double().abs() * weight.double().abs().amax(0)[at[1]]).sum())
+        assert abs(slope - float(grads[0][at])) <= torch.finfo(dtype).eps * abs(slope) + 26 * STEP * size + 1e-9
+    for at in ((0, 0, 0), (1, 3, 4), (2, 39, 23)):
+        moved = weight.double()
+        moved[at] += 1
+        slope = float(total(src, moved) - base)
+        size = float((src[:, at[1]].double().abs() * grad[:, at[2]].double().abs()).sum())
+        assert abs(slope - float(grads[1][at])) <= torch.finfo(dtype).eps * abs(slope) + 70 * STEP * size + 1e-9
+
+
+@requires_gpu
+def test_segment_matmul_is_reproducible_and_refuses_second_derivatives(cuda_device):
+    from ops_gnn import segment_matmul
+
+    src, ptr, weight, grad = [t.to(cuda_device) for t in _matmul_inputs(([500, 3, 900], 0, 0, 256, 256), torch.bfloat16)]
+    x, w = src.requires_grad_(), weight.requires_grad_()
+    runs = []
+    for _ in range(3):
+        out = segment_matmul(x, ptr, w)
+        runs.append((out.detach(),) + torch.autograd.grad(out, (x, w), grad))
+    assert all(torch.equal(a, b) for run in runs[1:] for a, b in zip(runs[0], run))
+    out = segment_matmul(x, ptr, w)
+    first, = torch.autograd.grad(out.float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.float().sum(), w)
+
+
+# ---- quantize_fp8 --------------------------------------------------------------------------------------------------------
+
+def _plain_quantize(x, block_rows):
+    """Block by block on the CPU; torch's own conversion to float8 rounds to nearest even."""
+    x = x.double()
+    values = torch.empty(x.shape, dtype=torch.float8_e4m3fn)
+    rows, width = x.shape
+    scale = torch.empty(-(-rows // block_rows), -(-width // 128))
+    for i in range(scale.size(0)):
+        for j in range(scale.size(1)):
+            part = x[i * block_rows:(i + 1) * block_rows, j * 128:(j + 1) * 128]
+            finite = part[torch.isfinite(part)].abs()
+            top = float(finite.max()) if finite.numel() else 0.0
+            p = -126
+            while top > 0 and top > 448 * 2.0 ** p:
+                p += 1
+            s = 2.0 ** p if top > 0 else 1.0
+            scale[i, j] = s
+            values[i * block_rows:(i + 1) * block_rows, j * 128:(j + 1) * 128] = \
+                (part / s).clamp(-448, 448).float().to(torch.float8_e4m3fn)
+    return values, scale
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", KINDS, ids=str)
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("rows,width", [(1, 1), (1, 128), (3, 130), (130, 256), (129, 257), (5, 1000), (260, 24)])
+def test_quantize_fp8(cuda_device, rows, width, block_rows, dtype):
+    from ops_gnn import quantize_fp8
+
+    gen = _gen(rows * 1000 + width)
+    x = torch.randn(rows, width, generator=gen) * torch.exp2(torch.randint(-30, 12, (rows, 1), generator=gen).float())
+    x = x.clamp(-60000, 60000).to(dtype)
+    if rows > 2:
+        x[1] = 0
+        x[2, 0] = 448.0
+    if width > 128:
+        x[0, 5], x[0, 6], x[0, 7] = math.nan, math.inf, -math.inf
+    values, scale = quantize_fp8(x.to(cuda_device), block_rows)
+    want, want_scale = _plain_quantize(x, block_rows)
+    assert torch.equal(scale.cpu(), want_scale)
+    assert values.dtype == torch.float8_e4m3fn and values.shape == x.shape
+    got, want = values.cpu().float(), want.float()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+
+
+@requires_gpu
+def test_quantize_fp8_extremes_and_borders(cuda_device):
+    """The largest and smallest numbers, exact borders of the scale, ties of the rounding, batches, views, no rows."""
+    from ops_gnn import quantize_fp8
+
+    big, tiny = torch.finfo(torch.float32).max, torch.finfo(torch.float32).tiny
+    x = torch.zeros(8, 128)
+    x[0, 0], x[1, 0], x[2, 0], x[3, 0] = big, tiny, 448.0, math.nextafter(448.0, 1000)
+    x[3, 0] = float(torch.nextafter(torch.tensor(448.0), torch.tensor(1000.0)))
+    x[4, 3] = 2.0 ** -149
+    x[5, :3] = torch.tensor([256.0, 17.0, 19.0])     # 17 and 19 lie between 16, 18 and 20: ties to even
+    x[6, :2] = torch.tensor([math.inf, math.nan])    # nothing finite: scale 1
+    values, scale = quantize_fp8(x.to(cuda_device))
+    want, want_scale = _plain_quantize(x, 1)
+    assert torch.equal(scale.cpu(), want_scale) and torch.equal(torch.nan_to_num(values.cpu().float()), torch.nan_to_num(want.float()))
+    assert scale[2, 0] == 1 and scale[3, 0] == 2 and scale[6, 0] == 1 and scale[7, 0] == 1
+    assert values[5, :3].float().tolist() == [256.0, 16.0, 20.0] and values[6, 0].float() == 448
+
+    y = torch.randn(2, 3, 140, 200, generator=_gen(4)).to(cuda_device)
+    for block_rows in (1, 128):
+        values, scale = quantize_fp8(y, block_rows)
+        assert values.shape == y.shape and scale.shape == ((2, 3, 140, 2) if block_rows == 1 else (2, 3, 2, 2))
+        one, one_scale = quantize_fp8(y[1, 2], block_rows)
+        assert torch.equal(values[1, 2].float(), one.float()) and torch.equal(scale[1, 2], one_scale)
+        again, again_scale = quantize_fp8(y.transpose(2, 3).contiguous().transpose(2, 3), block_rows)
+        assert torch.equal(values.float(), again.float()) and torch.equal(scale, again_scale)
+    values, scale = quantize_fp8(y[:, :, :0])
+    assert values.shape == (2, 3, 0, 200) and scale.shape == (2, 3, 0, 2)
+
+
+# ---- segment_matmul_fp8 --------------------------------------------------------------------------------------------------
+
+def _fp8_inputs(lengths, before, behind, k, n, seed=21, power=False):
+    gen = _gen(seed)
+    rows = before + sum(lengths) + behind
+    src = (torch.randn(rows, k, generator=gen) * 60).clamp(-448, 448).to(torch.float8_e4m3fn)
+    weight = (torch.randn(len(lengths), n, k, generator=gen) * 60).clamp(-448, 448).to(torch.float8_e4m3fn)
+    blocks, bands = -(-k // 128), -(-n // 128)
+    src_scale = torch.rand(rows, blocks, generator=gen) + 0.1
+    weight_scale = torch.rand(len(lengths), bands, blocks, generator=gen) + 0.1
+    if power:
+        src_scale, weight_scale = torch.exp2(torch.round(src_scale * 9 - 5)), torch.exp2(torch.round(weight_scale * 9 - 5))
+    return src, src_scale, weight, weight_scale, _pointers(lengths, before)
+
+
+def _stands_for(values, scale, block_rows):
+    v = values.float().double()
+    s = scale.double().repeat_interleave(block_rows, -2)[..., :v.size(-2), :].repeat_interleave(128, -1)[..., :v.size(-1)]
+    return v * s
+
+
+FP8S = [
+    ([5], 0, 0, 128, 128),
+    ([1, 0, 2], 1, 2, 16, 8),
+    ([129, 0, 64, 1], 0, 5, 272, 136),
+    ([300, 40], 3, 0, 1040, 264),
+    ([17, 3], 0, 0, 37, 21),           # nothing is a whole vector
+    ([2] * 40, 0, 0, 144, 48),
+]
+
+
+@requires_gpu
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+@pytest.mark.parametrize("case", FP8S, ids=str)
+def test_segment_matmul_fp8(cuda_device, case, out_dtype):
+    from ops_gnn import segment_matmul_fp8
+
+    args = _fp8_inputs(*case, power=out_dtype == torch.float16)
+    if out_dtype == torch.float16:  # keep the sums inside the type's range
+        args = (args[0], args[1] * 2.0 ** -9, args[2], args[3] * 2.0 ** -9, args[4])
+    src, src_scale, weight, weight_scale, ptr = args
+    a, b = _stands_for(src, src_scale, 1), _stands_for(weight, weight_scale, 128).transpose(1, 2)
+    got = segment_matmul_fp8(*[t.to(cuda_device) for t in args[:4]], ptr.to(cuda_device), out_dtype)
+    assert got.dtype == out_dtype
+    # K products, one more rounding for each product of two scales and each block's multiply-add
+    _within(got, _plain_matmul(a, ptr, b), _plain_matmul(a.abs(), ptr, b.abs()), case[3] + 4, str(case))
+
+
+@requires_gpu
+@pytest.mark.parametrize("m,k,n", [(1, 128, 128), (200, 384, 264), (1, 2048, 16), (130, 48, 1), (0, 128, 128), (5, 0, 9)])
+def test_segment_matmul_fp8_dense(cuda_device, m, k, n):
+    from ops_gnn import segment_matmul_fp8
+
+    src, src_scale, weight, weight_scale, _ = _fp8_inputs([m], 0, 0, k, n)
+    got = segment_matmul_fp8(src.to(cuda_device), src_scale.to(cuda_device), weight[0].to(cuda_device), weight_scale[0].to(cuda_device),
+                             out_dtype=torch.float32)
+    a, b = _stands_for(src, src_scale, 1), _stands_for(weight, weight_scale, 128)[0]
+    assert got.shape == (m, n)
+    _within(got, a @ b.t(), a.abs() @ b.abs().t(), k + 4, "dense")
+
+
+@requires_gpu
+def test_segment_matmul_fp8_layouts_and_special_values(cuda_device):
+    from ops_gnn import segment_matmul_fp8
+
+    args = _fp8_inputs([70, 0, 130, 4], 0, 3, 256, 128)
+    dev = [t.to(cuda_device) for t in args]
+    plain = segment_matmul_fp8(*dev, out_dtype=torch.float32)
+    assert not plain[-3:].any()
+    wide = torch.zeros(207, 300, dtype=torch.uint8, device=cuda_device).view(torch.float8_e4m3fn)
+    for offset in (0, 16, 5):
+        view = wide[:, offset:offset + 256]
+        view.view(torch.uint8).copy_(dev[0].view(torch.uint8))
+        assert torch.equal(segment_matmul_fp8(view, *dev[1:], out_dtype=torch.float32), plain), offset
+    turned = dev[2].view(torch.uint8).transpose(1, 2).contiguous().transpose(1, 2).view(torch.float8_e4m3fn)
+    assert torch.equal(segment_matmul_fp8(dev[0], dev[1].t().contiguous().t(), turned, dev[3], dev[4].int(), torch.float32), plain)
+    bits = dev[0].view(torch.uint8).clone()
+    bits[70:200, 9] = 0x7f                                     # NaN in one segment
+    other = segment_matmul_fp8(bits.view(torch.float8_e4m3fn), *dev[1:], out_dtype=torch.float32)
+    assert torch.isnan(other[70:200]).all() and torch.equal(other[:70], plain[:70]) and torch.equal(other[200:], plain[200:])
+
+
+# ---- together ------------------------------------------------------------------------------------------------------------
+
+def _layer(ops_gnn, x, logits, bias, up, down, k):
+    """Rows through their experts: route, dispatch, two products, combine by a CSR product over (row, place) edges."""
+    from ops_gnn.torch_sparse_spmm import csr_spmm
+
+    weight, index = ops_gnn.topk_route(logits, k, "sigmoid", bias, groups=4, kept_groups=2)
+    indptr, perm, position = ops_gnn.route_csr(index, up.size(0))
+    hidden = torch.nn.functional.silu(ops_gnn.segment_matmul(x[perm // k], indptr, up))
+    y = ops_gnn.segment_matmul(hidden, indptr, down)
+    rows = torch.arange(0, position.numel() + 1, k, device=x.device)
+    return csr_spmm(rows, position.view(-1), weight.reshape(-1), y, "sum"), index
+
+
+@requires_gpu
+def test_layer_of_experts(cuda_device):
+    """The operators as a layer uses them, forward and backward, against a loop over rows and experts in float64."""
+    import ops_gnn
+
+    rows, width, hidden, experts, k = 150, 48, 40, 16, 3
+    gen = _gen(31)
+    x, logits = torch.randn(rows, width, generator=gen), torch.randn(rows, experts, generator=gen)
+    bias = torch.randn(experts, generator=gen) * 0.1
+    up = torch.randn(experts, width, hidden, generator=gen) / width ** 0.5
+    down = torch.randn(experts, hidden, width, generator=gen) / hidden ** 0.5
+    upstream = torch.randn(rows, width, generator=gen)
+    leaves = [t.to(cuda_device).requires_grad_() for t in (x, logits, up, down)]
+    out, index = _layer(ops_gnn, leaves[0], leaves[1], bias.to(cuda_device), leaves[2], leaves[3], k)
+    grads = torch.autograd.grad(out, leaves, upstream.to(cuda_device))
+
+    assert torch.equal(index.cpu(), _plain_choice(logits, k, "sigmoid", bias, 4, 2, 2))
+    plain = [t.double().requires_grad_() for t in (x, logits, up, down)]
+    weight = _plain_weight(plain[1], index.cpu(), "sigmoid", True, 1.0)
+    lines = []
+    for r in range(rows):
+        parts = [weight[r, j] * (torch.nn.functional.silu(plain[0][r] @ plain[2][e]) @ plain[3][e])
+                 for j, e in enumerate(index[r].tolist())]
+        lines.append(sum(parts))
+    want = torch.stack(lines)
+    want_grads = torch.autograd.grad(want, plain, upstream.double())
+    # Four stages of fp32 sums of at most 150 terms each, values of order 1: 4 * 150 steps of the largest magnitude
+    for got, exact in zip((out,) + grads, (want,) + want_grads):
+        bound = 600 * STEP * float(exact.detach().abs().max()) * 4
+        assert float((got.detach().cpu().double() - exact.detach()).abs().max()) <= bound
+
+
+@requires_gpu
+def test_layer_in_a_graph_and_on_another_stream(cuda_device):
+    """Captured once and replayed with other inputs (other pointers among them), and run on a side stream."""
+    import ops_gnn
+
+    rows, width, experts, k = 96, 64, 16, 2
+    gen = _gen(41)
+
+    def inputs(seed):
+        g = _gen(seed)
+        return [torch.randn(rows, width, generator=g).bfloat16().to(cuda_device),
+                torch.randn(rows, experts, generator=g).bfloat16().to(cuda_device)]
+
+    up = (torch.randn(experts, width, width, generator=gen) / 8).bfloat16().to(cuda_device)
+    quantised = ops_gnn.quantize_fp8(up.transpose(1, 2).contiguous(), 128)
+
+    def run(x, logits):
+        weight, index = ops_gnn.topk_route(logits, k)
+        indptr, perm, position = ops_gnn.route_csr(index, experts)
+        rows_of = x[perm // k]
+        y = ops_gnn.segment_matmul(rows_of, indptr, up)
+        z = ops_gnn.segment_matmul_fp8(*ops_gnn.quantize_fp8(rows_of), *quantised, indptr)
+        return weight, index, indptr, perm, position, y, z
+
+    static = inputs(1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_side = run(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    plain = run(*static)
+    assert all(torch.equal(a, b) for a, b in zip(plain, on_side))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run(*static)
+    for seed in (2, 3):
+        fresh = inputs(seed)
+        for buffer, value in zip(static, fresh):
+            buffer.copy_(value)
+        graph.replay()
+        want = run(*fresh)
+        assert all(torch.equal(a, b) for a, b in zip(captured, want)), seed
+    del graph
