@@ -33,6 +33,13 @@ inline int LaunchStatus()
     return OPSGNN_OK;
 }
 
+// How long a device-side wait may last and where it reports; read once per launch (csr_abi.cu).
+struct WaitSettings {
+    unsigned long long* sink;  // device-visible word that marks a wait that ran out, or null
+    uint32_t polls;            // polls of one wait before it gives up
+};
+int CurrentWaitSettings(WaitSettings* settings);
+
 inline cudaStream_t AsStream(void* stream) { return reinterpret_cast<cudaStream_t>(stream); }
 
 inline int SmCount()

@@ -393,6 +393,21 @@ extern "C" int opsgnn_csr_reduce_status(const void* workspace, void* stream, int
     return count == 0 ? OPSGNN_OK : OPSGNN_ERR_TIMEOUT;
 }
 
+namespace opsgnn {
+
+// The same for kernels outside the engine; 0 or a cudaError_t.
+int CurrentWaitSettings(WaitSettings* settings)
+{
+    int device = 0;
+    OPSGNN_CUDA_TRY(cudaGetDevice(&device));
+    settings->sink = (device >= 0 && device < kMaxDevices) ? g_status_sink[device].load(std::memory_order_relaxed) : nullptr;
+    const int64_t polls = g_wait_polls.load(std::memory_order_relaxed);
+    settings->polls = polls < 0 ? kBulkSpinLimit : static_cast<uint32_t>(polls > 0xffffffffLL ? 0xffffffffLL : polls);
+    return OPSGNN_OK;
+}
+
+}  // namespace opsgnn
+
 extern "C" int opsgnn_set_status_sink(void* sink)
 {
     int device = 0;

@@ -64,7 +64,8 @@ extern "C" int opsgnn_segment_matmul(const OpsgnnSegmentMatmulDesc* desc, const 
     p.b_n = desc->weight_out_stride;
     p.in_type = desc->in_type;
     p.out_type = desc->out_type;
-    return segmm::RunRowsSimple(p, AsStream(stream));
+    const int ran = segmm::RunRowsTensor(p, AsStream(stream));
+    return ran == OPSGNN_ERR_UNSUPPORTED ? segmm::RunRowsSimple(p, AsStream(stream)) : ran;
 }
 
 extern "C" int opsgnn_segment_matmul_weight_grad(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src,
@@ -90,7 +91,8 @@ extern "C" int opsgnn_segment_matmul_weight_grad(const OpsgnnSegmentMatmulDesc* 
     p.lda = desc->src_stride;
     p.ldb = grad_stride;
     p.type = desc->in_type;
-    return segmm::RunOuterSimple(p, AsStream(stream));
+    const int ran = segmm::RunOuterTensor(p, AsStream(stream));
+    return ran == OPSGNN_ERR_UNSUPPORTED ? segmm::RunOuterSimple(p, AsStream(stream)) : ran;
 }
 
 extern "C" int opsgnn_segment_matmul_fp8(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src, const float* src_scale,

@@ -35,6 +35,10 @@ struct OuterProblem {
 // Any type, size, stride and alignment (segment_matmul_simple.cu).
 int RunRowsSimple(const RowsProblem& p, cudaStream_t stream);
 int RunOuterSimple(const OuterProblem& p, cudaStream_t stream);
+// 16-bit types on the tensor cores (segment_matmul_tc.cu): widths and strides of whole 16-byte vectors, 16-byte aligned
+// bases.  OPSGNN_ERR_UNSUPPORTED, with nothing launched, for anything else.
+int RunRowsTensor(const RowsProblem& p, cudaStream_t stream);
+int RunOuterTensor(const OuterProblem& p, cudaStream_t stream);
 
 }  // namespace segmm
 }  // namespace opsgnn

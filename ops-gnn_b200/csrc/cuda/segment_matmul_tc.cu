@@ -1,0 +1,451 @@
+// Segment products of 16-bit types on the tensor cores (tcgen05.mma, operands by TMA, accumulators in TMEM).
+//
+// One persistent thread block per SM walks over output tiles of 128 x BN:
+//   warp 0      loads the tiles' operands, 64 values of the reduced index at a time, into a ring of shared-memory stages
+//   warp 1      issues the matrix instructions; accumulators alternate between two halves of TMEM
+//   warps 4-7   move a finished accumulator to memory (32 rows each) while the next tile is multiplied
+// Rows form (out and grad_src): tiles are row tiles of one segment times BN columns, found on the device (SegmentWalk).  A
+// tile's last rows may belong to the next segment: they are multiplied and not stored, rows do not mix.  The weight is read as
+// it lies: its reduced index along memory (K-major operand) or its columns (MN-major).
+// Outer form (grad_weight): the rows of a segment are the reduced index, both operands MN-major.  The last load of a segment
+// reaches into the next one; those rows are zeroed in shared memory, in both operands (0 * NaN is NaN).
+#include <algorithm>
+
+#include "segment_matmul.cuh"
+#include "tensor_core.cuh"
+
+namespace opsgnn {
+
+namespace tc {
+
+bool EncodeMap(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* sizes, const uint64_t* strides,
+               const uint32_t* box)
+{
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = []() -> Encode {
+        void* entry = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &entry, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess) {
+            (void)cudaGetLastError();
+            return nullptr;
+        }
+        return reinterpret_cast<Encode>(entry);
+    }();
+    if (encode == nullptr) {
+        return false;
+    }
+    const cuuint32_t ones[3] = {1, 1, 1};
+    return encode(map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), reinterpret_cast<const cuuint64_t*>(sizes),
+                  reinterpret_cast<const cuuint64_t*>(strides), box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace tc
+
+namespace segmm {
+namespace {
+
+constexpr int kRows = 128;     // rows of a tile
+constexpr int kDepth = 64;     // reduced index per stage: one 128-byte row of 16-bit values
+constexpr int kThreads = 256;
+constexpr int kSlab = kDepth * 128;          // bytes of 64 rows of 128 bytes
+constexpr int kStagingBytes = 4 * 32 * 128;  // per epilogue warp 32 rows of 64 values
+
+enum Form { kRowsWide, kRowsTurned, kOuter };  // weight's columns along memory; its reduced index along memory; grad_weight
+
+template <int BN> constexpr int Stages() { return BN == 256 ? 4 : 6; }
+template <int BN> constexpr int StageBytes() { return kRows * 128 + BN * 128; }
+template <int BN> constexpr int SharedBytes() { return 1024 + Stages<BN>() * StageBytes<BN>() + kStagingBytes + 256; }
+
+struct Params {
+    SegmentPointers ptr;
+    void* out;
+    int64_t m, n, k;   // rows form: n columns, k reduced; outer form: m x n results per segment
+    WaitSettings wait;
+};
+
+struct Barriers {
+    uint64_t full[6], empty[6], done[2], free[2], drain;
+    uint32_t tmem, stop;
+};
+
+template <class T> __device__ __forceinline__ uint32_t TwoOf(uint32_t a, uint32_t b)
+{
+    uint32_t word;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(__uint_as_float(a), __uint_as_float(b));
+        memcpy(&word, &p, 4);
+    } else {
+        const __half2 p = __floats2half2_rn(__uint_as_float(a), __uint_as_float(b));
+        memcpy(&word, &p, 4);
+    }
+    return word;
+}
+
+template <class T, int BN, int FORM>
+__global__ void __launch_bounds__(kThreads, 1)
+    TensorKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p)
+{
+    constexpr int kStages = Stages<BN>();
+    constexpr int kStage = StageBytes<BN>();
+    extern __shared__ unsigned char raw[];
+    unsigned char* smem = raw + ((1024 - (tc::Shared(raw) & 1023)) & 1023);
+    unsigned char* staging = smem + kStages * kStage;
+    Barriers& bar = *reinterpret_cast<Barriers*>(staging + kStagingBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            tc::BarInit(&bar.full[i], 1);
+            tc::BarInit(&bar.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::BarInit(&bar.done[i], 1);
+            tc::BarInit(&bar.free[i], 4);
+        }
+        tc::BarInit(&bar.drain, 1);
+        bar.stop = 0;
+        tc::BarInitFence();
+    }
+    if (warp == 2) {
+        tc::TmemAlloc(&bar.tmem);
+    }
+    tc::FenceBefore();
+    __syncthreads();
+    tc::FenceAfter();
+    const uint32_t tmem = bar.tmem;
+    const tc::Waiter wait{&bar.stop, p.wait};
+
+    const int64_t across = (p.n + BN - 1) / BN;
+    const int64_t down = FORM == kOuter ? (p.m + kRows - 1) / kRows : 0;
+    const int64_t outer_tiles = FORM == kOuter ? p.ptr.segments * down * across : 0;
+    SegmentWalk<kRows> walk;
+    if constexpr (FORM != kOuter) {
+        if (warp != 2 && warp != 3) {
+            walk.Start(p.ptr);
+        }
+    }
+    // Tile t: its segment, first result row and column, and the range of the reduced index.
+    int64_t segment = 0, row = 0, row_end = 0, column = 0, from = 0, depth = 0;
+    auto find = [&](int64_t t) {
+        column = t % across * BN;
+        if constexpr (FORM == kOuter) {
+            if (t >= outer_tiles) {
+                return false;
+            }
+            segment = t / (down * across);
+            row = t / across % down * kRows;
+            row_end = p.m;
+            int64_t end;
+            p.ptr.Range(segment, from, end);
+            depth = end - from;
+            return true;
+        } else {
+            if (!walk.Seek(t / across)) {
+                return false;
+            }
+            segment = walk.segment;
+            row = walk.row;
+            row_end = walk.row_end;
+            depth = p.k;
+            return true;
+        }
+    };
+
+    uint32_t filled = 0;  // stages the loading warp has asked for
+    if (warp == 0) {
+        bool going = true;
+        for (int64_t t = blockIdx.x; going && find(t); t += gridDim.x) {
+            for (int64_t k = 0; k < depth; k += kDepth, ++filled) {
+                const uint32_t s = filled % kStages;
+                going = wait.Warp(&bar.empty[s], ((filled / kStages) & 1) ^ 1);
+                if (!going) {
+                    break;
+                }
+                if (lane == 0) {
+                    const uint32_t a = tc::Shared(smem) + s * kStage, b = a + kRows * 128;
+                    tc::BarExpect(&bar.full[s], kStage);
+                    if constexpr (FORM == kOuter) {
+#pragma unroll
+                        for (int i = 0; i < kRows / 64; ++i) {
+                            tc::Load2(map_a, &bar.full[s], a + i * kSlab, static_cast<int>(row) + i * 64, static_cast<int>(from + k));
+                        }
+#pragma unroll
+                        for (int i = 0; i < BN / 64; ++i) {
+                            tc::Load2(map_b, &bar.full[s], b + i * kSlab, static_cast<int>(column) + i * 64, static_cast<int>(from + k));
+                        }
+                    } else {
+                        tc::Load2(map_a, &bar.full[s], a, static_cast<int>(k), static_cast<int>(row));
+                        if constexpr (FORM == kRowsTurned) {
+                            tc::Load3(map_b, &bar.full[s], b, static_cast<int>(k), static_cast<int>(column), static_cast<int>(segment));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < BN / 64; ++i) {
+                                tc::Load3(map_b, &bar.full[s], b + i * kSlab, static_cast<int>(column) + i * 64, static_cast<int>(k),
+                                          static_cast<int>(segment));
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == 1) {
+        constexpr uint32_t shape = tc::Shape(kRows, BN, std::is_same<T, __nv_bfloat16>::value ? 1 : 0, FORM == kOuter, FORM != kRowsTurned);
+        uint32_t used = 0, tiles = 0;
+        bool going = true;
+        for (int64_t t = blockIdx.x; going && find(t); t += gridDim.x) {
+            if (depth == 0) {
+                continue;
+            }
+            const uint32_t half = tiles & 1;
+            going = wait.Warp(&bar.free[half], ((tiles >> 1) & 1) ^ 1);
+            tc::FenceAfter();
+            for (int64_t k = 0; going && k < depth; k += kDepth, ++used) {
+                const uint32_t s = used % kStages;
+                going = wait.Warp(&bar.full[s], (used / kStages) & 1);
+                if (!going) {
+                    break;
+                }
+                unsigned char* stage = smem + s * kStage;
+                if constexpr (FORM == kOuter) {
+                    if (depth - k < kDepth) {
+                        // Rows of the next segment: zero them in every slab of both operands.
+                        const int first = static_cast<int>(depth - k);
+                        for (int i = first * 8 + lane; i < kDepth * 8; i += 32) {
+#pragma unroll
+                            for (int slab = 0; slab < kStage / kSlab; ++slab) {
+                                *reinterpret_cast<uint4*>(stage + slab * kSlab + i * 16) = make_uint4(0, 0, 0, 0);
+                            }
+                        }
+                        tc::FenceAsync();
+                        __syncwarp();
+                    }
+                }
+                tc::FenceAfter();
+                if (lane == 0) {
+                    const uint32_t a = tc::Shared(stage), b = a + kRows * 128;
+                    uint64_t da = tc::Operand(a, FORM == kOuter ? kSlab : 16, 1024);
+                    uint64_t db = tc::Operand(b, FORM == kRowsTurned ? 16 : kSlab, 1024);
+#pragma unroll
+                    for (int i = 0; i < kDepth / 16; ++i) {
+                        tc::MmaF16(tmem + half * BN, da, db, shape, k > 0 || i > 0);
+                        da += FORM == kOuter ? 2048 >> 4 : 32 >> 4;
+                        db += FORM == kRowsTurned ? 32 >> 4 : 2048 >> 4;
+                    }
+                    tc::Commit(&bar.empty[s]);
+                }
+                __syncwarp();
+            }
+            if (going) {
+                if (lane == 0) {
+                    tc::Commit(&bar.done[half]);
+                }
+                __syncwarp();
+                ++tiles;
+            }
+        }
+        if (!going) {  // let what was issued end before TMEM is freed
+            if (lane == 0) {
+                tc::Commit(&bar.drain);
+                for (uint32_t i = 0; i < (1u << 15) && !tc::BarTry(&bar.drain, 0); ++i) {
+                }
+            }
+            __syncwarp();
+        }
+    } else if (warp >= 4) {
+        const int quarter = warp - 4;
+        unsigned char* mine = staging + quarter * (32 * 128);
+        T* out = static_cast<T*>(p.out);
+        uint32_t tiles = 0;
+        bool going = true;
+        for (int64_t t = blockIdx.x; going && find(t); t += gridDim.x) {
+            const uint32_t half = tiles & 1;
+            if (depth > 0) {
+                going = wait.Warp(&bar.done[half], (tiles >> 1) & 1);
+                if (!going) {
+                    break;
+                }
+                tc::FenceAfter();
+            }
+            T* to = out + (FORM == kOuter ? segment * p.m * p.n : 0);
+            const int64_t first = row + quarter * 32;
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 64) {
+                if (column + c >= p.n) {
+                    break;
+                }
+                uint32_t words[32];
+                if (depth > 0) {
+                    uint32_t low[32], high[32];
+                    const uint32_t at = tmem + half * BN + c + (static_cast<uint32_t>(quarter * 32) << 16);
+                    tc::TmemLoad32(at, low);
+                    tc::TmemLoad32(at + 32, high);
+                    tc::TmemWait();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        words[i] = TwoOf<T>(low[2 * i], low[2 * i + 1]);
+                        words[16 + i] = TwoOf<T>(high[2 * i], high[2 * i + 1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        words[i] = 0;
+                    }
+                }
+                // Through shared memory, so that 8 lanes write 128 consecutive bytes of a row; the 16-byte pieces of a row
+                // are permuted by its number against bank conflicts.
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    *reinterpret_cast<uint4*>(mine + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+                        make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
+                }
+                __syncwarp();
+                const int piece = lane & 7;
+                const int64_t col = column + c + piece * 8;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int r = i * 4 + (lane >> 3);
+                    const uint4 value = *reinterpret_cast<const uint4*>(mine + r * 128 + ((piece ^ (r & 7)) << 4));
+                    if (first + r < row_end && col < p.n) {
+                        *reinterpret_cast<uint4*>(to + (first + r) * p.n + col) = value;
+                    }
+                }
+                __syncwarp();
+            }
+            if (depth > 0) {
+                tc::FenceBefore();
+                __syncwarp();
+                if (lane == 0) {
+                    tc::BarArrive(&bar.free[half]);
+                }
+                ++tiles;
+            }
+        }
+        if constexpr (FORM != kOuter) {
+            // Rows of no segment.
+            const int64_t before = p.ptr.Raw(0), behind = p.ptr.Raw(p.ptr.segments);
+            const int64_t pieces = p.n / 8;
+            for (int64_t r = blockIdx.x * 4 + quarter; r < before + (p.ptr.rows - behind); r += gridDim.x * 4) {
+                const int64_t at = r < before ? r : behind + (r - before);
+                for (int64_t c = lane; c < pieces; c += 32) {
+                    *reinterpret_cast<uint4*>(out + at * p.n + c * 8) = make_uint4(0, 0, 0, 0);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    if (warp == 0 && lane == 0 && bar.stop != 0) {
+        // Copies in flight must land before the block's shared memory is given up.
+        for (uint32_t f = filled > kStages ? filled - kStages : 0; f < filled; ++f) {
+            for (uint32_t i = 0; i < (1u << 15) && !tc::BarTry(&bar.full[f % kStages], (f / kStages) & 1); ++i) {
+            }
+        }
+    }
+    tc::FenceBefore();
+    __syncthreads();
+    if (warp == 2) {
+        tc::FenceAfter();
+        tc::TmemFree(tmem);
+    }
+}
+
+// What TMA asks of an operand: 16-byte aligned base and strides, extents that fit its fields.
+bool Loadable(const void* base, int64_t stride, int64_t limit)
+{
+    return Aligned(base, 16) && stride % 8 == 0 && stride < (INT64_C(1) << 38) && limit < (INT64_C(1) << 31) - 512;
+}
+
+CUtensorMapDataType TypeOf(int type) { return type == OPSGNN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16; }
+
+bool Map2(CUtensorMap* map, int type, const void* base, int64_t inner, int64_t rows, int64_t stride, int box_inner, int box_rows)
+{
+    const uint64_t sizes[2] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(rows)};
+    const uint64_t strides[1] = {static_cast<uint64_t>(stride) * 2};
+    const uint32_t box[2] = {static_cast<uint32_t>(box_inner), static_cast<uint32_t>(box_rows)};
+    return tc::EncodeMap(map, TypeOf(type), 2, base, sizes, strides, box);
+}
+
+template <class T, int BN, int FORM>
+int Launch(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int64_t tiles, cudaStream_t stream)
+{
+    OPSGNN_CUDA_TRY(cudaFuncSetAttribute(TensorKernel<T, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, SharedBytes<BN>()));
+    const int grid = static_cast<int>(std::min<int64_t>(std::max<int64_t>(tiles, 1), SmCount()));
+    TensorKernel<T, BN, FORM><<<grid, kThreads, SharedBytes<BN>(), stream>>>(a, b, p);
+    return LaunchStatus();
+}
+
+template <int FORM, class F> int ByType(int type, bool narrow, F&& f)
+{
+    using std::integral_constant;
+    if (type == OPSGNN_BF16) {
+        return narrow ? f(__nv_bfloat16(), integral_constant<int, 128>()) : f(__nv_bfloat16(), integral_constant<int, 256>());
+    }
+    return narrow ? f(__half(), integral_constant<int, 128>()) : f(__half(), integral_constant<int, 256>());
+}
+
+}  // namespace
+
+int RunRowsTensor(const RowsProblem& p, cudaStream_t stream)
+{
+    const bool turned = p.b_k == 1 && p.b_n != 1;
+    const int64_t inner = turned ? p.k : p.n, other = turned ? p.n : p.k, stride = turned ? p.b_n : p.b_k;
+    if ((p.in_type != OPSGNN_BF16 && p.in_type != OPSGNN_F16) || p.out_type != p.in_type || p.k < 1 || p.ptr.data == nullptr ||
+        p.ptr.segments < 1 || p.n % 8 != 0 || p.ldo != p.n || (!turned && p.b_n != 1) || !Aligned(p.out, 16) || stride < inner ||
+        p.b_segment % 8 != 0 || p.b_segment >= (INT64_C(1) << 38) || p.b_segment < 1 || p.ptr.segments >= (INT64_C(1) << 31) ||
+        !Loadable(p.a, p.lda, std::max(p.k, p.ptr.rows)) || !Loadable(p.b, stride, std::max(inner, other))) {
+        return OPSGNN_ERR_UNSUPPORTED;
+    }
+    Params q{};
+    q.ptr = p.ptr;
+    q.out = p.out;
+    q.n = p.n;
+    q.k = p.k;
+    OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
+    const bool narrow = p.n <= 128;
+    CUtensorMap a, b;
+    const uint64_t sizes[3] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(other), static_cast<uint64_t>(p.ptr.segments)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(stride) * 2, static_cast<uint64_t>(p.b_segment) * 2};
+    const uint32_t box[3] = {64, turned ? (narrow ? 128u : 256u) : static_cast<uint32_t>(kDepth), 1};
+    if (!Map2(&a, p.in_type, p.a, p.k, p.ptr.rows, p.lda, kDepth, kRows) ||
+        !tc::EncodeMap(&b, TypeOf(p.in_type), 3, p.b, sizes, strides, box)) {
+        return OPSGNN_ERR_UNSUPPORTED;
+    }
+    auto run = [&](auto tag, auto width) {
+        using T = decltype(tag);
+        constexpr int BN = decltype(width)::value;
+        const int64_t tiles = (p.ptr.rows / kRows + p.ptr.segments) * CeilDiv(p.n, BN);
+        return turned ? Launch<T, BN, kRowsTurned>(a, b, q, tiles, stream) : Launch<T, BN, kRowsWide>(a, b, q, tiles, stream);
+    };
+    return ByType<0>(p.in_type, narrow, run);
+}
+
+int RunOuterTensor(const OuterProblem& p, cudaStream_t stream)
+{
+    if ((p.type != OPSGNN_BF16 && p.type != OPSGNN_F16) || p.ptr.rows < 1 || p.n % 8 != 0 || !Aligned(p.out, 16) ||
+        !Loadable(p.a, p.lda, std::max(p.k, p.ptr.rows)) || !Loadable(p.b, p.ldb, std::max(p.n, p.ptr.rows))) {
+        return OPSGNN_ERR_UNSUPPORTED;
+    }
+    Params q{};
+    q.ptr = p.ptr;
+    q.out = p.out;
+    q.m = p.k;
+    q.n = p.n;
+    OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
+    CUtensorMap a, b;
+    if (!Map2(&a, p.type, p.a, p.k, p.ptr.rows, p.lda, 64, kDepth) || !Map2(&b, p.type, p.b, p.n, p.ptr.rows, p.ldb, 64, kDepth)) {
+        return OPSGNN_ERR_UNSUPPORTED;
+    }
+    auto run = [&](auto tag, auto width) {
+        using T = decltype(tag);
+        constexpr int BN = decltype(width)::value;
+        return Launch<T, BN, kOuter>(a, b, q, p.ptr.segments * CeilDiv(p.k, kRows) * CeilDiv(p.n, BN), stream);
+    };
+    return ByType<0>(p.type, p.n <= 128, run);
+}
+
+}  // namespace segmm
+}  // namespace opsgnn

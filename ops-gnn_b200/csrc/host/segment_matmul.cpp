@@ -73,6 +73,7 @@ at::Tensor segment_matmul_forward(const at::Tensor& src, const at::Tensor& indpt
                 api, ": src must be [rows, width] and weight [segments, width, out] of one dtype on one GPU");
     CheckPointers(indptr, src, weight.size(0), api);
     c10::cuda::CUDAGuard guard(src.device());
+    RaiseIfDeviceStalled(src, api);
     const at::Tensor rows = RowMajor(src), matrices = Matrices(weight);
     at::Tensor out = at::empty({src.size(0), weight.size(2)}, src.options());
     OpsgnnSegmentMatmulDesc desc = DescOf(rows, indptr, weight.size(0), weight.size(2), src.scalar_type(), api);
@@ -93,6 +94,7 @@ at::Tensor segment_matmul_weight_grad(const at::Tensor& src, const at::Tensor& i
     const int64_t segments = indptr.numel() - 1;
     CheckPointers(indptr, src, segments, api);
     c10::cuda::CUDAGuard guard(src.device());
+    RaiseIfDeviceStalled(src, api);
     const at::Tensor rows = RowMajor(src), upstream = RowMajor(grad);
     at::Tensor out = at::empty({segments, src.size(1), grad.size(1)}, src.options());
     const OpsgnnSegmentMatmulDesc desc = DescOf(rows, indptr, segments, grad.size(1), src.scalar_type(), api);
@@ -124,6 +126,7 @@ at::Tensor segment_matmul_fp8(const at::Tensor& src, const at::Tensor& src_scale
         TORCH_CHECK(segments == 1, api, ": without indptr there is one weight");
     }
     c10::cuda::CUDAGuard guard(src.device());
+    RaiseIfDeviceStalled(src, api);
     const at::Tensor rows = RowMajor(src), matrices = weight.contiguous();
     const at::Tensor row_scale = src_scale.contiguous(), tile_scale = weight_scale.contiguous();
     at::Tensor out = at::empty({src.size(0), weight.size(1)}, src.options().dtype(out_type));
