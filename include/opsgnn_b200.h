@@ -466,13 +466,17 @@ typedef struct OpsgnnSegmentMatmulDesc {
     int32_t out_type;              /* = in_type; fp8: F32 / F16 / BF16                      */
 } OpsgnnSegmentMatmulDesc;
 
+/* Bytes of scratch (16-byte aligned) of opsgnn_segment_matmul (weight_grad 0) or opsgnn_segment_matmul_weight_grad (1); 0 for
+ * 16-bit types. */
+OPSGNN_API int opsgnn_segment_matmul_workspace_bytes(const OpsgnnSegmentMatmulDesc* desc, int weight_grad, int64_t* bytes);
 /* out[r, :] = src[r, :] @ weight[e] for the rows of segment e; 0 in rows of no segment.  out is contiguous. */
 OPSGNN_API int opsgnn_segment_matmul(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src, const void* weight,
-                                     void* out, void* stream);
+                                     void* out, void* workspace, int64_t workspace_bytes, void* stream);
 /* grad_weight[e] = src[rows of e]^T @ grad[rows of e], contiguous [segments, width, out]; the weight strides of desc are not
  * used.  grad_stride: elements between rows of grad. */
 OPSGNN_API int opsgnn_segment_matmul_weight_grad(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src,
-                                                 const void* grad, int64_t grad_stride, void* grad_weight, void* stream);
+                                                 const void* grad, int64_t grad_stride, void* grad_weight, void* workspace,
+                                                 int64_t workspace_bytes, void* stream);
 /* The same product on float8_e4m3 values: src[rows, width] with src_scale[rows, ceil(width / 128)], weight[e, out, width]
  * (its strides in desc as above) with weight_scale[e, ceil(out / 128), ceil(width / 128)], all scales contiguous fp32.
  * indptr NULL (with segments = 1): one dense product. */

@@ -21,6 +21,14 @@ int CheckDesc(const OpsgnnSegmentMatmulDesc* d, bool eight_bits)
     return OPSGNN_OK;
 }
 
+// fp32 products that go through bf16 terms on the tensor cores, as far as sizes and strides say (a base address off 16 bytes
+// sends the call to the simple kernel all the same).
+bool Splits(const OpsgnnSegmentMatmulDesc& d)
+{
+    return d.in_type == OPSGNN_F32 && d.rows > 0 && d.segments > 0 && d.width > 0 && d.width % 8 == 0 && d.out > 0 && d.out % 8 == 0 &&
+           d.src_stride % 4 == 0;
+}
+
 SegmentPointers Pointers(const OpsgnnSegmentMatmulDesc& d, const void* indptr)
 {
     SegmentPointers p;
@@ -37,10 +45,28 @@ SegmentPointers Pointers(const OpsgnnSegmentMatmulDesc& d, const void* indptr)
 
 using namespace opsgnn;
 
-extern "C" int opsgnn_segment_matmul(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src, const void* weight,
-                                     void* out, void* stream)
+extern "C" int opsgnn_segment_matmul_workspace_bytes(const OpsgnnSegmentMatmulDesc* desc, int weight_grad, int64_t* bytes)
 {
     const int status = segmm::CheckDesc(desc, false);
+    if (status != OPSGNN_OK) {
+        return status;
+    }
+    if (bytes == nullptr) {
+        return OPSGNN_ERR_INVALID;
+    }
+    *bytes = 0;
+    if (segmm::Splits(*desc)) {
+        *bytes = weight_grad ? segmm::OuterSplitBytes(desc->rows, desc->width, desc->out)
+                             : segmm::RowsSplitBytes(desc->rows, desc->segments, desc->width, desc->out);
+    }
+    return OPSGNN_OK;
+}
+
+extern "C" int opsgnn_segment_matmul(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src, const void* weight,
+                                     void* out, void* workspace, int64_t workspace_bytes, void* stream)
+{
+    int64_t need = 0;
+    const int status = opsgnn_segment_matmul_workspace_bytes(desc, 0, &need);
     if (status != OPSGNN_OK) {
         return status;
     }
@@ -64,14 +90,19 @@ extern "C" int opsgnn_segment_matmul(const OpsgnnSegmentMatmulDesc* desc, const 
     p.b_n = desc->weight_out_stride;
     p.in_type = desc->in_type;
     p.out_type = desc->out_type;
-    const int ran = segmm::RunRowsTensor(p, AsStream(stream));
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !Aligned(workspace, 16))) {
+        return OPSGNN_ERR_WORKSPACE;
+    }
+    const int ran = need > 0 ? segmm::RunRowsSplit(p, workspace, AsStream(stream)) : segmm::RunRowsTensor(p, AsStream(stream));
     return ran == OPSGNN_ERR_UNSUPPORTED ? segmm::RunRowsSimple(p, AsStream(stream)) : ran;
 }
 
 extern "C" int opsgnn_segment_matmul_weight_grad(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src,
-                                                 const void* grad, int64_t grad_stride, void* grad_weight, void* stream)
+                                                 const void* grad, int64_t grad_stride, void* grad_weight, void* workspace,
+                                                 int64_t workspace_bytes, void* stream)
 {
-    const int status = segmm::CheckDesc(desc, false);
+    int64_t need = 0;
+    const int status = opsgnn_segment_matmul_workspace_bytes(desc, 1, &need);
     if (status != OPSGNN_OK) {
         return status;
     }
@@ -91,7 +122,10 @@ extern "C" int opsgnn_segment_matmul_weight_grad(const OpsgnnSegmentMatmulDesc* 
     p.lda = desc->src_stride;
     p.ldb = grad_stride;
     p.type = desc->in_type;
-    const int ran = segmm::RunOuterTensor(p, AsStream(stream));
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !Aligned(workspace, 16))) {
+        return OPSGNN_ERR_WORKSPACE;
+    }
+    const int ran = need > 0 ? segmm::RunOuterSplit(p, workspace, AsStream(stream)) : segmm::RunOuterTensor(p, AsStream(stream));
     return ran == OPSGNN_ERR_UNSUPPORTED ? segmm::RunOuterSimple(p, AsStream(stream)) : ran;
 }
 
@@ -125,5 +159,6 @@ extern "C" int opsgnn_segment_matmul_fp8(const OpsgnnSegmentMatmulDesc* desc, co
     p.b_n = desc->weight_out_stride;
     p.in_type = desc->in_type;
     p.out_type = desc->out_type;
-    return segmm::RunRowsSimple(p, AsStream(stream));
+    const int ran = segmm::RunRowsFp8(p, AsStream(stream));
+    return ran == OPSGNN_ERR_UNSUPPORTED ? segmm::RunRowsSimple(p, AsStream(stream)) : ran;
 }

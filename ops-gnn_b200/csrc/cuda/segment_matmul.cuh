@@ -39,6 +39,12 @@ int RunOuterSimple(const OuterProblem& p, cudaStream_t stream);
 // bases.  OPSGNN_ERR_UNSUPPORTED, with nothing launched, for anything else.
 int RunRowsTensor(const RowsProblem& p, cudaStream_t stream);
 int RunOuterTensor(const OuterProblem& p, cudaStream_t stream);
+// 8-bit and fp32 operands on the tensor cores (segment_matmul_promoted.cu), under the same conditions; fp32 needs a workspace.
+int RunRowsFp8(const RowsProblem& p, cudaStream_t stream);
+int RunRowsSplit(const RowsProblem& p, void* workspace, cudaStream_t stream);
+int RunOuterSplit(const OuterProblem& p, void* workspace, cudaStream_t stream);
+int64_t RowsSplitBytes(int64_t rows, int64_t segments, int64_t k, int64_t n);
+int64_t OuterSplitBytes(int64_t rows, int64_t k, int64_t n);
 
 }  // namespace segmm
 }  // namespace opsgnn

@@ -1,0 +1,617 @@
+// Segment products whose tensor-core sums are short and are added up in fp32 registers: block-scaled 8-bit values, and fp32.
+//
+// 8 bits: a sum over 128 values of the reduced index (one block, one scale per row and one per weight tile) is formed by
+// tcgen05.mma in TMEM; the epilogue warps multiply it by the two scales and add it to registers while the next block is
+// multiplied into the other half of TMEM.
+//
+// fp32: every operand value is x = x1 + x2 + x3 with bf16 terms (8 significant bits each, so the three hold all 24), and
+//     a b = a1 b1 + (a1 b2 + a2 b1) + (a1 b3 + a2 b2 + a3 b1) + terms below 2^-24 of |a b|, which are left out.
+// The six products are exact; 64 values of the reduced index are summed in TMEM, smallest terms first, so that only the last
+// four instructions add at full magnitude, then the sum moves to registers, which round to nearest.  Six bf16 products cost
+// 1/6 of the bf16 rate, four times what fp32 multiply-adds reach.  An infinity or NaN among the operands breaks the split
+// (inf - inf): a result that is not finite is computed again from the fp32 operands, one multiply-add at a time.  Values below
+// 2^-110 lose low bits, as their third term lies below the smallest bf16.
+//
+// Layout as in segment_matmul_tc.cu (one persistent block per SM: a loading warp, a multiplying warp), with eight epilogue
+// warps, each 32 rows x half the columns of a tile, whose sums need BN / 2 registers a thread: the first four warps hand
+// registers over.
+#include <algorithm>
+
+#include "segment_matmul.cuh"
+#include "tensor_core.cuh"
+
+namespace opsgnn {
+namespace segmm {
+namespace {
+
+constexpr int kRows = 128;
+constexpr int kThreads = 384;
+constexpr int kStages = 4;
+constexpr int kSlab = 64 * 128;
+constexpr int kStagingBytes = 8 * 32 * 128;
+// 384 threads are launched with 168 registers each; 128 * 72 + 256 * 216 = 384 * 168.
+constexpr int kRegsIssue = 72, kRegsSum = 216;
+
+enum Form { kRowsWide, kRowsTurned, kOuter };
+
+template <int BN> constexpr int StageBytes() { return kRows * 128 + BN * 128; }
+template <int BN> constexpr int SharedBytes() { return 1024 + kStages * StageBytes<BN>() + kStagingBytes + 256; }
+
+struct Params {
+    SegmentPointers ptr;
+    void* out;
+    const float* a_scale;
+    const float* b_scale;
+    int64_t m, n, k;                 // rows form: n columns, k reduced; outer form: m x n results per segment
+    const float* a;                  // fp32: the operands as given, for results that are not finite
+    const float* b;
+    int64_t lda, ldb;                // outer form: ldb = row stride of b
+    int64_t b_segment, b_k, b_n;
+    WaitSettings wait;
+};
+
+struct Barriers {
+    uint64_t full[kStages], empty[kStages], done[2], free[2], drain;
+    uint32_t tmem, stop;
+};
+
+// The six products of the fp32 split, smallest first: planes of a and b.
+__device__ __forceinline__ int PlaneA(int term) { return term == 0 ? 2 : (term == 1 || term == 3 ? 1 : 0); }
+__device__ __forceinline__ int PlaneB(int term) { return term == 2 ? 2 : (term == 1 || term == 4 ? 1 : 0); }
+
+template <class O> __device__ __forceinline__ uint32_t Word(const float* v)  // one 32-bit word of results
+{
+    uint32_t word;
+    if constexpr (std::is_same<O, float>::value) {
+        word = __float_as_uint(v[0]);
+    } else if constexpr (std::is_same<O, __nv_bfloat16>::value) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(v[0], v[1]);
+        memcpy(&word, &p, 4);
+    } else {
+        const __half2 p = __floats2half2_rn(v[0], v[1]);
+        memcpy(&word, &p, 4);
+    }
+    return word;
+}
+
+// sum[i] += scale * part[i], two at a time.
+template <int N> __device__ __forceinline__ void Add(float (&sum)[N], int at, const uint32_t (&part)[32], float scale)
+{
+    const float2 s = make_float2(scale, scale);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        const float2 r = __ffma2_rn(s, make_float2(__uint_as_float(part[i]), __uint_as_float(part[i + 1])),
+                                    make_float2(sum[at + i], sum[at + i + 1]));
+        sum[at + i] = r.x;
+        sum[at + i + 1] = r.y;
+    }
+}
+
+template <bool F8, class O, int BN, int FORM>
+__global__ void __launch_bounds__(kThreads, 1)
+    PromotedKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p)
+{
+    constexpr int kStage = StageBytes<BN>();
+    constexpr int kTerms = F8 ? 1 : 6;
+    constexpr int kDepth = F8 ? 128 : 64;  // values of the reduced index in one 128-byte row
+    extern __shared__ unsigned char raw[];
+    unsigned char* smem = raw + ((1024 - (tc::Shared(raw) & 1023)) & 1023);
+    unsigned char* staging = smem + kStages * kStage;
+    Barriers& bar = *reinterpret_cast<Barriers*>(staging + kStagingBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            tc::BarInit(&bar.full[i], 1);
+            tc::BarInit(&bar.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::BarInit(&bar.done[i], 1);
+            tc::BarInit(&bar.free[i], 8);
+        }
+        tc::BarInit(&bar.drain, 1);
+        bar.stop = 0;
+        tc::BarInitFence();
+    }
+    if (warp == 2) {
+        tc::TmemAlloc(&bar.tmem);
+    }
+    tc::FenceBefore();
+    __syncthreads();
+    tc::FenceAfter();
+    const uint32_t tmem = bar.tmem;
+    const tc::Waiter wait{&bar.stop, p.wait};
+
+    const int64_t across = (p.n + BN - 1) / BN;
+    const int64_t down = FORM == kOuter ? (p.m + kRows - 1) / kRows : 0;
+    const int64_t outer_tiles = FORM == kOuter ? p.ptr.segments * down * across : 0;
+    SegmentWalk<kRows> walk;
+    if constexpr (FORM != kOuter) {
+        if (warp != 2 && warp != 3) {
+            walk.Start(p.ptr);
+        }
+    }
+    int64_t segment = 0, row = 0, row_end = 0, column = 0, from = 0, depth = 0;
+    auto find = [&](int64_t t) {
+        column = t % across * BN;
+        if constexpr (FORM == kOuter) {
+            if (t >= outer_tiles) {
+                return false;
+            }
+            segment = t / (down * across);
+            row = t / across % down * kRows;
+            row_end = p.m;
+            int64_t end;
+            p.ptr.Range(segment, from, end);
+            depth = end - from;
+            return true;
+        } else {
+            if (!walk.Seek(t / across)) {
+                return false;
+            }
+            segment = walk.segment;
+            row = walk.row;
+            row_end = walk.row_end;
+            depth = p.k;
+            return true;
+        }
+    };
+
+    uint32_t filled = 0;
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+        if (warp == 0) {
+            bool going = true;
+            for (int64_t t = blockIdx.x; going && find(t); t += gridDim.x) {
+                for (int64_t k = 0; going && k < depth; k += kDepth) {
+#pragma unroll 1
+                    for (int term = 0; term < kTerms; ++term, ++filled) {
+                        const uint32_t s = filled % kStages;
+                        going = wait.Warp(&bar.empty[s], ((filled / kStages) & 1) ^ 1);
+                        if (!going) {
+                            break;
+                        }
+                        if (lane == 0) {
+                            const int pa = F8 ? 0 : PlaneA(term), pb = F8 ? 0 : PlaneB(term);
+                            const uint32_t a = tc::Shared(smem) + s * kStage, b = a + kRows * 128;
+                            tc::BarExpect(&bar.full[s], kStage);
+                            if constexpr (FORM == kOuter) {
+                                const int r = static_cast<int>(from + k);
+#pragma unroll
+                                for (int i = 0; i < kRows / 64; ++i) {
+                                    tc::Load3(map_a, &bar.full[s], a + i * kSlab, static_cast<int>(row) + i * 64, r, pa);
+                                }
+#pragma unroll
+                                for (int i = 0; i < BN / 64; ++i) {
+                                    tc::Load3(map_b, &bar.full[s], b + i * kSlab, static_cast<int>(column) + i * 64, r, pb);
+                                }
+                            } else {
+                                const int matrix = static_cast<int>(pb * p.ptr.segments + segment);
+                                tc::Load3(map_a, &bar.full[s], a, static_cast<int>(k), static_cast<int>(row), pa);
+                                if constexpr (FORM == kRowsTurned) {
+                                    tc::Load3(map_b, &bar.full[s], b, static_cast<int>(k), static_cast<int>(column), matrix);
+                                } else {
+#pragma unroll
+                                    for (int i = 0; i < BN / 64; ++i) {
+                                        tc::Load3(map_b, &bar.full[s], b + i * kSlab, static_cast<int>(column) + i * 64,
+                                                  static_cast<int>(k), matrix);
+                                    }
+                                }
+                            }
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+        } else if (warp == 1) {
+            constexpr uint32_t shape = tc::Shape(kRows, BN, F8 ? 0 : 1, FORM == kOuter, FORM != kRowsTurned);
+            uint32_t used = 0, blocks = 0;
+            bool going = true;
+            for (int64_t t = blockIdx.x; going && find(t); t += gridDim.x) {
+                for (int64_t k = 0; going && k < depth; k += kDepth, ++blocks) {
+                    const uint32_t half = blocks & 1;
+                    going = wait.Warp(&bar.free[half], ((blocks >> 1) & 1) ^ 1);
+                    tc::FenceAfter();
+#pragma unroll 1
+                    for (int term = 0; going && term < kTerms; ++term, ++used) {
+                        const uint32_t s = used % kStages;
+                        going = wait.Warp(&bar.full[s], (used / kStages) & 1);
+                        if (!going) {
+                            break;
+                        }
+                        unsigned char* stage = smem + s * kStage;
+                        if constexpr (FORM == kOuter) {
+                            if (depth - k < kDepth) {  // rows of the next segment
+                                const int first = static_cast<int>(depth - k);
+                                for (int i = first * 8 + lane; i < kDepth * 8; i += 32) {
+#pragma unroll
+                                    for (int slab = 0; slab < kStage / kSlab; ++slab) {
+                                        *reinterpret_cast<uint4*>(stage + slab * kSlab + i * 16) = make_uint4(0, 0, 0, 0);
+                                    }
+                                }
+                                tc::FenceAsync();
+                                __syncwarp();
+                            }
+                        }
+                        tc::FenceAfter();
+                        if (lane == 0) {
+                            const uint32_t a = tc::Shared(stage), b = a + kRows * 128;
+                            uint64_t da = tc::Operand(a, FORM == kOuter ? kSlab : 16, 1024);
+                            uint64_t db = tc::Operand(b, FORM == kRowsTurned ? 16 : kSlab, 1024);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if constexpr (F8) {
+                                    tc::MmaF8(tmem + half * BN, da, db, shape, i > 0);
+                                } else {
+                                    tc::MmaF16(tmem + half * BN, da, db, shape, term > 0 || i > 0);
+                                }
+                                da += FORM == kOuter ? 2048 >> 4 : 32 >> 4;
+                                db += FORM == kRowsTurned ? 32 >> 4 : 2048 >> 4;
+                            }
+                            tc::Commit(&bar.empty[s]);
+                        }
+                        __syncwarp();
+                    }
+                    if (!going) {
+                        break;
+                    }
+                    if (lane == 0) {
+                        tc::Commit(&bar.done[half]);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (!going) {  // let what was issued end before TMEM is freed
+                if (lane == 0) {
+                    tc::Commit(&bar.drain);
+                    for (uint32_t i = 0; i < (1u << 15) && !tc::BarTry(&bar.drain, 0); ++i) {
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSum));
+        constexpr int kMine = BN / 2;  // columns of this warp
+        const int quarter = warp & 3, side = (warp - 4) >> 2;
+        unsigned char* mine = staging + (warp - 4) * (32 * 128);
+        O* out = static_cast<O*>(p.out);
+        const int64_t scale_blocks = F8 ? (p.k + 127) / 128 : 0, scale_bands = F8 ? (p.n + 127) / 128 : 0;
+        uint32_t blocks = 0;
+        bool going = true;
+        for (int64_t t = blockIdx.x; going && find(t); t += gridDim.x) {
+            float sum[kMine];
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                sum[i] = 0.0f;
+            }
+            const int64_t col0 = column + side * kMine;
+            const bool some = col0 < p.n;
+            const int64_t r0 = row + quarter * 32;
+            const float* sa = nullptr;
+            const float* sb = nullptr;
+            float scale = 1.0f;
+            if constexpr (F8) {
+                sa = p.a_scale + (r0 + lane < row_end ? r0 + lane : row) * scale_blocks;
+                sb = p.b_scale + (segment * scale_bands + (some ? col0 / 128 : 0)) * scale_blocks;
+            }
+            for (int64_t k = 0, kb = 0; k < depth; k += kDepth, ++kb, ++blocks) {
+                const uint32_t half = blocks & 1;
+                if constexpr (F8) {
+                    scale = __ldg(sa + kb) * __ldg(sb + kb);
+                }
+                going = wait.Warp(&bar.done[half], (blocks >> 1) & 1);
+                if (!going) {
+                    break;
+                }
+                tc::FenceAfter();
+                if (some) {
+                    const uint32_t at = tmem + half * BN + side * kMine + (static_cast<uint32_t>(quarter * 32) << 16);
+                    uint32_t part[2][32];
+                    tc::TmemLoad32(at, part[0]);
+#pragma unroll
+                    for (int c = 0; c < kMine; c += 32) {
+                        tc::TmemWait();
+                        if (c + 32 < kMine) {
+                            tc::TmemLoad32(at + c + 32, part[(c / 32 + 1) & 1]);
+                        }
+                        Add(sum, c, part[(c / 32) & 1], scale);
+                    }
+                }
+                tc::FenceBefore();
+                __syncwarp();
+                if (lane == 0) {
+                    tc::BarArrive(&bar.free[half]);
+                }
+            }
+            if (!going) {
+                break;
+            }
+            O* to = out + (FORM == kOuter ? segment * p.m * p.n : 0);
+            constexpr int kLine = 128 / sizeof(O);       // columns in 128 bytes
+            constexpr int kPerWord = 4 / sizeof(O);
+            bool odd = false;
+#pragma unroll
+            for (int c = 0; c < kMine; c += kLine) {
+                if (col0 + c < p.n) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        uint4 v;
+                        v.x = Word<O>(&sum[c + (4 * i) * kPerWord]);
+                        v.y = Word<O>(&sum[c + (4 * i + 1) * kPerWord]);
+                        v.z = Word<O>(&sum[c + (4 * i + 2) * kPerWord]);
+                        v.w = Word<O>(&sum[c + (4 * i + 3) * kPerWord]);
+                        *reinterpret_cast<uint4*>(mine + lane * 128 + ((i ^ (lane & 7)) << 4)) = v;
+                    }
+                    __syncwarp();
+                    const int piece = lane & 7;
+                    const int64_t col = col0 + c + piece * (kLine / 8);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = i * 4 + (lane >> 3);
+                        const uint4 value = *reinterpret_cast<const uint4*>(mine + r * 128 + ((piece ^ (r & 7)) << 4));
+                        if (r0 + r < row_end && col < p.n) {
+                            *reinterpret_cast<uint4*>(to + (r0 + r) * p.n + col) = value;
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            if constexpr (!F8) {
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) {
+                    odd |= !(fabsf(sum[i]) < INFINITY);
+                }
+                if (__any_sync(0xffffffffu, odd)) {
+                    // Results that are not finite, from the operands as given: the row of a lane, column by column.
+                    for (int64_t i = lane; i < 32 * kMine; i += 32) {
+                        const int64_t r = r0 + i / kMine, c = col0 + i % kMine;
+                        if (r >= row_end || c >= p.n) {
+                            continue;
+                        }
+                        float* place = reinterpret_cast<float*>(to) + r * p.n + c;
+                        if (fabsf(*place) < INFINITY) {
+                            continue;
+                        }
+                        const float* x = FORM == kOuter ? p.a + from * p.lda + r : p.a + r * p.lda;
+                        const float* y = FORM == kOuter ? p.b + from * p.ldb + c : p.b + segment * p.b_segment + c * p.b_n;
+                        const int64_t dx = FORM == kOuter ? p.lda : 1, dy = FORM == kOuter ? p.ldb : p.b_k;
+                        float v = 0.0f;
+                        for (int64_t d = 0; d < depth && v == v; ++d) {  // NaN stays NaN
+                            v = fmaf(__ldg(x + d * dx), __ldg(y + d * dy), v);
+                        }
+                        *place = v;
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        if constexpr (FORM != kOuter) {
+            // Rows of no segment.
+            const int64_t before = p.ptr.data != nullptr ? p.ptr.Raw(0) : 0;
+            const int64_t behind = p.ptr.data != nullptr ? p.ptr.Raw(p.ptr.segments) : p.ptr.rows;
+            constexpr int kVec = 16 / sizeof(O);
+            const int64_t pieces = p.n / kVec;
+            for (int64_t r = blockIdx.x * 8 + warp - 4; r < before + (p.ptr.rows - behind); r += gridDim.x * 8) {
+                const int64_t at = r < before ? r : behind + (r - before);
+                for (int64_t c = lane; c < pieces; c += 32) {
+                    *reinterpret_cast<uint4*>(out + at * p.n + c * kVec) = make_uint4(0, 0, 0, 0);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    if (warp == 0 && lane == 0 && bar.stop != 0) {
+        // Copies in flight must land before the block's shared memory is given up.
+        for (uint32_t f = filled > kStages ? filled - kStages : 0; f < filled; ++f) {
+            for (uint32_t i = 0; i < (1u << 15) && !tc::BarTry(&bar.full[f % kStages], (f / kStages) & 1); ++i) {
+            }
+        }
+    }
+    tc::FenceBefore();
+    __syncthreads();
+    if (warp == 2) {
+        tc::FenceAfter();
+        tc::TmemFree(tmem);
+    }
+}
+
+// planes[3][count] <- the three bf16 terms of src[matrices][rows][width] (rows of whole 16-byte vectors, strides in elements).
+__global__ void __launch_bounds__(256) SplitKernel(const float* __restrict__ src, int64_t matrices, int64_t rows, int64_t width,
+                                                   int64_t matrix_stride, int64_t row_stride, __nv_bfloat16* __restrict__ planes)
+{
+    const int64_t vectors = width / 4, total = matrices * rows * vectors, plane = matrices * rows * width;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int64_t line = i / vectors, c = (i - line * vectors) * 4;
+        const int64_t e = line / rows, r = line - e * rows;
+        const float4 v = __ldg(reinterpret_cast<const float4*>(src + e * matrix_stride + r * row_stride + c));
+        const float x[4] = {v.x, v.y, v.z, v.w};
+        __nv_bfloat16 t[3][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            t[0][j] = __float2bfloat16_rn(x[j]);
+            const float first = __bfloat162float(t[0][j]);
+            const bool finite = fabsf(first) < INFINITY;
+            const float rest = finite ? x[j] - first : 0.0f;   // exact
+            t[1][j] = __float2bfloat16_rn(rest);
+            t[2][j] = __float2bfloat16_rn(rest - __bfloat162float(t[1][j]));
+        }
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+            uint2 words;
+            memcpy(&words, t[j], 8);
+            *reinterpret_cast<uint2*>(planes + j * plane + line * width + c) = words;
+        }
+    }
+}
+
+int Split(const float* src, int64_t matrices, int64_t rows, int64_t width, int64_t matrix_stride, int64_t row_stride, void* planes,
+          cudaStream_t stream)
+{
+    const int64_t total = matrices * rows * (width / 4);
+    const int grid = static_cast<int>(std::min<int64_t>(CeilDiv(total, 256), static_cast<int64_t>(SmCount()) * 16));
+    SplitKernel<<<grid, 256, 0, stream>>>(src, matrices, rows, width, matrix_stride, row_stride, static_cast<__nv_bfloat16*>(planes));
+    return LaunchStatus();
+}
+
+bool Fits(int64_t v) { return v < (INT64_C(1) << 31) - 512; }
+
+// A map of planes or 8-bit values: [depth][rows][inner], rows `stride` elements apart, boxes of 128 bytes x box_rows.
+bool Map3(CUtensorMap* map, bool f8, const void* base, int64_t inner, int64_t rows, int64_t depth, int64_t stride, int64_t depth_stride,
+          int box_rows)
+{
+    const int size = f8 ? 1 : 2;
+    const uint64_t sizes[3] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(rows), static_cast<uint64_t>(depth)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(stride) * size, static_cast<uint64_t>(depth_stride) * size};
+    const uint32_t box[3] = {static_cast<uint32_t>(128 / size), static_cast<uint32_t>(box_rows), 1};
+    return tc::EncodeMap(map, f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, sizes, strides, box);
+}
+
+template <bool F8, class O, int BN, int FORM>
+int Launch(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int64_t tiles, cudaStream_t stream)
+{
+    OPSGNN_CUDA_TRY(cudaFuncSetAttribute(PromotedKernel<F8, O, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, SharedBytes<BN>()));
+    const int grid = static_cast<int>(std::min<int64_t>(std::max<int64_t>(tiles, 1), SmCount()));
+    PromotedKernel<F8, O, BN, FORM><<<grid, kThreads, SharedBytes<BN>(), stream>>>(a, b, p);
+    return LaunchStatus();
+}
+
+int64_t PlaneBytes(int64_t values) { return AlignUp(values * 3 * 2, 1024); }
+
+bool RowsSplittable(const RowsProblem& p, bool& turned)
+{
+    turned = p.b_k == 1 && p.b_n != 1;
+    const int64_t inner = turned ? p.k : p.n, other = turned ? p.n : p.k, stride = turned ? p.b_n : p.b_k;
+    return p.in_type == OPSGNN_F32 && p.k >= 1 && p.k % 8 == 0 && p.n % 8 == 0 && p.ldo == p.n && (turned || p.b_n == 1) &&
+           p.ptr.segments >= 1 && p.ptr.data != nullptr && p.lda % 4 == 0 && stride % 4 == 0 && p.b_segment % 4 == 0 && stride >= inner &&
+           Aligned(p.a, 16) && Aligned(p.b, 16) && Aligned(p.out, 16) && Fits(p.ptr.rows) && Fits(p.k) && Fits(p.n) &&
+           Fits(p.ptr.segments * 3) && Fits(other);
+}
+
+bool OuterSplittable(const OuterProblem& p)
+{
+    return p.type == OPSGNN_F32 && p.ptr.rows >= 1 && p.k % 8 == 0 && p.n % 8 == 0 && p.lda % 4 == 0 && p.ldb % 4 == 0 &&
+           Aligned(p.a, 16) && Aligned(p.b, 16) && Aligned(p.out, 16) && Fits(p.ptr.rows) && Fits(p.k) && Fits(p.n);
+}
+
+}  // namespace
+
+int64_t RowsSplitBytes(int64_t rows, int64_t segments, int64_t k, int64_t n) { return PlaneBytes(rows * k) + PlaneBytes(segments * k * n); }
+int64_t OuterSplitBytes(int64_t rows, int64_t k, int64_t n) { return PlaneBytes(rows * k) + PlaneBytes(rows * n); }
+
+int RunRowsSplit(const RowsProblem& p, void* workspace, cudaStream_t stream)
+{
+    bool turned;
+    if (!RowsSplittable(p, turned) || !Aligned(workspace, 16)) {
+        return OPSGNN_ERR_UNSUPPORTED;
+    }
+    Params q{};
+    q.ptr = p.ptr;
+    q.out = p.out;
+    q.n = p.n;
+    q.k = p.k;
+    q.a = static_cast<const float*>(p.a);
+    q.b = static_cast<const float*>(p.b);
+    q.lda = p.lda;
+    q.b_segment = p.b_segment;
+    q.b_k = p.b_k;
+    q.b_n = p.b_n;
+    OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
+    char* planes_a = static_cast<char*>(workspace);
+    char* planes_b = planes_a + PlaneBytes(p.ptr.rows * p.k);
+    const int64_t inner = turned ? p.k : p.n, other = turned ? p.n : p.k, e = p.ptr.segments;
+    const bool narrow = p.n <= 128;
+    CUtensorMap a, b;
+    if (!Map3(&a, false, planes_a, p.k, p.ptr.rows, 3, p.k, p.ptr.rows * p.k, kRows) ||
+        !Map3(&b, false, planes_b, inner, other, 3 * e, inner, inner * other, turned ? (narrow ? 128 : 256) : 64)) {
+        return OPSGNN_ERR_UNSUPPORTED;
+    }
+    int status = Split(q.a, 1, p.ptr.rows, p.k, 0, p.lda, planes_a, stream);
+    if (status == OPSGNN_OK) {
+        status = Split(q.b, e, other, inner, p.b_segment, turned ? p.b_n : p.b_k, planes_b, stream);
+    }
+    if (status != OPSGNN_OK) {
+        return status;
+    }
+    const int64_t down = p.ptr.rows / kRows + e;
+    if (narrow) {
+        return turned ? Launch<false, float, 128, kRowsTurned>(a, b, q, down, stream) : Launch<false, float, 128, kRowsWide>(a, b, q, down, stream);
+    }
+    const int64_t tiles = down * CeilDiv(p.n, 256);
+    return turned ? Launch<false, float, 256, kRowsTurned>(a, b, q, tiles, stream) : Launch<false, float, 256, kRowsWide>(a, b, q, tiles, stream);
+}
+
+int RunOuterSplit(const OuterProblem& p, void* workspace, cudaStream_t stream)
+{
+    if (!OuterSplittable(p) || !Aligned(workspace, 16)) {
+        return OPSGNN_ERR_UNSUPPORTED;
+    }
+    Params q{};
+    q.ptr = p.ptr;
+    q.out = p.out;
+    q.m = p.k;
+    q.n = p.n;
+    q.a = static_cast<const float*>(p.a);
+    q.b = static_cast<const float*>(p.b);
+    q.lda = p.lda;
+    q.ldb = p.ldb;
+    OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
+    char* planes_a = static_cast<char*>(workspace);
+    char* planes_b = planes_a + PlaneBytes(p.ptr.rows * p.k);
+    CUtensorMap a, b;
+    if (!Map3(&a, false, planes_a, p.k, p.ptr.rows, 3, p.k, p.ptr.rows * p.k, 64) ||
+        !Map3(&b, false, planes_b, p.n, p.ptr.rows, 3, p.n, p.ptr.rows * p.n, 64)) {
+        return OPSGNN_ERR_UNSUPPORTED;
+    }
+    int status = Split(q.a, 1, p.ptr.rows, p.k, 0, p.lda, planes_a, stream);
+    if (status == OPSGNN_OK) {
+        status = Split(q.b, 1, p.ptr.rows, p.n, 0, p.ldb, planes_b, stream);
+    }
+    if (status != OPSGNN_OK) {
+        return status;
+    }
+    const int64_t down = p.ptr.segments * CeilDiv(p.k, kRows);
+    return p.n <= 128 ? Launch<false, float, 128, kOuter>(a, b, q, down, stream)
+                      : Launch<false, float, 256, kOuter>(a, b, q, down * CeilDiv(p.n, 256), stream);
+}
+
+int RunRowsFp8(const RowsProblem& p, cudaStream_t stream)
+{
+    const int vec = 16 / DtypeBytes(p.out_type);
+    if (p.in_type != OPSGNN_F8E4M3 || p.k < 1 || p.ptr.segments < 1 || p.b_k != 1 || p.lda % 16 != 0 || p.b_n % 16 != 0 ||
+        p.b_segment % 16 != 0 || p.b_segment < 1 || p.b_n < p.k || p.n % vec != 0 || p.ldo != p.n || !Aligned(p.a, 16) ||
+        !Aligned(p.b, 16) || !Aligned(p.out, 16) || !Fits(p.ptr.rows) || !Fits(p.k) || !Fits(p.n) || !Fits(p.ptr.segments) ||
+        p.lda >= (INT64_C(1) << 39) || p.b_segment >= (INT64_C(1) << 39)) {
+        return OPSGNN_ERR_UNSUPPORTED;
+    }
+    Params q{};
+    q.ptr = p.ptr;
+    q.out = p.out;
+    q.a_scale = p.a_scale;
+    q.b_scale = p.b_scale;
+    q.n = p.n;
+    q.k = p.k;
+    OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
+    const bool narrow = p.n <= 128;
+    CUtensorMap a, b;
+    if (!Map3(&a, true, p.a, p.k, p.ptr.rows, 1, p.lda, p.lda, kRows) ||
+        !Map3(&b, true, p.b, p.k, p.n, p.ptr.segments, p.b_n, p.b_segment, narrow ? 128 : 256)) {
+        return OPSGNN_ERR_UNSUPPORTED;
+    }
+    const int64_t tiles = (p.ptr.rows / kRows + p.ptr.segments) * CeilDiv(p.n, narrow ? 128 : 256);
+    auto run = [&](auto tag) {
+        using O = decltype(tag);
+        return narrow ? Launch<true, O, 128, kRowsTurned>(a, b, q, tiles, stream) : Launch<true, O, 256, kRowsTurned>(a, b, q, tiles, stream);
+    };
+    switch (p.out_type) {
+        case OPSGNN_F32:
+            return run(float());
+        case OPSGNN_F16:
+            return run(__half());
+        default:
+            return run(__nv_bfloat16());
+    }
+}
+
+}  // namespace segmm
+}  // namespace opsgnn

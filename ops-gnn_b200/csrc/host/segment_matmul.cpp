@@ -78,8 +78,11 @@ at::Tensor segment_matmul_forward(const at::Tensor& src, const at::Tensor& indpt
     at::Tensor out = at::empty({src.size(0), weight.size(2)}, src.options());
     OpsgnnSegmentMatmulDesc desc = DescOf(rows, indptr, weight.size(0), weight.size(2), src.scalar_type(), api);
     SetWeight(desc, matrices);
+    int64_t bytes = 0;
+    CheckStatus(opsgnn_segment_matmul_workspace_bytes(&desc, 0, &bytes), api);
+    const at::Tensor scratch = bytes > 0 ? Scratch(bytes, src) : at::Tensor();
     CheckStatus(opsgnn_segment_matmul(&desc, indptr.const_data_ptr(), rows.const_data_ptr(), matrices.const_data_ptr(), out.data_ptr(),
-                                      CurrentStream(src)),
+                                      bytes > 0 ? scratch.data_ptr() : nullptr, bytes, CurrentStream(src)),
                 api);
     return out;
 }
@@ -98,8 +101,12 @@ at::Tensor segment_matmul_weight_grad(const at::Tensor& src, const at::Tensor& i
     const at::Tensor rows = RowMajor(src), upstream = RowMajor(grad);
     at::Tensor out = at::empty({segments, src.size(1), grad.size(1)}, src.options());
     const OpsgnnSegmentMatmulDesc desc = DescOf(rows, indptr, segments, grad.size(1), src.scalar_type(), api);
+    int64_t bytes = 0;
+    CheckStatus(opsgnn_segment_matmul_workspace_bytes(&desc, 1, &bytes), api);
+    const at::Tensor scratch = bytes > 0 ? Scratch(bytes, src) : at::Tensor();
     CheckStatus(opsgnn_segment_matmul_weight_grad(&desc, indptr.const_data_ptr(), rows.const_data_ptr(), upstream.const_data_ptr(),
-                                                  std::max(RowStride(upstream), upstream.size(1)), out.data_ptr(), CurrentStream(src)),
+                                                  std::max(RowStride(upstream), upstream.size(1)), out.data_ptr(),
+                                                  bytes > 0 ? scratch.data_ptr() : nullptr, bytes, CurrentStream(src)),
                 api);
     return out;
 }

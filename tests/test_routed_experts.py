@@ -243,14 +243,18 @@ def test_c_abi_refuses():
         return call(ref(_cabi.SegmentMatmulDesc(*fields.values())), *pointers)
 
     rows, outer, fp8 = lib.opsgnn_segment_matmul, lib.opsgnn_segment_matmul_weight_grad, lib.opsgnn_segment_matmul_fp8
-    assert matmul(rows, None, None, None, None, None) == -1
-    assert matmul(rows, None, None, None, None, None, rows=0) == 0
-    assert matmul(rows, None, None, None, None, None, src_stride=7) == -1
-    assert matmul(rows, None, None, None, None, None, out_type=_cabi.F32) == -2
-    assert matmul(rows, None, None, None, None, None, in_type=_cabi.F64, out_type=_cabi.F64) == -2
-    assert matmul(rows, None, None, None, None, None, index_type=_cabi.F32) == -1
-    assert matmul(outer, None, None, None, 8, None, None) == -1
-    assert matmul(outer, None, None, None, 8, None, None, segments=0) == 0
+    assert matmul(rows, None, None, None, None, None, 0, None) == -1
+    assert matmul(rows, None, None, None, None, None, 0, None, rows=0) == 0
+    assert matmul(rows, None, None, None, None, None, 0, None, src_stride=7) == -1
+    assert matmul(rows, None, None, None, None, None, 0, None, out_type=_cabi.F32) == -2
+    assert matmul(rows, None, None, None, None, None, 0, None, in_type=_cabi.F64, out_type=_cabi.F64) == -2
+    assert matmul(rows, None, None, None, None, None, 0, None, index_type=_cabi.F32) == -1
+    assert matmul(outer, None, None, None, 8, None, None, 0, None) == -1
+    assert matmul(outer, None, None, None, 8, None, None, 0, None, segments=0) == 0
+    four = dict(in_type=_cabi.F32, out_type=_cabi.F32)
+    assert matmul(lib.opsgnn_segment_matmul_workspace_bytes, 0, ref(size), **four) == 0 and size.value >= 6 * (4 * 8 + 2 * 64)
+    assert matmul(rows, 16, 16, 16, 16, None, 0, None, **four) == -3
+    assert matmul(lib.opsgnn_segment_matmul_workspace_bytes, 1, ref(size)) == 0 and size.value == 0
     assert matmul(fp8, None, None, None, None, None, None, None) == -2
     assert matmul(fp8, None, None, None, None, None, None, None, in_type=_cabi.F8E4M3) == -1
     assert lib.opsgnn_quantize_fp8(None, _cabi.BF16, 1, 4, 4, 1, None, None, None) == -1
@@ -549,6 +553,12 @@ def test_segment_matmul_layouts(cuda_device, dtype):
         view.copy_(d_weight)
         _within(segment_matmul(d_src, d_ptr, view), want, size, 66, f"weight at {k0}, {n0}")
         view.fill_(math.nan)
+    padded = torch.full((4, 80, 104), math.nan, dtype=dtype, device=cuda_device)  # whole vectors, rows apart
+    for turned in (False, True):
+        view = padded[:, 8:80, 16:80].transpose(1, 2) if turned else padded[:, 8:72, 16:88]
+        view.copy_(d_weight)
+        _within(segment_matmul(d_src, d_ptr, view), want, size, 66, f"weight of a wider tensor, turned: {turned}")
+        view.fill_(math.nan)
     shared = weight[:1].expand(4, -1, -1)
     leaf = weight[:1].to(cuda_device).requires_grad_()
     out = segment_matmul(d_src, d_ptr, leaf.expand(4, -1, -1))
@@ -840,11 +850,16 @@ def test_segment_matmul_fp8_layouts_and_special_values(cuda_device):
     dev = [t.to(cuda_device) for t in args]
     plain = segment_matmul_fp8(*dev, out_dtype=torch.float32)
     assert not plain[-3:].any()
-    wide = torch.zeros(207, 300, dtype=torch.uint8, device=cuda_device).view(torch.float8_e4m3fn)
-    for offset in (0, 16, 5):
-        view = wide[:, offset:offset + 256]
-        view.view(torch.uint8).copy_(dev[0].view(torch.uint8))
-        assert torch.equal(segment_matmul_fp8(view, *dev[1:], out_dtype=torch.float32), plain), offset
+    # Rows of a wider matrix.  Layouts that are not whole 16-byte vectors are summed in another order than the others, so
+    # each is held to the bound of its sum, not to the bits of `plain`.
+    a, b = _stands_for(args[0], args[1], 1), _stands_for(args[2], args[3], 128).transpose(1, 2)
+    want, size = _plain_matmul(a, args[4], b), _plain_matmul(a.abs(), args[4], b.abs())
+    for width in (300, 304):
+        wide = torch.zeros(207, width, dtype=torch.uint8, device=cuda_device).view(torch.float8_e4m3fn)
+        for offset in (0, 16, 5):
+            view = wide[:, offset:offset + 256]
+            view.view(torch.uint8).copy_(dev[0].view(torch.uint8))
+            _within(segment_matmul_fp8(view, *dev[1:], out_dtype=torch.float32), want, size, 260, f"{width}, {offset}")
     turned = dev[2].view(torch.uint8).transpose(1, 2).contiguous().transpose(1, 2).view(torch.float8_e4m3fn)
     assert torch.equal(segment_matmul_fp8(dev[0], dev[1].t().contiguous().t(), turned, dev[3], dev[4].int(), torch.float32), plain)
     bits = dev[0].view(torch.uint8).clone()
