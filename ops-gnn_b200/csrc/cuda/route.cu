@@ -7,7 +7,7 @@
 //     index = the k largest c of the open groups, descending, ties to the lowest index (groups likewise)
 //     weight = scale * s[index] / (renormalize ? sum s[index] : 1), 0 where that sum is 0
 // The choice must not hang on how exp rounds.  Without bias, and with groups ranked by one score, c orders as l does and the
-// choice compares the logits themselves, exactly.  Otherwise c is formed in 64 bits.
+// choice compares the logits themselves, exactly.  Otherwise it compares scores, in 64 bits where fp32 cannot tell.
 //
 // Backward (u = grad * scale, sums over the chosen i):
 //     softmax, renormalized:  dl_i = w_i (u_i - sum u w)                     with w the softmax over the chosen logits
@@ -104,167 +104,432 @@ template <class T, int VPL> __device__ __forceinline__ void LoadRow(const T* row
     }
 }
 
-template <class Key, class T, int VPL>
-__global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T* __restrict__ logits, const float* __restrict__ bias,
-                                                          T* __restrict__ weight, int64_t* __restrict__ index, bool wide)
+// Value of a key that came from a number.
+__device__ __forceinline__ float ValueOf(uint32_t key) { return __uint_as_float((key >> 31) ? (key & 0x7fffffffu) : ~key); }
+constexpr uint32_t kMasked = 0x007fffffu;  // KeyOf(-inf)
+
+__device__ __forceinline__ float Sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+// Sorts a lane's keys, largest first (odd-even merge; VPL a power of two).
+template <int VPL> __device__ __forceinline__ void SortDown(uint32_t (&key)[VPL])
 {
-    // The keys of a warp's row, needed across lanes only where groups are ranked.
-    extern __shared__ __align__(16) unsigned char shared[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    Key* row_keys = reinterpret_cast<Key*>(shared) + static_cast<size_t>(warp) * p.experts;
-    constexpr bool kFine = sizeof(Key) == 8;
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWarps + warp; r < p.rows; r += static_cast<int64_t>(gridDim.x) * kWarps) {
-        float l[VPL];
-        LoadRow<T, VPL>(logits + r * p.experts, p.experts, wide, lane, l);
-        float top = -INFINITY;
-        bool nan = false;
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-            top = fmaxf(top, l[j]);
-            nan |= l[j] != l[j];
-        }
-        if (p.softmax) {
-            top = WarpMax(top);
-            nan = __any_sync(kFull, nan);
-        }
-        // A softmax over NaN or +inf has no finite value: the whole row is NaN, as torch.softmax has it.
-        const float base = p.softmax ? ((nan || top == INFINITY) ? NAN : top) : 0.0f;
-
-        Key key[VPL];
-        if constexpr (kFine) {
-            double c[VPL];
-            double total = 1.0;
-            if (p.softmax) {
-                double part = 0.0;
+    for (int p = 1; p < VPL; p <<= 1) {
 #pragma unroll
-                for (int j = 0; j < VPL; ++j) {
-                    const bool real = lane * VPL + j < p.experts && l[j] != -INFINITY;
-                    c[j] = real ? exp(static_cast<double>(l[j]) - static_cast<double>(base)) : 0.0;
-                    part += c[j];
-                }
-                total = WarpSum(part);
-            }
+        for (int q = p; q >= 1; q >>= 1) {
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) {
-                const int at = lane * VPL + j;
-                double v = p.softmax ? c[j] / total : 1.0 / (1.0 + exp(-static_cast<double>(l[j])));
-                if (bias != nullptr && at < p.experts) {
-                    v += static_cast<double>(__ldg(bias + at));
-                }
-                v = l[j] == -INFINITY ? -static_cast<double>(INFINITY) : v;
-                key[j] = at < p.experts ? KeyOf(v) : 0;
-            }
-        } else {
+            for (int j = q % p; j + q < VPL; j += 2 * q) {
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) {
-                key[j] = lane * VPL + j < p.experts ? KeyOf(p.softmax && base != base ? NAN : l[j]) : 0;
-            }
-        }
-
-        if (p.groups > 1) {
-            const int size = p.experts / p.groups;
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < VPL; ++j) {
-                if (lane * VPL + j < p.experts) {
-                    row_keys[lane * VPL + j] = key[j];
-                }
-            }
-            __syncwarp();
-            // Lane g ranks group g (at most 32 groups).
-            Key mine = 0;
-            if (lane < p.groups) {
-                Key first = 0, second = 0;
-                for (int i = 0; i < size; ++i) {
-                    const Key v = row_keys[lane * size + i];
-                    second = v > first ? first : (v > second ? v : second);
-                    first = v > first ? v : first;
-                }
-                mine = first;
-                if constexpr (kFine) {
-                    if (p.group_top == 2) {
-                        // back from keys to values; both are numbers or -inf
-                        const uint64_t a = (first >> 63) ? (first & 0x7fffffffffffffffULL) : ~static_cast<uint64_t>(first);
-                        const uint64_t b = (second >> 63) ? (second & 0x7fffffffffffffffULL) : ~static_cast<uint64_t>(second);
-                        mine = KeyOf(__longlong_as_double(static_cast<long long>(a)) + __longlong_as_double(static_cast<long long>(b)));
+                for (int i = 0; i < q; ++i) {
+                    if (j + i + q < VPL && (j + i) / (2 * p) == (j + i + q) / (2 * p)) {
+                        const uint32_t a = key[j + i], b = key[j + i + q];
+                        key[j + i] = max(a, b);
+                        key[j + i + q] = min(a, b);
                     }
                 }
             }
-            int ahead = 0;
-            for (int g = 0; g < p.groups; ++g) {
-                const Key other = __shfl_sync(kFull, mine, g);
-                ahead += (other > mine || (other == mine && g < lane)) ? 1 : 0;
-            }
-            const unsigned open = __ballot_sync(kFull, lane < p.groups && ahead < p.kept_groups);
+        }
+    }
+}
+
+// Ranks the groups of a row by the sum of the `top` largest keys' values (keys themselves for top 1) and tells whether the
+// lane's experts are in an open one.  `gap`: how far the worst open group is above the best closed one.
+// A group of whole lanes, a power of two of them, is ranked by shuffles; other sizes go through shared memory.
+template <int VPL>
+__device__ __forceinline__ void CloseGroups(const RouteParams& p, uint32_t (&key)[VPL], uint32_t* row_keys, int lane, float& gap)
+{
+    const int size = p.experts / p.groups;
+    const int lanes = size / VPL;
+    const bool whole = size % VPL == 0 && (lanes & (lanes - 1)) == 0;
+    uint32_t first = 0, second = 0;
+    if (whole) {
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) {
-                const int at = lane * VPL + j;
-                if (at < p.experts && !((open >> (at / size)) & 1u)) {
-                    key[j] = 0;
-                }
+        for (int j = 0; j < VPL; ++j) {
+            second = max(second, min(first, key[j]));
+            first = max(first, key[j]);
+        }
+        for (int d = 1; d < lanes; d <<= 1) {
+            const uint32_t a = __shfl_xor_sync(kFull, first, d), b = __shfl_xor_sync(kFull, second, d);
+            second = max(max(second, b), min(first, a));
+            first = max(first, a);
+        }
+    } else {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            if (lane * VPL + j < p.experts) {
+                row_keys[lane * VPL + j] = key[j];
             }
         }
-
-        // k times: the largest key, at the lowest lane that has it (lanes hold ascending ranges of experts).
-        Key best = 0;
-        int where = 0;
+        __syncwarp();
+        if (lane < p.groups) {
+            for (int i = 0; i < size; ++i) {
+                const uint32_t v = row_keys[lane * size + i];
+                second = max(second, min(first, v));
+                first = max(first, v);
+            }
+        }
+    }
+    // Group g is at lane g * lanes (whole) or g.
+    const int step = whole ? lanes : 1;
+    const int mine = whole ? lane / lanes : lane;
+    const uint32_t score = mine < p.groups ? (p.group_top == 2 ? KeyOf(ValueOf(first) + ValueOf(second)) : first) : 0u;
+    int ahead = 0;
+    for (int g = 0; g < p.groups; ++g) {
+        const uint32_t other = __shfl_sync(kFull, score, g * step);
+        ahead += (other > score || (other == score && g < mine)) ? 1 : 0;
+    }
+    const bool open = mine < p.groups && ahead < p.kept_groups;
+    const uint32_t worst = ~__reduce_max_sync(kFull, open ? ~score : 0u);
+    const uint32_t best = __reduce_max_sync(kFull, open ? 0u : score);
+    gap = best == 0 ? INFINITY : ValueOf(worst) - ValueOf(best);
+    if (whole) {
 #pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            key[j] = open ? key[j] : 0u;
+        }
+    } else {
+        const unsigned set = __ballot_sync(kFull, open);
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            const int at = lane * VPL + j;
+            if (at < p.experts && !((set >> (at / size)) & 1u)) {
+                key[j] = 0;
+            }
+        }
+    }
+}
+
+// The choice with scores in 64 bits, for rows whose fp32 scores are too close to tell.  Lane i < k gets the i-th choice.
+template <int VPL>
+__device__ __noinline__ void ChooseFine(const RouteParams& p, const float (&l)[VPL], const float* bias, float base, uint64_t* row_keys,
+                                        int lane, int& chosen, float& chosen_logit)
+{
+    uint64_t key[VPL];
+    double total = 1.0;
+    if (p.softmax) {
+        double part = 0.0;
+#pragma unroll 1
+        for (int j = 0; j < VPL; ++j) {
+            part += l[j] != -INFINITY ? exp(static_cast<double>(l[j]) - static_cast<double>(base)) : 0.0;
+        }
+        total = WarpSum(part);
+    }
+#pragma unroll 1
+    for (int j = 0; j < VPL; ++j) {
+        const int at = lane * VPL + j;
+        const double x = static_cast<double>(l[j]);
+        double v = p.softmax ? exp(x - static_cast<double>(base)) / total : 1.0 / (1.0 + exp(-x));
+        if (bias != nullptr && at < p.experts) {
+            v += static_cast<double>(__ldg(bias + at));
+        }
+        v = l[j] == -INFINITY ? -static_cast<double>(INFINITY) : v;
+        key[j] = at < p.experts ? KeyOf(v) : 0;
+    }
+    if (p.groups > 1) {
+        const int size = p.experts / p.groups;
+        __syncwarp();
+#pragma unroll 1
+        for (int j = 0; j < VPL; ++j) {
+            if (lane * VPL + j < p.experts) {
+                row_keys[lane * VPL + j] = key[j];
+            }
+        }
+        __syncwarp();
+        uint64_t mine = 0;
+        if (lane < p.groups) {
+            uint64_t first = 0, second = 0;
+            for (int i = 0; i < size; ++i) {
+                const uint64_t v = row_keys[lane * size + i];
+                second = v > first ? first : (v > second ? v : second);
+                first = v > first ? v : first;
+            }
+            mine = first;
+            if (p.group_top == 2) {
+                // back from keys to values; both are numbers or -inf
+                const uint64_t a = (first >> 63) ? (first & 0x7fffffffffffffffULL) : ~first;
+                const uint64_t b = (second >> 63) ? (second & 0x7fffffffffffffffULL) : ~second;
+                mine = KeyOf(__longlong_as_double(static_cast<long long>(a)) + __longlong_as_double(static_cast<long long>(b)));
+            }
+        }
+        int ahead = 0;
+        for (int g = 0; g < p.groups; ++g) {
+            const uint64_t other = __shfl_sync(kFull, mine, g);
+            ahead += (other > mine || (other == mine && g < lane)) ? 1 : 0;
+        }
+        const unsigned open = __ballot_sync(kFull, lane < p.groups && ahead < p.kept_groups);
+#pragma unroll 1
+        for (int j = 0; j < VPL; ++j) {
+            const int at = lane * VPL + j;
+            if (at < p.experts && !((open >> (at / size)) & 1u)) {
+                key[j] = 0;
+            }
+        }
+    }
+    for (int i = 0; i < p.k; ++i) {
+        uint64_t best = 0;
+        int where = 0;
+#pragma unroll 1
         for (int j = 0; j < VPL; ++j) {
             where = key[j] > best ? j : where;
             best = key[j] > best ? key[j] : best;
         }
-        int chosen = 0;
-        float chosen_logit = -INFINITY;
-        for (int i = 0; i < p.k; ++i) {
-            const Key winner = WarpMax(best);
-            const int owner = __ffs(__ballot_sync(kFull, best == winner)) - 1;
-            float value = 0.0f;
-            int at = 0;
-            if (lane == owner) {
-                at = lane * VPL + where;
+        const uint64_t winner = WarpMax(best);
+        const int owner = __ffs(__ballot_sync(kFull, best == winner)) - 1;
+        const int at = __shfl_sync(kFull, lane * VPL + where, owner);
+        const float value = __shfl_sync(kFull, l[where], owner);
+        if (lane == owner) {
+            key[where] = 0;
+        }
+        if (lane == i) {
+            chosen = at;
+            chosen_logit = value;
+        }
+    }
+}
+
+// BIASED: the choice needs the scores themselves (a bias, or groups ranked by a sum of two); otherwise it compares logits.
+//
+// Logits of 16 bits and their expert's number fit one 32-bit key, all keys differ, and each step of the choice is one warp
+// maximum (redux) and a pop from the winning lane's sorted keys.  32-bit keys take a second step to find the winner's lane.
+//
+// BIASED scores are formed in fp32 first.  Each is off by at most 2^-20 of the largest score (exp, a division, a sum) and
+// 2^-24 of itself (the bias); where two neighbours in the order, or a group let in and one left out, are closer than twice
+// that and not equal by their inputs, the row is chosen again in 64 bits: about one row in a hundred at 256 experts.
+template <class T, int VPL, bool BIASED>
+__global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T* __restrict__ logits, const float* __restrict__ bias,
+                                                          T* __restrict__ weight, int64_t* __restrict__ index, bool wide)
+{
+    extern __shared__ __align__(16) unsigned char shared[];
+    constexpr bool PACKED = sizeof(T) == 2 && !BIASED;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // The keys of a warp's row, needed across lanes only where groups are not whole lanes (64-bit ones in ChooseFine).
+    unsigned char* row_keys = shared + static_cast<size_t>(warp) * p.experts * (BIASED ? 8 : 4);
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWarps + warp; r < p.rows; r += static_cast<int64_t>(gridDim.x) * kWarps) {
+        float l[VPL];
+        LoadRow<T, VPL>(logits + r * p.experts, p.experts, wide, lane, l);
+        // A softmax over NaN or +inf has no finite value: the whole row is NaN, as torch.softmax has it.
+        float top = -INFINITY;
+        bool bad = false;
+        if (p.softmax) {
+            bool odd = false;
 #pragma unroll
-                for (int j = 0; j < VPL; ++j) {
-                    if (j == where) {
-                        value = l[j];
-                        key[j] = 0;
-                    }
-                }
-                best = 0;
-#pragma unroll
-                for (int j = 0; j < VPL; ++j) {
-                    where = key[j] > best ? j : where;
-                    best = key[j] > best ? key[j] : best;
-                }
+            for (int j = 0; j < VPL; ++j) {
+                top = fmaxf(top, l[j]);
+                odd |= !(l[j] < INFINITY);
             }
-            at = __shfl_sync(kFull, at, owner);
-            value = __shfl_sync(kFull, value, owner);
-            if (lane == i) {
-                chosen = at;
-                chosen_logit = value;
+            bad = __any_sync(kFull, odd);
+            if (BIASED || !p.renormalize) {
+                top = ValueOf(__reduce_max_sync(kFull, KeyOf(top)));
             }
         }
 
-        float s = 0.0f;
-        if (lane < p.k) {
+        uint32_t key[VPL];
+        float margin = 0.0f, whole_sum = 1.0f;
+        if constexpr (BIASED) {
+            float c[VPL];
             if (p.softmax) {
-                s = chosen_logit == -INFINITY && base == base ? 0.0f : expf(chosen_logit - base);
+                float part = 0.0f;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) {
+                    c[j] = l[j] == -INFINITY ? 0.0f : expf(l[j] - top);
+                    part += c[j];
+                }
+                whole_sum = WarpSum(part);
+                const float inverse = 1.0f / whole_sum;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) {
+                    c[j] *= inverse;
+                }
+                margin = inverse * 0x1p-18f;
             } else {
-                s = 1.0f / (1.0f + expf(-chosen_logit));
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) {
+                    c[j] = Sigmoid(l[j]);
+                }
+                margin = 0x1p-18f;
             }
-        }
-        float total = 1.0f;
-        if (p.renormalize) {
-            total = WarpSum(s);
-        } else if (p.softmax) {
-            float part = 0.0f;
+            float largest = 0.0f;
 #pragma unroll
             for (int j = 0; j < VPL; ++j) {
-                part += l[j] == -INFINITY && base == base ? 0.0f : expf(l[j] - base);
+                const int at = lane * VPL + j;
+                if (bias != nullptr && at < p.experts) {
+                    c[j] += __ldg(bias + at);
+                }
+                largest = fmaxf(largest, fabsf(c[j]));
+                c[j] = l[j] == -INFINITY ? -INFINITY : (bad ? NAN : c[j]);
+                key[j] = at < p.experts ? KeyOf(c[j]) : 0u;
             }
-            total = WarpSum(part);
+            margin += __uint_as_float(__reduce_max_sync(kFull, __float_as_uint(largest))) * 0x1p-22f;
+        } else {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                const int at = lane * VPL + j;
+                key[j] = KeyOf(bad ? -INFINITY : l[j]);
+                if constexpr (PACKED) {
+                    // the 16 bits of the logit, ordered, then the lower expert first
+                    uint32_t bits;
+                    if constexpr (std::is_same<T, __half>::value) {
+                        const float v = bad || l[j] != l[j] ? -INFINITY : l[j] + 0.0f;
+                        bits = __half_as_ushort(__float2half_rn(v));
+                        bits = (bits & 0x8000u) ? (~bits & 0xffffu) : (bits | 0x8000u);
+                    } else {
+                        bits = key[j] >> 16;  // bf16 is the upper half of fp32, and so is its order
+                    }
+                    key[j] = (bits << 16) | (0xffffu - static_cast<uint32_t>(at));
+                }
+                key[j] = at < p.experts ? key[j] : 0u;
+            }
         }
-        if (lane < p.k) {
-            weight[r * p.k + lane] = Narrow<T, float>(total == 0.0f ? 0.0f : s / total * p.scale);
+
+        bool sure = true;
+        if (p.groups > 1) {
+            float gap;
+            if constexpr (PACKED) {
+                // Rank by the logit alone, ties to the lower group: the expert's number inside the key orders the same way.
+                CloseGroups<VPL>(p, key, reinterpret_cast<uint32_t*>(row_keys), lane, gap);
+            } else {
+                CloseGroups<VPL>(p, key, reinterpret_cast<uint32_t*>(row_keys), lane, gap);
+                sure = !BIASED || gap > 2.0f * margin;
+            }
+        }
+
+        int chosen = 0;
+        float chosen_logit = -INFINITY;
+        if constexpr (PACKED) {
+            if constexpr (VPL <= 8) {
+                SortDown<VPL>(key);
+            }
+            uint32_t head = key[0];
+            if constexpr (VPL > 8) {
+#pragma unroll
+                for (int j = 1; j < VPL; ++j) {
+                    head = max(head, key[j]);
+                }
+            }
+            uint32_t mine = 0;
+            for (int i = 0; i < p.k; ++i) {
+                const uint32_t winner = __reduce_max_sync(kFull, head);
+                mine = lane == i ? winner : mine;
+                if (head == winner) {
+                    if constexpr (VPL <= 8) {
+#pragma unroll
+                        for (int j = 0; j + 1 < VPL; ++j) {
+                            key[j] = key[j + 1];
+                        }
+                        key[VPL - 1] = 0;
+                        head = key[0];
+                    } else {
+                        head = 0;
+#pragma unroll
+                        for (int j = 0; j < VPL; ++j) {
+                            head = max(head, key[j] < winner ? key[j] : 0u);
+                        }
+                    }
+                }
+            }
+            if (lane < p.k) {
+                chosen = static_cast<int>(0xffffu - (mine & 0xffffu));
+                uint32_t bits = mine >> 16;
+                bits = (bits & 0x8000u) ? (bits & 0x7fffu) : (~bits & 0xffffu);
+                if constexpr (std::is_same<T, __half>::value) {
+                    chosen_logit = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+                } else {
+                    chosen_logit = __uint_as_float(bits << 16);
+                }
+                if (chosen_logit == -INFINITY) {  // the key of a masked expert is that of a NaN, too
+                    chosen_logit = Widen<float, T>(LoadNc(logits + r * p.experts + chosen));
+                }
+            }
+        } else {
+            uint32_t best = 0;
+            int where = 0;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                where = key[j] > best ? j : where;
+                best = key[j] > best ? key[j] : best;
+            }
+            uint32_t before = 0;
+            float before_value = 0.0f;
+            int before_at = 0;
+            // BIASED looks one step further: the first expert left out must be clear of the last one taken.
+            const int steps = BIASED && p.k < p.experts ? p.k + 1 : p.k;
+            for (int i = 0; sure && i < steps; ++i) {
+                const uint32_t winner = __reduce_max_sync(kFull, best);
+                if (winner == 0) {
+                    break;  // only the look-ahead can run out of experts
+                }
+                const int owner = __ffs(__ballot_sync(kFull, best == winner)) - 1;
+                float value = l[0];
+#pragma unroll
+                for (int j = 1; j < VPL; ++j) {
+                    value = where == j ? l[j] : value;
+                }
+                const int at = __shfl_sync(kFull, lane * VPL + where, owner);
+                value = __shfl_sync(kFull, value, owner);
+                if (lane == owner) {
+#pragma unroll
+                    for (int j = 0; j < VPL; ++j) {
+                        key[j] = j == where ? 0u : key[j];
+                    }
+                    best = 0;
+#pragma unroll
+                    for (int j = 0; j < VPL; ++j) {
+                        where = key[j] > best ? j : where;
+                        best = key[j] > best ? key[j] : best;
+                    }
+                }
+                if (lane == i) {
+                    chosen = at;
+                    chosen_logit = value;
+                }
+                if constexpr (BIASED) {
+                    if (i > 0 && !(ValueOf(before) - ValueOf(winner) > margin)) {
+                        // Equal by their inputs, or both masked: a tie in every precision.
+                        const bool tie = (before == kMasked && winner == kMasked) ||
+                                         (value == before_value && (bias == nullptr || __ldg(bias + at) == __ldg(bias + before_at)));
+                        sure = tie;
+                    }
+                    before = winner;
+                    before_value = value;
+                    before_at = at;
+                }
+            }
+            if constexpr (BIASED) {
+                if (!sure) {
+                    ChooseFine<VPL>(p, l, bias, bad ? NAN : top, reinterpret_cast<uint64_t*>(row_keys), lane, chosen, chosen_logit);
+                }
+            }
+        }
+
+        // Weights.  A softmax renormalized over the chosen experts is the softmax of their logits.
+        const bool taken = lane < p.k;
+        float s = 0.0f, total = 1.0f;
+        if (p.softmax) {
+            float base = top;
+            if (p.renormalize) {
+                base = ValueOf(__reduce_max_sync(kFull, taken ? KeyOf(chosen_logit) : 0u));
+            }
+            s = taken && chosen_logit != -INFINITY ? expf(chosen_logit - base) : 0.0f;
+            if (p.renormalize) {
+                total = WarpSum(s);
+            } else if (BIASED) {
+                total = whole_sum;
+            } else {
+                float part = 0.0f;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) {
+                    part += l[j] == -INFINITY ? 0.0f : expf(l[j] - top);
+                }
+                total = WarpSum(part);
+            }
+        } else {
+            s = taken ? Sigmoid(chosen_logit) : 0.0f;
+            total = p.renormalize ? WarpSum(s) : 1.0f;
+        }
+        if (taken) {
+            const float w = bad ? NAN : (total == 0.0f ? 0.0f : s / total * p.scale);
+            weight[r * p.k + lane] = Narrow<T, float>(w);
             index[r * p.k + lane] = chosen;
         }
     }
@@ -568,15 +833,15 @@ template <class T, int VPL>
 int RunTopk(const OpsgnnRouteDesc& d, const void* logits, const float* bias, void* weight, int64_t* index, cudaStream_t stream)
 {
     const RouteParams p = ParamsOf(d);
-    const bool fine = bias != nullptr || (d.groups > 1 && d.group_top == 2);
+    const bool biased = bias != nullptr || (d.groups > 1 && d.group_top == 2);
     const bool wide = Wide<T, VPL>(d.experts, logits, logits);
-    const size_t shared = d.groups > 1 ? static_cast<size_t>(kWarps) * d.experts * (fine ? 8 : 4) : 0;
+    const size_t shared = d.groups > 1 ? static_cast<size_t>(kWarps) * d.experts * (biased ? 8 : 4) : 0;
     const T* in = static_cast<const T*>(logits);
     T* out = static_cast<T*>(weight);
-    if (fine) {
-        TopkKernel<uint64_t, T, VPL><<<Grid(d.rows), kWarps * 32, shared, stream>>>(p, in, bias, out, index, wide);
+    if (biased) {
+        TopkKernel<T, VPL, true><<<Grid(d.rows), kWarps * 32, shared, stream>>>(p, in, bias, out, index, wide);
     } else {
-        TopkKernel<uint32_t, T, VPL><<<Grid(d.rows), kWarps * 32, shared, stream>>>(p, in, bias, out, index, wide);
+        TopkKernel<T, VPL, false><<<Grid(d.rows), kWarps * 32, shared, stream>>>(p, in, bias, out, index, wide);
     }
     return LaunchStatus();
 }

@@ -353,6 +353,41 @@ def test_topk_route_nan_and_infinity(cuda_device):
 
 
 @requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+def test_topk_route_nan_under_sigmoid(cuda_device, dtype):
+    """A NaN comes after every number; where nothing else is left it is chosen and shows as NaN, a masked expert as 0."""
+    from ops_gnn import topk_route
+
+    x = torch.full((4, 40), -math.inf, dtype=dtype)
+    x[0, 4], x[0, 9], x[0, 30] = 1.0, math.nan, 2.0
+    x[1, 2] = math.nan
+    x[2] = math.nan
+    x[3, 1], x[3, 7] = math.nan, 0.0
+    for bias in (None, torch.zeros(40, device=cuda_device)):
+        weight, index = topk_route(x.to(cuda_device), 3, score="sigmoid", bias=bias, renormalize=False)
+        assert index.tolist() == [[30, 4, 0], [0, 1, 2], [0, 1, 2], [7, 0, 1]]
+        nan = [[False, False, False], [False, False, True], [True, True, True], [False, False, True]]
+        assert torch.isnan(weight).tolist() == nan
+        assert weight[0, 2] == 0 and weight[1, 0] == 0 and weight[3, 1] == 0 and weight[3, 0] == 0.5
+
+
+@requires_gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups,kept", [(1, 1), (8, 3), (10, 4)])
+def test_topk_route_many_close_rows(cuda_device, score, groups, kept):
+    """Rows whose biased scores come from few logits and few biases: ties by input, and gaps from 1 ulp of fp32 up."""
+    from ops_gnn import topk_route
+
+    gen = _gen(51)
+    rows, experts, k = 200, 80, 6
+    logits = torch.randint(-2, 3, (rows, experts), generator=gen).float() * 0.25
+    bias = torch.randint(0, 3, (experts,), generator=gen).float() * 2.0 ** -24 + 0.5
+    bias[torch.rand(experts, generator=gen) < 0.3] = 0.75
+    weight, index = topk_route(logits.to(cuda_device), k, score, bias.to(cuda_device), groups, kept)
+    assert torch.equal(index.cpu(), _plain_choice(logits, k, score, bias, groups, kept, 1 if groups == 1 else 2))
+
+
+@requires_gpu
 def test_topk_route_close_scores(cuda_device):
     """Scores that differ by less than fp32 tells apart: the bias is the only difference, in its last bits."""
     from ops_gnn import topk_route
