@@ -72,7 +72,25 @@ template <class T> __device__ __forceinline__ T WarpSum(T v)
     return v;
 }
 
-// Lane l holds experts l * VPL + j, j < VPL, of its warp's row: a row of whole vectors is read with wide loads.
+// The same over teams of LANES neighbouring lanes (the whole warp calls).
+template <int LANES> __device__ __forceinline__ float TeamMax(float v)
+{
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d >>= 1) {
+        v = fmaxf(v, __shfl_xor_sync(kFull, v, d));
+    }
+    return v;
+}
+template <int LANES> __device__ __forceinline__ float TeamSum(float v)
+{
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d >>= 1) {
+        v += __shfl_xor_sync(kFull, v, d);
+    }
+    return v;
+}
+
+// Lane l of a row's lanes holds experts l * VPL + j, j < VPL: a row of whole vectors is read with wide loads.
 template <class T, int VPL> __device__ __forceinline__ void LoadRow(const T* row, int experts, bool wide, int lane, float (&out)[VPL])
 {
     constexpr int VEC = VPL * sizeof(T) >= 16 ? 16 / sizeof(T) : VPL;
@@ -535,22 +553,165 @@ __global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T
     }
 }
 
+// 16-bit logits without bias and groups, k <= 8, at most 256 experts: four rows per warp, eight lanes each.  A lane sorts its
+// VPL packed keys eight at a time and merges the lists (of two sorted lists of eight, the eight largest are the pairwise
+// maxima of one with the other reversed, a bitonic list), three more merges with its neighbours leave the row's eight largest in
+// every lane; lane i then owns the i-th choice.  Per row a quarter of the instructions of the one-row-per-warp form, which
+// is bound by them: 131072 x 128, k 8: 56 -> 21 us.
+constexpr int kList = 8;
+
+__device__ __forceinline__ void Exchange(uint32_t& a, uint32_t& b)
+{
+    const uint32_t high = max(a, b), low = min(a, b);
+    a = high;
+    b = low;
+}
+// list <- the eight largest of list and other (both descending), descending.
+__device__ __forceinline__ void Merge(uint32_t (&list)[kList], const uint32_t (&other)[kList])
+{
+#pragma unroll
+    for (int i = 0; i < kList; ++i) {
+        list[i] = max(list[i], other[kList - 1 - i]);
+    }
+#pragma unroll
+    for (int d = kList / 2; d > 0; d >>= 1) {
+#pragma unroll
+        for (int i = 0; i < kList; ++i) {
+            if ((i & d) == 0) {
+                Exchange(list[i], list[i + d]);
+            }
+        }
+    }
+}
+
 template <class T, int VPL>
+__global__ void __launch_bounds__(kWarps * 32) TopkTeamKernel(RouteParams p, const T* __restrict__ logits, T* __restrict__ weight,
+                                                              int64_t* __restrict__ index, bool wide)
+{
+    const int lane = threadIdx.x & 31, member = lane & 7;
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarps;
+    for (int64_t r0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * 4; r0 < p.rows; r0 += warps * 4) {
+        const bool real = r0 + (lane >> 3) < p.rows;
+        const int64_t r = real ? r0 + (lane >> 3) : r0;
+        float l[VPL];
+        LoadRow<T, VPL>(logits + r * p.experts, p.experts, wide, member, l);
+        float top = -INFINITY;
+        uint32_t odd = 0;
+        if (p.softmax) {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                odd |= l[j] < INFINITY ? 0u : 1u;
+            }
+            // NaN or +inf in a row makes it NaN
+#pragma unroll
+            for (int d = 4; d > 0; d >>= 1) {
+                odd |= __shfl_xor_sync(kFull, odd, d);
+            }
+        }
+        const bool bad = odd != 0;
+        uint32_t list[kList];
+#pragma unroll
+        for (int first = 0; first < VPL; first += kList) {
+            uint32_t key[kList];
+#pragma unroll
+            for (int j = 0; j < kList; ++j) {
+                const int at = member * VPL + first + j;
+                uint32_t bits;
+                if constexpr (std::is_same<T, __half>::value) {
+                    const float v = bad || l[first + j] != l[first + j] ? -INFINITY : l[first + j] + 0.0f;
+                    bits = __half_as_ushort(__float2half_rn(v));
+                    bits = (bits & 0x8000u) ? (~bits & 0xffffu) : (bits | 0x8000u);
+                } else {
+                    bits = KeyOf(bad ? -INFINITY : l[first + j]) >> 16;
+                }
+                key[j] = at < p.experts ? (bits << 16) | (0xffffu - static_cast<uint32_t>(at)) : 0u;
+            }
+            SortDown<kList>(key);
+            if (first == 0) {
+#pragma unroll
+                for (int j = 0; j < kList; ++j) {
+                    list[j] = key[j];
+                }
+            } else {
+                Merge(list, key);
+            }
+        }
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) {
+            uint32_t other[kList];
+#pragma unroll
+            for (int j = 0; j < kList; ++j) {
+                other[j] = __shfl_xor_sync(kFull, list[j], d);
+            }
+            Merge(list, other);
+        }
+        uint32_t mine = list[0];
+#pragma unroll
+        for (int j = 1; j < kList; ++j) {
+            mine = member == j ? list[j] : mine;
+        }
+        const bool taken = member < p.k;
+        const int chosen = taken ? static_cast<int>(0xffffu - (mine & 0xffffu)) : 0;
+        auto value_of = [](uint32_t key) {
+            uint32_t bits = key >> 16;
+            bits = (bits & 0x8000u) ? (bits & 0x7fffu) : (~bits & 0xffffu);
+            if constexpr (std::is_same<T, __half>::value) {
+                return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+            } else {
+                return __uint_as_float(bits << 16);
+            }
+        };
+        float x = value_of(mine);
+        if (taken && x == -INFINITY) {  // the key of a masked expert is that of a NaN, too
+            x = Widen<float, T>(LoadNc(logits + r * p.experts + chosen));
+        }
+        float s, total = 1.0f;
+        if (p.softmax) {
+            top = value_of(list[0]);  // the row's largest logit, the first choice
+            s = taken && x != -INFINITY ? expf(x - top) : 0.0f;
+            if (p.renormalize) {
+                total = TeamSum<8>(s);
+            } else {
+                float part = 0.0f;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) {
+                    part += l[j] == -INFINITY ? 0.0f : expf(l[j] - top);
+                }
+                total = TeamSum<8>(part);
+            }
+        } else {
+            s = taken ? Sigmoid(x) : 0.0f;
+            total = p.renormalize ? TeamSum<8>(s) : 1.0f;
+        }
+        if (taken && real) {
+            const float w = bad ? NAN : (total == 0.0f ? 0.0f : s / total * p.scale);
+            weight[r * p.k + member] = Narrow<T, float>(w);
+            index[r * p.k + member] = chosen;
+        }
+    }
+}
+
+// LANES lanes per row: 8 where k and the row fit (four rows per warp), else 32.
+template <class T, int VPL, int LANES>
 __global__ void __launch_bounds__(kWarps * 32) TopkBackwardKernel(RouteParams p, const T* __restrict__ logits,
                                                                   const int64_t* __restrict__ index, const T* __restrict__ grad,
                                                                   T* __restrict__ grad_logits, bool wide)
 {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int ROWS = 32 / LANES;
     constexpr int VEC = VPL * sizeof(T) >= 16 ? 16 / sizeof(T) : VPL;
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWarps + warp; r < p.rows; r += static_cast<int64_t>(gridDim.x) * kWarps) {
+    const int lane = threadIdx.x & 31, member = lane % LANES;
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarps;
+    for (int64_t r0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * ROWS; r0 < p.rows; r0 += warps * ROWS) {
+        const bool real = r0 + lane / LANES < p.rows;
+        const int64_t r = real ? r0 + lane / LANES : r0;
         const T* row = logits + r * p.experts;
         T* out = grad_logits + r * p.experts;
         int64_t at = -1;
         float u = 0.0f, x = -INFINITY;
-        if (lane < p.k) {
-            at = index[r * p.k + lane];
+        if (member < p.k) {
+            at = index[r * p.k + member];
             if (at >= 0 && at < p.experts) {
-                u = Widen<float, T>(grad[r * p.k + lane]) * p.scale;
+                u = Widen<float, T>(grad[r * p.k + member]) * p.scale;
                 x = Widen<float, T>(row[at]);
             } else {
                 at = -1;
@@ -562,36 +723,38 @@ __global__ void __launch_bounds__(kWarps * 32) TopkBackwardKernel(RouteParams p,
         float l[VPL];
         if (p.softmax) {
             if (p.renormalize) {
-                top = WarpMax(at >= 0 ? x : -INFINITY);
-                float e = at < 0 || (x == -INFINITY && top == -INFINITY) ? 0.0f : expf(x - top);
-                const float sum = WarpSum(e);
+                top = TeamMax<LANES>(at >= 0 ? x : -INFINITY);
+                const float e = at < 0 || (x == -INFINITY && top == -INFINITY) ? 0.0f : expf(x - top);
+                const float sum = TeamSum<LANES>(e);
                 const float w = sum == 0.0f ? 0.0f : e / sum;
-                value = w * (u - WarpSum(u * w));
+                value = w * (u - TeamSum<LANES>(u * w));
             } else {
-                LoadRow<T, VPL>(row, p.experts, wide, lane, l);
+                LoadRow<T, VPL>(row, p.experts, wide, member, l);
                 top = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < VPL; ++j) {
                     top = fmaxf(top, l[j]);
                 }
-                top = WarpMax(top);
+                top = TeamMax<LANES>(top);
                 float part = 0.0f;
 #pragma unroll
                 for (int j = 0; j < VPL; ++j) {
-                    part += l[j] == -INFINITY ? 0.0f : expf(l[j] - top);
+                    l[j] = l[j] == -INFINITY ? 0.0f : expf(l[j] - top);
+                    part += l[j];
                 }
-                total = WarpSum(part);
-                const float s = at < 0 || x == -INFINITY ? 0.0f : expf(x - top) / total;
-                spread = WarpSum(u * s);
+                total = TeamSum<LANES>(part);
+                total = total == 0.0f ? 0.0f : 1.0f / total;
+                const float s = at < 0 || x == -INFINITY ? 0.0f : expf(x - top) * total;
+                spread = TeamSum<LANES>(u * s);
                 value = s * (u - spread);
             }
         } else {
-            const float s = at < 0 ? 0.0f : 1.0f / (1.0f + expf(-x));
+            const float s = at < 0 ? 0.0f : Sigmoid(x);
             float v = u;
             if (p.renormalize) {
-                const float sum = WarpSum(s);
+                const float sum = TeamSum<LANES>(s);
                 const float w = sum == 0.0f ? 0.0f : s / sum;
-                v = sum == 0.0f ? 0.0f : (u - WarpSum(u * w)) / sum;
+                v = sum == 0.0f ? 0.0f : (u - TeamSum<LANES>(u * w)) / sum;
             }
             value = v * s * (1.0f - s);
         }
@@ -600,25 +763,25 @@ __global__ void __launch_bounds__(kWarps * 32) TopkBackwardKernel(RouteParams p,
         if (wide) {
 #pragma unroll
             for (int j = 0; j < VPL; j += VEC) {
-                if (lane * VPL + j < p.experts) {
+                if (real && member * VPL + j < p.experts) {
                     float f[VEC];
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
-                        f[i] = dense && l[j + i] != -INFINITY ? -expf(l[j + i] - top) / total * spread : 0.0f;
+                        f[i] = dense ? -l[j + i] * total * spread : 0.0f;
                     }
-                    *reinterpret_cast<Pack<T, VEC>*>(out + lane * VPL + j) = Repack<T, float, VEC>(f);
+                    *reinterpret_cast<Pack<T, VEC>*>(out + member * VPL + j) = Repack<T, float, VEC>(f);
                 }
             }
         } else {
 #pragma unroll
             for (int j = 0; j < VPL; ++j) {
-                if (lane * VPL + j < p.experts) {
-                    out[lane * VPL + j] = Narrow<T, float>(dense && l[j] != -INFINITY ? -expf(l[j] - top) / total * spread : 0.0f);
+                if (real && member * VPL + j < p.experts) {
+                    out[member * VPL + j] = Narrow<T, float>(dense ? -l[j] * total * spread : 0.0f);
                 }
             }
         }
         __syncwarp();
-        if (at >= 0) {
+        if (real && at >= 0) {
             out[at] = Narrow<T, float>(value);
         }
     }
@@ -820,7 +983,10 @@ RouteParams ParamsOf(const OpsgnnRouteDesc& d)
     return p;
 }
 
-int Grid(int64_t rows) { return static_cast<int>(std::min<int64_t>(CeilDiv(rows, kWarps), static_cast<int64_t>(SmCount()) * 16)); }
+int Grid(int64_t rows, int per_warp)
+{
+    return static_cast<int>(std::min<int64_t>(CeilDiv(rows, kWarps * per_warp), static_cast<int64_t>(SmCount()) * 16));
+}
 
 // Whole vectors: a lane's VPL values start on a vector boundary in every row.
 template <class T, int VPL> bool Wide(int64_t experts, const void* a, const void* b)
@@ -834,14 +1000,21 @@ int RunTopk(const OpsgnnRouteDesc& d, const void* logits, const float* bias, voi
 {
     const RouteParams p = ParamsOf(d);
     const bool biased = bias != nullptr || (d.groups > 1 && d.group_top == 2);
-    const bool wide = Wide<T, VPL>(d.experts, logits, logits);
-    const size_t shared = d.groups > 1 ? static_cast<size_t>(kWarps) * d.experts * (biased ? 8 : 4) : 0;
     const T* in = static_cast<const T*>(logits);
     T* out = static_cast<T*>(weight);
+    if constexpr (sizeof(T) == 2 && VPL <= 8) {
+        if (!biased && d.groups == 1 && d.k <= kList) {
+            constexpr int TEAM = VPL >= 2 ? 4 * VPL : 8;  // eight lanes hold what 32 do
+            TopkTeamKernel<T, TEAM><<<Grid(d.rows, 4), kWarps * 32, 0, stream>>>(p, in, out, index, Wide<T, TEAM>(d.experts, in, in));
+            return LaunchStatus();
+        }
+    }
+    const bool wide = Wide<T, VPL>(d.experts, logits, logits);
+    const size_t shared = d.groups > 1 ? static_cast<size_t>(kWarps) * d.experts * (biased ? 8 : 4) : 0;
     if (biased) {
-        TopkKernel<T, VPL, true><<<Grid(d.rows), kWarps * 32, shared, stream>>>(p, in, bias, out, index, wide);
+        TopkKernel<T, VPL, true><<<Grid(d.rows, 1), kWarps * 32, shared, stream>>>(p, in, bias, out, index, wide);
     } else {
-        TopkKernel<T, VPL, false><<<Grid(d.rows), kWarps * 32, shared, stream>>>(p, in, bias, out, index, wide);
+        TopkKernel<T, VPL, false><<<Grid(d.rows, 1), kWarps * 32, shared, stream>>>(p, in, bias, out, index, wide);
     }
     return LaunchStatus();
 }
@@ -850,14 +1023,22 @@ template <class T, int VPL>
 int RunTopkBackward(const OpsgnnRouteDesc& d, const void* logits, const int64_t* index, const void* grad, void* grad_logits,
                     cudaStream_t stream)
 {
-    const bool wide = Wide<T, VPL>(d.experts, logits, grad_logits);
-    TopkBackwardKernel<T, VPL><<<Grid(d.rows), kWarps * 32, 0, stream>>>(ParamsOf(d), static_cast<const T*>(logits), index,
-                                                                        static_cast<const T*>(grad), static_cast<T*>(grad_logits),
-                                                                        wide);
+    const T* in = static_cast<const T*>(logits);
+    const T* g = static_cast<const T*>(grad);
+    T* out = static_cast<T*>(grad_logits);
+    if constexpr (VPL <= 8) {
+        if (d.k <= 8) {
+            TopkBackwardKernel<T, 4 * VPL, 8><<<Grid(d.rows, 4), kWarps * 32, 0, stream>>>(ParamsOf(d), in, index, g, out,
+                                                                                           Wide<T, 4 * VPL>(d.experts, in, out));
+            return LaunchStatus();
+        }
+    }
+    TopkBackwardKernel<T, VPL, 32><<<Grid(d.rows, 1), kWarps * 32, 0, stream>>>(ParamsOf(d), in, index, g, out,
+                                                                              Wide<T, VPL>(d.experts, in, out));
     return LaunchStatus();
 }
 
-// f(type tag, integral constant VPL): experts a lane holds, a power of two.
+// f(type tag, integral constant VPL): experts a lane of a warp holds, a power of two.
 template <class F> int Dispatch(const OpsgnnRouteDesc& d, F&& f)
 {
     auto by_width = [&](auto tag) {
