@@ -218,47 +218,48 @@ __device__ __forceinline__ void CloseGroups(const RouteParams& p, uint32_t (&key
     }
 }
 
-// The choice with scores in 64 bits, for rows whose fp32 scores are too close to tell.  Lane i < k gets the i-th choice.
-template <int VPL>
-__device__ __noinline__ void ChooseFine(const RouteParams& p, const float (&l)[VPL], const float* bias, float base, uint64_t* row_keys,
-                                        int lane, int& chosen, float& chosen_logit)
+// One score in 64 bits; `inverse`: 1 / the softmax's sum.
+__device__ __forceinline__ double FineScore(const RouteParams& p, float l, float base, double inverse)
 {
-    uint64_t key[VPL];
-    double total = 1.0;
+    const double x = static_cast<double>(l);
+    return p.softmax ? exp(x - static_cast<double>(base)) * inverse : 1.0 / (1.0 + exp(-x));
+}
+
+// The choice with scores in 64 bits, for rows whose fp32 scores are too close to tell.  Lane i < k gets the i-th choice.  The
+// keys live in shared memory (experts keys per warp), so that nothing of this weighs on the registers of the common path.
+template <class T>
+__device__ __noinline__ void ChooseFine(const RouteParams& p, const T* row, const float* bias, float base, uint64_t* keys, int& chosen)
+{
+    const int lane = threadIdx.x & 31;
+    double inverse = 1.0;
     if (p.softmax) {
         double part = 0.0;
-#pragma unroll 1
-        for (int j = 0; j < VPL; ++j) {
-            part += l[j] != -INFINITY ? exp(static_cast<double>(l[j]) - static_cast<double>(base)) : 0.0;
+#pragma unroll 4
+        for (int at = lane; at < p.experts; at += 32) {
+            const float l = Widen<float, T>(LoadNc(row + at));
+            part += l != -INFINITY ? exp(static_cast<double>(l) - static_cast<double>(base)) : 0.0;
         }
-        total = WarpSum(part);
+        inverse = 1.0 / WarpSum(part);
     }
-#pragma unroll 1
-    for (int j = 0; j < VPL; ++j) {
-        const int at = lane * VPL + j;
-        const double x = static_cast<double>(l[j]);
-        double v = p.softmax ? exp(x - static_cast<double>(base)) / total : 1.0 / (1.0 + exp(-x));
-        if (bias != nullptr && at < p.experts) {
+    __syncwarp();
+#pragma unroll 4
+    for (int at = lane; at < p.experts; at += 32) {
+        const float l = Widen<float, T>(LoadNc(row + at));
+        double v = FineScore(p, l, base, inverse);
+        if (bias != nullptr) {
             v += static_cast<double>(__ldg(bias + at));
         }
-        v = l[j] == -INFINITY ? -static_cast<double>(INFINITY) : v;
-        key[j] = at < p.experts ? KeyOf(v) : 0;
+        keys[at] = KeyOf(l == -INFINITY ? -static_cast<double>(INFINITY) : v);
     }
+    __syncwarp();
     if (p.groups > 1) {
         const int size = p.experts / p.groups;
-        __syncwarp();
-#pragma unroll 1
-        for (int j = 0; j < VPL; ++j) {
-            if (lane * VPL + j < p.experts) {
-                row_keys[lane * VPL + j] = key[j];
-            }
-        }
-        __syncwarp();
         uint64_t mine = 0;
         if (lane < p.groups) {
             uint64_t first = 0, second = 0;
+#pragma unroll 4
             for (int i = 0; i < size; ++i) {
-                const uint64_t v = row_keys[lane * size + i];
+                const uint64_t v = keys[lane * size + i];
                 second = v > first ? first : (v > second ? v : second);
                 first = v > first ? v : first;
             }
@@ -276,33 +277,30 @@ __device__ __noinline__ void ChooseFine(const RouteParams& p, const float (&l)[V
             ahead += (other > mine || (other == mine && g < lane)) ? 1 : 0;
         }
         const unsigned open = __ballot_sync(kFull, lane < p.groups && ahead < p.kept_groups);
-#pragma unroll 1
-        for (int j = 0; j < VPL; ++j) {
-            const int at = lane * VPL + j;
-            if (at < p.experts && !((open >> (at / size)) & 1u)) {
-                key[j] = 0;
+        __syncwarp();
+        for (int at = lane; at < p.experts; at += 32) {
+            if (!((open >> (at / size)) & 1u)) {
+                keys[at] = 0;
             }
         }
+        __syncwarp();
     }
     for (int i = 0; i < p.k; ++i) {
         uint64_t best = 0;
         int where = 0;
-#pragma unroll 1
-        for (int j = 0; j < VPL; ++j) {
-            where = key[j] > best ? j : where;
-            best = key[j] > best ? key[j] : best;
+#pragma unroll 4
+        for (int at = lane; at < p.experts; at += 32) {
+            const uint64_t v = keys[at];
+            where = v > best ? at : where;
+            best = v > best ? v : best;
         }
         const uint64_t winner = WarpMax(best);
-        const int owner = __ffs(__ballot_sync(kFull, best == winner)) - 1;
-        const int at = __shfl_sync(kFull, lane * VPL + where, owner);
-        const float value = __shfl_sync(kFull, l[where], owner);
-        if (lane == owner) {
-            key[where] = 0;
+        const int at = static_cast<int>(__reduce_min_sync(kFull, best == winner ? static_cast<uint32_t>(where) : 0xffffffffu));
+        if ((at & 31) == lane) {
+            keys[at] = 0;
         }
-        if (lane == i) {
-            chosen = at;
-            chosen_logit = value;
-        }
+        chosen = lane == i ? at : chosen;
+        __syncwarp();
     }
 }
 
@@ -311,9 +309,10 @@ __device__ __noinline__ void ChooseFine(const RouteParams& p, const float (&l)[V
 // Logits of 16 bits and their expert's number fit one 32-bit key, all keys differ, and each step of the choice is one warp
 // maximum (redux) and a pop from the winning lane's sorted keys.  32-bit keys take a second step to find the winner's lane.
 //
-// BIASED scores are formed in fp32 first.  Each is off by at most 2^-20 of the largest score (exp, a division, a sum) and
-// 2^-24 of itself (the bias); where two neighbours in the order, or a group let in and one left out, are closer than twice
-// that and not equal by their inputs, the row is chosen again in 64 bits: about one row in a hundred at 256 experts.
+// BIASED scores are formed in fp32 first.  A sigmoid is off by at most 2^-22 (exp to 2 ulp at a slope of 1/4, an addition, a
+// division), a softmax by 2^-20 of its largest score, less the error of the sum, which all share; the bias adds 2^-24 of the
+// result.  Where two neighbours in the order, or a group let in and one left out, are closer than twice that and not equal by
+// their inputs, the row is chosen again in 64 bits: about one row in 300 at 256 experts.
 template <class T, int VPL, bool BIASED>
 __global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T* __restrict__ logits, const float* __restrict__ bias,
                                                           T* __restrict__ weight, int64_t* __restrict__ index, bool wide)
@@ -359,13 +358,13 @@ __global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T
                 for (int j = 0; j < VPL; ++j) {
                     c[j] *= inverse;
                 }
-                margin = inverse * 0x1p-18f;
+                margin = inverse * 0x1p-19f;
             } else {
 #pragma unroll
                 for (int j = 0; j < VPL; ++j) {
                     c[j] = Sigmoid(l[j]);
                 }
-                margin = 0x1p-18f;
+                margin = 0x1p-20f;
             }
             float largest = 0.0f;
 #pragma unroll
@@ -515,7 +514,11 @@ __global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T
             }
             if constexpr (BIASED) {
                 if (!sure) {
-                    ChooseFine<VPL>(p, l, bias, bad ? NAN : top, reinterpret_cast<uint64_t*>(row_keys), lane, chosen, chosen_logit);
+                    const T* row = logits + r * p.experts;
+                    ChooseFine<T>(p, row, bias, bad ? NAN : top, reinterpret_cast<uint64_t*>(row_keys), chosen);
+                    if (lane < p.k) {
+                        chosen_logit = Widen<float, T>(LoadNc(row + chosen));
+                    }
                 }
             }
         }
@@ -1010,7 +1013,7 @@ int RunTopk(const OpsgnnRouteDesc& d, const void* logits, const float* bias, voi
         }
     }
     const bool wide = Wide<T, VPL>(d.experts, logits, logits);
-    const size_t shared = d.groups > 1 ? static_cast<size_t>(kWarps) * d.experts * (biased ? 8 : 4) : 0;
+    const size_t shared = biased || d.groups > 1 ? static_cast<size_t>(kWarps) * d.experts * (biased ? 8 : 4) : 0;
     if (biased) {
         TopkKernel<T, VPL, true><<<Grid(d.rows, 1), kWarps * 32, shared, stream>>>(p, in, bias, out, index, wide);
     } else {

@@ -6,6 +6,7 @@
 #include <c10/cuda/CUDAException.h>
 #include <c10/util/intrusive_ptr.h>
 #include <cuda_runtime_api.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <atomic>
 #include <list>
@@ -82,6 +83,21 @@ PlannerScope::~PlannerScope()
 {
     --t_planner_depth;
     t_observable = could_observe_;
+}
+
+std::vector<at::Tensor> OnceDifferentiable(std::vector<at::Tensor> grads, const char* api)
+{
+    if (!at::GradMode::is_enabled()) {
+        return grads;
+    }
+    torch::autograd::variable_list marked;
+    for (const auto& grad : grads) {
+        marked.push_back(grad.defined() ? grad.detach().requires_grad_(true) : grad);
+    }
+    auto error = std::make_shared<torch::autograd::DelayedError>(std::string(api) + ": second derivatives are not built",
+                                                                 static_cast<int64_t>(marked.size()));
+    auto tied = (*error)(std::move(marked));
+    return {tied.begin(), tied.end()};
 }
 
 std::optional<TensorKey> TensorKey::Of(const at::Tensor& t)

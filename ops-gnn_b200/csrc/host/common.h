@@ -116,6 +116,10 @@ private:
     bool could_observe_;
 };
 
+// First-order gradients only: what a backward pass returns while another differentiation is being recorded
+// (create_graph = true) is tied to a node that raises when somebody differentiates through it.
+std::vector<at::Tensor> OnceDifferentiable(std::vector<at::Tensor> grads, const char* api);
+
 // Wraps a planner for binding: the whole call runs inside a PlannerScope.
 template <class R, class... A> auto Scoped(R (*fn)(A...))
 {

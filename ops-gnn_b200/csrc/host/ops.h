@@ -82,12 +82,15 @@ at::Tensor scatter_logsumexp_backward(const at::Tensor& src, const at::Tensor& o
                                       const at::Tensor& index, int64_t dim, int64_t dim_size);
 
 // routed experts (route.cpp, segment_matmul.cpp)
+std::tuple<at::Tensor, at::Tensor> topk_route(const at::Tensor& logits, const std::optional<at::Tensor>& bias, int64_t k, int64_t score,
+                                              int64_t groups, int64_t kept_groups, int64_t group_top, bool renormalize, double scale);
 std::tuple<at::Tensor, at::Tensor> topk_route_forward(const at::Tensor& logits, const std::optional<at::Tensor>& bias, int64_t k,
                                                       int64_t score, int64_t groups, int64_t kept_groups, int64_t group_top,
                                                       bool renormalize, double scale);
 at::Tensor topk_route_backward(const at::Tensor& logits, const at::Tensor& index, const at::Tensor& grad_weight, int64_t score,
                                bool renormalize, double scale);
 std::tuple<at::Tensor, at::Tensor, at::Tensor> route_csr(const at::Tensor& index, int64_t experts);
+at::Tensor segment_matmul(const at::Tensor& src, const at::Tensor& indptr, const at::Tensor& weight);
 at::Tensor segment_matmul_forward(const at::Tensor& src, const at::Tensor& indptr, const at::Tensor& weight);
 at::Tensor segment_matmul_weight_grad(const at::Tensor& src, const at::Tensor& indptr, const at::Tensor& grad);
 at::Tensor segment_matmul_fp8(const at::Tensor& src, const at::Tensor& src_scale, const at::Tensor& weight,

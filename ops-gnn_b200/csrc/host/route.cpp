@@ -64,6 +64,51 @@ at::Tensor topk_route_backward(const at::Tensor& logits, const at::Tensor& index
     return grad_logits;
 }
 
+namespace {
+
+// The autograd node lives in C++: a router's pass is a few microseconds of GPU time, which a Python node would exceed.
+class TopkRoute : public torch::autograd::Function<TopkRoute> {
+public:
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits,
+                                                  const std::optional<at::Tensor>& bias, int64_t k, int64_t score, int64_t groups,
+                                                  int64_t kept_groups, int64_t group_top, bool renormalize, double scale)
+    {
+        auto [weight, index] = topk_route_forward(logits, bias, k, score, groups, kept_groups, group_top, renormalize, scale);
+        ctx->save_for_backward({logits, index});
+        ctx->saved_data["score"] = score;
+        ctx->saved_data["renormalize"] = renormalize;
+        ctx->saved_data["scale"] = scale;
+        ctx->mark_non_differentiable({index});
+        ctx->set_materialize_grads(false);
+        return {weight, index};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads)
+    {
+        torch::autograd::variable_list out(9);
+        if (grads[0].defined()) {
+            PlannerScope scope;
+            const auto saved = ctx->get_saved_variables();
+            const at::Tensor grad = topk_route_backward(saved[0].detach(), saved[1], grads[0].detach().contiguous(),
+                                                        ctx->saved_data["score"].toInt(), ctx->saved_data["renormalize"].toBool(),
+                                                        ctx->saved_data["scale"].toDouble());
+            out[0] = OnceDifferentiable({grad}, "topk_route")[0];
+        }
+        return out;
+    }
+};
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor> topk_route(const at::Tensor& logits, const std::optional<at::Tensor>& bias, int64_t k, int64_t score,
+                                              int64_t groups, int64_t kept_groups, int64_t group_top, bool renormalize, double scale)
+{
+    if (logits.requires_grad() && at::GradMode::is_enabled()) {
+        const auto out = TopkRoute::apply(logits, bias, k, score, groups, kept_groups, group_top, renormalize, scale);
+        return {out[0], out[1]};
+    }
+    return topk_route_forward(logits, bias, k, score, groups, kept_groups, group_top, renormalize, scale);
+}
+
 std::tuple<at::Tensor, at::Tensor, at::Tensor> route_csr(const at::Tensor& index, int64_t experts)
 {
     const char* api = "route_csr";
@@ -94,6 +139,9 @@ namespace py = pybind11;
 
 void BindRoute(py::module_& m)
 {
+    m.def("topk_route", opsgnn::Scoped(&opsgnn::topk_route), py::arg("logits"), py::arg("bias"), py::arg("k"), py::arg("score"),
+          py::arg("groups"), py::arg("kept_groups"), py::arg("group_top"), py::arg("renormalize"), py::arg("scale"),
+          "topk_route_forward with its gradient; not part of the reference binding", py::call_guard<py::gil_scoped_release>());
     m.def("topk_route_forward", opsgnn::Scoped(&opsgnn::topk_route_forward), py::arg("logits"), py::arg("bias"), py::arg("k"),
           py::arg("score"), py::arg("groups"), py::arg("kept_groups"), py::arg("group_top"), py::arg("renormalize"), py::arg("scale"),
           "The k best experts of each row and their weights; not part of the reference binding",

@@ -111,6 +111,46 @@ at::Tensor segment_matmul_weight_grad(const at::Tensor& src, const at::Tensor& i
     return out;
 }
 
+namespace {
+
+class SegmentMatmul : public torch::autograd::Function<SegmentMatmul> {
+public:
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& src, const at::Tensor& indptr,
+                              const at::Tensor& weight)
+    {
+        ctx->save_for_backward({src, indptr, weight});
+        return segment_matmul_forward(src, indptr, weight);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads)
+    {
+        PlannerScope scope;
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor src = saved[0].detach(), indptr = saved[1], weight = saved[2].detach(), grad = grads[0].detach();
+        at::Tensor grad_src, grad_weight;
+        if (ctx->needs_input_grad(0)) {
+            grad_src = segment_matmul_forward(grad, indptr, weight.transpose(1, 2));
+        }
+        if (ctx->needs_input_grad(2)) {
+            // in the layout of the weight
+            grad_weight = weight.stride(1) == 1 && weight.stride(2) != 1
+                              ? segment_matmul_weight_grad(grad, indptr, src).transpose(1, 2)
+                              : segment_matmul_weight_grad(src, indptr, grad);
+        }
+        auto out = OnceDifferentiable({grad_src, grad_weight}, "segment_matmul");
+        return {out[0], at::Tensor(), out[1]};
+    }
+};
+
+}  // namespace
+
+at::Tensor segment_matmul(const at::Tensor& src, const at::Tensor& indptr, const at::Tensor& weight)
+{
+    if (at::GradMode::is_enabled() && (src.requires_grad() || weight.requires_grad())) {
+        return SegmentMatmul::apply(src, indptr, weight);
+    }
+    return segment_matmul_forward(src, indptr, weight);
+}
+
 at::Tensor segment_matmul_fp8(const at::Tensor& src, const at::Tensor& src_scale, const at::Tensor& weight,
                               const at::Tensor& weight_scale, const std::optional<at::Tensor>& indptr, at::ScalarType out_type)
 {
@@ -173,6 +213,8 @@ namespace py = pybind11;
 
 void BindSegmentMatmul(py::module_& m)
 {
+    m.def("segment_matmul", opsgnn::Scoped(&opsgnn::segment_matmul), py::arg("src"), py::arg("indptr"), py::arg("weight"),
+          "segment_matmul_forward with both gradients; not part of the reference binding", py::call_guard<py::gil_scoped_release>());
     m.def("segment_matmul_forward", opsgnn::Scoped(&opsgnn::segment_matmul_forward), py::arg("src"), py::arg("indptr"),
           py::arg("weight"), "out[r] = src[r] @ weight[segment of r]; not part of the reference binding",
           py::call_guard<py::gil_scoped_release>());

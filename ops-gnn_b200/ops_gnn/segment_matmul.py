@@ -8,27 +8,6 @@ _SUPPORTED_DTYPES = (torch.float16, torch.float32, torch.bfloat16)
 _SUPPORTED_PTR_DTYPES = (torch.int32, torch.int64)
 
 
-class _SegmentMatmul(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, src, indptr, weight):
-        ctx.save_for_backward(src, indptr, weight)
-        return _pybind.segment_matmul_forward(src, indptr, weight)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        src, indptr, weight = ctx.saved_tensors
-        grad_src = grad_weight = None
-        if ctx.needs_input_grad[0]:
-            grad_src = _pybind.segment_matmul_forward(grad, indptr, weight.transpose(1, 2))
-        if ctx.needs_input_grad[2]:
-            if weight.stride(1) == 1 and weight.stride(2) != 1:  # the gradient in the layout of the weight
-                grad_weight = _pybind.segment_matmul_weight_grad(grad, indptr, src).transpose(1, 2)
-            else:
-                grad_weight = _pybind.segment_matmul_weight_grad(src, indptr, grad)
-        return grad_src, None, grad_weight
-
-
 def check_segments(src: torch.Tensor, indptr: torch.Tensor, segments: int) -> torch.Tensor:
     if not isinstance(indptr, torch.Tensor):
         raise TypeError(f"indptr must be a torch.Tensor, got {type(indptr).__name__}")
@@ -76,6 +55,4 @@ def segment_matmul(src: torch.Tensor, indptr: torch.Tensor, weight: torch.Tensor
     indptr = check_segments(src, indptr, weight.size(0))
     if src.device.type != "cuda":
         raise RuntimeError("segment_matmul requires CUDA tensors")
-    if torch.is_grad_enabled() and (src.requires_grad or weight.requires_grad):
-        return _SegmentMatmul.apply(src, indptr, weight)
-    return _pybind.segment_matmul_forward(src, indptr, weight)
+    return _pybind.segment_matmul(src, indptr, weight)

@@ -18,25 +18,6 @@ def _check_int(name: str, value, low: int, high: int) -> None:
         raise ValueError(f"{name} must be in [{low}, {high}], got {value}")
 
 
-class _TopkRoute(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, bias, k, score, groups, kept_groups, group_top, renormalize, scale):
-        weight, index = _pybind.topk_route_forward(logits, bias, k, score, groups, kept_groups, group_top, renormalize, scale)
-        ctx.save_for_backward(logits, index)
-        ctx.rule = (score, renormalize, scale)
-        ctx.mark_non_differentiable(index)
-        ctx.set_materialize_grads(False)
-        return weight, index
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_weight, _):
-        logits, index = ctx.saved_tensors
-        if grad_weight is None:
-            return (None,) * 9
-        return (_pybind.topk_route_backward(logits, index, grad_weight.contiguous(), *ctx.rule),) + (None,) * 8
-
-
 def topk_route(logits: torch.Tensor, k: int, score: str = "softmax", bias: Optional[torch.Tensor] = None, groups: int = 1,
                kept_groups: Optional[int] = None, group_top: int = 2, renormalize: bool = True,
                scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -93,11 +74,8 @@ def topk_route(logits: torch.Tensor, k: int, score: str = "softmax", bias: Optio
     if logits.device.type != "cuda":
         raise RuntimeError("topk_route requires CUDA tensors")
     rows = logits if logits.dim() == 2 else logits.reshape(-1, experts)
-    args = (rows.contiguous(), bias, k, _SCORES[score], groups, kept_groups, group_top, bool(renormalize), float(scale))
-    if logits.requires_grad and torch.is_grad_enabled():
-        weight, index = _TopkRoute.apply(*args)
-    else:
-        weight, index = _pybind.topk_route_forward(*args)
+    weight, index = _pybind.topk_route(rows.contiguous(), bias, k, _SCORES[score], groups, kept_groups, group_top, bool(renormalize),
+                                       float(scale))
     if logits.dim() == 2:
         return weight, index
     shape = logits.shape[:-1] + (k,)
