@@ -466,8 +466,7 @@ typedef struct OpsgnnSegmentMatmulDesc {
     int32_t out_type;              /* = in_type; fp8: F32 / F16 / BF16                      */
 } OpsgnnSegmentMatmulDesc;
 
-/* Bytes of scratch (16-byte aligned) of opsgnn_segment_matmul (weight_grad 0) or opsgnn_segment_matmul_weight_grad (1); 0 for
- * 16-bit types. */
+/* Bytes of scratch (16-byte aligned) of opsgnn_segment_matmul (weight_grad 0) or opsgnn_segment_matmul_weight_grad (1). */
 OPSGNN_API int opsgnn_segment_matmul_workspace_bytes(const OpsgnnSegmentMatmulDesc* desc, int weight_grad, int64_t* bytes);
 /* out[r, :] = src[r, :] @ weight[e] for the rows of segment e; 0 in rows of no segment.  out is contiguous. */
 OPSGNN_API int opsgnn_segment_matmul(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src, const void* weight,

@@ -56,8 +56,11 @@ extern "C" int opsgnn_segment_matmul_workspace_bytes(const OpsgnnSegmentMatmulDe
     }
     *bytes = 0;
     if (segmm::Splits(*desc)) {
-        *bytes = weight_grad ? segmm::OuterSplitBytes(desc->rows, desc->width, desc->out)
+        *bytes = weight_grad ? segmm::OuterSplitBytes(desc->rows, desc->segments, desc->width, desc->out)
                              : segmm::RowsSplitBytes(desc->rows, desc->segments, desc->width, desc->out);
+    } else if (desc->in_type != OPSGNN_F32 && weight_grad && desc->rows > 0 && desc->segments > 0 && desc->width > 0 && desc->out > 0 &&
+               desc->out % 8 == 0) {
+        *bytes = segmm::OuterPartialBytes(desc->rows, desc->segments, desc->width, desc->out);
     }
     return OPSGNN_OK;
 }
@@ -125,7 +128,8 @@ extern "C" int opsgnn_segment_matmul_weight_grad(const OpsgnnSegmentMatmulDesc* 
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !Aligned(workspace, 16))) {
         return OPSGNN_ERR_WORKSPACE;
     }
-    const int ran = need > 0 ? segmm::RunOuterSplit(p, workspace, AsStream(stream)) : segmm::RunOuterTensor(p, AsStream(stream));
+    const int ran = p.type == OPSGNN_F32 ? (need > 0 ? segmm::RunOuterSplit(p, workspace, AsStream(stream)) : OPSGNN_ERR_UNSUPPORTED)
+                                         : segmm::RunOuterTensor(p, workspace, AsStream(stream));
     return ran == OPSGNN_ERR_UNSUPPORTED ? segmm::RunOuterSimple(p, AsStream(stream)) : ran;
 }
 

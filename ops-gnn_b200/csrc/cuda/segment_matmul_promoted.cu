@@ -47,6 +47,8 @@ struct Params {
     const float* b;
     int64_t lda, ldb;                // outer form: ldb = row stride of b
     int64_t b_segment, b_k, b_n;
+    int64_t chunk;     // outer form: rows per partial result; 0: a segment's rows in one piece
+    float* partial;    // [pieces][m][n]
     WaitSettings wait;
 };
 
@@ -125,22 +127,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int64_t across = (p.n + BN - 1) / BN;
     const int64_t down = FORM == kOuter ? (p.m + kRows - 1) / kRows : 0;
     const int64_t outer_tiles = FORM == kOuter ? p.ptr.segments * down * across : 0;
-    SegmentWalk<kRows> walk;
-    if constexpr (FORM != kOuter) {
-        if (warp != 2 && warp != 3) {
-            walk.Start(p.ptr);
-        }
+    SegmentWalk<FORM == kOuter ? 0 : kRows> walk;
+    if (warp != 2 && warp != 3 && (FORM != kOuter || p.chunk > 0)) {
+        walk.Start(p.ptr, FORM == kOuter ? p.chunk : kRows);
     }
     int64_t segment = 0, row = 0, row_end = 0, column = 0, from = 0, depth = 0;
     auto find = [&](int64_t t) {
         column = t % across * BN;
         if constexpr (FORM == kOuter) {
+            row = t / across % down * kRows;
+            row_end = p.m;
+            segment = t / (down * across);  // of the result to write: a segment or a piece
+            if (p.chunk > 0) {
+                if (!walk.Seek(segment)) {
+                    return false;
+                }
+                from = walk.row;
+                depth = walk.row_end - from < p.chunk ? walk.row_end - from : p.chunk;
+                return true;
+            }
             if (t >= outer_tiles) {
                 return false;
             }
-            segment = t / (down * across);
-            row = t / across % down * kRows;
-            row_end = p.m;
             int64_t end;
             p.ptr.Range(segment, from, end);
             depth = end - from;
@@ -275,7 +283,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr int kMine = BN / 2;  // columns of this warp
         const int quarter = warp & 3, side = (warp - 4) >> 2;
         unsigned char* mine = staging + (warp - 4) * (32 * 128);
-        O* out = static_cast<O*>(p.out);
+        // a piece of a segment's sum (outer form in pieces; fp32 then) goes to `partial`
+        O* out = FORM == kOuter && p.chunk > 0 ? reinterpret_cast<O*>(p.partial) : static_cast<O*>(p.out);
         const int64_t scale_blocks = F8 ? (p.k + 127) / 128 : 0, scale_bands = F8 ? (p.n + 127) / 128 : 0;
         uint32_t blocks = 0;
         bool going = true;
@@ -497,7 +506,10 @@ bool OuterSplittable(const OuterProblem& p)
 }  // namespace
 
 int64_t RowsSplitBytes(int64_t rows, int64_t segments, int64_t k, int64_t n) { return PlaneBytes(rows * k) + PlaneBytes(segments * k * n); }
-int64_t OuterSplitBytes(int64_t rows, int64_t k, int64_t n) { return PlaneBytes(rows * k) + PlaneBytes(rows * n); }
+int64_t OuterSplitBytes(int64_t rows, int64_t segments, int64_t k, int64_t n)
+{
+    return PlaneBytes(rows * k) + PlaneBytes(rows * n) + OuterPartialBytes(rows, segments, k, n);
+}
 
 int RunRowsSplit(const RowsProblem& p, void* workspace, cudaStream_t stream)
 {
@@ -551,6 +563,7 @@ int RunOuterSplit(const OuterProblem& p, void* workspace, cudaStream_t stream)
     q.out = p.out;
     q.m = p.k;
     q.n = p.n;
+    q.chunk = OuterChunk(p.ptr.rows, p.ptr.segments, p.k, p.n);
     q.a = static_cast<const float*>(p.a);
     q.b = static_cast<const float*>(p.b);
     q.lda = p.lda;
@@ -558,6 +571,7 @@ int RunOuterSplit(const OuterProblem& p, void* workspace, cudaStream_t stream)
     OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
     char* planes_a = static_cast<char*>(workspace);
     char* planes_b = planes_a + PlaneBytes(p.ptr.rows * p.k);
+    q.partial = reinterpret_cast<float*>(planes_b + PlaneBytes(p.ptr.rows * p.n));
     CUtensorMap a, b;
     if (!Map3(&a, false, planes_a, p.k, p.ptr.rows, 3, p.k, p.ptr.rows * p.k, 64) ||
         !Map3(&b, false, planes_b, p.n, p.ptr.rows, 3, p.n, p.ptr.rows * p.n, 64)) {
@@ -570,9 +584,10 @@ int RunOuterSplit(const OuterProblem& p, void* workspace, cudaStream_t stream)
     if (status != OPSGNN_OK) {
         return status;
     }
-    const int64_t down = p.ptr.segments * CeilDiv(p.k, kRows);
-    return p.n <= 128 ? Launch<false, float, 128, kOuter>(a, b, q, down, stream)
-                      : Launch<false, float, 256, kOuter>(a, b, q, down * CeilDiv(p.n, 256), stream);
+    const int64_t down = (q.chunk > 0 ? p.ptr.rows / q.chunk + p.ptr.segments : p.ptr.segments) * CeilDiv(p.k, kRows);
+    status = p.n <= 128 ? Launch<false, float, 128, kOuter>(a, b, q, down, stream)
+                        : Launch<false, float, 256, kOuter>(a, b, q, down * CeilDiv(p.n, 256), stream);
+    return status == OPSGNN_OK && q.chunk > 0 ? JoinPieces(p, q.chunk, q.partial, stream) : status;
 }
 
 int RunRowsFp8(const RowsProblem& p, cudaStream_t stream)

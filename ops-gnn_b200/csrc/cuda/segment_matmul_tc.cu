@@ -64,6 +64,8 @@ struct Params {
     SegmentPointers ptr;
     void* out;
     int64_t m, n, k;   // rows form: n columns, k reduced; outer form: m x n results per segment
+    int64_t chunk;     // outer form: rows per partial result; 0: a segment's rows in one piece
+    float* partial;    // [pieces][m][n]
     WaitSettings wait;
 };
 
@@ -122,23 +124,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int64_t across = (p.n + BN - 1) / BN;
     const int64_t down = FORM == kOuter ? (p.m + kRows - 1) / kRows : 0;
     const int64_t outer_tiles = FORM == kOuter ? p.ptr.segments * down * across : 0;
-    SegmentWalk<kRows> walk;
-    if constexpr (FORM != kOuter) {
-        if (warp != 2 && warp != 3) {
-            walk.Start(p.ptr);
-        }
+    SegmentWalk<FORM == kOuter ? 0 : kRows> walk;
+    if (warp != 2 && warp != 3 && (FORM != kOuter || p.chunk > 0)) {
+        walk.Start(p.ptr, FORM == kOuter ? p.chunk : kRows);
     }
     // Tile t: its segment, first result row and column, and the range of the reduced index.
     int64_t segment = 0, row = 0, row_end = 0, column = 0, from = 0, depth = 0;
     auto find = [&](int64_t t) {
         column = t % across * BN;
         if constexpr (FORM == kOuter) {
+            row = t / across % down * kRows;
+            row_end = p.m;
+            segment = t / (down * across);  // of the result to write: a segment or a piece
+            if (p.chunk > 0) {
+                if (!walk.Seek(segment)) {
+                    return false;
+                }
+                from = walk.row;
+                depth = walk.row_end - from < p.chunk ? walk.row_end - from : p.chunk;
+                return true;
+            }
             if (t >= outer_tiles) {
                 return false;
             }
-            segment = t / (down * across);
-            row = t / across % down * kRows;
-            row_end = p.m;
             int64_t end;
             p.ptr.Range(segment, from, end);
             depth = end - from;
@@ -279,12 +287,37 @@ __global__ void __launch_bounds__(kThreads, 1)
                     break;
                 }
                 uint32_t words[32];
+                const int piece = lane & 7;
                 if (depth > 0) {
                     uint32_t low[32], high[32];
                     const uint32_t at = tmem + half * BN + c + (static_cast<uint32_t>(quarter * 32) << 16);
                     tc::TmemLoad32(at, low);
                     tc::TmemLoad32(at + 32, high);
                     tc::TmemWait();
+                    if (FORM == kOuter && p.chunk > 0) {
+                        // A piece of the sum, kept in fp32: 32 columns are 128 bytes.
+#pragma unroll
+                        for (int side = 0; side < 2; ++side) {
+                            const uint32_t(&v)[32] = side == 0 ? low : high;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                *reinterpret_cast<uint4*>(mine + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+                                    make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                            }
+                            __syncwarp();
+                            const int64_t col = column + c + side * 32 + piece * 4;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int r = i * 4 + (lane >> 3);
+                                const uint4 value = *reinterpret_cast<const uint4*>(mine + r * 128 + ((piece ^ (r & 7)) << 4));
+                                if (first + r < row_end && col < p.n) {
+                                    *reinterpret_cast<uint4*>(p.partial + segment * p.m * p.n + (first + r) * p.n + col) = value;
+                                }
+                            }
+                            __syncwarp();
+                        }
+                        continue;
+                    }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         words[i] = TwoOf<T>(low[2 * i], low[2 * i + 1]);
@@ -304,7 +337,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                         make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
                 }
                 __syncwarp();
-                const int piece = lane & 7;
                 const int64_t col = column + c + piece * 8;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -423,7 +455,84 @@ int RunRowsTensor(const RowsProblem& p, cudaStream_t stream)
     return ByType<0>(p.in_type, narrow, run);
 }
 
-int RunOuterTensor(const OuterProblem& p, cudaStream_t stream)
+namespace {
+
+// out[e][i] <- the sum of the pieces of segment e, in their order.  blockIdx.y: segment.
+template <class T>
+__global__ void __launch_bounds__(256) JoinKernel(SegmentPointers ptr, int64_t chunk, int64_t size, const float* __restrict__ partial,
+                                                  T* __restrict__ out)
+{
+    const int64_t e = blockIdx.y;
+    const int lane = threadIdx.x & 31;
+    int64_t before = 0, begin, end;
+    for (int64_t s = lane; s < e; s += 32) {
+        ptr.Range(s, begin, end);
+        before += (end - begin + chunk - 1) / chunk;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        before += __shfl_xor_sync(0xffffffffu, before, d);
+    }
+    ptr.Range(e, begin, end);
+    const int64_t pieces = (end - begin + chunk - 1) / chunk;
+    const int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 4;
+    if (i >= size) {
+        return;
+    }
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int64_t c = 0; c < pieces; ++c) {
+        const float4 v = __ldcs(reinterpret_cast<const float4*>(partial + (before + c) * size + i));
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
+    }
+    const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+    StorePlain<T, 4>(out + e * size + i, Repack<T, float, 4>(f));
+}
+
+}  // namespace
+
+int64_t OuterChunk(int64_t rows, int64_t segments, int64_t k, int64_t n)
+{
+    // A result tile is one block's sequential sum over a segment's rows.  With fewer tiles than SMs the rows are cut into
+    // pieces, four rounds of tiles over the SMs (typed layer of 13 segments, 200003 x 256 -> 256, bf16: 26 tiles 0.63 ms, in
+    // pieces 0.09 ms); with more, partial results would cost more than they give (32 segments, 2048 x 1024: 8 MB a piece).
+    const int64_t tiles = CeilDiv(k, kRows) * CeilDiv(n, n <= 128 ? 128 : 256);
+    if (tiles * segments >= SmCount()) {
+        return 0;
+    }
+    const int64_t pieces = std::max<int64_t>(1, static_cast<int64_t>(SmCount()) * 4 / tiles);
+    const int64_t chunk = std::max<int64_t>(256, AlignUp(CeilDiv(rows, pieces), kDepth));
+    return chunk >= rows ? 0 : chunk;
+}
+
+int64_t OuterPartialBytes(int64_t rows, int64_t segments, int64_t k, int64_t n)
+{
+    const int64_t chunk = OuterChunk(rows, segments, k, n);
+    return chunk > 0 ? AlignUp((rows / chunk + segments) * k * n * 4, 256) : 0;
+}
+
+int JoinPieces(const OuterProblem& p, int64_t chunk, const float* partial, cudaStream_t stream)
+{
+    const int64_t size = p.k * p.n;
+    const dim3 grid(static_cast<unsigned>(CeilDiv(size, 1024)), static_cast<unsigned>(p.ptr.segments));
+    switch (p.type) {
+        case OPSGNN_F32:
+            JoinKernel<float><<<grid, 256, 0, stream>>>(p.ptr, chunk, size, partial, static_cast<float*>(p.out));
+            break;
+        case OPSGNN_F16:
+            JoinKernel<__half><<<grid, 256, 0, stream>>>(p.ptr, chunk, size, partial, static_cast<__half*>(p.out));
+            break;
+        default:
+            JoinKernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p.ptr, chunk, size, partial, static_cast<__nv_bfloat16*>(p.out));
+            break;
+    }
+    return LaunchStatus();
+}
+
+int RunOuterTensor(const OuterProblem& p, void* workspace, cudaStream_t stream)
 {
     if ((p.type != OPSGNN_BF16 && p.type != OPSGNN_F16) || p.ptr.rows < 1 || p.n % 8 != 0 || !Aligned(p.out, 16) ||
         !Loadable(p.a, p.lda, std::max(p.k, p.ptr.rows)) || !Loadable(p.b, p.ldb, std::max(p.n, p.ptr.rows))) {
@@ -434,6 +543,8 @@ int RunOuterTensor(const OuterProblem& p, cudaStream_t stream)
     q.out = p.out;
     q.m = p.k;
     q.n = p.n;
+    q.chunk = OuterChunk(p.ptr.rows, p.ptr.segments, p.k, p.n);
+    q.partial = static_cast<float*>(workspace);
     OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
     CUtensorMap a, b;
     if (!Map2(&a, p.type, p.a, p.k, p.ptr.rows, p.lda, 64, kDepth) || !Map2(&b, p.type, p.b, p.n, p.ptr.rows, p.ldb, 64, kDepth)) {
@@ -442,9 +553,11 @@ int RunOuterTensor(const OuterProblem& p, cudaStream_t stream)
     auto run = [&](auto tag, auto width) {
         using T = decltype(tag);
         constexpr int BN = decltype(width)::value;
-        return Launch<T, BN, kOuter>(a, b, q, p.ptr.segments * CeilDiv(p.k, kRows) * CeilDiv(p.n, BN), stream);
+        const int64_t results = q.chunk > 0 ? p.ptr.rows / q.chunk + p.ptr.segments : p.ptr.segments;
+        return Launch<T, BN, kOuter>(a, b, q, results * CeilDiv(p.k, kRows) * CeilDiv(p.n, BN), stream);
     };
-    return ByType<0>(p.type, p.n <= 128, run);
+    const int status = ByType<0>(p.type, p.n <= 128, run);
+    return status == OPSGNN_OK && q.chunk > 0 ? JoinPieces(p, q.chunk, q.partial, stream) : status;
 }
 
 }  // namespace segmm

@@ -32,15 +32,21 @@ struct SegmentPointers {
 
 // Row tiles of all segments in order, TILE rows each (a segment's last one may be short; an empty segment has none).
 // Seek(t) is called by a whole warp with ascending t and finds tile t by a running warp scan over 32 segments at a time:
-// no tile table, no workspace, no limit on the number of segments.
+// no tile table, no workspace, no limit on the number of segments.  TILE 0: the number of rows is given to Start.
 template <int TILE> struct SegmentWalk {
     SegmentPointers ptr;
+    int64_t length;              // rows per tile
     int64_t from, base;          // first segment of the 32 at hand; tiles before them
     int64_t begin, end;          // this lane's segment
     int64_t inclusive;           // tiles of the 32 up to and with this lane's segment
     // what Seek found
     int64_t segment, row, row_end;
 
+    __device__ __forceinline__ int64_t Tiles() const
+    {
+        const int64_t tile = TILE > 0 ? TILE : length;
+        return (end - begin + tile - 1) / tile;
+    }
     __device__ __forceinline__ void Load()
     {
         const int lane = threadIdx.x & 31;
@@ -48,16 +54,17 @@ template <int TILE> struct SegmentWalk {
         if (from + lane < ptr.segments) {
             ptr.Range(from + lane, begin, end);
         }
-        inclusive = (end - begin + TILE - 1) / TILE;
+        inclusive = Tiles();
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int64_t up = __shfl_up_sync(0xffffffffu, inclusive, d);
             inclusive += lane >= d ? up : 0;
         }
     }
-    __device__ __forceinline__ void Start(const SegmentPointers& p)
+    __device__ __forceinline__ void Start(const SegmentPointers& p, int64_t tile = TILE)
     {
         ptr = p;
+        length = tile;
         from = 0;
         base = 0;
         Load();
@@ -69,10 +76,9 @@ template <int TILE> struct SegmentWalk {
             const unsigned there = __ballot_sync(0xffffffffu, t < base + inclusive);
             if (there != 0) {
                 const int owner = __ffs(there) - 1;
-                const int64_t tiles = (end - begin + TILE - 1) / TILE;
-                const int64_t first = __shfl_sync(0xffffffffu, base + inclusive - tiles, owner);
+                const int64_t first = __shfl_sync(0xffffffffu, base + inclusive - Tiles(), owner);
                 row_end = __shfl_sync(0xffffffffu, end, owner);
-                row = __shfl_sync(0xffffffffu, begin, owner) + (t - first) * TILE;
+                row = __shfl_sync(0xffffffffu, begin, owner) + (t - first) * (TILE > 0 ? TILE : length);
                 segment = from + owner;
                 return true;
             }

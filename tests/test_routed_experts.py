@@ -992,3 +992,19 @@ def test_layer_in_a_graph_and_on_another_stream(cuda_device):
         want = run(*fresh)
         assert all(torch.equal(a, b) for a, b in zip(captured, want)), seed
     del graph
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", KINDS, ids=str)
+@pytest.mark.parametrize("lengths,k,n", [([5000, 0, 70, 1, 3000], 64, 40), ([20000], 8, 136), ([0, 900, 0], 264, 264), ([256, 320, 64], 16, 16)])
+def test_segment_matmul_long_sums_in_pieces(cuda_device, dtype, lengths, k, n):
+    """Few results and many rows: the weight gradient is summed in pieces of rows and joined, in a fixed order."""
+    from ops_gnn import segment_matmul
+
+    src, ptr, weight, grad = _matmul_inputs((lengths, 3, 9, k, n), dtype, 61)
+    w = weight.to(cuda_device).requires_grad_()
+    args = src.to(cuda_device), ptr.to(cuda_device)
+    first, = torch.autograd.grad(segment_matmul(*args, w), w, grad.to(cuda_device))
+    again, = torch.autograd.grad(segment_matmul(*args, w), w, grad.to(cuda_device))
+    assert torch.equal(first, again)
+    _within(first, _plain_weight_grad(src, ptr, grad), _plain_weight_grad(src.abs(), ptr, grad.abs()), max(lengths) + 2, "grad_weight")
