@@ -56,125 +56,213 @@ template <class T, int VEC> __device__ __forceinline__ void StoreBytes(uint8_t* 
     }
 }
 
-// One scale per row and 128 columns.  Lanes x VEC = 128: a block is one 16-byte (VEC = 16 / sizeof(T)) vector per lane of a
-// half warp (16-bit types) or a warp (fp32); the scalar form takes any width and alignment.
-template <class T, int VEC>
-__global__ void __launch_bounds__(256) RowKernel(const T* __restrict__ src, int64_t rows, int64_t width, uint8_t* __restrict__ values,
-                                                 float* __restrict__ scales)
+// 16 bytes that are read once.
+template <class T, int VEC> __device__ __forceinline__ Pack<T, VEC> LoadStream16(const T* p)
 {
-    constexpr int PER = VEC == 1 ? 4 : 1;             // strided elements a lane takes in the scalar form
-    constexpr int LANES = VEC == 1 ? 32 : kBlock / VEC;
-    constexpr int GROUPS = 256 / LANES;
-    const int lane = threadIdx.x % LANES;
-    const int64_t across = (width + kBlock - 1) / kBlock;
-    const int64_t blocks = rows * across;
-    // All lanes of a warp stay in the loop together: the shuffles below name the whole warp.
-    const int64_t steps = (blocks + static_cast<int64_t>(gridDim.x) * GROUPS - 1) / (static_cast<int64_t>(gridDim.x) * GROUPS);
-    for (int64_t s = 0; s < steps; ++s) {
-        const int64_t b = (s * gridDim.x + blockIdx.x) * GROUPS + threadIdx.x / LANES;
-        const bool real = b < blocks;
-        const int64_t row = real ? b / across : 0, block = real ? b % across : 0;
-        const int64_t first = row * width + block * kBlock;
-        const int left = static_cast<int>(width - block * kBlock < kBlock ? width - block * kBlock : kBlock);
-        float v[VEC * PER];
+    static_assert(sizeof(T) * VEC == 16, "one vector");
+    const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(p));
+    Pack<T, VEC> out;
+    memcpy(&out, &raw, 16);
+    return out;
+}
+
+// Largest magnitude of a 16-byte vector; NaN has no part.  An infinity shows as +inf.
+template <class T, int VEC> __device__ __forceinline__ float TopOf(const Pack<T, VEC>& p)
+{
+    if constexpr (std::is_same<T, float>::value) {
         float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < VEC * PER; ++i) {
-            v[i] = 0.0f;
+        for (int i = 0; i < VEC; ++i) {
+            top = fmaxf(top, fabsf(p.v[i]));
         }
-        if constexpr (VEC == 1) {
+        return top;
+    } else {
+        using Two = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        Two pair[VEC / 2];
+        memcpy(pair, &p, sizeof(pair));
+        Two top = __habs2(pair[0]);
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                if (real && i * LANES + lane < left) {
-                    v[i] = Widen<float, T>(LoadNc(src + first + i * LANES + lane));
-                }
+        for (int i = 1; i < VEC / 2; ++i) {
+            top = __hmax2(top, __habs2(pair[i]));  // of a number and a NaN, the number
+        }
+        return fmaxf(fmaxf(Widen<float, T>(top.x), Widen<float, T>(top.y)), 0.0f);
+    }
+}
+template <class T, int VEC> __device__ __forceinline__ float FiniteTopOf(const Pack<T, VEC>& p)
+{
+    float v[VEC], top = 0.0f;
+    Unpack<float, T, VEC>(p, v);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        top = fmaxf(top, FiniteAbs(v[i]));
+    }
+    return top;
+}
+template <int LANES> __device__ __forceinline__ float GroupMax(float top)
+{
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
+    }
+    return top;
+}
+
+// One scale per row and 128 columns, whole vectors: a block of 128 is one 16-byte vector per lane of a half warp (16-bit
+// types) or a warp (fp32).  Bound by memory: every lane has kAhead vectors in flight (16381 x 4096 bf16: two 33.3 us,
+// four 36.1, eight 37.8).  FULL: the width is a multiple of 128, so the blocks lie one after the other.
+constexpr int kAhead = 2;
+
+template <class T, bool FULL>
+__global__ void __launch_bounds__(256) RowKernel(const T* __restrict__ src, int64_t blocks, int64_t width, int64_t across,
+                                                 uint8_t* __restrict__ values, float* __restrict__ scales)
+{
+    constexpr int VEC = 16 / sizeof(T);
+    constexpr int LANES = kBlock / VEC;
+    constexpr int GROUPS = 256 / LANES;
+    const int lane = threadIdx.x % LANES;
+    // kAhead runs of GROUPS blocks, one after the other in memory; every lane of a warp stays in the loop, as the shuffles name
+    // the whole warp.
+    for (int64_t first = static_cast<int64_t>(blockIdx.x) * (GROUPS * kAhead); first < blocks;
+         first += static_cast<int64_t>(gridDim.x) * (GROUPS * kAhead)) {
+        const int64_t b0 = first + threadIdx.x / LANES;
+        Pack<T, VEC> p[kAhead];
+        int64_t at[FULL ? 1 : kAhead];
+        unsigned mine = 0;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t b = b0 + i * GROUPS;
+            bool here = b < blocks;
+            const T* from;
+            if constexpr (FULL) {
+                from = src + b * kBlock + lane * VEC;
+            } else {
+                const int64_t row = here ? b / across : 0, column = (b - row * across) * kBlock + lane * VEC;
+                at[i] = row * width + column;
+                from = src + at[i];
+                here = here && column < width;
             }
-        } else {
-            if (real && lane * VEC < left) {
-                Unpack<float, T, VEC>(LoadGather<T, VEC>(src + first + lane * VEC), v);
+            mine |= here ? 1u << i : 0u;
+            memset(&p[i], 0, sizeof(p[i]));
+            if (here) {
+                p[i] = LoadStream16<T, VEC>(from);
             }
         }
 #pragma unroll
-        for (int i = 0; i < VEC * PER; ++i) {
-            top = fmaxf(top, FiniteAbs(v[i]));
-        }
-#pragma unroll
-        for (int d = LANES / 2; d > 0; d >>= 1) {
-            top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
-        }
-        float scale, inverse;
-        ScaleOf(top, scale, inverse);
-        if (real && lane == 0) {
-            scales[b] = scale;
-        }
-        if constexpr (VEC == 1) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                if (real && i * LANES + lane < left) {
-                    const float one[1] = {v[i]};
-                    StoreBytes<T, 1>(values + first + i * LANES + lane, one, inverse);
-                }
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t b = b0 + i * GROUPS;
+            float top = GroupMax<LANES>(TopOf<T, VEC>(p[i]));
+            if (__any_sync(kFull, top == INFINITY)) {
+                top = GroupMax<LANES>(FiniteTopOf<T, VEC>(p[i]));
             }
-        } else {
-            if (real && lane * VEC < left) {
-                StoreBytes<T, VEC>(values + first + lane * VEC, v, inverse);
+            float scale, inverse;
+            ScaleOf(top, scale, inverse);
+            if (lane == 0 && b < blocks) {
+                scales[b] = scale;
+            }
+            if ((mine >> i) & 1u) {
+                float v[VEC];
+                Unpack<float, T, VEC>(p[i], v);
+                StoreBytes<T, VEC>(values + (FULL ? b * kBlock + lane * VEC : at[FULL ? 0 : i]), v, inverse);
             }
         }
     }
 }
 
-// One scale per tile of 128 x 128: a thread block per tile, the tile's values stay in registers between the maximum and the
-// conversion.
-template <class T, int VEC>
-__global__ void __launch_bounds__(512) TileKernel(const T* __restrict__ src, int64_t rows, int64_t width, int64_t down, int64_t across,
-                                                  uint8_t* __restrict__ values, float* __restrict__ scales)
+// The same for any width and alignment, a block of 128 per warp.
+template <class T>
+__global__ void __launch_bounds__(256) RowScalarKernel(const T* __restrict__ src, int64_t blocks, int64_t width, int64_t across,
+                                                       uint8_t* __restrict__ values, float* __restrict__ scales)
 {
-    constexpr int LANES = kBlock / VEC;       // threads along a row of the tile
-    constexpr int STEP = 512 / LANES;         // rows taken at once
-    constexpr int PER = kBlock / STEP;
-    __shared__ float tops[16];
-    const int lane = threadIdx.x % LANES, line = threadIdx.x / LANES;
-    const int64_t tile = blockIdx.x;
-    const int64_t batch = tile / (down * across), row0 = tile / across % down * kBlock, col0 = tile % across * kBlock;
-    const int64_t at = (batch * rows + row0) * width + col0;
-    const int high = static_cast<int>(rows - row0 < kBlock ? rows - row0 : kBlock);
-    const int left = static_cast<int>(width - col0 < kBlock ? width - col0 : kBlock);
-    float v[PER][VEC];
-    float top = 0.0f;
+    constexpr int PER = kBlock / 32;
+    const int lane = threadIdx.x & 31;
+    for (int64_t b = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); b < blocks; b += static_cast<int64_t>(gridDim.x) * 8) {
+        const int64_t row = b / across, column = (b - row * across) * kBlock;
+        const int64_t first = row * width + column;
+        const int left = static_cast<int>(width - column < kBlock ? width - column : kBlock);
+        float v[PER], top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int r = i * STEP + line;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            v[i][j] = 0.0f;
+        for (int i = 0; i < PER; ++i) {
+            v[i] = i * 32 + lane < left ? Widen<float, T>(LoadNc(src + first + i * 32 + lane)) : 0.0f;
+            top = fmaxf(top, FiniteAbs(v[i]));
         }
-        if (r < high && lane * VEC < left) {
-            const T* from = src + at + r * width + lane * VEC;
-            if constexpr (VEC == 1) {
-                v[i][0] = Widen<float, T>(LoadNc(from));
-            } else {
-                Unpack<float, T, VEC>(LoadGather<T, VEC>(from), v[i]);
+        top = GroupMax<32>(top);
+        float scale, inverse;
+        ScaleOf(top, scale, inverse);
+        if (lane == 0) {
+            scales[b] = scale;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (i * 32 + lane < left) {
+                const float one[1] = {v[i]};
+                StoreBytes<T, 1>(values + first + i * 32 + lane, one, inverse);
             }
         }
     }
+}
+
+// One scale per tile of 128 x 128: a thread block per tile, the tile stays in registers (as loaded) between the maximum and
+// the conversion.
+constexpr int kTileThreads = 256;
+
+template <class T, int VEC>
+__global__ void __launch_bounds__(kTileThreads) TileKernel(const T* __restrict__ src, int64_t rows, int64_t width, int down, int across,
+                                                           uint8_t* __restrict__ values, float* __restrict__ scales)
+{
+    constexpr int LANES = kBlock / VEC;         // threads along a row of the tile
+    constexpr int STEP = kTileThreads / LANES;  // rows taken at once
+    constexpr int PER = kBlock / STEP;
+    __shared__ float tops[2][kTileThreads / 32];
+    const int lane = threadIdx.x % LANES, line = threadIdx.x / LANES;
+    const unsigned tile = blockIdx.x;
+    const unsigned band = tile / across;
+    const int64_t batch = band / down, row0 = static_cast<int64_t>(band % down) * kBlock, col0 = static_cast<int64_t>(tile % across) * kBlock;
+    const int64_t at = (batch * rows + row0) * width + col0 + lane * VEC;
+    const int high = static_cast<int>(rows - row0 < kBlock ? rows - row0 : kBlock);
+    const bool inside = lane * VEC < width - col0;
+    Pack<T, VEC> p[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            top = fmaxf(top, FiniteAbs(v[i][j]));
+        const int r = i * STEP + line;
+        memset(&p[i], 0, sizeof(p[i]));
+        if (r < high && inside) {
+            if constexpr (VEC == 1) {
+                p[i].v[0] = LoadNc(src + at + r * width);
+            } else {
+                p[i] = LoadStream16<T, VEC>(src + at + r * width);
+            }
         }
     }
+    float top = 0.0f;
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
+    for (int i = 0; i < PER; ++i) {
+        if constexpr (VEC == 1) {
+            top = fmaxf(top, fabsf(Widen<float, T>(p[i].v[0])));
+        } else {
+            top = fmaxf(top, TopOf<T, VEC>(p[i]));
+        }
     }
-    if ((threadIdx.x & 31) == 0) {
-        tops[threadIdx.x >> 5] = top;
-    }
-    __syncthreads();
+    auto over_block = [&](float mine, float* shared) {
+        mine = GroupMax<32>(mine);
+        if ((threadIdx.x & 31) == 0) {
+            shared[threadIdx.x >> 5] = mine;
+        }
+        __syncthreads();
+        float all = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) {
-        top = fmaxf(top, tops[w]);
+        for (int w = 0; w < kTileThreads / 32; ++w) {
+            all = fmaxf(all, shared[w]);
+        }
+        return all;
+    };
+    top = over_block(top, tops[0]);
+    if (top == INFINITY) {  // the same in every thread
+        top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            top = fmaxf(top, FiniteTopOf<T, VEC>(p[i]));
+        }
+        top = over_block(top, tops[1]);
     }
     float scale, inverse;
     ScaleOf(top, scale, inverse);
@@ -184,8 +272,10 @@ __global__ void __launch_bounds__(512) TileKernel(const T* __restrict__ src, int
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int r = i * STEP + line;
-        if (r < high && lane * VEC < left) {
-            StoreBytes<T, VEC>(values + at + r * width + lane * VEC, v[i], inverse);
+        if (r < high && inside) {
+            float v[VEC];
+            Unpack<float, T, VEC>(p[i], v);
+            StoreBytes<T, VEC>(values + at + r * width, v, inverse);
         }
     }
 }
@@ -199,22 +289,25 @@ int Run(const void* src, int64_t batch, int64_t rows, int64_t width, int block_r
     const int64_t across = CeilDiv(width, kBlock);
     if (block_rows == 1) {
         const int64_t blocks = batch * rows * across;
-        const int64_t groups = wide ? 256 / (kBlock / VEC) : 8;
+        const int64_t groups = wide ? 256 / (kBlock / VEC) * kAhead : 8;
         const int grid = static_cast<int>(std::min<int64_t>(CeilDiv(blocks, groups), static_cast<int64_t>(SmCount()) * 64));
-        if (wide) {
-            RowKernel<T, VEC><<<grid, 256, 0, stream>>>(in, batch * rows, width, values, scales);
+        if (!wide) {
+            RowScalarKernel<T><<<grid, 256, 0, stream>>>(in, blocks, width, across, values, scales);
+        } else if (width % kBlock == 0) {
+            RowKernel<T, true><<<grid, 256, 0, stream>>>(in, blocks, width, across, values, scales);
         } else {
-            RowKernel<T, 1><<<grid, 256, 0, stream>>>(in, batch * rows, width, values, scales);
+            RowKernel<T, false><<<grid, 256, 0, stream>>>(in, blocks, width, across, values, scales);
         }
     } else {
         const int64_t down = CeilDiv(rows, kBlock), tiles = batch * down * across;
         if (tiles > INT32_MAX) {
             return OPSGNN_ERR_LIMIT;
         }
+        const unsigned grid = static_cast<unsigned>(tiles);
         if (wide) {
-            TileKernel<T, VEC><<<static_cast<unsigned>(tiles), 512, 0, stream>>>(in, rows, width, down, across, values, scales);
+            TileKernel<T, VEC><<<grid, kTileThreads, 0, stream>>>(in, rows, width, static_cast<int>(down), static_cast<int>(across), values, scales);
         } else {
-            TileKernel<T, 1><<<static_cast<unsigned>(tiles), 512, 0, stream>>>(in, rows, width, down, across, values, scales);
+            TileKernel<T, 1><<<grid, kTileThreads, 0, stream>>>(in, rows, width, static_cast<int>(down), static_cast<int>(across), values, scales);
         }
     }
     return LaunchStatus();
