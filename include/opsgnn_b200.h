@@ -466,8 +466,11 @@ typedef struct OpsgnnSegmentMatmulDesc {
     int32_t out_type;              /* = in_type; fp8: F32 / F16 / BF16                      */
 } OpsgnnSegmentMatmulDesc;
 
-/* Bytes of scratch (16-byte aligned) of opsgnn_segment_matmul (weight_grad 0) or opsgnn_segment_matmul_weight_grad (1). */
-OPSGNN_API int opsgnn_segment_matmul_workspace_bytes(const OpsgnnSegmentMatmulDesc* desc, int weight_grad, int64_t* bytes);
+#define OPSGNN_SEGMENT_MATMUL_FORWARD 0
+#define OPSGNN_SEGMENT_MATMUL_WEIGHT_GRAD 1
+#define OPSGNN_SEGMENT_MATMUL_GRADS 2
+/* Bytes of scratch (16-byte aligned) of opsgnn_segment_matmul, _weight_grad or _grads (what: OPSGNN_SEGMENT_MATMUL_*). */
+OPSGNN_API int opsgnn_segment_matmul_workspace_bytes(const OpsgnnSegmentMatmulDesc* desc, int what, int64_t* bytes);
 /* out[r, :] = src[r, :] @ weight[e] for the rows of segment e; 0 in rows of no segment.  out is contiguous. */
 OPSGNN_API int opsgnn_segment_matmul(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src, const void* weight,
                                      void* out, void* workspace, int64_t workspace_bytes, void* stream);
@@ -476,6 +479,11 @@ OPSGNN_API int opsgnn_segment_matmul(const OpsgnnSegmentMatmulDesc* desc, const 
 OPSGNN_API int opsgnn_segment_matmul_weight_grad(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src,
                                                  const void* grad, int64_t grad_stride, void* grad_weight, void* workspace,
                                                  int64_t workspace_bytes, void* stream);
+/* Both gradients of opsgnn_segment_matmul(desc, indptr, src, weight) in one call (fp32 operands are prepared once for the two):
+ * grad_src[rows, width] and grad_weight [segments, width, out], or [segments, out, width] when `turned`, both contiguous. */
+OPSGNN_API int opsgnn_segment_matmul_grads(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src, const void* weight,
+                                           const void* grad, int64_t grad_stride, void* grad_src, void* grad_weight, int turned,
+                                           void* workspace, int64_t workspace_bytes, void* stream);
 /* The same product on float8_e4m3 values: src[rows, width] with src_scale[rows, ceil(width / 128)], weight[e, out, width]
  * (its strides in desc as above) with weight_scale[e, ceil(out / 128), ceil(width / 128)], all scales contiguous fp32.
  * indptr NULL (with segments = 1): one dense product. */

@@ -1,4 +1,6 @@
 // C ABI of the segment products: argument checks and the choice of a kernel.
+#include <algorithm>
+
 #include "segment_matmul.cuh"
 
 namespace opsgnn {
@@ -29,6 +31,12 @@ bool Splits(const OpsgnnSegmentMatmulDesc& d)
            d.src_stride % 4 == 0;
 }
 
+// Weight gradients of 16-bit types that may be summed in pieces.
+bool Pieces(const OpsgnnSegmentMatmulDesc& d)
+{
+    return d.in_type != OPSGNN_F32 && d.rows > 0 && d.segments > 0 && d.width > 0 && d.out > 0;
+}
+
 SegmentPointers Pointers(const OpsgnnSegmentMatmulDesc& d, const void* indptr)
 {
     SegmentPointers p;
@@ -39,13 +47,36 @@ SegmentPointers Pointers(const OpsgnnSegmentMatmulDesc& d, const void* indptr)
     return p;
 }
 
+// The fastest kernel that takes the problem; fp32 goes through bf16 terms where there is a workspace for them.
+int RunRows(const RowsProblem& p, void* workspace, cudaStream_t stream)
+{
+    int ran = OPSGNN_ERR_UNSUPPORTED;
+    if (p.in_type != OPSGNN_F32) {
+        ran = RunRowsTensor(p, stream);
+    } else if (workspace != nullptr) {
+        ran = RunRowsSplit(p, workspace, stream);
+    }
+    return ran == OPSGNN_ERR_UNSUPPORTED ? RunRowsSimple(p, stream) : ran;
+}
+
+int RunOuter(const OuterProblem& p, void* workspace, cudaStream_t stream)
+{
+    int ran = OPSGNN_ERR_UNSUPPORTED;
+    if (p.type != OPSGNN_F32) {
+        ran = RunOuterTensor(p, workspace, stream);
+    } else if (workspace != nullptr) {
+        ran = RunOuterSplit(p, workspace, stream);
+    }
+    return ran == OPSGNN_ERR_UNSUPPORTED ? RunOuterSimple(p, stream) : ran;
+}
+
 }  // namespace
 }  // namespace segmm
 }  // namespace opsgnn
 
 using namespace opsgnn;
 
-extern "C" int opsgnn_segment_matmul_workspace_bytes(const OpsgnnSegmentMatmulDesc* desc, int weight_grad, int64_t* bytes)
+extern "C" int opsgnn_segment_matmul_workspace_bytes(const OpsgnnSegmentMatmulDesc* desc, int what, int64_t* bytes)
 {
     const int status = segmm::CheckDesc(desc, false);
     if (status != OPSGNN_OK) {
@@ -54,13 +85,21 @@ extern "C" int opsgnn_segment_matmul_workspace_bytes(const OpsgnnSegmentMatmulDe
     if (bytes == nullptr) {
         return OPSGNN_ERR_INVALID;
     }
+    const int64_t rows = desc->rows, segments = desc->segments, width = desc->width, out = desc->out;
+    const bool split = segmm::Splits(*desc);
     *bytes = 0;
-    if (segmm::Splits(*desc)) {
-        *bytes = weight_grad ? segmm::OuterSplitBytes(desc->rows, desc->segments, desc->width, desc->out)
-                             : segmm::RowsSplitBytes(desc->rows, desc->segments, desc->width, desc->out);
-    } else if (desc->in_type != OPSGNN_F32 && weight_grad && desc->rows > 0 && desc->segments > 0 && desc->width > 0 && desc->out > 0 &&
-               desc->out % 8 == 0) {
-        *bytes = segmm::OuterPartialBytes(desc->rows, desc->segments, desc->width, desc->out);
+    if (what == OPSGNN_SEGMENT_MATMUL_FORWARD) {
+        *bytes = split ? segmm::RowsSplitBytes(rows, segments, width, out) : 0;
+    } else if (what == OPSGNN_SEGMENT_MATMUL_WEIGHT_GRAD) {
+        *bytes = split ? segmm::OuterSplitBytes(rows, segments, width, out)
+                       : (segmm::Pieces(*desc) ? segmm::OuterPartialBytes(rows, segments, width, out) : 0);
+    } else if (what == OPSGNN_SEGMENT_MATMUL_GRADS) {
+        *bytes = split ? segmm::GradsSplitBytes(rows, segments, width, out)
+                       : (segmm::Pieces(*desc) ? std::max(segmm::OuterPartialBytes(rows, segments, width, out),
+                                                          segmm::OuterPartialBytes(rows, segments, out, width))
+                                               : 0);
+    } else {
+        return OPSGNN_ERR_INVALID;
     }
     return OPSGNN_OK;
 }
@@ -69,7 +108,7 @@ extern "C" int opsgnn_segment_matmul(const OpsgnnSegmentMatmulDesc* desc, const 
                                      void* out, void* workspace, int64_t workspace_bytes, void* stream)
 {
     int64_t need = 0;
-    const int status = opsgnn_segment_matmul_workspace_bytes(desc, 0, &need);
+    const int status = opsgnn_segment_matmul_workspace_bytes(desc, OPSGNN_SEGMENT_MATMUL_FORWARD, &need);
     if (status != OPSGNN_OK) {
         return status;
     }
@@ -96,8 +135,7 @@ extern "C" int opsgnn_segment_matmul(const OpsgnnSegmentMatmulDesc* desc, const 
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !Aligned(workspace, 16))) {
         return OPSGNN_ERR_WORKSPACE;
     }
-    const int ran = need > 0 ? segmm::RunRowsSplit(p, workspace, AsStream(stream)) : segmm::RunRowsTensor(p, AsStream(stream));
-    return ran == OPSGNN_ERR_UNSUPPORTED ? segmm::RunRowsSimple(p, AsStream(stream)) : ran;
+    return segmm::RunRows(p, need > 0 ? workspace : nullptr, AsStream(stream));
 }
 
 extern "C" int opsgnn_segment_matmul_weight_grad(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src,
@@ -105,7 +143,7 @@ extern "C" int opsgnn_segment_matmul_weight_grad(const OpsgnnSegmentMatmulDesc* 
                                                  int64_t workspace_bytes, void* stream)
 {
     int64_t need = 0;
-    const int status = opsgnn_segment_matmul_workspace_bytes(desc, 1, &need);
+    const int status = opsgnn_segment_matmul_workspace_bytes(desc, OPSGNN_SEGMENT_MATMUL_WEIGHT_GRAD, &need);
     if (status != OPSGNN_OK) {
         return status;
     }
@@ -128,9 +166,67 @@ extern "C" int opsgnn_segment_matmul_weight_grad(const OpsgnnSegmentMatmulDesc* 
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !Aligned(workspace, 16))) {
         return OPSGNN_ERR_WORKSPACE;
     }
-    const int ran = p.type == OPSGNN_F32 ? (need > 0 ? segmm::RunOuterSplit(p, workspace, AsStream(stream)) : OPSGNN_ERR_UNSUPPORTED)
-                                         : segmm::RunOuterTensor(p, workspace, AsStream(stream));
-    return ran == OPSGNN_ERR_UNSUPPORTED ? segmm::RunOuterSimple(p, AsStream(stream)) : ran;
+    return segmm::RunOuter(p, need > 0 ? workspace : nullptr, AsStream(stream));
+}
+
+extern "C" int opsgnn_segment_matmul_grads(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src, const void* weight,
+                                           const void* grad, int64_t grad_stride, void* grad_src, void* grad_weight, int turned,
+                                           void* workspace, int64_t workspace_bytes, void* stream)
+{
+    int64_t need = 0;
+    const int status = opsgnn_segment_matmul_workspace_bytes(desc, OPSGNN_SEGMENT_MATMUL_GRADS, &need);
+    if (status != OPSGNN_OK) {
+        return status;
+    }
+    if (indptr == nullptr || grad_stride < desc->out) {
+        return OPSGNN_ERR_INVALID;
+    }
+    const bool rows = desc->rows > 0 && desc->width > 0, outer = desc->segments > 0 && desc->width > 0 && desc->out > 0;
+    const bool sums = desc->out > 0 && desc->segments > 0;
+    if ((rows && (grad_src == nullptr || (sums && (grad == nullptr || weight == nullptr)))) ||
+        (outer && (grad_weight == nullptr || (desc->rows > 0 && (src == nullptr || grad == nullptr))))) {
+        return OPSGNN_ERR_INVALID;
+    }
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !Aligned(workspace, 16))) {
+        return OPSGNN_ERR_WORKSPACE;
+    }
+    segmm::RowsProblem p{};
+    p.ptr = segmm::Pointers(*desc, indptr);
+    p.a = grad;
+    p.b = weight;
+    p.out = grad_src;
+    p.k = desc->out;
+    p.n = desc->width;
+    p.lda = grad_stride;
+    p.ldo = desc->width;
+    p.b_segment = desc->weight_segment_stride;
+    p.b_k = desc->weight_out_stride;
+    p.b_n = desc->weight_width_stride;
+    p.in_type = desc->in_type;
+    p.out_type = desc->out_type;
+    segmm::OuterProblem q{};
+    q.ptr = p.ptr;
+    q.a = turned ? grad : src;
+    q.b = turned ? src : grad;
+    q.out = grad_weight;
+    q.k = turned ? desc->out : desc->width;
+    q.n = turned ? desc->width : desc->out;
+    q.lda = turned ? grad_stride : desc->src_stride;
+    q.ldb = turned ? desc->src_stride : grad_stride;
+    q.type = desc->in_type;
+    if (rows && outer && segmm::Splits(*desc)) {
+        const int ran = segmm::RunGradsSplit(p, q, turned != 0, workspace, AsStream(stream));
+        if (ran != OPSGNN_ERR_UNSUPPORTED) {
+            return ran;
+        }
+    }
+    // fp32 that cannot be split goes through the simple kernels: no workspace for it below
+    void* scratch = need > 0 && !segmm::Splits(*desc) ? workspace : nullptr;
+    int ran = rows ? segmm::RunRows(p, scratch, AsStream(stream)) : OPSGNN_OK;
+    if (ran == OPSGNN_OK && outer) {
+        ran = segmm::RunOuter(q, scratch, AsStream(stream));
+    }
+    return ran;
 }
 
 extern "C" int opsgnn_segment_matmul_fp8(const OpsgnnSegmentMatmulDesc* desc, const void* indptr, const void* src, const float* src_scale,

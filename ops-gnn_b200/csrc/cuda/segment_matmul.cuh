@@ -45,6 +45,10 @@ int RunRowsSplit(const RowsProblem& p, void* workspace, cudaStream_t stream);
 int RunOuterSplit(const OuterProblem& p, void* workspace, cudaStream_t stream);
 int64_t RowsSplitBytes(int64_t rows, int64_t segments, int64_t k, int64_t n);
 int64_t OuterSplitBytes(int64_t rows, int64_t segments, int64_t k, int64_t n);
+// Both gradients in one call: the terms of the upstream gradient are made once.
+int64_t GradsSplitBytes(int64_t rows, int64_t segments, int64_t k, int64_t n);
+// `turned`: outer is grad^T src.
+int RunGradsSplit(const RowsProblem& rows, const OuterProblem& outer, bool turned, void* workspace, cudaStream_t stream);
 // Outer form with few result tiles: rows per piece (0: one piece per segment), fp32 scratch for the pieces, and their sum.
 int64_t OuterChunk(int64_t rows, int64_t segments, int64_t k, int64_t n);
 int64_t OuterPartialBytes(int64_t rows, int64_t segments, int64_t k, int64_t n);

@@ -25,12 +25,13 @@ namespace segmm {
 namespace {
 
 constexpr int kRows = 128;
+constexpr int kBoxRows = 32;  // rows of a per load where a tile is not full
 constexpr int kThreads = 384;
 constexpr int kStages = 4;
 constexpr int kSlab = 64 * 128;
 constexpr int kStagingBytes = 8 * 32 * 128;
 // 384 threads are launched with 168 registers each; 128 * 72 + 256 * 216 = 384 * 168.
-constexpr int kRegsIssue = 72, kRegsSum = 216;
+constexpr int kRegsIssue = 104, kRegsSum = 200;
 
 enum Form { kRowsWide, kRowsTurned, kOuter };
 
@@ -47,6 +48,7 @@ struct Params {
     const float* b;
     int64_t lda, ldb;                // outer form: ldb = row stride of b
     int64_t b_segment, b_k, b_n;
+    bool whole_a, whole_b;  // MN-major operands: all slabs in one load
     int64_t chunk;     // outer form: rows per partial result; 0: a segment's rows in one piece
     float* partial;    // [pieces][m][n]
     WaitSettings wait;
@@ -54,12 +56,9 @@ struct Params {
 
 struct Barriers {
     uint64_t full[kStages], empty[kStages], done[2], free[2], drain;
+    uint32_t fills[kStages];  // loads asked for, per stage (loading warp)
     uint32_t tmem, stop;
 };
-
-// The six products of the fp32 split, smallest first: planes of a and b.
-__device__ __forceinline__ int PlaneA(int term) { return term == 0 ? 2 : (term == 1 || term == 3 ? 1 : 0); }
-__device__ __forceinline__ int PlaneB(int term) { return term == 2 ? 2 : (term == 1 || term == 4 ? 1 : 0); }
 
 template <class O> __device__ __forceinline__ uint32_t Word(const float* v)  // one 32-bit word of results
 {
@@ -91,10 +90,10 @@ template <int N> __device__ __forceinline__ void Add(float (&sum)[N], int at, co
 
 template <bool F8, class O, int BN, int FORM>
 __global__ void __launch_bounds__(kThreads, 1)
-    PromotedKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p)
+    PromotedKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_tail,
+                   const __grid_constant__ CUtensorMap map_b, const Params p)
 {
     constexpr int kStage = StageBytes<BN>();
-    constexpr int kTerms = F8 ? 1 : 6;
     constexpr int kDepth = F8 ? 128 : 64;  // values of the reduced index in one 128-byte row
     extern __shared__ unsigned char raw[];
     unsigned char* smem = raw + ((1024 - (tc::Shared(raw) & 1023)) & 1023);
@@ -106,6 +105,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < kStages; ++i) {
             tc::BarInit(&bar.full[i], 1);
             tc::BarInit(&bar.empty[i], 1);
+            bar.fills[i] = 0;
         }
         for (int i = 0; i < 2; ++i) {
             tc::BarInit(&bar.done[i], 1);
@@ -124,148 +124,189 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = bar.tmem;
     const tc::Waiter wait{&bar.stop, p.wait};
 
-    const int64_t across = (p.n + BN - 1) / BN;
-    const int64_t down = FORM == kOuter ? (p.m + kRows - 1) / kRows : 0;
-    const int64_t outer_tiles = FORM == kOuter ? p.ptr.segments * down * across : 0;
-    SegmentWalk<FORM == kOuter ? 0 : kRows> walk;
-    if (warp != 2 && warp != 3 && (FORM != kOuter || p.chunk > 0)) {
-        walk.Start(p.ptr, FORM == kOuter ? p.chunk : kRows);
+    // Rows, widths and tile numbers fit 32 bits (checked on the host); offsets in memory are formed in 64.
+    const int n = static_cast<int>(p.n), m = static_cast<int>(p.m), width = static_cast<int>(p.k), chunk = static_cast<int>(p.chunk);
+    const int across = (n + BN - 1) / BN;
+    const int down = FORM == kOuter ? (m + kRows - 1) / kRows : 1;
+    SegmentWalk<FORM == kOuter ? 0 : kRows, int> walk;
+    if (warp != 2 && warp != 3 && (FORM != kOuter || chunk > 0)) {
+        walk.Start(p.ptr, FORM == kOuter ? chunk : kRows);
     }
-    int64_t segment = 0, row = 0, row_end = 0, column = 0, from = 0, depth = 0;
-    auto find = [&](int64_t t) {
+    // Tile t: its segment, first result row and column, and the range of the reduced index.
+    int segment = 0, row = 0, row_end = 0, column = 0, from = 0, depth = 0;
+    auto find = [&](int t) {
         column = t % across * BN;
+        t /= across;
         if constexpr (FORM == kOuter) {
-            row = t / across % down * kRows;
-            row_end = p.m;
-            segment = t / (down * across);  // of the result to write: a segment or a piece
-            if (p.chunk > 0) {
-                if (!walk.Seek(segment)) {
+            row = t % down * kRows;
+            row_end = m;
+            segment = t / down;  // of the result to write: a segment or a piece
+            if (chunk > 0) {
+                if (!walk.Seek(p.ptr, segment)) {
                     return false;
                 }
                 from = walk.row;
-                depth = walk.row_end - from < p.chunk ? walk.row_end - from : p.chunk;
+                depth = min(walk.row_end - from, chunk);
                 return true;
             }
-            if (t >= outer_tiles) {
+            if (segment >= p.ptr.segments) {
                 return false;
             }
-            int64_t end;
-            p.ptr.Range(segment, from, end);
+            int end;
+            p.ptr.Range<int>(segment, from, end);
             depth = end - from;
             return true;
         } else {
-            if (!walk.Seek(t / across)) {
+            if (!walk.Seek(p.ptr, t)) {
                 return false;
             }
             segment = walk.segment;
             row = walk.row;
             row_end = walk.row_end;
-            depth = p.k;
+            depth = width;
             return true;
         }
     };
 
-    uint32_t filled = 0;
+    // 8 bits: the stages are a ring.  fp32: stages 0 and 1 take turns with (third term of a, first of b), stage 2 holds the
+    // second terms of both, stage 3 (first of a, third of b); every term is loaded once per 64 values of the reduced index and
+    // used in one to three products (a ring of operand pairs per product read 288 KB in place of 144 and was bound by that).
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
         if (warp == 0) {
-            bool going = true;
-            for (int64_t t = blockIdx.x; going && find(t); t += gridDim.x) {
-                for (int64_t k = 0; going && k < depth; k += kDepth) {
-#pragma unroll 1
-                    for (int term = 0; term < kTerms; ++term, ++filled) {
-                        const uint32_t s = filled % kStages;
-                        going = wait.Warp(&bar.empty[s], ((filled / kStages) & 1) ^ 1);
-                        if (!going) {
-                            break;
-                        }
-                        if (lane == 0) {
-                            const int pa = F8 ? 0 : PlaneA(term), pb = F8 ? 0 : PlaneB(term);
-                            const uint32_t a = tc::Shared(smem) + s * kStage, b = a + kRows * 128;
-                            tc::BarExpect(&bar.full[s], kStage);
-                            if constexpr (FORM == kOuter) {
-                                const int r = static_cast<int>(from + k);
-#pragma unroll
-                                for (int i = 0; i < kRows / 64; ++i) {
-                                    tc::Load3(map_a, &bar.full[s], a + i * kSlab, static_cast<int>(row) + i * 64, r, pa);
-                                }
-#pragma unroll
-                                for (int i = 0; i < BN / 64; ++i) {
-                                    tc::Load3(map_b, &bar.full[s], b + i * kSlab, static_cast<int>(column) + i * 64, r, pb);
-                                }
-                            } else {
-                                const int matrix = static_cast<int>(pb * p.ptr.segments + segment);
-                                tc::Load3(map_a, &bar.full[s], a, static_cast<int>(k), static_cast<int>(row), pa);
-                                if constexpr (FORM == kRowsTurned) {
-                                    tc::Load3(map_b, &bar.full[s], b, static_cast<int>(k), static_cast<int>(column), matrix);
-                                } else {
-#pragma unroll
-                                    for (int i = 0; i < BN / 64; ++i) {
-                                        tc::Load3(map_b, &bar.full[s], b + i * kSlab, static_cast<int>(column) + i * 64,
-                                                  static_cast<int>(k), matrix);
-                                    }
-                                }
+            // One stage: rows and columns of the tile at k, terms pa and pb.
+            auto load = [&](uint32_t s, uint32_t use, int k, int pa, int pb) {
+                if (!wait.Warp(&bar.empty[s], (use & 1) ^ 1)) {
+                    return false;
+                }
+                if (lane == 0) {
+                    const uint32_t a = tc::Shared(smem) + s * kStage, b = a + kRows * 128;
+                    bar.fills[s] = use + 1;
+                    if constexpr (FORM == kOuter) {
+                        tc::BarExpect(&bar.full[s], kStage);
+                        tc::LoadSlabs(map_a, &bar.full[s], a, row, from + k, pa, kRows / 64, p.whole_a);
+                        tc::LoadSlabs(map_b, &bar.full[s], b, column, from + k, pb, BN / 64, p.whole_b);
+                    } else {
+                        // Only the rows that are the segment's, to the next 32; what else lies in the stage is multiplied into
+                        // rows that are not stored.
+                        const int boxes = min(row_end - row + kBoxRows - 1, kRows) / kBoxRows;
+                        const int matrix = pb * static_cast<int>(p.ptr.segments) + segment;
+                        tc::BarExpect(&bar.full[s], boxes * kBoxRows * 128 + BN * 128);
+                        if (boxes * kBoxRows == kRows) {
+                            tc::Load3(map_a, &bar.full[s], a, k, row, pa);
+                        } else {
+                            for (int i = 0; i < boxes; ++i) {
+                                tc::Load3(map_tail, &bar.full[s], a + i * kBoxRows * 128, k, row + i * kBoxRows, pa);
                             }
                         }
-                        __syncwarp();
+                        if constexpr (FORM == kRowsTurned) {
+                            tc::Load3(map_b, &bar.full[s], b, k, column, matrix);
+                        } else {
+                            tc::LoadSlabs(map_b, &bar.full[s], b, column, k, matrix, BN / 64, p.whole_b);
+                        }
+                    }
+                }
+                __syncwarp();
+                return true;
+            };
+            uint32_t blocks = 0;
+            bool going = true;
+            for (int t = blockIdx.x; going && find(t); t += gridDim.x) {
+                for (int k = 0; going && k < depth; k += kDepth, ++blocks) {
+                    if constexpr (F8) {
+                        going = load(blocks % kStages, blocks / kStages, k, 0, 0);
+                    } else {
+                        going = load(blocks & 1, blocks >> 1, k, 2, 0) && load(2, blocks, k, 1, 1) && load(3, blocks, k, 0, 2);
                     }
                 }
             }
         } else if (warp == 1) {
             constexpr uint32_t shape = tc::Shape(kRows, BN, F8 ? 0 : 1, FORM == kOuter, FORM != kRowsTurned);
-            uint32_t used = 0, blocks = 0;
+            uint32_t blocks = 0;
+            int at = 0;
             bool going = true;
-            for (int64_t t = blockIdx.x; going && find(t); t += gridDim.x) {
-                for (int64_t k = 0; going && k < depth; k += kDepth, ++blocks) {
+            // The stage's operands have landed; rows that belong to the next segment are zeroed.
+            auto ready = [&](uint32_t s, uint32_t use) {
+                if (!wait.Warp(&bar.full[s], use & 1)) {
+                    return false;
+                }
+                if constexpr (FORM == kOuter) {
+                    if (depth - at < kDepth) {
+                        unsigned char* stage = smem + s * kStage;
+                        const int first = (depth - at);
+                        for (int i = first * 8 + lane; i < kDepth * 8; i += 32) {
+#pragma unroll
+                            for (int slab = 0; slab < kStage / kSlab; ++slab) {
+                                *reinterpret_cast<uint4*>(stage + slab * kSlab + i * 16) = make_uint4(0, 0, 0, 0);
+                            }
+                        }
+                        tc::FenceAsync();
+                        __syncwarp();
+                    }
+                }
+                tc::FenceAfter();
+                return true;
+            };
+            // One product of kDepth values: a of one stage, b of another.
+            auto multiply = [&](uint32_t sa, uint32_t sb, uint32_t half, bool add) {
+                if (lane == 0) {
+                    uint64_t da = tc::Operand(tc::Shared(smem) + sa * kStage, FORM == kOuter ? kSlab : 16, 1024);
+                    uint64_t db = tc::Operand(tc::Shared(smem) + sb * kStage + kRows * 128, FORM == kRowsTurned ? 16 : kSlab, 1024);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (F8) {
+                            tc::MmaF8(tmem + half * BN, da, db, shape, add || i > 0);
+                        } else {
+                            tc::MmaF16(tmem + half * BN, da, db, shape, add || i > 0);
+                        }
+                        da += FORM == kOuter ? 2048 >> 4 : 32 >> 4;
+                        db += FORM == kRowsTurned ? 32 >> 4 : 2048 >> 4;
+                    }
+                }
+            };
+            auto commit = [&](uint64_t* to) {
+                if (lane == 0) {
+                    tc::Commit(to);
+                }
+            };
+            for (int t = blockIdx.x; going && find(t); t += gridDim.x) {
+                for (at = 0; going && at < depth; at += kDepth, ++blocks) {
                     const uint32_t half = blocks & 1;
                     going = wait.Warp(&bar.free[half], ((blocks >> 1) & 1) ^ 1);
                     tc::FenceAfter();
-#pragma unroll 1
-                    for (int term = 0; going && term < kTerms; ++term, ++used) {
-                        const uint32_t s = used % kStages;
-                        going = wait.Warp(&bar.full[s], (used / kStages) & 1);
+                    if constexpr (F8) {
+                        const uint32_t s = blocks % kStages;
+                        going = going && ready(s, blocks / kStages);
                         if (!going) {
                             break;
                         }
-                        unsigned char* stage = smem + s * kStage;
-                        if constexpr (FORM == kOuter) {
-                            if (depth - k < kDepth) {  // rows of the next segment
-                                const int first = static_cast<int>(depth - k);
-                                for (int i = first * 8 + lane; i < kDepth * 8; i += 32) {
-#pragma unroll
-                                    for (int slab = 0; slab < kStage / kSlab; ++slab) {
-                                        *reinterpret_cast<uint4*>(stage + slab * kSlab + i * 16) = make_uint4(0, 0, 0, 0);
-                                    }
-                                }
-                                tc::FenceAsync();
-                                __syncwarp();
-                            }
+                        multiply(s, s, half, false);
+                        commit(&bar.empty[s]);
+                    } else {
+                        const uint32_t s = blocks & 1;
+                        going = going && ready(s, blocks >> 1);
+                        if (!going) {
+                            break;
                         }
-                        tc::FenceAfter();
-                        if (lane == 0) {
-                            const uint32_t a = tc::Shared(stage), b = a + kRows * 128;
-                            uint64_t da = tc::Operand(a, FORM == kOuter ? kSlab : 16, 1024);
-                            uint64_t db = tc::Operand(b, FORM == kRowsTurned ? 16 : kSlab, 1024);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                if constexpr (F8) {
-                                    tc::MmaF8(tmem + half * BN, da, db, shape, i > 0);
-                                } else {
-                                    tc::MmaF16(tmem + half * BN, da, db, shape, term > 0 || i > 0);
-                                }
-                                da += FORM == kOuter ? 2048 >> 4 : 32 >> 4;
-                                db += FORM == kRowsTurned ? 32 >> 4 : 2048 >> 4;
-                            }
-                            tc::Commit(&bar.empty[s]);
+                        multiply(s, s, half, false);     // a3 b1
+                        going = ready(2, blocks);
+                        if (!going) {
+                            break;
                         }
-                        __syncwarp();
+                        multiply(2, 2, half, true);      // a2 b2
+                        going = ready(3, blocks);
+                        if (!going) {
+                            break;
+                        }
+                        multiply(3, 3, half, true);      // a1 b3
+                        multiply(2, s, half, true);      // a2 b1
+                        multiply(3, 2, half, true);      // a1 b2
+                        commit(&bar.empty[2]);
+                        multiply(3, s, half, true);      // a1 b1
+                        commit(&bar.empty[s]);
+                        commit(&bar.empty[3]);
                     }
-                    if (!going) {
-                        break;
-                    }
-                    if (lane == 0) {
-                        tc::Commit(&bar.done[half]);
-                    }
+                    commit(&bar.done[half]);
                     __syncwarp();
                 }
             }
@@ -285,46 +326,51 @@ __global__ void __launch_bounds__(kThreads, 1)
         unsigned char* mine = staging + (warp - 4) * (32 * 128);
         // a piece of a segment's sum (outer form in pieces; fp32 then) goes to `partial`
         O* out = FORM == kOuter && p.chunk > 0 ? reinterpret_cast<O*>(p.partial) : static_cast<O*>(p.out);
-        const int64_t scale_blocks = F8 ? (p.k + 127) / 128 : 0, scale_bands = F8 ? (p.n + 127) / 128 : 0;
+        const int scale_blocks = F8 ? (width + 127) / 128 : 0, scale_bands = F8 ? (n + 127) / 128 : 0;
         uint32_t blocks = 0;
         bool going = true;
-        for (int64_t t = blockIdx.x; going && find(t); t += gridDim.x) {
+        for (int t = blockIdx.x; going && find(t); t += gridDim.x) {
             float sum[kMine];
 #pragma unroll
             for (int i = 0; i < kMine; ++i) {
                 sum[i] = 0.0f;
             }
-            const int64_t col0 = column + side * kMine;
-            const bool some = col0 < p.n;
-            const int64_t r0 = row + quarter * 32;
+            const int col0 = column + side * kMine;
+            const bool some = col0 < n;
+            const int r0 = row + quarter * 32;
             const float* sa = nullptr;
             const float* sb = nullptr;
             float scale = 1.0f;
             if constexpr (F8) {
-                sa = p.a_scale + (r0 + lane < row_end ? r0 + lane : row) * scale_blocks;
-                sb = p.b_scale + (segment * scale_bands + (some ? col0 / 128 : 0)) * scale_blocks;
+                sa = p.a_scale + static_cast<int64_t>(r0 + lane < row_end ? r0 + lane : row) * scale_blocks;
+                sb = p.b_scale + (static_cast<int64_t>(segment) * scale_bands + (some ? col0 / 128 : 0)) * scale_blocks;
             }
-            for (int64_t k = 0, kb = 0; k < depth; k += kDepth, ++kb, ++blocks) {
+            float next_a = 1.0f, next_b = 1.0f;  // the next block's scales, asked for one block ahead
+            if constexpr (F8) {
+                next_a = __ldg(sa);
+                next_b = __ldg(sb);
+            }
+            const int last = (depth + kDepth - 1) / kDepth - 1;
+            for (int kb = 0; kb <= last; ++kb, ++blocks) {
                 const uint32_t half = blocks & 1;
                 if constexpr (F8) {
-                    scale = __ldg(sa + kb) * __ldg(sb + kb);
+                    scale = next_a * next_b;
+                    next_a = __ldg(sa + min(kb + 1, last));
+                    next_b = __ldg(sb + min(kb + 1, last));
                 }
                 going = wait.Warp(&bar.done[half], (blocks >> 1) & 1);
                 if (!going) {
                     break;
                 }
                 tc::FenceAfter();
+                const uint32_t at = tmem + half * BN + side * kMine + (static_cast<uint32_t>(quarter * 32) << 16);
                 if (some) {
-                    const uint32_t at = tmem + half * BN + side * kMine + (static_cast<uint32_t>(quarter * 32) << 16);
-                    uint32_t part[2][32];
-                    tc::TmemLoad32(at, part[0]);
+                    uint32_t part[32];
 #pragma unroll
                     for (int c = 0; c < kMine; c += 32) {
+                        tc::TmemLoad32(at + c, part);
                         tc::TmemWait();
-                        if (c + 32 < kMine) {
-                            tc::TmemLoad32(at + c + 32, part[(c / 32 + 1) & 1]);
-                        }
-                        Add(sum, c, part[(c / 32) & 1], scale);
+                        Add(sum, c, part, scale);
                     }
                 }
                 tc::FenceBefore();
@@ -342,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool odd = false;
 #pragma unroll
             for (int c = 0; c < kMine; c += kLine) {
-                if (col0 + c < p.n) {
+                if (col0 + c < n) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         uint4 v;
@@ -354,12 +400,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     __syncwarp();
                     const int piece = lane & 7;
-                    const int64_t col = col0 + c + piece * (kLine / 8);
+                    const int col = col0 + c + piece * (kLine / 8);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int r = i * 4 + (lane >> 3);
                         const uint4 value = *reinterpret_cast<const uint4*>(mine + r * 128 + ((piece ^ (r & 7)) << 4));
-                        if (r0 + r < row_end && col < p.n) {
+                        if (r0 + r < row_end && col < n) {
                             *reinterpret_cast<uint4*>(to + (r0 + r) * p.n + col) = value;
                         }
                     }
@@ -373,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (__any_sync(0xffffffffu, odd)) {
                     // Results that are not finite, from the operands as given: the row of a lane, column by column.
-                    for (int64_t i = lane; i < 32 * kMine; i += 32) {
+                    for (int i = lane; i < 32 * kMine; i += 32) {
                         const int64_t r = r0 + i / kMine, c = col0 + i % kMine;
                         if (r >= row_end || c >= p.n) {
                             continue;
@@ -382,8 +428,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (fabsf(*place) < INFINITY) {
                             continue;
                         }
-                        const float* x = FORM == kOuter ? p.a + from * p.lda + r : p.a + r * p.lda;
-                        const float* y = FORM == kOuter ? p.b + from * p.ldb + c : p.b + segment * p.b_segment + c * p.b_n;
+                        const float* x = FORM == kOuter ? p.a + static_cast<int64_t>(from) * p.lda + r : p.a + r * p.lda;
+                        const float* y = FORM == kOuter ? p.b + static_cast<int64_t>(from) * p.ldb + c : p.b + segment * p.b_segment + c * p.b_n;
                         const int64_t dx = FORM == kOuter ? p.lda : 1, dy = FORM == kOuter ? p.ldb : p.b_k;
                         float v = 0.0f;
                         for (int64_t d = 0; d < depth && v == v; ++d) {  // NaN stays NaN
@@ -412,8 +458,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     if (warp == 0 && lane == 0 && bar.stop != 0) {
         // Copies in flight must land before the block's shared memory is given up.
-        for (uint32_t f = filled > kStages ? filled - kStages : 0; f < filled; ++f) {
-            for (uint32_t i = 0; i < (1u << 15) && !tc::BarTry(&bar.full[f % kStages], (f / kStages) & 1); ++i) {
+        for (int s = 0; s < kStages; ++s) {
+            for (uint32_t i = 0; bar.fills[s] > 0 && i < (1u << 15) && !tc::BarTry(&bar.full[s], (bar.fills[s] - 1) & 1); ++i) {
             }
         }
     }
@@ -477,11 +523,14 @@ bool Map3(CUtensorMap* map, bool f8, const void* base, int64_t inner, int64_t ro
 }
 
 template <bool F8, class O, int BN, int FORM>
-int Launch(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int64_t tiles, cudaStream_t stream)
+int Launch(const CUtensorMap& a, const CUtensorMap& tail, const CUtensorMap& b, const Params& p, int64_t tiles, cudaStream_t stream)
 {
+    if (tiles >= INT32_MAX - 4096) {
+        return OPSGNN_ERR_UNSUPPORTED;
+    }
     OPSGNN_CUDA_TRY(cudaFuncSetAttribute(PromotedKernel<F8, O, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, SharedBytes<BN>()));
     const int grid = static_cast<int>(std::min<int64_t>(std::max<int64_t>(tiles, 1), SmCount()));
-    PromotedKernel<F8, O, BN, FORM><<<grid, kThreads, SharedBytes<BN>(), stream>>>(a, b, p);
+    PromotedKernel<F8, O, BN, FORM><<<grid, kThreads, SharedBytes<BN>(), stream>>>(a, tail, b, p);
     return LaunchStatus();
 }
 
@@ -511,12 +560,12 @@ int64_t OuterSplitBytes(int64_t rows, int64_t segments, int64_t k, int64_t n)
     return PlaneBytes(rows * k) + PlaneBytes(rows * n) + OuterPartialBytes(rows, segments, k, n);
 }
 
-int RunRowsSplit(const RowsProblem& p, void* workspace, cudaStream_t stream)
+namespace {
+
+// The products from planes that are there.
+int RowsFromPlanes(const RowsProblem& p, const void* planes_a, const void* planes_b, cudaStream_t stream)
 {
-    bool turned;
-    if (!RowsSplittable(p, turned) || !Aligned(workspace, 16)) {
-        return OPSGNN_ERR_UNSUPPORTED;
-    }
+    const bool turned = p.b_k == 1 && p.b_n != 1;
     Params q{};
     q.ptr = p.ptr;
     q.out = p.out;
@@ -529,28 +578,78 @@ int RunRowsSplit(const RowsProblem& p, void* workspace, cudaStream_t stream)
     q.b_k = p.b_k;
     q.b_n = p.b_n;
     OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
-    char* planes_a = static_cast<char*>(workspace);
-    char* planes_b = planes_a + PlaneBytes(p.ptr.rows * p.k);
     const int64_t inner = turned ? p.k : p.n, other = turned ? p.n : p.k, e = p.ptr.segments;
     const bool narrow = p.n <= 128;
-    CUtensorMap a, b;
+    q.whole_b = tc::WholeSlabs(p.n);
+    CUtensorMap a, tail, b;
     if (!Map3(&a, false, planes_a, p.k, p.ptr.rows, 3, p.k, p.ptr.rows * p.k, kRows) ||
-        !Map3(&b, false, planes_b, inner, other, 3 * e, inner, inner * other, turned ? (narrow ? 128 : 256) : 64)) {
+        !Map3(&tail, false, planes_a, p.k, p.ptr.rows, 3, p.k, p.ptr.rows * p.k, kBoxRows) ||
+        !(turned ? Map3(&b, false, planes_b, inner, other, 3 * e, inner, inner * other, narrow ? 128 : 256)
+                 : tc::EncodeSlabs(&b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, planes_b, p.n, p.k, 3 * e, p.n * 2, p.n * p.k * 2, narrow ? 2 : 4))) {
         return OPSGNN_ERR_UNSUPPORTED;
-    }
-    int status = Split(q.a, 1, p.ptr.rows, p.k, 0, p.lda, planes_a, stream);
-    if (status == OPSGNN_OK) {
-        status = Split(q.b, e, other, inner, p.b_segment, turned ? p.b_n : p.b_k, planes_b, stream);
-    }
-    if (status != OPSGNN_OK) {
-        return status;
     }
     const int64_t down = p.ptr.rows / kRows + e;
     if (narrow) {
-        return turned ? Launch<false, float, 128, kRowsTurned>(a, b, q, down, stream) : Launch<false, float, 128, kRowsWide>(a, b, q, down, stream);
+        return turned ? Launch<false, float, 128, kRowsTurned>(a, tail, b, q, down, stream) : Launch<false, float, 128, kRowsWide>(a, tail, b, q, down, stream);
     }
     const int64_t tiles = down * CeilDiv(p.n, 256);
-    return turned ? Launch<false, float, 256, kRowsTurned>(a, b, q, tiles, stream) : Launch<false, float, 256, kRowsWide>(a, b, q, tiles, stream);
+    return turned ? Launch<false, float, 256, kRowsTurned>(a, tail, b, q, tiles, stream) : Launch<false, float, 256, kRowsWide>(a, tail, b, q, tiles, stream);
+}
+
+int OuterFromPlanes(const OuterProblem& p, const void* planes_a, const void* planes_b, void* partial, cudaStream_t stream)
+{
+    Params q{};
+    q.ptr = p.ptr;
+    q.out = p.out;
+    q.m = p.k;
+    q.n = p.n;
+    q.chunk = OuterChunk(p.ptr.rows, p.ptr.segments, p.k, p.n);
+    q.partial = static_cast<float*>(partial);
+    q.a = static_cast<const float*>(p.a);
+    q.b = static_cast<const float*>(p.b);
+    q.lda = p.lda;
+    q.ldb = p.ldb;
+    OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
+    q.whole_a = tc::WholeSlabs(p.k);
+    q.whole_b = tc::WholeSlabs(p.n);
+    const CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const int64_t rows = p.ptr.rows;
+    CUtensorMap a, b;
+    if (!tc::EncodeSlabs(&a, type, planes_a, p.k, rows, 3, p.k * 2, rows * p.k * 2, kRows / 64) ||
+        !tc::EncodeSlabs(&b, type, planes_b, p.n, rows, 3, p.n * 2, rows * p.n * 2, p.n <= 128 ? 2 : 4)) {
+        return OPSGNN_ERR_UNSUPPORTED;
+    }
+    const int64_t down = (q.chunk > 0 ? p.ptr.rows / q.chunk + p.ptr.segments : p.ptr.segments) * CeilDiv(p.k, kRows);
+    const int status = p.n <= 128 ? Launch<false, float, 128, kOuter>(a, a, b, q, down, stream)
+                                  : Launch<false, float, 256, kOuter>(a, a, b, q, down * CeilDiv(p.n, 256), stream);
+    return status == OPSGNN_OK && q.chunk > 0 ? JoinPieces(p, q.chunk, q.partial, stream) : status;
+}
+
+int SplitWeight(const RowsProblem& p, void* planes, cudaStream_t stream)
+{
+    const bool turned = p.b_k == 1 && p.b_n != 1;
+    return Split(static_cast<const float*>(p.b), p.ptr.segments, turned ? p.n : p.k, turned ? p.k : p.n, p.b_segment,
+                 turned ? p.b_n : p.b_k, planes, stream);
+}
+
+int SplitMatrix(const void* src, int64_t rows, int64_t width, int64_t stride, void* planes, cudaStream_t stream)
+{
+    return Split(static_cast<const float*>(src), 1, rows, width, 0, stride, planes, stream);
+}
+
+}  // namespace
+
+int RunRowsSplit(const RowsProblem& p, void* workspace, cudaStream_t stream)
+{
+    bool turned;
+    if (!RowsSplittable(p, turned) || !Aligned(workspace, 16)) {
+        return OPSGNN_ERR_UNSUPPORTED;
+    }
+    char* planes_a = static_cast<char*>(workspace);
+    char* planes_b = planes_a + PlaneBytes(p.ptr.rows * p.k);
+    int status = SplitMatrix(p.a, p.ptr.rows, p.k, p.lda, planes_a, stream);
+    status = status != OPSGNN_OK ? status : SplitWeight(p, planes_b, stream);
+    return status != OPSGNN_OK ? status : RowsFromPlanes(p, planes_a, planes_b, stream);
 }
 
 int RunOuterSplit(const OuterProblem& p, void* workspace, cudaStream_t stream)
@@ -558,36 +657,40 @@ int RunOuterSplit(const OuterProblem& p, void* workspace, cudaStream_t stream)
     if (!OuterSplittable(p) || !Aligned(workspace, 16)) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
-    Params q{};
-    q.ptr = p.ptr;
-    q.out = p.out;
-    q.m = p.k;
-    q.n = p.n;
-    q.chunk = OuterChunk(p.ptr.rows, p.ptr.segments, p.k, p.n);
-    q.a = static_cast<const float*>(p.a);
-    q.b = static_cast<const float*>(p.b);
-    q.lda = p.lda;
-    q.ldb = p.ldb;
-    OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
     char* planes_a = static_cast<char*>(workspace);
     char* planes_b = planes_a + PlaneBytes(p.ptr.rows * p.k);
-    q.partial = reinterpret_cast<float*>(planes_b + PlaneBytes(p.ptr.rows * p.n));
-    CUtensorMap a, b;
-    if (!Map3(&a, false, planes_a, p.k, p.ptr.rows, 3, p.k, p.ptr.rows * p.k, 64) ||
-        !Map3(&b, false, planes_b, p.n, p.ptr.rows, 3, p.n, p.ptr.rows * p.n, 64)) {
+    char* partial = planes_b + PlaneBytes(p.ptr.rows * p.n);
+    int status = SplitMatrix(p.a, p.ptr.rows, p.k, p.lda, planes_a, stream);
+    status = status != OPSGNN_OK ? status : SplitMatrix(p.b, p.ptr.rows, p.n, p.ldb, planes_b, stream);
+    return status != OPSGNN_OK ? status : OuterFromPlanes(p, planes_a, planes_b, partial, stream);
+}
+
+int64_t GradsSplitBytes(int64_t rows, int64_t segments, int64_t k, int64_t n)
+{
+    return PlaneBytes(rows * k) + PlaneBytes(rows * n) + PlaneBytes(segments * k * n) +
+           std::max(OuterPartialBytes(rows, segments, k, n), OuterPartialBytes(rows, segments, n, k));
+}
+
+int RunGradsSplit(const RowsProblem& rows, const OuterProblem& outer, bool turned, void* workspace, cudaStream_t stream)
+{
+    bool ignored;
+    if (!RowsSplittable(rows, ignored) || !OuterSplittable(outer) || !Aligned(workspace, 16)) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
-    int status = Split(q.a, 1, p.ptr.rows, p.k, 0, p.lda, planes_a, stream);
-    if (status == OPSGNN_OK) {
-        status = Split(q.b, 1, p.ptr.rows, p.n, 0, p.ldb, planes_b, stream);
-    }
+    const void* src = turned ? outer.b : outer.a;
+    const int64_t width = turned ? outer.n : outer.k, stride = turned ? outer.ldb : outer.lda;
+    char* planes_src = static_cast<char*>(workspace);
+    char* planes_grad = planes_src + PlaneBytes(rows.ptr.rows * width);
+    char* planes_weight = planes_grad + PlaneBytes(rows.ptr.rows * rows.k);
+    char* partial = planes_weight + PlaneBytes(rows.ptr.segments * rows.k * rows.n);
+    int status = SplitMatrix(rows.a, rows.ptr.rows, rows.k, rows.lda, planes_grad, stream);
+    status = status != OPSGNN_OK ? status : SplitWeight(rows, planes_weight, stream);
+    status = status != OPSGNN_OK ? status : RowsFromPlanes(rows, planes_grad, planes_weight, stream);
+    status = status != OPSGNN_OK ? status : SplitMatrix(src, rows.ptr.rows, width, stride, planes_src, stream);
     if (status != OPSGNN_OK) {
         return status;
     }
-    const int64_t down = (q.chunk > 0 ? p.ptr.rows / q.chunk + p.ptr.segments : p.ptr.segments) * CeilDiv(p.k, kRows);
-    status = p.n <= 128 ? Launch<false, float, 128, kOuter>(a, b, q, down, stream)
-                        : Launch<false, float, 256, kOuter>(a, b, q, down * CeilDiv(p.n, 256), stream);
-    return status == OPSGNN_OK && q.chunk > 0 ? JoinPieces(p, q.chunk, q.partial, stream) : status;
+    return OuterFromPlanes(outer, turned ? planes_grad : planes_src, turned ? planes_src : planes_grad, partial, stream);
 }
 
 int RunRowsFp8(const RowsProblem& p, cudaStream_t stream)
@@ -608,15 +711,15 @@ int RunRowsFp8(const RowsProblem& p, cudaStream_t stream)
     q.k = p.k;
     OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
     const bool narrow = p.n <= 128;
-    CUtensorMap a, b;
-    if (!Map3(&a, true, p.a, p.k, p.ptr.rows, 1, p.lda, p.lda, kRows) ||
+    CUtensorMap a, tail, b;
+    if (!Map3(&a, true, p.a, p.k, p.ptr.rows, 1, p.lda, p.lda, kRows) || !Map3(&tail, true, p.a, p.k, p.ptr.rows, 1, p.lda, p.lda, kBoxRows) ||
         !Map3(&b, true, p.b, p.k, p.n, p.ptr.segments, p.b_n, p.b_segment, narrow ? 128 : 256)) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
     const int64_t tiles = (p.ptr.rows / kRows + p.ptr.segments) * CeilDiv(p.n, narrow ? 128 : 256);
     auto run = [&](auto tag) {
         using O = decltype(tag);
-        return narrow ? Launch<true, O, 128, kRowsTurned>(a, b, q, tiles, stream) : Launch<true, O, 256, kRowsTurned>(a, b, q, tiles, stream);
+        return narrow ? Launch<true, O, 128, kRowsTurned>(a, tail, b, q, tiles, stream) : Launch<true, O, 256, kRowsTurned>(a, tail, b, q, tiles, stream);
     };
     switch (p.out_type) {
         case OPSGNN_F32:

@@ -74,10 +74,10 @@ template <class T, class O> __global__ void __launch_bounds__(kThreads) RowsKern
     O* out = static_cast<O*>(p.out);
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
     const int64_t across = (p.n + kTile - 1) / kTile;
-    SegmentWalk<kTile> walk;
+    SegmentWalk<kTile, int64_t> walk;
     walk.Start(p.ptr);
     for (int64_t t = blockIdx.x;; t += gridDim.x) {
-        if (!walk.Seek(t / across)) {
+        if (!walk.Seek(p.ptr, t / across)) {
             break;
         }
         const int64_t col0 = t % across * kTile;
@@ -144,7 +144,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) OuterKernel(Outer
     for (int64_t t = blockIdx.x; t < p.ptr.segments * down * across; t += gridDim.x) {
         const int64_t e = t / (down * across), k0 = t / across % down * kTile, n0 = t % across * kTile;
         int64_t begin, end;
-        p.ptr.Range(e, begin, end);
+        p.ptr.Range<int64_t>(e, begin, end);
         float total[4][4] = {};
         Multiply([&](int r, int64_t d) { return k0 + r < p.k ? ValueOf(a + (begin + d) * p.lda + k0 + r) : 0.0f; },
                  [&](int64_t d, int c) { return n0 + c < p.n ? ValueOf(b + (begin + d) * p.ldb + n0 + c) : 0.0f; }, false, false,

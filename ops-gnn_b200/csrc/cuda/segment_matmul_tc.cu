@@ -37,10 +37,21 @@ bool EncodeMap(CUtensorMap* map, CUtensorMapDataType type, int rank, const void*
     if (encode == nullptr) {
         return false;
     }
-    const cuuint32_t ones[3] = {1, 1, 1};
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
     return encode(map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), reinterpret_cast<const cuuint64_t*>(sizes),
                   reinterpret_cast<const cuuint64_t*>(strides), box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool EncodeSlabs(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t extent, int64_t rows, int64_t depth,
+                 int64_t row_bytes, int64_t depth_bytes, int slabs)
+{
+    const bool whole = WholeSlabs(extent);
+    const uint64_t sizes[4] = {static_cast<uint64_t>(whole ? 64 : extent), static_cast<uint64_t>(rows),
+                               static_cast<uint64_t>(whole ? extent / 64 : 1), static_cast<uint64_t>(depth)};
+    const uint64_t strides[3] = {static_cast<uint64_t>(row_bytes), 128, static_cast<uint64_t>(depth_bytes)};
+    const uint32_t box[4] = {64, 64, whole ? static_cast<uint32_t>(slabs) : 1u, 1};
+    return EncodeMap(map, type, 4, base, sizes, strides, box);
 }
 
 }  // namespace tc
@@ -49,6 +60,7 @@ namespace segmm {
 namespace {
 
 constexpr int kRows = 128;     // rows of a tile
+constexpr int kBoxRows = 32;   // rows of a per load where a tile is not full
 constexpr int kDepth = 64;     // reduced index per stage: one 128-byte row of 16-bit values
 constexpr int kThreads = 256;
 constexpr int kSlab = kDepth * 128;          // bytes of 64 rows of 128 bytes
@@ -64,6 +76,7 @@ struct Params {
     SegmentPointers ptr;
     void* out;
     int64_t m, n, k;   // rows form: n columns, k reduced; outer form: m x n results per segment
+    bool whole_a, whole_b;  // MN-major operands: all slabs in one load
     int64_t chunk;     // outer form: rows per partial result; 0: a segment's rows in one piece
     float* partial;    // [pieces][m][n]
     WaitSettings wait;
@@ -89,7 +102,8 @@ template <class T> __device__ __forceinline__ uint32_t TwoOf(uint32_t a, uint32_
 
 template <class T, int BN, int FORM>
 __global__ void __launch_bounds__(kThreads, 1)
-    TensorKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p)
+    TensorKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_tail,
+                 const __grid_constant__ CUtensorMap map_b, const Params p)
 {
     constexpr int kStages = Stages<BN>();
     constexpr int kStage = StageBytes<BN>();
@@ -121,44 +135,46 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = bar.tmem;
     const tc::Waiter wait{&bar.stop, p.wait};
 
-    const int64_t across = (p.n + BN - 1) / BN;
-    const int64_t down = FORM == kOuter ? (p.m + kRows - 1) / kRows : 0;
-    const int64_t outer_tiles = FORM == kOuter ? p.ptr.segments * down * across : 0;
-    SegmentWalk<FORM == kOuter ? 0 : kRows> walk;
-    if (warp != 2 && warp != 3 && (FORM != kOuter || p.chunk > 0)) {
-        walk.Start(p.ptr, FORM == kOuter ? p.chunk : kRows);
+    // Rows, widths and tile numbers fit 32 bits (checked on the host); offsets in memory are formed in 64.
+    const int n = static_cast<int>(p.n), m = static_cast<int>(p.m), width = static_cast<int>(p.k), chunk = static_cast<int>(p.chunk);
+    const int across = (n + BN - 1) / BN;
+    const int down = FORM == kOuter ? (m + kRows - 1) / kRows : 1;
+    SegmentWalk<FORM == kOuter ? 0 : kRows, int> walk;
+    if (warp != 2 && warp != 3 && (FORM != kOuter || chunk > 0)) {
+        walk.Start(p.ptr, FORM == kOuter ? chunk : kRows);
     }
     // Tile t: its segment, first result row and column, and the range of the reduced index.
-    int64_t segment = 0, row = 0, row_end = 0, column = 0, from = 0, depth = 0;
-    auto find = [&](int64_t t) {
+    int segment = 0, row = 0, row_end = 0, column = 0, from = 0, depth = 0;
+    auto find = [&](int t) {
         column = t % across * BN;
+        t /= across;
         if constexpr (FORM == kOuter) {
-            row = t / across % down * kRows;
-            row_end = p.m;
-            segment = t / (down * across);  // of the result to write: a segment or a piece
-            if (p.chunk > 0) {
-                if (!walk.Seek(segment)) {
+            row = t % down * kRows;
+            row_end = m;
+            segment = t / down;  // of the result to write: a segment or a piece
+            if (chunk > 0) {
+                if (!walk.Seek(p.ptr, segment)) {
                     return false;
                 }
                 from = walk.row;
-                depth = walk.row_end - from < p.chunk ? walk.row_end - from : p.chunk;
+                depth = min(walk.row_end - from, chunk);
                 return true;
             }
-            if (t >= outer_tiles) {
+            if (segment >= p.ptr.segments) {
                 return false;
             }
-            int64_t end;
-            p.ptr.Range(segment, from, end);
+            int end;
+            p.ptr.Range<int>(segment, from, end);
             depth = end - from;
             return true;
         } else {
-            if (!walk.Seek(t / across)) {
+            if (!walk.Seek(p.ptr, t)) {
                 return false;
             }
             segment = walk.segment;
             row = walk.row;
             row_end = walk.row_end;
-            depth = p.k;
+            depth = width;
             return true;
         }
     };
@@ -166,8 +182,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t filled = 0;  // stages the loading warp has asked for
     if (warp == 0) {
         bool going = true;
-        for (int64_t t = blockIdx.x; going && find(t); t += gridDim.x) {
-            for (int64_t k = 0; k < depth; k += kDepth, ++filled) {
+        for (int t = blockIdx.x; going && find(t); t += gridDim.x) {
+            for (int k = 0; k < depth; k += kDepth, ++filled) {
                 const uint32_t s = filled % kStages;
                 going = wait.Warp(&bar.empty[s], ((filled / kStages) & 1) ^ 1);
                 if (!going) {
@@ -175,26 +191,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (lane == 0) {
                     const uint32_t a = tc::Shared(smem) + s * kStage, b = a + kRows * 128;
-                    tc::BarExpect(&bar.full[s], kStage);
                     if constexpr (FORM == kOuter) {
-#pragma unroll
-                        for (int i = 0; i < kRows / 64; ++i) {
-                            tc::Load2(map_a, &bar.full[s], a + i * kSlab, static_cast<int>(row) + i * 64, static_cast<int>(from + k));
-                        }
-#pragma unroll
-                        for (int i = 0; i < BN / 64; ++i) {
-                            tc::Load2(map_b, &bar.full[s], b + i * kSlab, static_cast<int>(column) + i * 64, static_cast<int>(from + k));
-                        }
+                        tc::BarExpect(&bar.full[s], kStage);
+                        tc::LoadSlabs(map_a, &bar.full[s], a, row, from + k, 0, kRows / 64, p.whole_a);
+                        tc::LoadSlabs(map_b, &bar.full[s], b, column, from + k, 0, BN / 64, p.whole_b);
                     } else {
-                        tc::Load2(map_a, &bar.full[s], a, static_cast<int>(k), static_cast<int>(row));
-                        if constexpr (FORM == kRowsTurned) {
-                            tc::Load3(map_b, &bar.full[s], b, static_cast<int>(k), static_cast<int>(column), static_cast<int>(segment));
+                        // Only the rows that are the segment's, to the next 32; what else lies in the stage is multiplied into
+                        // rows that are not stored.
+                        const int boxes = min(row_end - row + kBoxRows - 1, kRows) / kBoxRows;
+                        tc::BarExpect(&bar.full[s], boxes * kBoxRows * 128 + BN * 128);
+                        if (boxes * kBoxRows == kRows) {
+                            tc::Load2(map_a, &bar.full[s], a, k, row);
                         } else {
-#pragma unroll
-                            for (int i = 0; i < BN / 64; ++i) {
-                                tc::Load3(map_b, &bar.full[s], b + i * kSlab, static_cast<int>(column) + i * 64, static_cast<int>(k),
-                                          static_cast<int>(segment));
+                            for (int i = 0; i < boxes; ++i) {
+                                tc::Load2(map_tail, &bar.full[s], a + i * kBoxRows * 128, k, row + i * kBoxRows);
                             }
+                        }
+                        if constexpr (FORM == kRowsTurned) {
+                            tc::Load3(map_b, &bar.full[s], b, k, column, segment);
+                        } else {
+                            tc::LoadSlabs(map_b, &bar.full[s], b, column, k, segment, BN / 64, p.whole_b);
                         }
                     }
                 }
@@ -205,14 +221,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t shape = tc::Shape(kRows, BN, std::is_same<T, __nv_bfloat16>::value ? 1 : 0, FORM == kOuter, FORM != kRowsTurned);
         uint32_t used = 0, tiles = 0;
         bool going = true;
-        for (int64_t t = blockIdx.x; going && find(t); t += gridDim.x) {
+        for (int t = blockIdx.x; going && find(t); t += gridDim.x) {
             if (depth == 0) {
                 continue;
             }
             const uint32_t half = tiles & 1;
             going = wait.Warp(&bar.free[half], ((tiles >> 1) & 1) ^ 1);
             tc::FenceAfter();
-            for (int64_t k = 0; going && k < depth; k += kDepth, ++used) {
+            for (int k = 0; going && k < depth; k += kDepth, ++used) {
                 const uint32_t s = used % kStages;
                 going = wait.Warp(&bar.full[s], (used / kStages) & 1);
                 if (!going) {
@@ -222,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if constexpr (FORM == kOuter) {
                     if (depth - k < kDepth) {
                         // Rows of the next segment: zero them in every slab of both operands.
-                        const int first = static_cast<int>(depth - k);
+                        const int first = (depth - k);
                         for (int i = first * 8 + lane; i < kDepth * 8; i += 32) {
 #pragma unroll
                             for (int slab = 0; slab < kStage / kSlab; ++slab) {
@@ -270,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         T* out = static_cast<T*>(p.out);
         uint32_t tiles = 0;
         bool going = true;
-        for (int64_t t = blockIdx.x; going && find(t); t += gridDim.x) {
+        for (int t = blockIdx.x; going && find(t); t += gridDim.x) {
             const uint32_t half = tiles & 1;
             if (depth > 0) {
                 going = wait.Warp(&bar.done[half], (tiles >> 1) & 1);
@@ -280,10 +296,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc::FenceAfter();
             }
             T* to = out + (FORM == kOuter ? segment * p.m * p.n : 0);
-            const int64_t first = row + quarter * 32;
+            const int first = row + quarter * 32;
 #pragma unroll 1
             for (int c = 0; c < BN; c += 64) {
-                if (column + c >= p.n) {
+                if (column + c >= n) {
                     break;
                 }
                 uint32_t words[32];
@@ -305,12 +321,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
                             }
                             __syncwarp();
-                            const int64_t col = column + c + side * 32 + piece * 4;
+                            const int col = column + c + side * 32 + piece * 4;
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
                                 const int r = i * 4 + (lane >> 3);
                                 const uint4 value = *reinterpret_cast<const uint4*>(mine + r * 128 + ((piece ^ (r & 7)) << 4));
-                                if (first + r < row_end && col < p.n) {
+                                if (first + r < row_end && col < n) {
                                     *reinterpret_cast<uint4*>(p.partial + segment * p.m * p.n + (first + r) * p.n + col) = value;
                                 }
                             }
@@ -337,12 +353,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
                 }
                 __syncwarp();
-                const int64_t col = column + c + piece * 8;
+                const int col = column + c + piece * 8;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int r = i * 4 + (lane >> 3);
                     const uint4 value = *reinterpret_cast<const uint4*>(mine + r * 128 + ((piece ^ (r & 7)) << 4));
-                    if (first + r < row_end && col < p.n) {
+                    if (first + r < row_end && col < n) {
                         *reinterpret_cast<uint4*>(to + (first + r) * p.n + col) = value;
                     }
                 }
@@ -402,11 +418,14 @@ bool Map2(CUtensorMap* map, int type, const void* base, int64_t inner, int64_t r
 }
 
 template <class T, int BN, int FORM>
-int Launch(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int64_t tiles, cudaStream_t stream)
+int Launch(const CUtensorMap& a, const CUtensorMap& tail, const CUtensorMap& b, const Params& p, int64_t tiles, cudaStream_t stream)
 {
+    if (tiles >= INT32_MAX - 4096) {
+        return OPSGNN_ERR_UNSUPPORTED;
+    }
     OPSGNN_CUDA_TRY(cudaFuncSetAttribute(TensorKernel<T, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, SharedBytes<BN>()));
     const int grid = static_cast<int>(std::min<int64_t>(std::max<int64_t>(tiles, 1), SmCount()));
-    TensorKernel<T, BN, FORM><<<grid, kThreads, SharedBytes<BN>(), stream>>>(a, b, p);
+    TensorKernel<T, BN, FORM><<<grid, kThreads, SharedBytes<BN>(), stream>>>(a, tail, b, p);
     return LaunchStatus();
 }
 
@@ -438,19 +457,23 @@ int RunRowsTensor(const RowsProblem& p, cudaStream_t stream)
     q.k = p.k;
     OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
     const bool narrow = p.n <= 128;
-    CUtensorMap a, b;
+    q.whole_b = tc::WholeSlabs(p.n);
+    CUtensorMap a, tail, b;
     const uint64_t sizes[3] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(other), static_cast<uint64_t>(p.ptr.segments)};
     const uint64_t strides[2] = {static_cast<uint64_t>(stride) * 2, static_cast<uint64_t>(p.b_segment) * 2};
-    const uint32_t box[3] = {64, turned ? (narrow ? 128u : 256u) : static_cast<uint32_t>(kDepth), 1};
+    const uint32_t box[3] = {64, narrow ? 128u : 256u, 1};
+    const CUtensorMapDataType type = TypeOf(p.in_type);
     if (!Map2(&a, p.in_type, p.a, p.k, p.ptr.rows, p.lda, kDepth, kRows) ||
-        !tc::EncodeMap(&b, TypeOf(p.in_type), 3, p.b, sizes, strides, box)) {
+        !Map2(&tail, p.in_type, p.a, p.k, p.ptr.rows, p.lda, kDepth, kBoxRows) ||
+        !(turned ? tc::EncodeMap(&b, type, 3, p.b, sizes, strides, box)
+                 : tc::EncodeSlabs(&b, type, p.b, p.n, p.k, p.ptr.segments, stride * 2, p.b_segment * 2, narrow ? 2 : 4))) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
     auto run = [&](auto tag, auto width) {
         using T = decltype(tag);
         constexpr int BN = decltype(width)::value;
         const int64_t tiles = (p.ptr.rows / kRows + p.ptr.segments) * CeilDiv(p.n, BN);
-        return turned ? Launch<T, BN, kRowsTurned>(a, b, q, tiles, stream) : Launch<T, BN, kRowsWide>(a, b, q, tiles, stream);
+        return turned ? Launch<T, BN, kRowsTurned>(a, tail, b, q, tiles, stream) : Launch<T, BN, kRowsWide>(a, tail, b, q, tiles, stream);
     };
     return ByType<0>(p.in_type, narrow, run);
 }
@@ -463,26 +486,18 @@ __global__ void __launch_bounds__(256) JoinKernel(SegmentPointers ptr, int64_t c
                                                   T* __restrict__ out)
 {
     const int64_t e = blockIdx.y;
-    const int lane = threadIdx.x & 31;
-    int64_t before = 0, begin, end;
-    for (int64_t s = lane; s < e; s += 32) {
-        ptr.Range(s, begin, end);
-        before += (end - begin + chunk - 1) / chunk;
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        before += __shfl_xor_sync(0xffffffffu, before, d);
-    }
-    ptr.Range(e, begin, end);
-    const int64_t pieces = (end - begin + chunk - 1) / chunk;
+    SegmentWalk<0, int> walk;  // numbers the pieces as the kernel that made them did
+    walk.Start(ptr, static_cast<int>(chunk));
+    int before, pieces;
+    walk.Count(ptr, static_cast<int>(e), before, pieces);
     const int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 4;
     if (i >= size) {
         return;
     }
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-    for (int64_t c = 0; c < pieces; ++c) {
-        const float4 v = __ldcs(reinterpret_cast<const float4*>(partial + (before + c) * size + i));
+    for (int c = 0; c < pieces; ++c) {
+        const float4 v = __ldcs(reinterpret_cast<const float4*>(partial + static_cast<int64_t>(before + c) * size + i));
         sum.x += v.x;
         sum.y += v.y;
         sum.z += v.z;
@@ -505,7 +520,7 @@ int64_t OuterChunk(int64_t rows, int64_t segments, int64_t k, int64_t n)
     }
     const int64_t pieces = std::max<int64_t>(1, static_cast<int64_t>(SmCount()) * 4 / tiles);
     const int64_t chunk = std::max<int64_t>(256, AlignUp(CeilDiv(rows, pieces), kDepth));
-    return chunk >= rows ? 0 : chunk;
+    return chunk >= rows || rows < 8192 ? 0 : chunk;
 }
 
 int64_t OuterPartialBytes(int64_t rows, int64_t segments, int64_t k, int64_t n)
@@ -546,17 +561,21 @@ int RunOuterTensor(const OuterProblem& p, void* workspace, cudaStream_t stream)
     q.chunk = OuterChunk(p.ptr.rows, p.ptr.segments, p.k, p.n);
     q.partial = static_cast<float*>(workspace);
     OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
+    const bool narrow = p.n <= 128;
+    q.whole_a = tc::WholeSlabs(p.k);
+    q.whole_b = tc::WholeSlabs(p.n);
     CUtensorMap a, b;
-    if (!Map2(&a, p.type, p.a, p.k, p.ptr.rows, p.lda, 64, kDepth) || !Map2(&b, p.type, p.b, p.n, p.ptr.rows, p.ldb, 64, kDepth)) {
+    if (!tc::EncodeSlabs(&a, TypeOf(p.type), p.a, p.k, p.ptr.rows, 1, p.lda * 2, 16, kRows / 64) ||
+        !tc::EncodeSlabs(&b, TypeOf(p.type), p.b, p.n, p.ptr.rows, 1, p.ldb * 2, 16, narrow ? 2 : 4)) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
     auto run = [&](auto tag, auto width) {
         using T = decltype(tag);
         constexpr int BN = decltype(width)::value;
         const int64_t results = q.chunk > 0 ? p.ptr.rows / q.chunk + p.ptr.segments : p.ptr.segments;
-        return Launch<T, BN, kOuter>(a, b, q, results * CeilDiv(p.k, kRows) * CeilDiv(p.n, BN), stream);
+        return Launch<T, BN, kOuter>(a, a, b, q, results * CeilDiv(p.k, kRows) * CeilDiv(p.n, BN), stream);
     };
-    const int status = ByType<0>(p.type, p.n <= 128, run);
+    const int status = ByType<0>(p.type, narrow, run);
     return status == OPSGNN_OK && q.chunk > 0 ? JoinPieces(p, q.chunk, q.partial, stream) : status;
 }
 

@@ -17,77 +17,104 @@ struct SegmentPointers {
         const int64_t v = wide ? __ldg(static_cast<const long long*>(data) + i) : __ldg(static_cast<const int*>(data) + i);
         return v < 0 ? 0 : (v > rows ? rows : v);
     }
-    __device__ __forceinline__ void Range(int64_t e, int64_t& begin, int64_t& end) const
+    template <class I> __device__ __forceinline__ void Range(I e, I& begin, I& end) const
     {
         if (data == nullptr) {  // one dense segment
             begin = 0;
-            end = rows;
+            end = static_cast<I>(rows);
             return;
         }
-        begin = Raw(e);
-        const int64_t last = Raw(e + 1);
+        begin = static_cast<I>(Raw(e));
+        const I last = static_cast<I>(Raw(static_cast<int64_t>(e) + 1));
         end = last > begin ? last : begin;
     }
 };
 
 // Row tiles of all segments in order, TILE rows each (a segment's last one may be short; an empty segment has none).
 // Seek(t) is called by a whole warp with ascending t and finds tile t by a running warp scan over 32 segments at a time:
-// no tile table, no workspace, no limit on the number of segments.  TILE 0: the number of rows is given to Start.
-template <int TILE> struct SegmentWalk {
-    SegmentPointers ptr;
-    int64_t length;              // rows per tile
-    int64_t from, base;          // first segment of the 32 at hand; tiles before them
-    int64_t begin, end;          // this lane's segment
-    int64_t inclusive;           // tiles of the 32 up to and with this lane's segment
+// no tile table, no workspace, no limit on the number of segments.  TILE 0: the number of rows is given to Start.  I: the
+// type of rows and tile numbers, int where the host has checked that they fit (half the registers).
+template <int TILE, class I> struct SegmentWalk {
+    I length;              // rows per tile
+    I segments;
+    I from, base;          // first segment of the 32 at hand; tiles before them
+    I high;                // largest pointer before them
+    I begin, end;          // this lane's segment
+    I inclusive;           // tiles of the 32 up to and with this lane's segment
     // what Seek found
-    int64_t segment, row, row_end;
+    I segment, row, row_end;
 
-    __device__ __forceinline__ int64_t Tiles() const
+    __device__ __forceinline__ I Tiles() const
     {
-        const int64_t tile = TILE > 0 ? TILE : length;
+        const I tile = TILE > 0 ? TILE : length;
         return (end - begin + tile - 1) / tile;
     }
-    __device__ __forceinline__ void Load()
+    __device__ __forceinline__ void Load(const SegmentPointers& p)
     {
         const int lane = threadIdx.x & 31;
-        begin = end = 0;
-        if (from + lane < ptr.segments) {
-            ptr.Range(from + lane, begin, end);
+        end = 0;
+        if (from + lane < segments) {
+            end = p.data != nullptr ? static_cast<I>(p.Raw(static_cast<int64_t>(from) + lane + 1)) : static_cast<I>(p.rows);
         }
+        // A pointer below an earlier one counts as that one: segments never overlap, and all tiles together are bounded.
+        end = end > high ? end : high;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const I up = __shfl_up_sync(0xffffffffu, end, d);
+            end = lane >= d && up > end ? up : end;
+        }
+        begin = __shfl_up_sync(0xffffffffu, end, 1);
+        begin = lane == 0 ? high : begin;
+        high = __shfl_sync(0xffffffffu, end, 31);
         inclusive = Tiles();
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int64_t up = __shfl_up_sync(0xffffffffu, inclusive, d);
+            const I up = __shfl_up_sync(0xffffffffu, inclusive, d);
             inclusive += lane >= d ? up : 0;
         }
     }
-    __device__ __forceinline__ void Start(const SegmentPointers& p, int64_t tile = TILE)
+    __device__ __forceinline__ void Start(const SegmentPointers& p, I tile = TILE)
     {
-        ptr = p;
         length = tile;
+        segments = static_cast<I>(p.segments);
         from = 0;
         base = 0;
-        Load();
+        high = p.data != nullptr ? static_cast<I>(p.Raw(0)) : 0;
+        Load(p);
+    }
+    // Tiles before segment e and of it (ascending e).
+    __device__ __forceinline__ void Count(const SegmentPointers& p, I e, I& before, I& tiles)
+    {
+        while (from + 32 <= e) {
+            Next(p);
+        }
+        const int owner = static_cast<int>(e - from);
+        tiles = __shfl_sync(0xffffffffu, Tiles(), owner);
+        before = __shfl_sync(0xffffffffu, base + inclusive, owner) - tiles;
+    }
+    __device__ __forceinline__ void Next(const SegmentPointers& p)
+    {
+        base += __shfl_sync(0xffffffffu, inclusive, 31);
+        from += 32;
+        Load(p);
     }
     // False past the last tile.
-    __device__ __forceinline__ bool Seek(int64_t t)
+    __device__ __forceinline__ bool Seek(const SegmentPointers& p, I t)
     {
         while (true) {
             const unsigned there = __ballot_sync(0xffffffffu, t < base + inclusive);
             if (there != 0) {
                 const int owner = __ffs(there) - 1;
-                const int64_t first = __shfl_sync(0xffffffffu, base + inclusive - Tiles(), owner);
+                const I first = __shfl_sync(0xffffffffu, base + inclusive - Tiles(), owner);
                 row_end = __shfl_sync(0xffffffffu, end, owner);
                 row = __shfl_sync(0xffffffffu, begin, owner) + (t - first) * (TILE > 0 ? TILE : length);
                 segment = from + owner;
                 return true;
             }
-            base += __shfl_sync(0xffffffffu, inclusive, 31);
-            from += 32;
-            if (from >= ptr.segments) {
+            if (from + 32 >= segments) {
                 return false;
             }
-            Load();
+            Next(p);
         }
     }
 };

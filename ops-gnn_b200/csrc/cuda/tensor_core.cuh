@@ -88,6 +88,13 @@ __device__ __forceinline__ void Load3(const CUtensorMap& map, uint64_t* bar, uin
                  "l"(&map), "r"(Shared(bar)), "r"(x), "r"(y), "r"(z)
                  : "memory");
 }
+__device__ __forceinline__ void Load4(const CUtensorMap& map, uint64_t* bar, uint32_t to, int x, int y, int z, int w)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(to),
+        "l"(&map), "r"(Shared(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
 // Writes to shared memory by this thread become visible to tcgen05.mma and TMA.
 __device__ __forceinline__ void FenceAsync() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -173,7 +180,27 @@ constexpr uint32_t Shape(int m, int n, int type, bool a_mn, bool b_mn)
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
 
-// A tile map of up to 3 dimensions with 128-byte swizzle; strides[i] (bytes, multiples of 16) belong to dimension i + 1.
+// An MN-major operand is a row of slabs, 64 values of the kept index by 64 of the reduced one.  Where the kept extent is a
+// multiple of 64 one load takes `slabs` of them (dimensions 64, rows, slab, depth); else each slab is a load of its own, with
+// the map's bounds filling zeros past the extent (dimensions extent, rows, 1, depth).  Loads are issued by one thread and
+// their number matters: four 32-row loads and four slabs a stage in place of one each cost a quarter of the rate.
+constexpr int kSlabBytes = 64 * 128;
+__device__ __forceinline__ void LoadSlabs(const CUtensorMap& map, uint64_t* bar, uint32_t to, int column, int row, int depth, int slabs,
+                                          bool whole)
+{
+    if (whole) {
+        Load4(map, bar, to, 0, row, column / 64, depth);
+    } else {
+        for (int i = 0; i < slabs; ++i) {
+            Load4(map, bar, to + i * kSlabBytes, column + i * 64, row, 0, depth);
+        }
+    }
+}
+inline bool WholeSlabs(int64_t extent) { return extent % 64 == 0; }
+bool EncodeSlabs(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t extent, int64_t rows, int64_t depth,
+                 int64_t row_bytes, int64_t depth_bytes, int slabs);
+
+// A tile map of up to 4 dimensions with 128-byte swizzle; strides[i] (bytes, multiples of 16) belong to dimension i + 1.
 // False where the driver refuses it.
 bool EncodeMap(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* sizes, const uint64_t* strides,
                const uint32_t* box);

@@ -79,7 +79,7 @@ at::Tensor segment_matmul_forward(const at::Tensor& src, const at::Tensor& indpt
     OpsgnnSegmentMatmulDesc desc = DescOf(rows, indptr, weight.size(0), weight.size(2), src.scalar_type(), api);
     SetWeight(desc, matrices);
     int64_t bytes = 0;
-    CheckStatus(opsgnn_segment_matmul_workspace_bytes(&desc, 0, &bytes), api);
+    CheckStatus(opsgnn_segment_matmul_workspace_bytes(&desc, OPSGNN_SEGMENT_MATMUL_FORWARD, &bytes), api);
     const at::Tensor scratch = bytes > 0 ? Scratch(bytes, src) : at::Tensor();
     CheckStatus(opsgnn_segment_matmul(&desc, indptr.const_data_ptr(), rows.const_data_ptr(), matrices.const_data_ptr(), out.data_ptr(),
                                       bytes > 0 ? scratch.data_ptr() : nullptr, bytes, CurrentStream(src)),
@@ -102,7 +102,7 @@ at::Tensor segment_matmul_weight_grad(const at::Tensor& src, const at::Tensor& i
     at::Tensor out = at::empty({segments, src.size(1), grad.size(1)}, src.options());
     const OpsgnnSegmentMatmulDesc desc = DescOf(rows, indptr, segments, grad.size(1), src.scalar_type(), api);
     int64_t bytes = 0;
-    CheckStatus(opsgnn_segment_matmul_workspace_bytes(&desc, 1, &bytes), api);
+    CheckStatus(opsgnn_segment_matmul_workspace_bytes(&desc, OPSGNN_SEGMENT_MATMUL_WEIGHT_GRAD, &bytes), api);
     const at::Tensor scratch = bytes > 0 ? Scratch(bytes, src) : at::Tensor();
     CheckStatus(opsgnn_segment_matmul_weight_grad(&desc, indptr.const_data_ptr(), rows.const_data_ptr(), upstream.const_data_ptr(),
                                                   std::max(RowStride(upstream), upstream.size(1)), out.data_ptr(),
@@ -112,6 +112,30 @@ at::Tensor segment_matmul_weight_grad(const at::Tensor& src, const at::Tensor& i
 }
 
 namespace {
+
+// grad_src and, in the layout of weight, grad_weight.
+std::vector<at::Tensor> Gradients(const at::Tensor& src, const at::Tensor& indptr, const at::Tensor& weight, const at::Tensor& grad)
+{
+    const char* api = "segment_matmul backward";
+    c10::cuda::CUDAGuard guard(src.device());
+    RaiseIfDeviceStalled(src, api);
+    const at::Tensor rows = RowMajor(src), matrices = Matrices(weight), upstream = RowMajor(grad);
+    const bool turned = weight.stride(1) == 1 && weight.stride(2) != 1;
+    OpsgnnSegmentMatmulDesc desc = DescOf(rows, indptr, weight.size(0), weight.size(2), src.scalar_type(), api);
+    SetWeight(desc, matrices);
+    at::Tensor grad_src = at::empty(src.sizes(), src.options());
+    at::Tensor grad_weight = turned ? at::empty({weight.size(0), weight.size(2), weight.size(1)}, src.options())
+                                    : at::empty(weight.sizes(), src.options());
+    int64_t bytes = 0;
+    CheckStatus(opsgnn_segment_matmul_workspace_bytes(&desc, OPSGNN_SEGMENT_MATMUL_GRADS, &bytes), api);
+    const at::Tensor scratch = bytes > 0 ? Scratch(bytes, src) : at::Tensor();
+    CheckStatus(opsgnn_segment_matmul_grads(&desc, indptr.const_data_ptr(), rows.const_data_ptr(), matrices.const_data_ptr(),
+                                            upstream.const_data_ptr(), std::max(RowStride(upstream), upstream.size(1)),
+                                            grad_src.data_ptr(), grad_weight.data_ptr(), turned ? 1 : 0,
+                                            bytes > 0 ? scratch.data_ptr() : nullptr, bytes, CurrentStream(src)),
+                api);
+    return {grad_src, turned ? grad_weight.transpose(1, 2) : grad_weight};
+}
 
 class SegmentMatmul : public torch::autograd::Function<SegmentMatmul> {
 public:
@@ -126,17 +150,17 @@ public:
         PlannerScope scope;
         const auto saved = ctx->get_saved_variables();
         const at::Tensor src = saved[0].detach(), indptr = saved[1], weight = saved[2].detach(), grad = grads[0].detach();
-        at::Tensor grad_src, grad_weight;
-        if (ctx->needs_input_grad(0)) {
-            grad_src = segment_matmul_forward(grad, indptr, weight.transpose(1, 2));
+        const bool of_src = ctx->needs_input_grad(0), of_weight = ctx->needs_input_grad(2);
+        std::vector<at::Tensor> out(2);
+        if (of_src && of_weight) {
+            out = Gradients(src, indptr, weight, grad);
+        } else if (of_src) {
+            out[0] = segment_matmul_forward(grad, indptr, weight.transpose(1, 2));
+        } else if (of_weight) {  // in the layout of the weight
+            out[1] = weight.stride(1) == 1 && weight.stride(2) != 1 ? segment_matmul_weight_grad(grad, indptr, src).transpose(1, 2)
+                                                                    : segment_matmul_weight_grad(src, indptr, grad);
         }
-        if (ctx->needs_input_grad(2)) {
-            // in the layout of the weight
-            grad_weight = weight.stride(1) == 1 && weight.stride(2) != 1
-                              ? segment_matmul_weight_grad(grad, indptr, src).transpose(1, 2)
-                              : segment_matmul_weight_grad(src, indptr, grad);
-        }
-        auto out = OnceDifferentiable({grad_src, grad_weight}, "segment_matmul");
+        out = OnceDifferentiable(std::move(out), "segment_matmul");
         return {out[0], at::Tensor(), out[1]};
     }
 };

@@ -36,7 +36,8 @@ EXPORTS = (
     "opsgnn_scatter_workspace_bytes", "opsgnn_scatter",
     "opsgnn_grouped_workspace_bytes", "opsgnn_grouped_forward", "opsgnn_grouped_forward_permuted", "opsgnn_grouped_backward",
     "opsgnn_topk_route", "opsgnn_topk_route_backward", "opsgnn_route_csr_workspace_bytes", "opsgnn_route_csr",
-    "opsgnn_segment_matmul_workspace_bytes", "opsgnn_segment_matmul", "opsgnn_segment_matmul_weight_grad", "opsgnn_segment_matmul_fp8", "opsgnn_quantize_fp8",
+    "opsgnn_segment_matmul_workspace_bytes", "opsgnn_segment_matmul", "opsgnn_segment_matmul_weight_grad", "opsgnn_segment_matmul_grads",
+    "opsgnn_segment_matmul_fp8", "opsgnn_quantize_fp8",
 )
 
 
@@ -149,6 +150,8 @@ _PROTOTYPES = {
                                       c_void_p]),
     "opsgnn_segment_matmul_weight_grad": (c_int, [POINTER(SegmentMatmulDesc), c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
                                                   c_void_p, c_int64, c_void_p]),
+    "opsgnn_segment_matmul_grads": (c_int, [POINTER(SegmentMatmulDesc), c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
+                                            c_void_p, c_int, c_void_p, c_int64, c_void_p]),
     "opsgnn_segment_matmul_fp8": (c_int, [POINTER(SegmentMatmulDesc), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                           c_void_p, c_void_p]),
     "opsgnn_quantize_fp8": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p]),

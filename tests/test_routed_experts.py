@@ -249,12 +249,17 @@ def test_c_abi_refuses():
     assert matmul(rows, None, None, None, None, None, 0, None, out_type=_cabi.F32) == -2
     assert matmul(rows, None, None, None, None, None, 0, None, in_type=_cabi.F64, out_type=_cabi.F64) == -2
     assert matmul(rows, None, None, None, None, None, 0, None, index_type=_cabi.F32) == -1
+    grads = lib.opsgnn_segment_matmul_grads
+    assert matmul(grads, None, None, None, None, 8, None, None, 0, None, 0, None) == -1
+    assert matmul(grads, 16, None, None, None, 8, None, None, 0, None, 0, None, rows=0, segments=0) == 0
+    assert matmul(grads, 16, 16, 16, 16, 8, 16, 16, 0, None, 0, None, in_type=_cabi.F32, out_type=_cabi.F32) == -3
+    assert matmul(lib.opsgnn_segment_matmul_workspace_bytes, 3, ref(size)) == -1
     assert matmul(outer, None, None, None, 8, None, None, 0, None) == -1
     assert matmul(outer, None, None, None, 8, None, None, 0, None, segments=0) == 0
     four = dict(in_type=_cabi.F32, out_type=_cabi.F32)
     assert matmul(lib.opsgnn_segment_matmul_workspace_bytes, 0, ref(size), **four) == 0 and size.value >= 6 * (4 * 8 + 2 * 64)
     assert matmul(rows, 16, 16, 16, 16, None, 0, None, **four) == -3
-    assert matmul(lib.opsgnn_segment_matmul_workspace_bytes, 1, ref(size)) == 0 and size.value == 0
+    assert matmul(lib.opsgnn_segment_matmul_workspace_bytes, 0, ref(size)) == 0 and size.value == 0
     assert matmul(fp8, None, None, None, None, None, None, None) == -2
     assert matmul(fp8, None, None, None, None, None, None, None, in_type=_cabi.F8E4M3) == -1
     assert lib.opsgnn_quantize_fp8(None, _cabi.BF16, 1, 4, 4, 1, None, None, None) == -1
@@ -1008,3 +1013,21 @@ def test_segment_matmul_long_sums_in_pieces(cuda_device, dtype, lengths, k, n):
     again, = torch.autograd.grad(segment_matmul(*args, w), w, grad.to(cuda_device))
     assert torch.equal(first, again)
     _within(first, _plain_weight_grad(src, ptr, grad), _plain_weight_grad(src.abs(), ptr, grad.abs()), max(lengths) + 2, "grad_weight")
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", KINDS, ids=str)
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("k,n", [(64, 200), (33, 7)])
+def test_segment_matmul_one_gradient_at_a_time(cuda_device, dtype, turned, k, n):
+    from ops_gnn import segment_matmul
+
+    src, ptr, weight, grad = [t.to(cuda_device) for t in _matmul_inputs(([90, 0, 300], 1, 2, k, n), dtype)]
+    if turned:
+        weight = weight.transpose(1, 2).contiguous().transpose(1, 2)
+    x, w = src.clone().requires_grad_(), weight.detach().requires_grad_()
+    both = torch.autograd.grad(segment_matmul(x, ptr, w), (x, w), grad)
+    only_src, = torch.autograd.grad(segment_matmul(x, ptr, weight), x, grad)
+    only_weight, = torch.autograd.grad(segment_matmul(src, ptr, w), w, grad)
+    assert torch.equal(both[0], only_src) and torch.equal(both[1], only_weight)
+    assert both[1].stride() == w.stride()
