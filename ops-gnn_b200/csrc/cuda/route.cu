@@ -791,165 +791,211 @@ __global__ void __launch_bounds__(kWarps * 32) TopkBackwardKernel(RouteParams p,
 }
 
 // ---- route_csr -----------------------------------------------------------------------------------------------------------
-// Pairs (in the order they come) sorted by expert, stable: a counting sort in tiles of kTile consecutive pairs.  A label
-// outside [0, experts) is a dropped pair and counts in one more bin behind the last expert.
+// Pairs (in the order they come) sorted by expert, stable: a counting sort in tiles of consecutive pairs, one thread block per
+// tile.  A label outside [0, experts) is a dropped pair and counts in one more bin behind the last expert.
 //   CountKernel  per tile: how many pairs of each bin                                  -> counts[bin][tile]
 //   ScanKernel   per bin: exclusive prefix of its counts over the tiles, and its total -> counts, totals[bin]
 //   PlaceKernel  per tile: where every bin starts (prefix of the totals), then every pair's place: bin start + pairs of the
 //                bin in earlier tiles, in earlier warps of the tile, in earlier rounds of the warp, in lower lanes
 // One tile needs the last kernel only.  No atomics on global memory; shared counters are per warp and commute.
-constexpr int kSortWarps = 8;
-constexpr int kRounds = 8;
-constexpr int kTile = kSortWarps * 32 * kRounds;
+// Bound by latency: three launches, and in the last a chain of counts, prefix and ranks.  1048576 pairs, 256 experts: 512 tiles
+// of eight warps 21.9 us, one tile per SM of 32 warps 17.9 us (24.5 with the scan inside the last kernel, where every block reads
+// all counts); 512 pairs, 128 experts in one tile: 5.0 us with eight warps, 3.8 with 32.
+constexpr int kMaxBins = 4096;
+constexpr int kSortWarps = 32;
 
-template <class I> __device__ __forceinline__ int BinOf(const I* index, int64_t at, int64_t count, int experts)
+// Warps of a block: as many tables of bins as shared memory holds.
+inline int SortWarps(int bins) { return bins <= 1500 ? kSortWarps : 8; }
+
+template <class I> __device__ __forceinline__ int BinOf(const I* index, int64_t at, int64_t end, int experts)
 {
-    if (at >= count) {
+    if (at >= end) {
         return -1;
     }
-    const int64_t v = static_cast<int64_t>(index[at]);
+    const int64_t v = static_cast<int64_t>(__ldg(index + at));
     return v >= 0 && v < experts ? static_cast<int>(v) : experts;
 }
 
 template <class I>
-__global__ void __launch_bounds__(kSortWarps * 32) CountKernel(const I* __restrict__ index, int64_t count, int experts, int64_t tiles,
-                                                               int32_t* __restrict__ counts)
+__global__ void __launch_bounds__(1024) CountKernel(const I* __restrict__ index, int64_t count, int experts, int64_t tile,
+                                                    int32_t* __restrict__ counts)
 {
     extern __shared__ int32_t bins[];
     for (int b = threadIdx.x; b <= experts; b += blockDim.x) {
         bins[b] = 0;
     }
     __syncthreads();
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kTile;
-    for (int i = threadIdx.x; i < kTile; i += blockDim.x) {
-        const int b = BinOf(index, first + i, count, experts);
-        if (b >= 0) {
-            atomicAdd(&bins[b], 1);
-        }
+    const int64_t first = blockIdx.x * tile, end = first + tile < count ? first + tile : count;
+#pragma unroll 4
+    for (int64_t at = first + threadIdx.x; at < end; at += blockDim.x) {
+        atomicAdd(&bins[BinOf(index, at, end, experts)], 1);
     }
     __syncthreads();
     for (int b = threadIdx.x; b <= experts; b += blockDim.x) {
-        counts[b * tiles + blockIdx.x] = bins[b];
+        counts[static_cast<int64_t>(b) * gridDim.x + blockIdx.x] = bins[b];
     }
 }
 
-__device__ __forceinline__ int64_t BlockExclusive(int64_t v, int64_t* scratch, int64_t& total)
+// A warp per bin: its counts over the tiles become the pairs of the bin in earlier tiles, and their total.
+__global__ void __launch_bounds__(256) ScanKernel(int32_t* __restrict__ counts, int bins, int tiles, int32_t* __restrict__ totals)
 {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t inclusive = v;
+    const int lane = threadIdx.x & 31, bin = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+    if (bin >= bins) {
+        return;
+    }
+    int32_t* mine = counts + static_cast<int64_t>(bin) * tiles;
+    int before = 0;
+    for (int t0 = 0; t0 < tiles; t0 += 256) {
+        int v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int t = t0 + i * 32 + lane;
+            v[i] = t < tiles ? mine[t] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            int inclusive = v[i];
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int up = __shfl_up_sync(kFull, inclusive, d);
+                inclusive += lane >= d ? up : 0;
+            }
+            const int t = t0 + i * 32 + lane;
+            if (t < tiles) {
+                mine[t] = before + inclusive - v[i];
+            }
+            before += __shfl_sync(kFull, inclusive, 31);
+        }
+    }
+    if (lane == 0) {
+        totals[bin] = before;
+    }
+}
+
+// Exclusive prefix of v over the block, and its total.
+__device__ __forceinline__ int BlockExclusive(int v, int* scratch, int& total)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    int inclusive = v;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int64_t up = __shfl_up_sync(kFull, inclusive, d);
+        const int up = __shfl_up_sync(kFull, inclusive, d);
         inclusive += lane >= d ? up : 0;
     }
     if (lane == 31) {
         scratch[warp] = inclusive;
     }
     __syncthreads();
-    int64_t before = 0;
-    total = 0;
+    int sums = lane < warps ? scratch[lane] : 0;
+    const int own = sums;
 #pragma unroll
-    for (int w = 0; w < kSortWarps; ++w) {
-        before += w < warp ? scratch[w] : 0;
-        total += scratch[w];
+    for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(kFull, sums, d);
+        sums += lane >= d ? up : 0;
     }
+    total = __shfl_sync(kFull, sums, 31);
+    const int before = __shfl_sync(kFull, sums - own, warp);
     __syncthreads();
     return before + inclusive - v;
 }
 
-__global__ void __launch_bounds__(kSortWarps * 32) ScanKernel(int32_t* __restrict__ counts, int64_t tiles, int64_t* __restrict__ totals)
+// Lanes with the same bin: one ballot per bit (match_any runs through the distinct values one by one, up to 32 of them).
+__device__ __forceinline__ unsigned Peers(int bin, int bits)
 {
-    __shared__ int64_t scratch[kSortWarps];
-    int32_t* mine = counts + static_cast<int64_t>(blockIdx.x) * tiles;
-    int64_t before = 0;
-    for (int64_t from = 0; from < tiles; from += blockDim.x) {
-        const int64_t t = from + threadIdx.x;
-        const int64_t v = t < tiles ? mine[t] : 0;
-        int64_t total;
-        const int64_t exclusive = BlockExclusive(v, scratch, total);
-        if (t < tiles) {
-            mine[t] = static_cast<int32_t>(before + exclusive);  // at most `count` < 2^31 pairs (checked on the host)
-        }
-        before += total;
+    unsigned peers = __ballot_sync(kFull, bin >= 0);
+    peers = bin >= 0 ? peers : ~peers;
+    for (int i = 0; i < bits; ++i) {
+        const bool set = (bin >> i) & 1;
+        const unsigned with = __ballot_sync(kFull, set);
+        peers &= set ? with : ~with;
     }
-    if (threadIdx.x == 0) {
-        totals[blockIdx.x] = before;
-    }
+    return peers;
 }
 
+// Counts and places fit 32 bits: fewer than 2^31 pairs (checked on the host).
 template <class I>
-__global__ void __launch_bounds__(kSortWarps * 32)
-    PlaceKernel(const I* __restrict__ index, int64_t count, int experts, int64_t tiles, const int32_t* __restrict__ counts,
-                const int64_t* __restrict__ totals, int64_t* __restrict__ indptr, int64_t* __restrict__ perm,
-                int64_t* __restrict__ position)
+__global__ void __launch_bounds__(1024)
+    PlaceKernel(const I* __restrict__ index, int64_t count, int experts, int64_t tile, const int32_t* __restrict__ counts,
+                const int32_t* __restrict__ totals, int64_t* __restrict__ indptr, int64_t* __restrict__ perm, int64_t* __restrict__ position)
 {
-    extern __shared__ int32_t place[];  // [kSortWarps][experts + 1]: where the warp's next pair of a bin goes
-    __shared__ int64_t scratch[kSortWarps];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    extern __shared__ int32_t place[];  // [warps][experts + 1]: where the warp's next pair of a bin goes
+    __shared__ int scratch[kSortWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int bins = experts + 1;
     int32_t* mine = place + warp * bins;
-    for (int b = threadIdx.x; b < bins * kSortWarps; b += blockDim.x) {
+    for (int b = threadIdx.x; b < bins * warps; b += blockDim.x) {
         place[b] = 0;
     }
     __syncthreads();
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kTile + warp * (32 * kRounds);
-    int bin[kRounds];
-#pragma unroll
-    for (int i = 0; i < kRounds; ++i) {
-        bin[i] = BinOf(index, first + i * 32 + lane, count, experts);
-        if (bin[i] >= 0) {
-            atomicAdd(&mine[bin[i]], 1);
-        }
+    // A warp takes consecutive pairs of the tile, 32 a round.
+    const int64_t first = blockIdx.x * tile, end = first + tile < count ? first + tile : count;
+    const int64_t share = ((tile + warps - 1) / warps + 31) / 32 * 32;
+    const int64_t from = first + warp * share, to = from + share < end ? from + share : end;
+#pragma unroll 4
+    for (int64_t at = from + lane; at < to; at += 32) {
+        atomicAdd(&mine[BinOf(index, at, to, experts)], 1);
     }
     __syncthreads();
-    int64_t before = 0;
-    for (int from = 0; from < bins; from += blockDim.x) {
-        const int b = from + threadIdx.x;
-        int64_t in_tile = 0;
+    int before = 0;
+    for (int b0 = 0; b0 < bins; b0 += blockDim.x) {
+        const int b = b0 + threadIdx.x;
+        int sum = 0, earlier = 0;
         if (b < bins) {
-            for (int w = 0; w < kSortWarps; ++w) {
-                in_tile += place[w * bins + b];
+            if (counts != nullptr) {
+                sum = totals[b];
+                earlier = counts[static_cast<int64_t>(b) * gridDim.x + blockIdx.x];
+            } else {
+#pragma unroll 8
+                for (int w = 0; w < warps; ++w) {
+                    sum += place[w * bins + b];
+                }
             }
         }
-        const int64_t v = b < bins ? (totals != nullptr ? totals[b] : in_tile) : 0;
-        int64_t total;
-        const int64_t start = before + BlockExclusive(v, scratch, total);
+        int total;
+        const int start = before + BlockExclusive(sum, scratch, total);
         before += total;
         if (b < bins) {
             if (blockIdx.x == 0) {
                 indptr[b] = start;  // bin `experts` starts where the last expert ends
             }
-            int64_t next = start + (counts != nullptr ? counts[b * tiles + blockIdx.x] : 0);
-            for (int w = 0; w < kSortWarps; ++w) {
-                const int32_t here = place[w * bins + b];
-                place[w * bins + b] = static_cast<int32_t>(next);
+            int next = start + earlier;
+#pragma unroll 8
+            for (int w = 0; w < warps; ++w) {
+                const int here = place[w * bins + b];
+                place[w * bins + b] = next;
                 next += here;
             }
         }
     }
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kRounds; ++i) {
-        const unsigned peers = __match_any_sync(kFull, bin[i]);
-        if (bin[i] >= 0) {
-            const int lower = __popc(peers & ((1u << lane) - 1u));
-            const int32_t to = mine[bin[i]] + lower;
-            const int64_t at = first + i * 32 + lane;
-            perm[to] = at;
-            position[at] = to;
+    const int bits = 32 - __clz(experts);  // of the largest bin
+    int next = BinOf(index, from + lane, to, experts);
+    for (int64_t round = from; round < to; round += 32) {
+        const int bin = next;
+        next = BinOf(index, round + 32 + lane, to, experts);
+        const unsigned peers = Peers(bin, bits);
+        int where = 0;
+        if (bin >= 0) {
+            where = mine[bin] + __popc(peers & ((1u << lane) - 1u));
         }
         __syncwarp();
-        if (bin[i] >= 0 && lane == __ffs(peers) - 1) {
-            mine[bin[i]] += __popc(peers);
+        if (bin >= 0) {
+            if ((peers >> lane) == 1u) {  // the highest lane of the bin
+                mine[bin] = where + 1;
+            }
+            perm[where] = round + lane;
+            position[round + lane] = where;
         }
         __syncwarp();
     }
 }
 
+// Tiles: at most one per SM, of 1024 pairs or more.
+inline int64_t SortTiles(int64_t count) { return count <= 4096 ? 1 : std::min<int64_t>(SmCount(), CeilDiv(count, 1024)); }
+
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxChosen = 32;
 constexpr int kMaxGroups = 32;
-constexpr int kMaxBins = 4096;
 
 int CheckRoute(const OpsgnnRouteDesc* d)
 {
@@ -1117,8 +1163,8 @@ extern "C" int opsgnn_route_csr_workspace_bytes(int64_t count, int64_t experts, 
     if (experts > route::kMaxBins || count >= (INT64_C(1) << 31)) {
         return OPSGNN_ERR_LIMIT;
     }
-    const int64_t tiles = CeilDiv(count, route::kTile);
-    *bytes = tiles > 1 ? AlignUp((experts + 1) * 8, 256) + (experts + 1) * tiles * 4 : 0;
+    const int64_t tiles = route::SortTiles(count);
+    *bytes = tiles > 1 ? (experts + 1) * (tiles + 1) * 4 : 0;
     return OPSGNN_OK;
 }
 
@@ -1137,25 +1183,26 @@ extern "C" int opsgnn_route_csr(const void* index, int index_type, int64_t count
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !Aligned(workspace, 8))) {
         return OPSGNN_ERR_WORKSPACE;
     }
-    const int64_t tiles = std::max<int64_t>(1, CeilDiv(count, route::kTile));
     const int bins = static_cast<int>(experts) + 1;
-    int64_t* totals = tiles > 1 ? static_cast<int64_t*>(workspace) : nullptr;
-    int32_t* counts =
-        tiles > 1 ? reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + AlignUp(static_cast<int64_t>(bins) * 8, 256)) : nullptr;
-    const size_t shared = static_cast<size_t>(route::kSortWarps) * bins * 4;
+    const int64_t tiles = route::SortTiles(count), tile = std::max<int64_t>(1, CeilDiv(count, tiles));
+    int32_t* counts = tiles > 1 ? static_cast<int32_t*>(workspace) : nullptr;
+    int32_t* totals = tiles > 1 ? counts + bins * tiles : nullptr;
+    const int warps = route::SortWarps(bins);
+    const int shared = warps * bins * 4;
     auto run = [&](auto tag) {
         using I = decltype(tag);
         const I* in = static_cast<const I*>(index);
-        const int threads = route::kSortWarps * 32;
-        OPSGNN_CUDA_TRY(cudaFuncSetAttribute(route::PlaceKernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(route::kSortWarps * (route::kMaxBins + 1) * 4)));
-        if (tiles > 1) {
-            route::CountKernel<I><<<static_cast<unsigned>(tiles), threads, bins * 4, AsStream(stream)>>>(
-                in, count, static_cast<int>(experts), tiles, counts);
-            route::ScanKernel<<<bins, threads, 0, AsStream(stream)>>>(counts, tiles, totals);
+        if (shared > 48 * 1024) {
+            OPSGNN_CUDA_TRY(cudaFuncSetAttribute(route::PlaceKernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
         }
-        route::PlaceKernel<I><<<static_cast<unsigned>(tiles), threads, shared, AsStream(stream)>>>(
-            in, count, static_cast<int>(experts), tiles, counts, totals, indptr, perm, position);
+        if (tiles > 1) {
+            route::CountKernel<I><<<static_cast<unsigned>(tiles), 1024, bins * 4, AsStream(stream)>>>(in, count, static_cast<int>(experts),
+                                                                                                    tile, counts);
+            route::ScanKernel<<<static_cast<unsigned>(CeilDiv(bins, 8)), 256, 0, AsStream(stream)>>>(counts, bins, static_cast<int>(tiles),
+                                                                                                    totals);
+        }
+        route::PlaceKernel<I><<<static_cast<unsigned>(tiles), warps * 32, shared, AsStream(stream)>>>(
+            in, count, static_cast<int>(experts), tile, counts, totals, indptr, perm, position);
         return LaunchStatus();
     };
     return index_type == OPSGNN_I32 ? run(int32_t()) : run(int64_t());

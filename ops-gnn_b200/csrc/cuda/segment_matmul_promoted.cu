@@ -12,9 +12,15 @@
 // (inf - inf): a result that is not finite is computed again from the fp32 operands, one multiply-add at a time.  Values below
 // 2^-110 lose low bits, as their third term lies below the smallest bf16.
 //
-// Layout as in segment_matmul_tc.cu (one persistent block per SM: a loading warp, a multiplying warp), with eight epilogue
-// warps, each 32 rows x half the columns of a tile, whose sums need BN / 2 registers a thread: the first four warps hand
-// registers over.
+// Layout as in segment_matmul_tc.cu (one persistent block per SM: a loading warp, a multiplying warp), with eight summing
+// warps, each 32 rows x half the columns of a tile, whose sums need BN / 2 registers a thread.  The first four warps hand
+// registers over, and a warp of these looks the tiles up for the summing warps: a register spilled in their inner loop
+// doubles the time, since waiting on a barrier drops the first-level cache that holds it.
+//
+// What bounds the 8-bit product: reading every block's sums out of TMEM.  128 x 256 sums are 128 KB at 128 bytes per cycle and
+// SM, twice the 512 cycles of the block's multiplication.  Measured, 18944 x 4096 -> 2048: 171 us (1.86 PFLOP/s); with the
+// sums left unread 130 us, with one sum over all of K 117 us, Sixteen
+// summing warps in place of eight (187 us) and pairs of blocks that halve the operand traffic (170 us) change nothing.
 #include <algorithm>
 
 #include "segment_matmul.cuh"
@@ -26,12 +32,13 @@ namespace {
 
 constexpr int kRows = 128;
 constexpr int kBoxRows = 32;  // rows of a per load where a tile is not full
-constexpr int kThreads = 384;
+constexpr int kSumWarps = 8;
+constexpr int kThreads = 128 + 32 * kSumWarps;
 constexpr int kStages = 4;
-constexpr int kSlab = 64 * 128;
+constexpr int kSlab = tc::kSlabBytes;
 constexpr int kStagingBytes = 8 * 32 * 128;
 // 384 threads are launched with 168 registers each; 128 * 72 + 256 * 216 = 384 * 168.
-constexpr int kRegsIssue = 104, kRegsSum = 200;
+constexpr int kRegsIssue = 72, kRegsSum = 216;
 
 enum Form { kRowsWide, kRowsTurned, kOuter };
 
@@ -56,9 +63,14 @@ struct Params {
 
 struct Barriers {
     uint64_t full[kStages], empty[kStages], done[2], free[2], drain;
+    uint64_t told[2], taken[2];
+    int32_t tile[2][6];          // for the summing warps: segment, row, row_end, column, from, depth
     uint32_t fills[kStages];  // loads asked for, per stage (loading warp)
     uint32_t tmem, stop;
 };
+
+// Loads of kBoxRows rows that cover the first `rows` of a block's rows.
+__device__ __forceinline__ int Boxes(int rows) { return rows <= 0 ? 0 : min(rows + kBoxRows - 1, kRows) / kBoxRows; }
 
 template <class O> __device__ __forceinline__ uint32_t Word(const float* v)  // one 32-bit word of results
 {
@@ -109,7 +121,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             tc::BarInit(&bar.done[i], 1);
-            tc::BarInit(&bar.free[i], 8);
+            tc::BarInit(&bar.free[i], kSumWarps);
+            tc::BarInit(&bar.told[i], 1);
+            tc::BarInit(&bar.taken[i], kSumWarps);
         }
         tc::BarInit(&bar.drain, 1);
         bar.stop = 0;
@@ -129,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int across = (n + BN - 1) / BN;
     const int down = FORM == kOuter ? (m + kRows - 1) / kRows : 1;
     SegmentWalk<FORM == kOuter ? 0 : kRows, int> walk;
-    if (warp != 2 && warp != 3 && (FORM != kOuter || chunk > 0)) {
+    if (warp != 2 && warp < 4 && (FORM != kOuter || chunk > 0)) {
         walk.Start(p.ptr, FORM == kOuter ? chunk : kRows);
     }
     // Tile t: its segment, first result row and column, and the range of the reduced index.
@@ -181,28 +195,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (lane == 0) {
                     const uint32_t a = tc::Shared(smem) + s * kStage, b = a + kRows * 128;
+                    const uint32_t full = tc::Shared(&bar.full[s]);
                     bar.fills[s] = use + 1;
                     if constexpr (FORM == kOuter) {
                         tc::BarExpect(&bar.full[s], kStage);
-                        tc::LoadSlabs(map_a, &bar.full[s], a, row, from + k, pa, kRows / 64, p.whole_a);
-                        tc::LoadSlabs(map_b, &bar.full[s], b, column, from + k, pb, BN / 64, p.whole_b);
+                        tc::LoadSlabs(map_a, full, a, row, from + k, pa, kRows / 64, p.whole_a);
+                        tc::LoadSlabs(map_b, full, b, column, from + k, pb, BN / 64, p.whole_b);
                     } else {
                         // Only the rows that are the segment's, to the next 32; what else lies in the stage is multiplied into
                         // rows that are not stored.
-                        const int boxes = min(row_end - row + kBoxRows - 1, kRows) / kBoxRows;
+                        const int boxes = Boxes(row_end - row);
                         const int matrix = pb * static_cast<int>(p.ptr.segments) + segment;
                         tc::BarExpect(&bar.full[s], boxes * kBoxRows * 128 + BN * 128);
                         if (boxes * kBoxRows == kRows) {
-                            tc::Load3(map_a, &bar.full[s], a, k, row, pa);
+                            tc::LoadTo(map_a, full, a, k, row, pa);
                         } else {
                             for (int i = 0; i < boxes; ++i) {
-                                tc::Load3(map_tail, &bar.full[s], a + i * kBoxRows * 128, k, row + i * kBoxRows, pa);
+                                tc::LoadTo(map_tail, full, a + i * kBoxRows * 128, k, row + i * kBoxRows, pa);
                             }
                         }
                         if constexpr (FORM == kRowsTurned) {
-                            tc::Load3(map_b, &bar.full[s], b, k, column, matrix);
+                            tc::LoadTo(map_b, full, b, k, column, matrix);
                         } else {
-                            tc::LoadSlabs(map_b, &bar.full[s], b, column, k, matrix, BN / 64, p.whole_b);
+                            tc::LoadSlabs(map_b, full, b, column, k, matrix, BN / 64, p.whole_b);
                         }
                     }
                 }
@@ -222,92 +237,107 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         } else if (warp == 1) {
             constexpr uint32_t shape = tc::Shape(kRows, BN, F8 ? 0 : 1, FORM == kOuter, FORM != kRowsTurned);
-            uint32_t blocks = 0;
-            int at = 0;
+            // One thread issues (but for the zeroing); see segment_matmul_tc.cu on why its loop is lean.
             bool going = true;
-            // The stage's operands have landed; rows that belong to the next segment are zeroed.
-            auto ready = [&](uint32_t s, uint32_t use) {
-                if (!wait.Warp(&bar.full[s], use & 1)) {
-                    return false;
-                }
-                if constexpr (FORM == kOuter) {
-                    if (depth - at < kDepth) {
-                        unsigned char* stage = smem + s * kStage;
-                        const int first = (depth - at);
-                        for (int i = first * 8 + lane; i < kDepth * 8; i += 32) {
-#pragma unroll
-                            for (int slab = 0; slab < kStage / kSlab; ++slab) {
-                                *reinterpret_cast<uint4*>(stage + slab * kSlab + i * 16) = make_uint4(0, 0, 0, 0);
-                            }
-                        }
-                        tc::FenceAsync();
-                        __syncwarp();
-                    }
-                }
-                tc::FenceAfter();
-                return true;
-            };
+            const uint64_t a0 = tc::Operand(tc::Shared(smem), FORM == kOuter ? kSlab : 16, 1024);
+            const uint64_t b0 = tc::Operand(tc::Shared(smem) + kRows * 128, FORM == kRowsTurned ? 16 : kSlab, 1024);
             // One product of kDepth values: a of one stage, b of another.
             auto multiply = [&](uint32_t sa, uint32_t sb, uint32_t half, bool add) {
-                if (lane == 0) {
-                    uint64_t da = tc::Operand(tc::Shared(smem) + sa * kStage, FORM == kOuter ? kSlab : 16, 1024);
-                    uint64_t db = tc::Operand(tc::Shared(smem) + sb * kStage + kRows * 128, FORM == kRowsTurned ? 16 : kSlab, 1024);
+                const uint64_t da = a0 + sa * (kStage >> 4), db = b0 + sb * (kStage >> 4);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (F8) {
-                            tc::MmaF8(tmem + half * BN, da, db, shape, add || i > 0);
-                        } else {
-                            tc::MmaF16(tmem + half * BN, da, db, shape, add || i > 0);
-                        }
-                        da += FORM == kOuter ? 2048 >> 4 : 32 >> 4;
-                        db += FORM == kRowsTurned ? 32 >> 4 : 2048 >> 4;
+                for (int i = 0; i < 4; ++i) {
+                    const uint64_t ai = da + i * (FORM == kOuter ? 2048 >> 4 : 32 >> 4);
+                    const uint64_t bi = db + i * (FORM == kRowsTurned ? 32 >> 4 : 2048 >> 4);
+                    if constexpr (F8) {
+                        tc::MmaF8(tmem + half * BN, ai, bi, shape, add || i > 0);
+                    } else {
+                        tc::MmaF16(tmem + half * BN, ai, bi, shape, add || i > 0);
                     }
                 }
             };
-            auto commit = [&](uint64_t* to) {
-                if (lane == 0) {
-                    tc::Commit(to);
+            if constexpr (F8) {
+                uint32_t s = 0, parity = 0, half = 0, half_parity = 1;
+                for (int t = blockIdx.x; going && find(t); t += gridDim.x) {
+                    if (lane == 0) {
+                        bool landed = tc::BarTest(&bar.full[s], parity), freed = tc::BarTest(&bar.free[half], half_parity);
+                        for (int k = 0; k < depth; k += kDepth) {
+                            going = (freed || wait(&bar.free[half], half_parity)) && (landed || wait(&bar.full[s], parity));
+                            if (!going) {
+                                break;
+                            }
+                            tc::FenceAfter();
+                            multiply(s, s, half, false);
+                            tc::Commit(&bar.empty[s]);
+                            tc::Commit(&bar.done[half]);
+                            if (++s == kStages) {
+                                s = 0;
+                                parity ^= 1;
+                            }
+                            half ^= 1;
+                            half_parity ^= half == 0 ? 1 : 0;
+                            landed = k + kDepth < depth && tc::BarTest(&bar.full[s], parity);
+                            freed = k + kDepth < depth && tc::BarTest(&bar.free[half], half_parity);
+                        }
+                    }
+                    going = __shfl_sync(0xffffffffu, going ? 1 : 0, 0) != 0;
                 }
-            };
-            for (int t = blockIdx.x; going && find(t); t += gridDim.x) {
-                for (at = 0; going && at < depth; at += kDepth, ++blocks) {
-                    const uint32_t half = blocks & 1;
-                    going = wait.Warp(&bar.free[half], ((blocks >> 1) & 1) ^ 1);
+            } else {
+                uint32_t blocks = 0;
+                int at = 0;
+                // The stage's operands have landed; rows that belong to the next segment are zeroed.
+                auto ready = [&](uint32_t s, uint32_t use) {
+                    if (!wait.Warp(&bar.full[s], use & 1)) {
+                        return false;
+                    }
+                    if constexpr (FORM == kOuter) {
+                        if (depth - at < kDepth) {
+                            unsigned char* stage = smem + s * kStage;
+                            for (int i = (depth - at) * 8 + lane; i < kDepth * 8; i += 32) {
+#pragma unroll
+                                for (int slab = 0; slab < kStage / kSlab; ++slab) {
+                                    *reinterpret_cast<uint4*>(stage + slab * kSlab + i * 16) = make_uint4(0, 0, 0, 0);
+                                }
+                            }
+                            tc::FenceAsync();
+                            __syncwarp();
+                        }
+                    }
                     tc::FenceAfter();
-                    if constexpr (F8) {
-                        const uint32_t s = blocks % kStages;
-                        going = going && ready(s, blocks / kStages);
+                    return true;
+                };
+                for (int t = blockIdx.x; going && find(t); t += gridDim.x) {
+                    for (at = 0; going && at < depth; at += kDepth, ++blocks) {
+                        const uint32_t half = blocks & 1, s = blocks & 1;
+                        going = wait.Warp(&bar.free[half], ((blocks >> 1) & 1) ^ 1) && ready(s, blocks >> 1);
                         if (!going) {
                             break;
                         }
-                        multiply(s, s, half, false);
-                        commit(&bar.empty[s]);
-                    } else {
-                        const uint32_t s = blocks & 1;
-                        going = going && ready(s, blocks >> 1);
-                        if (!going) {
-                            break;
+                        if (lane == 0) {
+                            multiply(s, s, half, false);     // a3 b1
                         }
-                        multiply(s, s, half, false);     // a3 b1
                         going = ready(2, blocks);
                         if (!going) {
                             break;
                         }
-                        multiply(2, 2, half, true);      // a2 b2
+                        if (lane == 0) {
+                            multiply(2, 2, half, true);      // a2 b2
+                        }
                         going = ready(3, blocks);
                         if (!going) {
                             break;
                         }
-                        multiply(3, 3, half, true);      // a1 b3
-                        multiply(2, s, half, true);      // a2 b1
-                        multiply(3, 2, half, true);      // a1 b2
-                        commit(&bar.empty[2]);
-                        multiply(3, s, half, true);      // a1 b1
-                        commit(&bar.empty[s]);
-                        commit(&bar.empty[3]);
+                        if (lane == 0) {
+                            multiply(3, 3, half, true);      // a1 b3
+                            multiply(2, s, half, true);      // a2 b1
+                            multiply(3, 2, half, true);      // a1 b2
+                            tc::Commit(&bar.empty[2]);
+                            multiply(3, s, half, true);      // a1 b1
+                            tc::Commit(&bar.empty[s]);
+                            tc::Commit(&bar.empty[3]);
+                            tc::Commit(&bar.done[half]);
+                        }
+                        __syncwarp();
                     }
-                    commit(&bar.done[half]);
-                    __syncwarp();
                 }
             }
             if (!going) {  // let what was issued end before TMEM is freed
@@ -315,6 +345,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc::Commit(&bar.drain);
                     for (uint32_t i = 0; i < (1u << 15) && !tc::BarTry(&bar.drain, 0); ++i) {
                     }
+                }
+                __syncwarp();
+            }
+        } else if (warp == 3) {
+            // The tiles, looked up for the summing warps, whose registers hold nothing but sums.
+            uint32_t turn = 0;
+            bool going = true, more = true;
+            for (int t = blockIdx.x; going && more; t += gridDim.x, ++turn) {
+                more = find(t);
+                going = wait.Warp(&bar.taken[turn & 1], ((turn >> 1) & 1) ^ 1);
+                if (going && lane == 0) {
+                    int32_t* tile = bar.tile[turn & 1];
+                    tile[0] = more ? segment : -1;
+                    tile[1] = row;
+                    tile[2] = row_end;
+                    tile[3] = column;
+                    tile[4] = from;
+                    tile[5] = depth;
+                    tc::BarArrive(&bar.told[turn & 1]);
                 }
                 __syncwarp();
             }
@@ -327,9 +376,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         // a piece of a segment's sum (outer form in pieces; fp32 then) goes to `partial`
         O* out = FORM == kOuter && p.chunk > 0 ? reinterpret_cast<O*>(p.partial) : static_cast<O*>(p.out);
         const int scale_blocks = F8 ? (width + 127) / 128 : 0, scale_bands = F8 ? (n + 127) / 128 : 0;
-        uint32_t blocks = 0;
+        uint32_t blocks = 0, turn = 0;
         bool going = true;
-        for (int t = blockIdx.x; going && find(t); t += gridDim.x) {
+        for (;; ++turn) {
+            going = wait.Warp(&bar.told[turn & 1], (turn >> 1) & 1);
+            if (!going) {
+                break;
+            }
+            const volatile int32_t* tile = bar.tile[turn & 1];
+            const int segment = tile[0], row = tile[1], row_end = tile[2], column = tile[3], depth = tile[5];
+            [[maybe_unused]] const int from = tile[4];
+            __syncwarp();
+            if (lane == 0) {
+                tc::BarArrive(&bar.taken[turn & 1]);
+            }
+            if (segment < 0) {
+                break;
+            }
             float sum[kMine];
 #pragma unroll
             for (int i = 0; i < kMine; ++i) {
@@ -364,19 +427,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 tc::FenceAfter();
                 const uint32_t at = tmem + half * BN + side * kMine + (static_cast<uint32_t>(quarter * 32) << 16);
+                // Two loads in flight at a time; the half is handed back as soon as the last one is in registers.
+                uint32_t low[32], high[32];
                 if (some) {
-                    uint32_t part[32];
-#pragma unroll
-                    for (int c = 0; c < kMine; c += 32) {
-                        tc::TmemLoad32(at + c, part);
+                    tc::TmemLoad32(at, low);
+                    tc::TmemLoad32(at + 32, high);
+                    tc::TmemWait();
+                    if constexpr (kMine == 128) {
+                        Add(sum, 0, low, scale);
+                        tc::TmemLoad32(at + 64, low);
+                        Add(sum, 32, high, scale);
+                        tc::TmemLoad32(at + 96, high);
                         tc::TmemWait();
-                        Add(sum, c, part, scale);
                     }
                 }
                 tc::FenceBefore();
                 __syncwarp();
                 if (lane == 0) {
                     tc::BarArrive(&bar.free[half]);
+                }
+                if (some) {
+                    Add(sum, kMine - 64, low, scale);
+                    Add(sum, kMine - 32, high, scale);
                 }
             }
             if (!going) {
@@ -463,6 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     }
+    __syncwarp();
     tc::FenceBefore();
     __syncthreads();
     if (warp == 2) {
@@ -528,9 +601,10 @@ int Launch(const CUtensorMap& a, const CUtensorMap& tail, const CUtensorMap& b, 
     if (tiles >= INT32_MAX - 4096) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
-    OPSGNN_CUDA_TRY(cudaFuncSetAttribute(PromotedKernel<F8, O, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, SharedBytes<BN>()));
+    constexpr int kShared = SharedBytes<BN>();
+    OPSGNN_CUDA_TRY(cudaFuncSetAttribute(PromotedKernel<F8, O, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
     const int grid = static_cast<int>(std::min<int64_t>(std::max<int64_t>(tiles, 1), SmCount()));
-    PromotedKernel<F8, O, BN, FORM><<<grid, kThreads, SharedBytes<BN>(), stream>>>(a, tail, b, p);
+    PromotedKernel<F8, O, BN, FORM><<<grid, kThreads, kShared, stream>>>(a, tail, b, p);
     return LaunchStatus();
 }
 
@@ -716,10 +790,11 @@ int RunRowsFp8(const RowsProblem& p, cudaStream_t stream)
         !Map3(&b, true, p.b, p.k, p.n, p.ptr.segments, p.b_n, p.b_segment, narrow ? 128 : 256)) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
-    const int64_t tiles = (p.ptr.rows / kRows + p.ptr.segments) * CeilDiv(p.n, narrow ? 128 : 256);
+    const int64_t across = CeilDiv(p.n, narrow ? 128 : 256), tiles = (p.ptr.rows / kRows + p.ptr.segments) * across;
     auto run = [&](auto tag) {
         using O = decltype(tag);
-        return narrow ? Launch<true, O, 128, kRowsTurned>(a, tail, b, q, tiles, stream) : Launch<true, O, 256, kRowsTurned>(a, tail, b, q, tiles, stream);
+        return narrow ? Launch<true, O, 128, kRowsTurned>(a, tail, b, q, tiles, stream)
+                      : Launch<true, O, 256, kRowsTurned>(a, tail, b, q, tiles, stream);
     };
     switch (p.out_type) {
         case OPSGNN_F32:

@@ -63,7 +63,7 @@ constexpr int kRows = 128;     // rows of a tile
 constexpr int kBoxRows = 32;   // rows of a per load where a tile is not full
 constexpr int kDepth = 64;     // reduced index per stage: one 128-byte row of 16-bit values
 constexpr int kThreads = 256;
-constexpr int kSlab = kDepth * 128;          // bytes of 64 rows of 128 bytes
+constexpr int kSlab = tc::kSlabBytes;
 constexpr int kStagingBytes = 4 * 32 * 128;  // per epilogue warp 32 rows of 64 values
 
 enum Form { kRowsWide, kRowsTurned, kOuter };  // weight's columns along memory; its reduced index along memory; grad_weight
@@ -86,6 +86,9 @@ struct Barriers {
     uint64_t full[6], empty[6], done[2], free[2], drain;
     uint32_t tmem, stop;
 };
+
+// Loads of kBoxRows rows that cover the first `rows` of a block's rows.
+__device__ __forceinline__ int Boxes(int rows) { return rows <= 0 ? 0 : min(rows + kBoxRows - 1, kRows) / kBoxRows; }
 
 template <class T> __device__ __forceinline__ uint32_t TwoOf(uint32_t a, uint32_t b)
 {
@@ -191,26 +194,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (lane == 0) {
                     const uint32_t a = tc::Shared(smem) + s * kStage, b = a + kRows * 128;
+                    const uint32_t full = tc::Shared(&bar.full[s]);
                     if constexpr (FORM == kOuter) {
                         tc::BarExpect(&bar.full[s], kStage);
-                        tc::LoadSlabs(map_a, &bar.full[s], a, row, from + k, 0, kRows / 64, p.whole_a);
-                        tc::LoadSlabs(map_b, &bar.full[s], b, column, from + k, 0, BN / 64, p.whole_b);
+                        tc::LoadSlabs(map_a, full, a, row, from + k, 0, kRows / 64, p.whole_a);
+                        tc::LoadSlabs(map_b, full, b, column, from + k, 0, BN / 64, p.whole_b);
                     } else {
                         // Only the rows that are the segment's, to the next 32; what else lies in the stage is multiplied into
                         // rows that are not stored.
-                        const int boxes = min(row_end - row + kBoxRows - 1, kRows) / kBoxRows;
+                        const int boxes = Boxes(row_end - row);
                         tc::BarExpect(&bar.full[s], boxes * kBoxRows * 128 + BN * 128);
                         if (boxes * kBoxRows == kRows) {
-                            tc::Load2(map_a, &bar.full[s], a, k, row);
+                            tc::LoadTo(map_a, full, a, k, row);
                         } else {
                             for (int i = 0; i < boxes; ++i) {
-                                tc::Load2(map_tail, &bar.full[s], a + i * kBoxRows * 128, k, row + i * kBoxRows);
+                                tc::LoadTo(map_tail, full, a + i * kBoxRows * 128, k, row + i * kBoxRows);
                             }
                         }
                         if constexpr (FORM == kRowsTurned) {
-                            tc::Load3(map_b, &bar.full[s], b, k, column, segment);
+                            tc::LoadTo(map_b, full, b, k, column, segment);
                         } else {
-                            tc::LoadSlabs(map_b, &bar.full[s], b, column, k, segment, BN / 64, p.whole_b);
+                            tc::LoadSlabs(map_b, full, b, column, k, segment, BN / 64, p.whole_b);
                         }
                     }
                 }
@@ -219,27 +223,56 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 1) {
         constexpr uint32_t shape = tc::Shape(kRows, BN, std::is_same<T, __nv_bfloat16>::value ? 1 : 0, FORM == kOuter, FORM != kRowsTurned);
-        uint32_t used = 0, tiles = 0;
+        // One thread issues.  The tensor cores run dry where it dawdles between two stages, so stage and parity advance without
+        // divisions, operand descriptors differ by a constant, and the next stage is looked at before it is needed (18944 x 4096 ->
+        // 2048 bf16, a warp-wide loop without these: 235 us; with them 223 us).
+        uint32_t s = 0, parity = 0, tiles = 0;
         bool going = true;
+        const uint64_t a0 = tc::Operand(tc::Shared(smem), FORM == kOuter ? kSlab : 16, 1024);
+        const uint64_t b0 = tc::Operand(tc::Shared(smem) + kRows * 128, FORM == kRowsTurned ? 16 : kSlab, 1024);
         for (int t = blockIdx.x; going && find(t); t += gridDim.x) {
             if (depth == 0) {
                 continue;
             }
             const uint32_t half = tiles & 1;
-            going = wait.Warp(&bar.free[half], ((tiles >> 1) & 1) ^ 1);
-            tc::FenceAfter();
-            for (int k = 0; going && k < depth; k += kDepth, ++used) {
-                const uint32_t s = used % kStages;
-                going = wait.Warp(&bar.full[s], (used / kStages) & 1);
-                if (!going) {
-                    break;
+            auto multiply = [&](int k) {  // one stage
+                tc::FenceAfter();
+                const uint64_t da = a0 + s * (kStage >> 4), db = b0 + s * (kStage >> 4);
+#pragma unroll
+                for (int i = 0; i < kDepth / 16; ++i) {
+                    tc::MmaF16(tmem + half * BN, da + i * (FORM == kOuter ? 2048 >> 4 : 32 >> 4),
+                                     db + i * (FORM == kRowsTurned ? 32 >> 4 : 2048 >> 4), shape, k > 0 || i > 0);
                 }
-                unsigned char* stage = smem + s * kStage;
-                if constexpr (FORM == kOuter) {
-                    if (depth - k < kDepth) {
+                tc::Commit(&bar.empty[s]);
+            };
+            const int whole = FORM == kOuter ? depth / kDepth * kDepth : depth;
+            if (lane == 0) {
+                going = wait(&bar.free[half], ((tiles >> 1) & 1) ^ 1);
+                tc::FenceAfter();
+                bool landed = going && whole > 0 && tc::BarTest(&bar.full[s], parity);
+                for (int k = 0; going && k < whole; k += kDepth) {
+                    going = landed || wait(&bar.full[s], parity);
+                    if (!going) {
+                        break;
+                    }
+                    multiply(k);
+                    if (++s == kStages) {
+                        s = 0;
+                        parity ^= 1;
+                    }
+                    landed = k + kDepth < whole && tc::BarTest(&bar.full[s], parity);
+                }
+            }
+            going = __shfl_sync(0xffffffffu, going ? 1 : 0, 0) != 0;
+            if constexpr (FORM == kOuter) {
+                s = __shfl_sync(0xffffffffu, s, 0);
+                parity = __shfl_sync(0xffffffffu, parity, 0);
+                if (whole < depth && going) {
+                    going = wait.Warp(&bar.full[s], parity);
+                    if (going) {
                         // Rows of the next segment: zero them in every slab of both operands.
-                        const int first = (depth - k);
-                        for (int i = first * 8 + lane; i < kDepth * 8; i += 32) {
+                        unsigned char* stage = smem + s * kStage;
+                        for (int i = (depth - whole) * 8 + lane; i < kDepth * 8; i += 32) {
 #pragma unroll
                             for (int slab = 0; slab < kStage / kSlab; ++slab) {
                                 *reinterpret_cast<uint4*>(stage + slab * kSlab + i * 16) = make_uint4(0, 0, 0, 0);
@@ -247,30 +280,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         tc::FenceAsync();
                         __syncwarp();
+                        if (lane == 0) {
+                            multiply(whole);
+                        }
+                        if (++s == kStages) {
+                            s = 0;
+                            parity ^= 1;
+                        }
                     }
                 }
-                tc::FenceAfter();
-                if (lane == 0) {
-                    const uint32_t a = tc::Shared(stage), b = a + kRows * 128;
-                    uint64_t da = tc::Operand(a, FORM == kOuter ? kSlab : 16, 1024);
-                    uint64_t db = tc::Operand(b, FORM == kRowsTurned ? 16 : kSlab, 1024);
-#pragma unroll
-                    for (int i = 0; i < kDepth / 16; ++i) {
-                        tc::MmaF16(tmem + half * BN, da, db, shape, k > 0 || i > 0);
-                        da += FORM == kOuter ? 2048 >> 4 : 32 >> 4;
-                        db += FORM == kRowsTurned ? 32 >> 4 : 2048 >> 4;
-                    }
-                    tc::Commit(&bar.empty[s]);
-                }
-                __syncwarp();
             }
-            if (going) {
-                if (lane == 0) {
-                    tc::Commit(&bar.done[half]);
-                }
-                __syncwarp();
-                ++tiles;
+            if (lane == 0 && going) {
+                tc::Commit(&bar.done[half]);
             }
+            __syncwarp();
+            ++tiles;
         }
         if (!going) {  // let what was issued end before TMEM is freed
             if (lane == 0) {
@@ -393,6 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     }
+    __syncwarp();
     tc::FenceBefore();
     __syncthreads();
     if (warp == 2) {
@@ -423,9 +448,10 @@ int Launch(const CUtensorMap& a, const CUtensorMap& tail, const CUtensorMap& b, 
     if (tiles >= INT32_MAX - 4096) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
-    OPSGNN_CUDA_TRY(cudaFuncSetAttribute(TensorKernel<T, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, SharedBytes<BN>()));
+    constexpr int kShared = SharedBytes<BN>();
+    OPSGNN_CUDA_TRY(cudaFuncSetAttribute(TensorKernel<T, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
     const int grid = static_cast<int>(std::min<int64_t>(std::max<int64_t>(tiles, 1), SmCount()));
-    TensorKernel<T, BN, FORM><<<grid, kThreads, SharedBytes<BN>(), stream>>>(a, tail, b, p);
+    TensorKernel<T, BN, FORM><<<grid, kThreads, kShared, stream>>>(a, tail, b, p);
     return LaunchStatus();
 }
 

@@ -31,29 +31,31 @@ struct SegmentPointers {
 };
 
 // Row tiles of all segments in order, TILE rows each (a segment's last one may be short; an empty segment has none).
-// Seek(t) is called by a whole warp with ascending t and finds tile t by a running warp scan over 32 segments at a time:
-// no tile table, no workspace, no limit on the number of segments.  TILE 0: the number of rows is given to Start.  I: the
-// type of rows and tile numbers, int where the host has checked that they fit (half the registers).
+// Seek(t) is called by a whole warp with ascending t and finds tile t by a warp scan over 32 segments at a time, from where it
+// last stood: no tile table, no workspace, no limit on the number of segments.  Three registers live between two calls (the
+// scan is done again each time: the products' summing warps have none to spare).  TILE 0: the number of rows is given to
+// Start.  I: the type of rows and tile numbers, int where the host has checked that they fit.
 template <int TILE, class I> struct SegmentWalk {
-    I length;              // rows per tile
-    I segments;
     I from, base;          // first segment of the 32 at hand; tiles before them
     I high;                // largest pointer before them
-    I begin, end;          // this lane's segment
-    I inclusive;           // tiles of the 32 up to and with this lane's segment
+    I length;              // rows per tile
     // what Seek found
     I segment, row, row_end;
 
-    __device__ __forceinline__ I Tiles() const
+    __device__ __forceinline__ I Rows() const { return TILE > 0 ? TILE : length; }
+    __device__ __forceinline__ void Start(const SegmentPointers& p, I tile = TILE)
     {
-        const I tile = TILE > 0 ? TILE : length;
-        return (end - begin + tile - 1) / tile;
+        length = tile;
+        from = 0;
+        base = 0;
+        high = p.data != nullptr ? static_cast<I>(p.Raw(0)) : 0;
     }
-    __device__ __forceinline__ void Load(const SegmentPointers& p)
+    // This lane's segment of the 32 at hand, and the tiles of the 32 up to and with it.
+    __device__ __forceinline__ void Scan(const SegmentPointers& p, I& begin, I& end, I& inclusive) const
     {
         const int lane = threadIdx.x & 31;
         end = 0;
-        if (from + lane < segments) {
+        if (from + lane < static_cast<I>(p.segments)) {
             end = p.data != nullptr ? static_cast<I>(p.Raw(static_cast<int64_t>(from) + lane + 1)) : static_cast<I>(p.rows);
         }
         // A pointer below an earlier one counts as that one: segments never overlap, and all tiles together are bounded.
@@ -65,57 +67,51 @@ template <int TILE, class I> struct SegmentWalk {
         }
         begin = __shfl_up_sync(0xffffffffu, end, 1);
         begin = lane == 0 ? high : begin;
-        high = __shfl_sync(0xffffffffu, end, 31);
-        inclusive = Tiles();
+        inclusive = (end - begin + Rows() - 1) / Rows();
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const I up = __shfl_up_sync(0xffffffffu, inclusive, d);
             inclusive += lane >= d ? up : 0;
         }
     }
-    __device__ __forceinline__ void Start(const SegmentPointers& p, I tile = TILE)
-    {
-        length = tile;
-        segments = static_cast<I>(p.segments);
-        from = 0;
-        base = 0;
-        high = p.data != nullptr ? static_cast<I>(p.Raw(0)) : 0;
-        Load(p);
-    }
-    // Tiles before segment e and of it (ascending e).
-    __device__ __forceinline__ void Count(const SegmentPointers& p, I e, I& before, I& tiles)
-    {
-        while (from + 32 <= e) {
-            Next(p);
-        }
-        const int owner = static_cast<int>(e - from);
-        tiles = __shfl_sync(0xffffffffu, Tiles(), owner);
-        before = __shfl_sync(0xffffffffu, base + inclusive, owner) - tiles;
-    }
-    __device__ __forceinline__ void Next(const SegmentPointers& p)
+    __device__ __forceinline__ void Next(I end, I inclusive)
     {
         base += __shfl_sync(0xffffffffu, inclusive, 31);
+        high = __shfl_sync(0xffffffffu, end, 31);
         from += 32;
-        Load(p);
     }
     // False past the last tile.
     __device__ __forceinline__ bool Seek(const SegmentPointers& p, I t)
     {
-        while (true) {
+        while (from < static_cast<I>(p.segments)) {
+            I begin, end, inclusive;
+            Scan(p, begin, end, inclusive);
             const unsigned there = __ballot_sync(0xffffffffu, t < base + inclusive);
             if (there != 0) {
                 const int owner = __ffs(there) - 1;
-                const I first = __shfl_sync(0xffffffffu, base + inclusive - Tiles(), owner);
+                const I before = __shfl_sync(0xffffffffu, base + inclusive - (end - begin + Rows() - 1) / Rows(), owner);
                 row_end = __shfl_sync(0xffffffffu, end, owner);
-                row = __shfl_sync(0xffffffffu, begin, owner) + (t - first) * (TILE > 0 ? TILE : length);
+                row = __shfl_sync(0xffffffffu, begin, owner) + (t - before) * Rows();
                 segment = from + owner;
                 return true;
             }
-            if (from + 32 >= segments) {
-                return false;
-            }
-            Next(p);
+            Next(end, inclusive);
         }
+        return false;
+    }
+    // Tiles before segment e and of it (ascending e).
+    __device__ __forceinline__ void Count(const SegmentPointers& p, I e, I& before, I& tiles)
+    {
+        I begin, end, inclusive;
+        Scan(p, begin, end, inclusive);
+        while (from + 32 <= e) {
+            Next(end, inclusive);
+            Scan(p, begin, end, inclusive);
+        }
+        const int owner = static_cast<int>(e - from);
+        const I mine = (end - begin + Rows() - 1) / Rows();
+        tiles = __shfl_sync(0xffffffffu, mine, owner);
+        before = __shfl_sync(0xffffffffu, base + inclusive - mine, owner);
     }
 };
 

@@ -43,6 +43,22 @@ __device__ __forceinline__ bool BarTry(uint64_t* bar, uint32_t parity)
     return done != 0;
 }
 
+// A look that does not wait.
+__device__ __forceinline__ bool BarTest(uint64_t* bar, uint32_t parity)
+{
+    uint32_t done;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(done)
+        : "r"(Shared(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
 // A bounded wait.  One that runs out marks the launch as stopped (every other wait of the block then ends too) and reports
 // to the host; the block leaves its remaining tiles unwritten, waits for what it has in flight and returns.
 struct Waiter {
@@ -75,24 +91,24 @@ struct Waiter {
 // ---- TMA -------------------------------------------------------------------------------------------------------------------
 
 // Tile loads into the own block's shared memory.  x counts elements and is a multiple of 16 bytes at every call site.
-__device__ __forceinline__ void Load2(const CUtensorMap& map, uint64_t* bar, uint32_t to, int x, int y)
+__device__ __forceinline__ void LoadTo(const CUtensorMap& map, uint32_t bar, uint32_t to, int x, int y)
 {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(to),
-                 "l"(&map), "r"(Shared(bar)), "r"(x), "r"(y)
+                 "l"(&map), "r"(bar), "r"(x), "r"(y)
                  : "memory");
 }
-__device__ __forceinline__ void Load3(const CUtensorMap& map, uint64_t* bar, uint32_t to, int x, int y, int z)
+__device__ __forceinline__ void LoadTo(const CUtensorMap& map, uint32_t bar, uint32_t to, int x, int y, int z)
 {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
                      to),
-                 "l"(&map), "r"(Shared(bar)), "r"(x), "r"(y), "r"(z)
+                 "l"(&map), "r"(bar), "r"(x), "r"(y), "r"(z)
                  : "memory");
 }
-__device__ __forceinline__ void Load4(const CUtensorMap& map, uint64_t* bar, uint32_t to, int x, int y, int z, int w)
+__device__ __forceinline__ void LoadTo(const CUtensorMap& map, uint32_t bar, uint32_t to, int x, int y, int z, int w)
 {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(to),
-        "l"(&map), "r"(Shared(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        "l"(&map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
 // Writes to shared memory by this thread become visible to tcgen05.mma and TMA.
@@ -185,14 +201,14 @@ constexpr uint32_t Shape(int m, int n, int type, bool a_mn, bool b_mn)
 // the map's bounds filling zeros past the extent (dimensions extent, rows, 1, depth).  Loads are issued by one thread and
 // their number matters: four 32-row loads and four slabs a stage in place of one each cost a quarter of the rate.
 constexpr int kSlabBytes = 64 * 128;
-__device__ __forceinline__ void LoadSlabs(const CUtensorMap& map, uint64_t* bar, uint32_t to, int column, int row, int depth, int slabs,
+__device__ __forceinline__ void LoadSlabs(const CUtensorMap& map, uint32_t bar, uint32_t to, int column, int row, int depth, int slabs,
                                           bool whole)
 {
     if (whole) {
-        Load4(map, bar, to, 0, row, column / 64, depth);
+        LoadTo(map, bar, to, 0, row, column / 64, depth);
     } else {
         for (int i = 0; i < slabs; ++i) {
-            Load4(map, bar, to + i * kSlabBytes, column + i * 64, row, 0, depth);
+            LoadTo(map, bar, to + i * kSlabBytes, column + i * 64, row, 0, depth);
         }
     }
 }
