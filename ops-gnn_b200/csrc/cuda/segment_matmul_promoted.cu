@@ -6,8 +6,8 @@
 //
 // fp32: every operand value is x = x1 + x2 + x3 with bf16 terms (8 significant bits each, so the three hold all 24), and
 //     a b = a1 b1 + (a1 b2 + a2 b1) + (a1 b3 + a2 b2 + a3 b1) + terms below 2^-24 of |a b|, which are left out.
-// The six products are exact; 64 values of the reduced index are summed in TMEM, smallest terms first, so that only the last
-// four instructions add at full magnitude, then the sum moves to registers, which round to nearest.  Six bf16 products cost
+// The six products are exact; 64 values of the reduced index are summed in TMEM, a1 b1 last, so that only the last four
+// instructions add at full magnitude, then the sum moves to registers, which round to nearest.  Six bf16 products cost
 // 1/6 of the bf16 rate, four times what fp32 multiply-adds reach.  An infinity or NaN among the operands breaks the split
 // (inf - inf): a result that is not finite is computed again from the fp32 operands, one multiply-add at a time.  Values below
 // 2^-110 lose low bits, as their third term lies below the smallest bf16.
@@ -182,9 +182,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     };
 
-    // 8 bits: the stages are a ring.  fp32: stages 0 and 1 take turns with (third term of a, first of b), stage 2 holds the
-    // second terms of both, stage 3 (first of a, third of b); every term is loaded once per 64 values of the reduced index and
-    // used in one to three products (a ring of operand pairs per product read 288 KB in place of 144 and was bound by that).
+    // 8 bits: the stages are a ring.  fp32: stages 0 and 1 take turns with the first terms of both operands, stage 2 holds the
+    // second, stage 3 the third; every term is loaded once per 64 values of the reduced index and used in up to three products
+    // (a ring of operand pairs per product read 288 KB in place of 144).  The single stages are read first and refilled while
+    // the other products run; a1 b1 comes last, see above.
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
         if (warp == 0) {
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if constexpr (F8) {
                         going = load(blocks % kStages, blocks / kStages, k, 0, 0);
                     } else {
-                        going = load(blocks & 1, blocks >> 1, k, 2, 0) && load(2, blocks, k, 1, 1) && load(3, blocks, k, 0, 2);
+                        going = load(blocks & 1, blocks >> 1, k, 0, 0) && load(3, blocks, k, 2, 2) && load(2, blocks, k, 1, 1);
                     }
                 }
             }
@@ -283,59 +284,64 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             } else {
                 uint32_t blocks = 0;
-                int at = 0;
-                // The stage's operands have landed; rows that belong to the next segment are zeroed.
-                auto ready = [&](uint32_t s, uint32_t use) {
-                    if (!wait.Warp(&bar.full[s], use & 1)) {
+                // The six products of 64 values, with a wait (one thread's or the warp's) where a stage is first read.
+                auto products = [&](auto&& ready) {
+                    const uint32_t half = blocks & 1, s = blocks & 1;
+                    if (!ready(&bar.free[half], ((blocks >> 1) & 1) ^ 1, -1) || !ready(&bar.full[s], (blocks >> 1) & 1, s) ||
+                        !ready(&bar.full[3], blocks & 1, 3)) {
                         return false;
                     }
-                    if constexpr (FORM == kOuter) {
-                        if (depth - at < kDepth) {
-                            unsigned char* stage = smem + s * kStage;
-                            for (int i = (depth - at) * 8 + lane; i < kDepth * 8; i += 32) {
-#pragma unroll
-                                for (int slab = 0; slab < kStage / kSlab; ++slab) {
-                                    *reinterpret_cast<uint4*>(stage + slab * kSlab + i * 16) = make_uint4(0, 0, 0, 0);
-                                }
-                            }
-                            tc::FenceAsync();
-                            __syncwarp();
-                        }
+                    tc::FenceAfter();
+                    if (lane == 0) {
+                        multiply(3, s, half, false);     // a3 b1
+                        multiply(s, 3, half, true);      // a1 b3
+                        tc::Commit(&bar.empty[3]);
+                    }
+                    if (!ready(&bar.full[2], blocks & 1, 2)) {
+                        return false;
                     }
                     tc::FenceAfter();
+                    if (lane == 0) {
+                        multiply(2, 2, half, true);      // a2 b2
+                        multiply(2, s, half, true);      // a2 b1
+                        multiply(s, 2, half, true);      // a1 b2
+                        tc::Commit(&bar.empty[2]);
+                        multiply(s, s, half, true);      // a1 b1
+                        tc::Commit(&bar.empty[s]);
+                        tc::Commit(&bar.done[half]);
+                    }
                     return true;
                 };
                 for (int t = blockIdx.x; going && find(t); t += gridDim.x) {
-                    for (at = 0; going && at < depth; at += kDepth, ++blocks) {
-                        const uint32_t half = blocks & 1, s = blocks & 1;
-                        going = wait.Warp(&bar.free[half], ((blocks >> 1) & 1) ^ 1) && ready(s, blocks >> 1);
-                        if (!going) {
-                            break;
+                    const int whole = FORM == kOuter ? depth / kDepth : (depth + kDepth - 1) / kDepth;
+                    const uint32_t before = blocks;
+                    if (lane == 0) {
+                        for (int i = 0; going && i < whole; ++i, ++blocks) {
+                            going = products([&](uint64_t* barrier, uint32_t parity, int) { return wait(barrier, parity); });
                         }
-                        if (lane == 0) {
-                            multiply(s, s, half, false);     // a3 b1
-                        }
-                        going = ready(2, blocks);
-                        if (!going) {
-                            break;
-                        }
-                        if (lane == 0) {
-                            multiply(2, 2, half, true);      // a2 b2
-                        }
-                        going = ready(3, blocks);
-                        if (!going) {
-                            break;
-                        }
-                        if (lane == 0) {
-                            multiply(3, 3, half, true);      // a1 b3
-                            multiply(2, s, half, true);      // a2 b1
-                            multiply(3, 2, half, true);      // a1 b2
-                            tc::Commit(&bar.empty[2]);
-                            multiply(3, s, half, true);      // a1 b1
-                            tc::Commit(&bar.empty[s]);
-                            tc::Commit(&bar.empty[3]);
-                            tc::Commit(&bar.done[half]);
-                        }
+                    }
+                    going = __shfl_sync(0xffffffffu, going ? 1 : 0, 0) != 0;
+                    blocks = before + whole;
+                    if (FORM == kOuter && whole * kDepth < depth && going) {
+                        // Rows of the next segment in the last stages are zeroed.
+                        going = products([&](uint64_t* barrier, uint32_t parity, int stage) {
+                            if (!wait.Warp(barrier, parity)) {
+                                return false;
+                            }
+                            if (stage >= 0) {
+                                unsigned char* data = smem + stage * kStage;
+                                for (int i = (depth - whole * kDepth) * 8 + lane; i < kDepth * 8; i += 32) {
+#pragma unroll
+                                    for (int slab = 0; slab < kStage / kSlab; ++slab) {
+                                        *reinterpret_cast<uint4*>(data + slab * kSlab + i * 16) = make_uint4(0, 0, 0, 0);
+                                    }
+                                }
+                                tc::FenceAsync();
+                                __syncwarp();
+                            }
+                            return true;
+                        });
+                        ++blocks;
                         __syncwarp();
                     }
                 }
@@ -544,31 +550,57 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
+__device__ __forceinline__ void SplitFour(float4 v, uint2 (&words)[3])
+{
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    __nv_bfloat16 t[3][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        t[0][j] = __float2bfloat16_rn(x[j]);
+        const float first = __bfloat162float(t[0][j]);
+        const float rest = fabsf(first) < INFINITY ? x[j] - first : 0.0f;  // exact
+        t[1][j] = __float2bfloat16_rn(rest);
+        t[2][j] = __float2bfloat16_rn(rest - __bfloat162float(t[1][j]));
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+        memcpy(&words[j], t[j], 8);
+    }
+}
+
 // planes[3][count] <- the three bf16 terms of src[matrices][rows][width] (rows of whole 16-byte vectors, strides in elements).
+// FLAT: src is contiguous.  Bound by memory: 200003 x 256 reads 205 MB and writes 307 MB.
+template <bool FLAT>
 __global__ void __launch_bounds__(256) SplitKernel(const float* __restrict__ src, int64_t matrices, int64_t rows, int64_t width,
                                                    int64_t matrix_stride, int64_t row_stride, __nv_bfloat16* __restrict__ planes)
 {
     const int64_t vectors = width / 4, total = matrices * rows * vectors, plane = matrices * rows * width;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t line = i / vectors, c = (i - line * vectors) * 4;
-        const int64_t e = line / rows, r = line - e * rows;
-        const float4 v = __ldg(reinterpret_cast<const float4*>(src + e * matrix_stride + r * row_stride + c));
-        const float x[4] = {v.x, v.y, v.z, v.w};
-        __nv_bfloat16 t[3][4];
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += 2 * stride) {
+        float4 v[2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            t[0][j] = __float2bfloat16_rn(x[j]);
-            const float first = __bfloat162float(t[0][j]);
-            const bool finite = fabsf(first) < INFINITY;
-            const float rest = finite ? x[j] - first : 0.0f;   // exact
-            t[1][j] = __float2bfloat16_rn(rest);
-            t[2][j] = __float2bfloat16_rn(rest - __bfloat162float(t[1][j]));
+        for (int u = 0; u < 2; ++u) {
+            const int64_t at = i + u * stride;
+            if (at < total) {
+                const float* from = src + at * 4;
+                if constexpr (!FLAT) {
+                    const int64_t line = at / vectors, e = line / rows;
+                    from = src + e * matrix_stride + (line - e * rows) * row_stride + (at - line * vectors) * 4;
+                }
+                v[u] = __ldcs(reinterpret_cast<const float4*>(from));
+            }
         }
 #pragma unroll
-        for (int j = 0; j < 3; ++j) {
-            uint2 words;
-            memcpy(&words, t[j], 8);
-            *reinterpret_cast<uint2*>(planes + j * plane + line * width + c) = words;
+        for (int u = 0; u < 2; ++u) {
+            const int64_t at = i + u * stride;
+            if (at < total) {
+                uint2 words[3];
+                SplitFour(v[u], words);
+#pragma unroll
+                for (int j = 0; j < 3; ++j) {
+                    *reinterpret_cast<uint2*>(planes + j * plane + at * 4) = words[j];
+                }
+            }
         }
     }
 }
@@ -577,8 +609,13 @@ int Split(const float* src, int64_t matrices, int64_t rows, int64_t width, int64
           cudaStream_t stream)
 {
     const int64_t total = matrices * rows * (width / 4);
-    const int grid = static_cast<int>(std::min<int64_t>(CeilDiv(total, 256), static_cast<int64_t>(SmCount()) * 16));
-    SplitKernel<<<grid, 256, 0, stream>>>(src, matrices, rows, width, matrix_stride, row_stride, static_cast<__nv_bfloat16*>(planes));
+    const int grid = static_cast<int>(std::min<int64_t>(CeilDiv(total, 512), static_cast<int64_t>(SmCount()) * 32));
+    __nv_bfloat16* to = static_cast<__nv_bfloat16*>(planes);
+    if (row_stride == width && (matrices == 1 || matrix_stride == rows * width)) {
+        SplitKernel<true><<<grid, 256, 0, stream>>>(src, matrices, rows, width, matrix_stride, row_stride, to);
+    } else {
+        SplitKernel<false><<<grid, 256, 0, stream>>>(src, matrices, rows, width, matrix_stride, row_stride, to);
+    }
     return LaunchStatus();
 }
 

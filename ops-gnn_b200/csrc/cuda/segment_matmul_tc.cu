@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(256) JoinKernel(SegmentPointers ptr, int64_t c
         return;
     }
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+#pragma unroll 8
     for (int c = 0; c < pieces; ++c) {
         const float4 v = __ldcs(reinterpret_cast<const float4*>(partial + static_cast<int64_t>(before + c) * size + i));
         sum.x += v.x;
@@ -538,15 +538,19 @@ __global__ void __launch_bounds__(256) JoinKernel(SegmentPointers ptr, int64_t c
 int64_t OuterChunk(int64_t rows, int64_t segments, int64_t k, int64_t n)
 {
     // A result tile is one block's sequential sum over a segment's rows.  With fewer tiles than SMs the rows are cut into
-    // pieces, four rounds of tiles over the SMs (typed layer of 13 segments, 200003 x 256 -> 256, bf16: 26 tiles 0.63 ms, in
-    // pieces 0.09 ms); with more, partial results would cost more than they give (32 segments, 2048 x 1024: 8 MB a piece).
+    // pieces (200003 x 256 -> 256 in 13 segments, fp32: one piece each 1271 us, in pieces 313 us); with more tiles, or few rows,
+    // partial results would cost more than they give (32 segments of 2048 x 1024: 8 MB a piece; 4096 x 256 -> 256 in 32 segments,
+    // bf16: 10.5 us in one piece each, 22.9 us in pieces).  Two rounds of tiles over the SMs where a piece is a few tiles (bf16,
+    // the first case: 55.7 us, four rounds 65.6 us), four where it is many and two would leave the second round half empty
+    // (two segments, 32768 x 2048 -> 1024: 131 us, two rounds 148 us).  A segment's last piece is half full on average.
     const int64_t tiles = CeilDiv(k, kRows) * CeilDiv(n, n <= 128 ? 128 : 256);
-    if (tiles * segments >= SmCount()) {
+    if (tiles * segments >= SmCount() || rows < 8192) {
         return 0;
     }
-    const int64_t pieces = std::max<int64_t>(1, static_cast<int64_t>(SmCount()) * 4 / tiles);
+    const int64_t rounds = tiles * 8 <= SmCount() ? 2 : 4;
+    const int64_t pieces = std::max<int64_t>(1, SmCount() * rounds / tiles - segments / 2);
     const int64_t chunk = std::max<int64_t>(256, AlignUp(CeilDiv(rows, pieces), kDepth));
-    return chunk >= rows || rows < 8192 ? 0 : chunk;
+    return chunk >= rows ? 0 : chunk;
 }
 
 int64_t OuterPartialBytes(int64_t rows, int64_t segments, int64_t k, int64_t n)
