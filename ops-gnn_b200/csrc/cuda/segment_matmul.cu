@@ -23,12 +23,17 @@ int CheckDesc(const OpsgnnSegmentMatmulDesc* d, bool eight_bits)
     return OPSGNN_OK;
 }
 
-// fp32 products that go through bf16 terms on the tensor cores, as far as sizes and strides say (a base address off 16 bytes
-// sends the call to the simple kernel all the same).
-bool Splits(const OpsgnnSegmentMatmulDesc& d)
+// fp32 products that go through bf16 terms on the tensor cores.  Making the terms costs launches and passes over the operands,
+// which small products do not earn back: forward 4096 x 128 -> 128 (134 MFLOP) 13.1 us against 11.2 us on the simple kernel,
+// 16384 x 101 -> 77 (255 MFLOP) 20.8 against 27.4 us, 32768 x 501 -> 333 157 against 586 us.  The simple weight gradient also
+// grows with the rows a block sums alone: 1000 x 128 -> 128 12.2 us in terms against 11.7 us, 4096 x 64 -> 64 20.1 against 38.7.
+bool Splits(const OpsgnnSegmentMatmulDesc& d, int what)
 {
-    return d.in_type == OPSGNN_F32 && d.rows > 0 && d.segments > 0 && d.width > 0 && d.width % 8 == 0 && d.out > 0 && d.out % 8 == 0 &&
-           d.src_stride % 4 == 0;
+    if (d.in_type != OPSGNN_F32 || d.rows <= 0 || d.segments <= 0 || d.width <= 0 || d.out <= 0) {
+        return false;
+    }
+    const double flops = 2.0 * static_cast<double>(d.rows) * static_cast<double>(d.width) * static_cast<double>(d.out);
+    return flops >= 2e8 || (what != OPSGNN_SEGMENT_MATMUL_FORWARD && d.rows >= 2048);
 }
 
 // Weight gradients of 16-bit types that may be summed in pieces.
@@ -86,7 +91,7 @@ extern "C" int opsgnn_segment_matmul_workspace_bytes(const OpsgnnSegmentMatmulDe
         return OPSGNN_ERR_INVALID;
     }
     const int64_t rows = desc->rows, segments = desc->segments, width = desc->width, out = desc->out;
-    const bool split = segmm::Splits(*desc);
+    const bool split = segmm::Splits(*desc, what);
     *bytes = 0;
     if (what == OPSGNN_SEGMENT_MATMUL_FORWARD) {
         *bytes = split ? segmm::RowsSplitBytes(rows, segments, width, out) : 0;
@@ -214,14 +219,14 @@ extern "C" int opsgnn_segment_matmul_grads(const OpsgnnSegmentMatmulDesc* desc, 
     q.lda = turned ? grad_stride : desc->src_stride;
     q.ldb = turned ? desc->src_stride : grad_stride;
     q.type = desc->in_type;
-    if (rows && outer && segmm::Splits(*desc)) {
+    if (rows && outer && segmm::Splits(*desc, OPSGNN_SEGMENT_MATMUL_GRADS)) {
         const int ran = segmm::RunGradsSplit(p, q, turned != 0, workspace, AsStream(stream));
         if (ran != OPSGNN_ERR_UNSUPPORTED) {
             return ran;
         }
     }
     // fp32 that cannot be split goes through the simple kernels: no workspace for it below
-    void* scratch = need > 0 && !segmm::Splits(*desc) ? workspace : nullptr;
+    void* scratch = need > 0 && !segmm::Splits(*desc, OPSGNN_SEGMENT_MATMUL_GRADS) ? workspace : nullptr;
     int ran = rows ? segmm::RunRows(p, scratch, AsStream(stream)) : OPSGNN_OK;
     if (ran == OPSGNN_OK && outer) {
         ran = segmm::RunOuter(q, scratch, AsStream(stream));

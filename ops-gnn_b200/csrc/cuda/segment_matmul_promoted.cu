@@ -56,6 +56,7 @@ struct Params {
     int64_t lda, ldb;                // outer form: ldb = row stride of b
     int64_t b_segment, b_k, b_n;
     bool whole_a, whole_b;  // MN-major operands: all slabs in one load
+    bool vec;               // rows of out start on 16-byte boundaries
     int64_t chunk;     // outer form: rows per partial result; 0: a segment's rows in one piece
     float* partial;    // [pieces][m][n]
     WaitSettings wait;
@@ -474,19 +475,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         v.y = Word<O>(&sum[c + (4 * i + 1) * kPerWord]);
                         v.z = Word<O>(&sum[c + (4 * i + 2) * kPerWord]);
                         v.w = Word<O>(&sum[c + (4 * i + 3) * kPerWord]);
-                        *reinterpret_cast<uint4*>(mine + lane * 128 + ((i ^ (lane & 7)) << 4)) = v;
+                        *reinterpret_cast<uint4*>(mine + tc::Staged<128>(lane, i)) = v;
                     }
                     __syncwarp();
-                    const int piece = lane & 7;
-                    const int col = col0 + c + piece * (kLine / 8);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = i * 4 + (lane >> 3);
-                        const uint4 value = *reinterpret_cast<const uint4*>(mine + r * 128 + ((piece ^ (r & 7)) << 4));
-                        if (r0 + r < row_end && col < n) {
-                            *reinterpret_cast<uint4*>(to + (r0 + r) * p.n + col) = value;
-                        }
-                    }
+                    tc::StoreStaged<128>(mine, to + r0 * p.n + col0 + c, p.n, row_end - r0, n - col0 - c, p.vec);
                     __syncwarp();
                 }
             }
@@ -523,12 +515,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             // Rows of no segment.
             const int64_t before = p.ptr.data != nullptr ? p.ptr.Raw(0) : 0;
             const int64_t behind = p.ptr.data != nullptr ? p.ptr.Raw(p.ptr.segments) : p.ptr.rows;
-            constexpr int kVec = 16 / sizeof(O);
-            const int64_t pieces = p.n / kVec;
-            for (int64_t r = blockIdx.x * 8 + warp - 4; r < before + (p.ptr.rows - behind); r += gridDim.x * 8) {
+            for (int64_t r = blockIdx.x * kSumWarps + warp - 4; r < before + (p.ptr.rows - behind); r += gridDim.x * kSumWarps) {
                 const int64_t at = r < before ? r : behind + (r - before);
-                for (int64_t c = lane; c < pieces; c += 32) {
-                    *reinterpret_cast<uint4*>(out + at * p.n + c * kVec) = make_uint4(0, 0, 0, 0);
+                for (int c = lane; c < n; c += 32) {
+                    out[at * p.n + c] = Narrow<O, float>(0.0f);
                 }
             }
         }
@@ -568,26 +558,39 @@ __device__ __forceinline__ void SplitFour(float4 v, uint2 (&words)[3])
     }
 }
 
-// planes[3][count] <- the three bf16 terms of src[matrices][rows][width] (rows of whole 16-byte vectors, strides in elements).
-// FLAT: src is contiguous.  Bound by memory: 200003 x 256 reads 205 MB and writes 307 MB.
+// A row of a plane: whole 16-byte vectors.
+__host__ __device__ inline int64_t PlaneWidth(int64_t width) { return (width + 7) / 8 * 8; }
+
+// planes[3][matrices * rows][PlaneWidth(width)] <- the three bf16 terms of src[matrices][rows][width], any strides and alignment
+// (`vec`: every row starts on a 16-byte boundary).  What lies past `width` in a plane is not read.  FLAT: src is one contiguous
+// run of vectors and width a multiple of 8.  Bound by memory: 200003 x 256 reads 205 MB and writes 307 MB.
 template <bool FLAT>
 __global__ void __launch_bounds__(256) SplitKernel(const float* __restrict__ src, int64_t matrices, int64_t rows, int64_t width,
-                                                   int64_t matrix_stride, int64_t row_stride, __nv_bfloat16* __restrict__ planes)
+                                                   int64_t matrix_stride, int64_t row_stride, bool vec, __nv_bfloat16* __restrict__ planes)
 {
-    const int64_t vectors = width / 4, total = matrices * rows * vectors, plane = matrices * rows * width;
+    const int64_t vectors = PlaneWidth(width) / 4, total = matrices * rows * vectors, plane = total * 4;
     const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += 2 * stride) {
         float4 v[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int64_t at = i + u * stride;
+            v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (at < total) {
-                const float* from = src + at * 4;
-                if constexpr (!FLAT) {
-                    const int64_t line = at / vectors, e = line / rows;
-                    from = src + e * matrix_stride + (line - e * rows) * row_stride + (at - line * vectors) * 4;
+                if constexpr (FLAT) {
+                    v[u] = __ldcs(reinterpret_cast<const float4*>(src + at * 4));
+                } else {
+                    const int64_t line = at / vectors, e = line / rows, c = (at - line * vectors) * 4;
+                    const float* from = src + e * matrix_stride + (line - e * rows) * row_stride + c;
+                    if (vec && c + 4 <= width) {
+                        v[u] = __ldcs(reinterpret_cast<const float4*>(from));
+                    } else {
+                        v[u].x = c < width ? from[0] : 0.0f;
+                        v[u].y = c + 1 < width ? from[1] : 0.0f;
+                        v[u].z = c + 2 < width ? from[2] : 0.0f;
+                        v[u].w = c + 3 < width ? from[3] : 0.0f;
+                    }
                 }
-                v[u] = __ldcs(reinterpret_cast<const float4*>(from));
             }
         }
 #pragma unroll
@@ -608,13 +611,14 @@ __global__ void __launch_bounds__(256) SplitKernel(const float* __restrict__ src
 int Split(const float* src, int64_t matrices, int64_t rows, int64_t width, int64_t matrix_stride, int64_t row_stride, void* planes,
           cudaStream_t stream)
 {
-    const int64_t total = matrices * rows * (width / 4);
+    const int64_t total = matrices * rows * (PlaneWidth(width) / 4);
     const int grid = static_cast<int>(std::min<int64_t>(CeilDiv(total, 512), static_cast<int64_t>(SmCount()) * 32));
     __nv_bfloat16* to = static_cast<__nv_bfloat16*>(planes);
-    if (row_stride == width && (matrices == 1 || matrix_stride == rows * width)) {
-        SplitKernel<true><<<grid, 256, 0, stream>>>(src, matrices, rows, width, matrix_stride, row_stride, to);
+    const bool vec = Aligned(src, 16) && row_stride % 4 == 0 && (matrices == 1 || matrix_stride % 4 == 0);
+    if (vec && width % 8 == 0 && row_stride == width && (matrices == 1 || matrix_stride == rows * width)) {
+        SplitKernel<true><<<grid, 256, 0, stream>>>(src, matrices, rows, width, matrix_stride, row_stride, vec, to);
     } else {
-        SplitKernel<false><<<grid, 256, 0, stream>>>(src, matrices, rows, width, matrix_stride, row_stride, to);
+        SplitKernel<false><<<grid, 256, 0, stream>>>(src, matrices, rows, width, matrix_stride, row_stride, vec, to);
     }
     return LaunchStatus();
 }
@@ -645,30 +649,36 @@ int Launch(const CUtensorMap& a, const CUtensorMap& tail, const CUtensorMap& b, 
     return LaunchStatus();
 }
 
-int64_t PlaneBytes(int64_t values) { return AlignUp(values * 3 * 2, 1024); }
+// Bytes of the planes of lines of `width` values.
+int64_t PlaneBytes(int64_t lines, int64_t width) { return AlignUp(lines * PlaneWidth(width) * 3 * 2, 1024); }
 
-bool RowsSplittable(const RowsProblem& p, bool& turned)
+bool RowsSplittable(const RowsProblem& p)
 {
-    turned = p.b_k == 1 && p.b_n != 1;
-    const int64_t inner = turned ? p.k : p.n, other = turned ? p.n : p.k, stride = turned ? p.b_n : p.b_k;
-    return p.in_type == OPSGNN_F32 && p.k >= 1 && p.k % 8 == 0 && p.n % 8 == 0 && p.ldo == p.n && (turned || p.b_n == 1) &&
-           p.ptr.segments >= 1 && p.ptr.data != nullptr && p.lda % 4 == 0 && stride % 4 == 0 && p.b_segment % 4 == 0 && stride >= inner &&
-           Aligned(p.a, 16) && Aligned(p.b, 16) && Aligned(p.out, 16) && Fits(p.ptr.rows) && Fits(p.k) && Fits(p.n) &&
-           Fits(p.ptr.segments * 3) && Fits(other);
+    return p.in_type == OPSGNN_F32 && p.k >= 1 && p.ldo == p.n && (p.b_k == 1 || p.b_n == 1) && p.ptr.segments >= 1 &&
+           p.ptr.data != nullptr && Fits(p.ptr.rows) && Fits(p.k) && Fits(p.n) && Fits(p.ptr.segments * 3);
 }
 
 bool OuterSplittable(const OuterProblem& p)
 {
-    return p.type == OPSGNN_F32 && p.ptr.rows >= 1 && p.k % 8 == 0 && p.n % 8 == 0 && p.lda % 4 == 0 && p.ldb % 4 == 0 &&
-           Aligned(p.a, 16) && Aligned(p.b, 16) && Aligned(p.out, 16) && Fits(p.ptr.rows) && Fits(p.k) && Fits(p.n);
+    return p.type == OPSGNN_F32 && p.ptr.rows >= 1 && Fits(p.ptr.rows) && Fits(p.k) && Fits(p.n);
 }
 
 }  // namespace
 
-int64_t RowsSplitBytes(int64_t rows, int64_t segments, int64_t k, int64_t n) { return PlaneBytes(rows * k) + PlaneBytes(segments * k * n); }
+// The planes of a weight [segments, k, n] in either layout.
+int64_t WeightPlaneBytes(int64_t segments, int64_t k, int64_t n)
+{
+    return std::max(PlaneBytes(segments * k, n), PlaneBytes(segments * n, k));
+}
+int64_t RowsSplitBytes(int64_t rows, int64_t segments, int64_t k, int64_t n) { return PlaneBytes(rows, k) + WeightPlaneBytes(segments, k, n); }
 int64_t OuterSplitBytes(int64_t rows, int64_t segments, int64_t k, int64_t n)
 {
-    return PlaneBytes(rows * k) + PlaneBytes(rows * n) + OuterPartialBytes(rows, segments, k, n);
+    return PlaneBytes(rows, k) + PlaneBytes(rows, n) + OuterPartialBytes(rows, segments, k, n);
+}
+int64_t GradsSplitBytes(int64_t rows, int64_t segments, int64_t k, int64_t n)
+{
+    return PlaneBytes(rows, k) + PlaneBytes(rows, n) + WeightPlaneBytes(segments, k, n) +
+           std::max(OuterPartialBytes(rows, segments, k, n), OuterPartialBytes(rows, segments, n, k));
 }
 
 namespace {
@@ -692,11 +702,13 @@ int RowsFromPlanes(const RowsProblem& p, const void* planes_a, const void* plane
     const int64_t inner = turned ? p.k : p.n, other = turned ? p.n : p.k, e = p.ptr.segments;
     const bool narrow = p.n <= 128;
     q.whole_b = tc::WholeSlabs(p.n);
+    const int64_t wide_a = PlaneWidth(p.k), wide_b = PlaneWidth(inner);
+    q.vec = p.n % 4 == 0 && Aligned(p.out, 16);
     CUtensorMap a, tail, b;
-    if (!Map3(&a, false, planes_a, p.k, p.ptr.rows, 3, p.k, p.ptr.rows * p.k, kRows) ||
-        !Map3(&tail, false, planes_a, p.k, p.ptr.rows, 3, p.k, p.ptr.rows * p.k, kBoxRows) ||
-        !(turned ? Map3(&b, false, planes_b, inner, other, 3 * e, inner, inner * other, narrow ? 128 : 256)
-                 : tc::EncodeSlabs(&b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, planes_b, p.n, p.k, 3 * e, p.n * 2, p.n * p.k * 2, narrow ? 2 : 4))) {
+    if (!Map3(&a, false, planes_a, p.k, p.ptr.rows, 3, wide_a, p.ptr.rows * wide_a, kRows) ||
+        !Map3(&tail, false, planes_a, p.k, p.ptr.rows, 3, wide_a, p.ptr.rows * wide_a, kBoxRows) ||
+        !(turned ? Map3(&b, false, planes_b, inner, other, 3 * e, wide_b, wide_b * other, narrow ? 128 : 256)
+                 : tc::EncodeSlabs(&b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, planes_b, p.n, p.k, 3 * e, wide_b * 2, wide_b * p.k * 2, narrow ? 2 : 4))) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
     const int64_t down = p.ptr.rows / kRows + e;
@@ -726,8 +738,10 @@ int OuterFromPlanes(const OuterProblem& p, const void* planes_a, const void* pla
     const CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const int64_t rows = p.ptr.rows;
     CUtensorMap a, b;
-    if (!tc::EncodeSlabs(&a, type, planes_a, p.k, rows, 3, p.k * 2, rows * p.k * 2, kRows / 64) ||
-        !tc::EncodeSlabs(&b, type, planes_b, p.n, rows, 3, p.n * 2, rows * p.n * 2, p.n <= 128 ? 2 : 4)) {
+    const int64_t wide_a = PlaneWidth(p.k) * 2, wide_b = PlaneWidth(p.n) * 2;
+    q.vec = p.n % 4 == 0 && Aligned(p.out, 16);
+    if (!tc::EncodeSlabs(&a, type, planes_a, p.k, rows, 3, wide_a, rows * wide_a, kRows / 64) ||
+        !tc::EncodeSlabs(&b, type, planes_b, p.n, rows, 3, wide_b, rows * wide_b, p.n <= 128 ? 2 : 4)) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
     const int64_t down = (q.chunk > 0 ? p.ptr.rows / q.chunk + p.ptr.segments : p.ptr.segments) * CeilDiv(p.k, kRows);
@@ -752,12 +766,11 @@ int SplitMatrix(const void* src, int64_t rows, int64_t width, int64_t stride, vo
 
 int RunRowsSplit(const RowsProblem& p, void* workspace, cudaStream_t stream)
 {
-    bool turned;
-    if (!RowsSplittable(p, turned) || !Aligned(workspace, 16)) {
+    if (!RowsSplittable(p) || !Aligned(workspace, 16)) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
     char* planes_a = static_cast<char*>(workspace);
-    char* planes_b = planes_a + PlaneBytes(p.ptr.rows * p.k);
+    char* planes_b = planes_a + PlaneBytes(p.ptr.rows, p.k);
     int status = SplitMatrix(p.a, p.ptr.rows, p.k, p.lda, planes_a, stream);
     status = status != OPSGNN_OK ? status : SplitWeight(p, planes_b, stream);
     return status != OPSGNN_OK ? status : RowsFromPlanes(p, planes_a, planes_b, stream);
@@ -769,31 +782,24 @@ int RunOuterSplit(const OuterProblem& p, void* workspace, cudaStream_t stream)
         return OPSGNN_ERR_UNSUPPORTED;
     }
     char* planes_a = static_cast<char*>(workspace);
-    char* planes_b = planes_a + PlaneBytes(p.ptr.rows * p.k);
-    char* partial = planes_b + PlaneBytes(p.ptr.rows * p.n);
+    char* planes_b = planes_a + PlaneBytes(p.ptr.rows, p.k);
+    char* partial = planes_b + PlaneBytes(p.ptr.rows, p.n);
     int status = SplitMatrix(p.a, p.ptr.rows, p.k, p.lda, planes_a, stream);
     status = status != OPSGNN_OK ? status : SplitMatrix(p.b, p.ptr.rows, p.n, p.ldb, planes_b, stream);
     return status != OPSGNN_OK ? status : OuterFromPlanes(p, planes_a, planes_b, partial, stream);
 }
 
-int64_t GradsSplitBytes(int64_t rows, int64_t segments, int64_t k, int64_t n)
-{
-    return PlaneBytes(rows * k) + PlaneBytes(rows * n) + PlaneBytes(segments * k * n) +
-           std::max(OuterPartialBytes(rows, segments, k, n), OuterPartialBytes(rows, segments, n, k));
-}
-
 int RunGradsSplit(const RowsProblem& rows, const OuterProblem& outer, bool turned, void* workspace, cudaStream_t stream)
 {
-    bool ignored;
-    if (!RowsSplittable(rows, ignored) || !OuterSplittable(outer) || !Aligned(workspace, 16)) {
+    if (!RowsSplittable(rows) || !OuterSplittable(outer) || !Aligned(workspace, 16)) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
     const void* src = turned ? outer.b : outer.a;
     const int64_t width = turned ? outer.n : outer.k, stride = turned ? outer.ldb : outer.lda;
     char* planes_src = static_cast<char*>(workspace);
-    char* planes_grad = planes_src + PlaneBytes(rows.ptr.rows * width);
-    char* planes_weight = planes_grad + PlaneBytes(rows.ptr.rows * rows.k);
-    char* partial = planes_weight + PlaneBytes(rows.ptr.segments * rows.k * rows.n);
+    char* planes_grad = planes_src + PlaneBytes(rows.ptr.rows, width);
+    char* planes_weight = planes_grad + PlaneBytes(rows.ptr.rows, rows.k);
+    char* partial = planes_weight + WeightPlaneBytes(rows.ptr.segments, rows.k, rows.n);
     int status = SplitMatrix(rows.a, rows.ptr.rows, rows.k, rows.lda, planes_grad, stream);
     status = status != OPSGNN_OK ? status : SplitWeight(rows, planes_weight, stream);
     status = status != OPSGNN_OK ? status : RowsFromPlanes(rows, planes_grad, planes_weight, stream);
@@ -806,10 +812,9 @@ int RunGradsSplit(const RowsProblem& rows, const OuterProblem& outer, bool turne
 
 int RunRowsFp8(const RowsProblem& p, cudaStream_t stream)
 {
-    const int vec = 16 / DtypeBytes(p.out_type);
     if (p.in_type != OPSGNN_F8E4M3 || p.k < 1 || p.ptr.segments < 1 || p.b_k != 1 || p.lda % 16 != 0 || p.b_n % 16 != 0 ||
-        p.b_segment % 16 != 0 || p.b_segment < 1 || p.b_n < p.k || p.n % vec != 0 || p.ldo != p.n || !Aligned(p.a, 16) ||
-        !Aligned(p.b, 16) || !Aligned(p.out, 16) || !Fits(p.ptr.rows) || !Fits(p.k) || !Fits(p.n) || !Fits(p.ptr.segments) ||
+        p.b_segment % 16 != 0 || p.b_segment < 1 || p.b_n < p.k || p.ldo != p.n || !Aligned(p.a, 16) ||
+        !Aligned(p.b, 16) || !Fits(p.ptr.rows) || !Fits(p.k) || !Fits(p.n) || !Fits(p.ptr.segments) ||
         p.lda >= (INT64_C(1) << 39) || p.b_segment >= (INT64_C(1) << 39)) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
@@ -821,6 +826,7 @@ int RunRowsFp8(const RowsProblem& p, cudaStream_t stream)
     q.n = p.n;
     q.k = p.k;
     OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
+    q.vec = p.n % (16 / DtypeBytes(p.out_type)) == 0 && Aligned(p.out, 16);
     const bool narrow = p.n <= 128;
     CUtensorMap a, tail, b;
     if (!Map3(&a, true, p.a, p.k, p.ptr.rows, 1, p.lda, p.lda, kRows) || !Map3(&tail, true, p.a, p.k, p.ptr.rows, 1, p.lda, p.lda, kBoxRows) ||

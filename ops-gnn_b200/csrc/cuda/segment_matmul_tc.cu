@@ -77,6 +77,7 @@ struct Params {
     void* out;
     int64_t m, n, k;   // rows form: n columns, k reduced; outer form: m x n results per segment
     bool whole_a, whole_b;  // MN-major operands: all slabs in one load
+    bool vec;               // rows of out start on 16-byte boundaries
     int64_t chunk;     // outer form: rows per partial result; 0: a segment's rows in one piece
     float* partial;    // [pieces][m][n]
     WaitSettings wait;
@@ -327,7 +328,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     break;
                 }
                 uint32_t words[32];
-                const int piece = lane & 7;
                 if (depth > 0) {
                     uint32_t low[32], high[32];
                     const uint32_t at = tmem + half * BN + c + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -341,19 +341,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const uint32_t(&v)[32] = side == 0 ? low : high;
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
-                                *reinterpret_cast<uint4*>(mine + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+                                *reinterpret_cast<uint4*>(mine + tc::Staged<128>(lane, i)) =
                                     make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
                             }
                             __syncwarp();
-                            const int col = column + c + side * 32 + piece * 4;
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const int r = i * 4 + (lane >> 3);
-                                const uint4 value = *reinterpret_cast<const uint4*>(mine + r * 128 + ((piece ^ (r & 7)) << 4));
-                                if (first + r < row_end && col < n) {
-                                    *reinterpret_cast<uint4*>(p.partial + segment * p.m * p.n + (first + r) * p.n + col) = value;
-                                }
-                            }
+                            const int col = column + c + side * 32;
+                            tc::StoreStaged<128>(mine, p.partial + segment * p.m * p.n + first * p.n + col, p.n, row_end - first, n - col,
+                                                 n % 4 == 0);
                             __syncwarp();
                         }
                         continue;
@@ -369,23 +363,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                         words[i] = 0;
                     }
                 }
-                // Through shared memory, so that 8 lanes write 128 consecutive bytes of a row; the 16-byte pieces of a row
-                // are permuted by its number against bank conflicts.
+                // Through shared memory, so that 8 lanes write 128 consecutive bytes of a row.
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    *reinterpret_cast<uint4*>(mine + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+                    *reinterpret_cast<uint4*>(mine + tc::Staged<128>(lane, i)) =
                         make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
                 }
                 __syncwarp();
-                const int col = column + c + piece * 8;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int r = i * 4 + (lane >> 3);
-                    const uint4 value = *reinterpret_cast<const uint4*>(mine + r * 128 + ((piece ^ (r & 7)) << 4));
-                    if (first + r < row_end && col < n) {
-                        *reinterpret_cast<uint4*>(to + (first + r) * p.n + col) = value;
-                    }
-                }
+                tc::StoreStaged<128>(mine, to + first * p.n + column + c, p.n, row_end - first, n - column - c, p.vec);
                 __syncwarp();
             }
             if (depth > 0) {
@@ -400,11 +385,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (FORM != kOuter) {
             // Rows of no segment.
             const int64_t before = p.ptr.Raw(0), behind = p.ptr.Raw(p.ptr.segments);
-            const int64_t pieces = p.n / 8;
             for (int64_t r = blockIdx.x * 4 + quarter; r < before + (p.ptr.rows - behind); r += gridDim.x * 4) {
                 const int64_t at = r < before ? r : behind + (r - before);
-                for (int64_t c = lane; c < pieces; c += 32) {
-                    *reinterpret_cast<uint4*>(out + at * p.n + c * 8) = make_uint4(0, 0, 0, 0);
+                for (int c = lane; c < n; c += 32) {
+                    out[at * p.n + c] = Narrow<T, float>(0.0f);
                 }
             }
         }
@@ -471,7 +455,7 @@ int RunRowsTensor(const RowsProblem& p, cudaStream_t stream)
     const bool turned = p.b_k == 1 && p.b_n != 1;
     const int64_t inner = turned ? p.k : p.n, other = turned ? p.n : p.k, stride = turned ? p.b_n : p.b_k;
     if ((p.in_type != OPSGNN_BF16 && p.in_type != OPSGNN_F16) || p.out_type != p.in_type || p.k < 1 || p.ptr.data == nullptr ||
-        p.ptr.segments < 1 || p.n % 8 != 0 || p.ldo != p.n || (!turned && p.b_n != 1) || !Aligned(p.out, 16) || stride < inner ||
+        p.ptr.segments < 1 || p.ldo != p.n || (!turned && p.b_n != 1) || stride < inner ||
         p.b_segment % 8 != 0 || p.b_segment >= (INT64_C(1) << 38) || p.b_segment < 1 || p.ptr.segments >= (INT64_C(1) << 31) ||
         !Loadable(p.a, p.lda, std::max(p.k, p.ptr.rows)) || !Loadable(p.b, stride, std::max(inner, other))) {
         return OPSGNN_ERR_UNSUPPORTED;
@@ -481,6 +465,7 @@ int RunRowsTensor(const RowsProblem& p, cudaStream_t stream)
     q.out = p.out;
     q.n = p.n;
     q.k = p.k;
+    q.vec = p.n % 8 == 0 && Aligned(p.out, 16);
     OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
     const bool narrow = p.n <= 128;
     q.whole_b = tc::WholeSlabs(p.n);
@@ -507,7 +492,7 @@ int RunRowsTensor(const RowsProblem& p, cudaStream_t stream)
 namespace {
 
 // out[e][i] <- the sum of the pieces of segment e, in their order.  blockIdx.y: segment.
-template <class T>
+template <class T, int VEC>
 __global__ void __launch_bounds__(256) JoinKernel(SegmentPointers ptr, int64_t chunk, int64_t size, const float* __restrict__ partial,
                                                   T* __restrict__ out)
 {
@@ -516,21 +501,20 @@ __global__ void __launch_bounds__(256) JoinKernel(SegmentPointers ptr, int64_t c
     walk.Start(ptr, static_cast<int>(chunk));
     int before, pieces;
     walk.Count(ptr, static_cast<int>(e), before, pieces);
-    const int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 4;
+    const int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * VEC;
     if (i >= size) {
         return;
     }
-    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float sum[VEC] = {};
 #pragma unroll 8
     for (int c = 0; c < pieces; ++c) {
-        const float4 v = __ldcs(reinterpret_cast<const float4*>(partial + static_cast<int64_t>(before + c) * size + i));
-        sum.x += v.x;
-        sum.y += v.y;
-        sum.z += v.z;
-        sum.w += v.w;
+        const Pack<float, VEC> v = LoadPlain<float, VEC>(partial + static_cast<int64_t>(before + c) * size + i);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            sum[j] += v.v[j];
+        }
     }
-    const float f[4] = {sum.x, sum.y, sum.z, sum.w};
-    StorePlain<T, 4>(out + e * size + i, Repack<T, float, 4>(f));
+    StorePlain<T, VEC>(out + e * size + i, Repack<T, float, VEC>(sum));
 }
 
 }  // namespace
@@ -562,24 +546,30 @@ int64_t OuterPartialBytes(int64_t rows, int64_t segments, int64_t k, int64_t n)
 int JoinPieces(const OuterProblem& p, int64_t chunk, const float* partial, cudaStream_t stream)
 {
     const int64_t size = p.k * p.n;
-    const dim3 grid(static_cast<unsigned>(CeilDiv(size, 1024)), static_cast<unsigned>(p.ptr.segments));
+    auto run = [&](auto tag) {
+        using T = decltype(tag);
+        const bool vec = size % 4 == 0 && Aligned(p.out, 16);
+        const dim3 grid(static_cast<unsigned>(CeilDiv(size, vec ? 1024 : 256)), static_cast<unsigned>(p.ptr.segments));
+        if (vec) {
+            JoinKernel<T, 4><<<grid, 256, 0, stream>>>(p.ptr, chunk, size, partial, static_cast<T*>(p.out));
+        } else {
+            JoinKernel<T, 1><<<grid, 256, 0, stream>>>(p.ptr, chunk, size, partial, static_cast<T*>(p.out));
+        }
+        return LaunchStatus();
+    };
     switch (p.type) {
         case OPSGNN_F32:
-            JoinKernel<float><<<grid, 256, 0, stream>>>(p.ptr, chunk, size, partial, static_cast<float*>(p.out));
-            break;
+            return run(float());
         case OPSGNN_F16:
-            JoinKernel<__half><<<grid, 256, 0, stream>>>(p.ptr, chunk, size, partial, static_cast<__half*>(p.out));
-            break;
+            return run(__half());
         default:
-            JoinKernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p.ptr, chunk, size, partial, static_cast<__nv_bfloat16*>(p.out));
-            break;
+            return run(__nv_bfloat16());
     }
-    return LaunchStatus();
 }
 
 int RunOuterTensor(const OuterProblem& p, void* workspace, cudaStream_t stream)
 {
-    if ((p.type != OPSGNN_BF16 && p.type != OPSGNN_F16) || p.ptr.rows < 1 || p.n % 8 != 0 || !Aligned(p.out, 16) ||
+    if ((p.type != OPSGNN_BF16 && p.type != OPSGNN_F16) || p.ptr.rows < 1 ||
         !Loadable(p.a, p.lda, std::max(p.k, p.ptr.rows)) || !Loadable(p.b, p.ldb, std::max(p.n, p.ptr.rows))) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
@@ -588,6 +578,7 @@ int RunOuterTensor(const OuterProblem& p, void* workspace, cudaStream_t stream)
     q.out = p.out;
     q.m = p.k;
     q.n = p.n;
+    q.vec = p.n % 8 == 0 && Aligned(p.out, 16);
     q.chunk = OuterChunk(p.ptr.rows, p.ptr.segments, p.k, p.n);
     q.partial = static_cast<float*>(workspace);
     OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));

@@ -194,6 +194,44 @@ constexpr uint32_t Shape(int m, int n, int type, bool a_mn, bool b_mn)
            (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n / 8) << 17) | (static_cast<uint32_t>(m / 16) << 24);
 }
 
+// ---- results ---------------------------------------------------------------------------------------------------------------
+
+// A warp writes 32 rows of BYTES bytes from its staging area, whose 16-byte pieces are permuted by the row's number against
+// bank conflicts (Staged gives a piece's place), to `to` + row * stride; rows and columns past the limits are left out.  VEC:
+// rows of the result start on 16-byte boundaries, so neighbouring lanes write neighbouring 16-byte pieces; else single values.
+template <int BYTES> __device__ __forceinline__ int Staged(int row, int piece)
+{
+    constexpr int PIECES = BYTES / 16;
+    return row * BYTES + ((piece ^ ((PIECES == 8 ? row : row >> 1) & (PIECES - 1))) << 4);
+}
+template <int BYTES, class O>
+__device__ __forceinline__ void StoreStaged(const unsigned char* staging, O* to, int64_t stride, int rows, int columns, bool vec)
+{
+    constexpr int PIECES = BYTES / 16, PER = 16 / sizeof(O), LINE = BYTES / sizeof(O);
+    const int lane = threadIdx.x & 31;
+    if (vec) {
+        const int piece = lane % PIECES;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int r = i * (32 / PIECES) + lane / PIECES;
+            const uint4 value = *reinterpret_cast<const uint4*>(staging + Staged<BYTES>(r, piece));
+            if (r < rows && piece * PER < columns) {
+                *reinterpret_cast<uint4*>(to + r * stride + piece * PER) = value;
+            }
+        }
+    } else {
+#pragma unroll 1
+        for (int r = 0; r < 32 && r < rows; ++r) {
+#pragma unroll 1
+            for (int c = lane; c < LINE; c += 32) {
+                if (c < columns) {
+                    to[r * stride + c] = *reinterpret_cast<const O*>(staging + Staged<BYTES>(r, c / PER) + c % PER * sizeof(O));
+                }
+            }
+        }
+    }
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------------
 
 // An MN-major operand is a row of slabs, 64 values of the kept index by 64 of the reduced one.  Where the kept extent is a

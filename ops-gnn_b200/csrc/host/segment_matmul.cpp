@@ -30,6 +30,38 @@ at::Tensor Matrices(const at::Tensor& t)
     return (out_fast || width_fast) && (e == 1 || t.stride(0) >= extent) ? t : t.contiguous();
 }
 
+// The tensor cores' loads want rows on 16-byte boundaries.  A product of this many multiply-adds or more is worth a copy of an
+// operand that has them elsewhere; smaller ones run as they are, on the kernel for any layout.
+constexpr double kWorthCopy = 5e7;
+
+bool Wants(const at::Tensor& rows, const at::Tensor& matrices)
+{
+    return rows.scalar_type() != at::kFloat &&
+           static_cast<double>(rows.size(0)) * static_cast<double>(matrices.size(1)) * static_cast<double>(matrices.size(2)) >= kWorthCopy;
+}
+
+// t itself, or a copy with rows (the last dimension or, `turned`, the one before it) on 16-byte boundaries.
+at::Tensor OnBoundaries(const at::Tensor& t, bool turned = false)
+{
+    const int64_t vec = 16 / t.element_size(), inner = turned ? t.dim() - 2 : t.dim() - 1;
+    bool fine = reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+    for (int64_t d = 0; d < t.dim(); ++d) {
+        fine = fine && (d == inner || t.size(d) <= 1 || t.stride(d) % vec == 0);
+    }
+    if (fine) {
+        return t;
+    }
+    at::Tensor from = turned ? t.transpose(-1, -2) : t;
+    auto shape = from.sizes().vec();
+    const int64_t width = shape.back();
+    shape.back() = (width + vec - 1) / vec * vec;
+    at::Tensor copy = at::empty(shape, t.options()).narrow(-1, 0, width);
+    copy.copy_(from);
+    return turned ? copy.transpose(-1, -2) : copy;
+}
+
+bool Turned(const at::Tensor& matrices) { return matrices.size(1) > 1 && matrices.stride(1) == 1 && matrices.stride(2) != 1; }
+
 OpsgnnSegmentMatmulDesc DescOf(const at::Tensor& src, const std::optional<at::Tensor>& indptr, int64_t segments, int64_t out,
                                at::ScalarType out_type, const char* api)
 {
@@ -74,7 +106,11 @@ at::Tensor segment_matmul_forward(const at::Tensor& src, const at::Tensor& indpt
     CheckPointers(indptr, src, weight.size(0), api);
     c10::cuda::CUDAGuard guard(src.device());
     RaiseIfDeviceStalled(src, api);
-    const at::Tensor rows = RowMajor(src), matrices = Matrices(weight);
+    at::Tensor rows = RowMajor(src), matrices = Matrices(weight);
+    if (Wants(rows, matrices)) {
+        rows = OnBoundaries(rows);
+        matrices = OnBoundaries(matrices, Turned(matrices));
+    }
     at::Tensor out = at::empty({src.size(0), weight.size(2)}, src.options());
     OpsgnnSegmentMatmulDesc desc = DescOf(rows, indptr, weight.size(0), weight.size(2), src.scalar_type(), api);
     SetWeight(desc, matrices);
@@ -98,7 +134,11 @@ at::Tensor segment_matmul_weight_grad(const at::Tensor& src, const at::Tensor& i
     CheckPointers(indptr, src, segments, api);
     c10::cuda::CUDAGuard guard(src.device());
     RaiseIfDeviceStalled(src, api);
-    const at::Tensor rows = RowMajor(src), upstream = RowMajor(grad);
+    at::Tensor rows = RowMajor(src), upstream = RowMajor(grad);
+    if (rows.scalar_type() != at::kFloat && static_cast<double>(rows.numel()) * static_cast<double>(grad.size(1)) >= kWorthCopy) {
+        rows = OnBoundaries(rows);
+        upstream = OnBoundaries(upstream);
+    }
     at::Tensor out = at::empty({segments, src.size(1), grad.size(1)}, src.options());
     const OpsgnnSegmentMatmulDesc desc = DescOf(rows, indptr, segments, grad.size(1), src.scalar_type(), api);
     int64_t bytes = 0;
@@ -119,7 +159,12 @@ std::vector<at::Tensor> Gradients(const at::Tensor& src, const at::Tensor& indpt
     const char* api = "segment_matmul backward";
     c10::cuda::CUDAGuard guard(src.device());
     RaiseIfDeviceStalled(src, api);
-    const at::Tensor rows = RowMajor(src), matrices = Matrices(weight), upstream = RowMajor(grad);
+    at::Tensor rows = RowMajor(src), matrices = Matrices(weight), upstream = RowMajor(grad);
+    if (Wants(rows, matrices)) {
+        rows = OnBoundaries(rows);
+        matrices = OnBoundaries(matrices, Turned(matrices));
+        upstream = OnBoundaries(upstream);
+    }
     const bool turned = weight.stride(1) == 1 && weight.stride(2) != 1;
     OpsgnnSegmentMatmulDesc desc = DescOf(rows, indptr, weight.size(0), weight.size(2), src.scalar_type(), api);
     SetWeight(desc, matrices);
@@ -198,13 +243,17 @@ at::Tensor segment_matmul_fp8(const at::Tensor& src, const at::Tensor& src_scale
     }
     c10::cuda::CUDAGuard guard(src.device());
     RaiseIfDeviceStalled(src, api);
-    const at::Tensor rows = RowMajor(src), matrices = weight.contiguous();
+    at::Tensor rows = RowMajor(src), matrices = weight.contiguous();
+    if (Wants(rows, matrices)) {
+        rows = OnBoundaries(rows);
+        matrices = OnBoundaries(matrices);
+    }
     const at::Tensor row_scale = src_scale.contiguous(), tile_scale = weight_scale.contiguous();
     at::Tensor out = at::empty({src.size(0), weight.size(1)}, src.options().dtype(out_type));
     OpsgnnSegmentMatmulDesc desc = DescOf(rows, indptr, segments, weight.size(1), out_type, api);
     desc.weight_width_stride = 1;
-    desc.weight_out_stride = src.size(1);
-    desc.weight_segment_stride = weight.size(1) * src.size(1);
+    desc.weight_out_stride = matrices.stride(1);
+    desc.weight_segment_stride = matrices.stride(0);
     CheckStatus(opsgnn_segment_matmul_fp8(&desc, indptr ? indptr->const_data_ptr() : nullptr, rows.const_data_ptr(),
                                           row_scale.const_data_ptr<float>(), matrices.const_data_ptr(),
                                           tile_scale.const_data_ptr<float>(), out.data_ptr(), CurrentStream(src)),

@@ -252,12 +252,12 @@ def test_c_abi_refuses():
     grads = lib.opsgnn_segment_matmul_grads
     assert matmul(grads, None, None, None, None, 8, None, None, 0, None, 0, None) == -1
     assert matmul(grads, 16, None, None, None, 8, None, None, 0, None, 0, None, rows=0, segments=0) == 0
-    assert matmul(grads, 16, 16, 16, 16, 8, 16, 16, 0, None, 0, None, in_type=_cabi.F32, out_type=_cabi.F32) == -3
+    assert matmul(grads, 16, 16, 16, 16, 8, 16, 16, 0, None, 0, None, in_type=_cabi.F32, out_type=_cabi.F32, rows=2_000_000) == -3
     assert matmul(lib.opsgnn_segment_matmul_workspace_bytes, 3, ref(size)) == -1
     assert matmul(outer, None, None, None, 8, None, None, 0, None) == -1
     assert matmul(outer, None, None, None, 8, None, None, 0, None, segments=0) == 0
-    four = dict(in_type=_cabi.F32, out_type=_cabi.F32)
-    assert matmul(lib.opsgnn_segment_matmul_workspace_bytes, 0, ref(size), **four) == 0 and size.value >= 6 * (4 * 8 + 2 * 64)
+    four = dict(in_type=_cabi.F32, out_type=_cabi.F32, rows=2_000_000)  # large enough to go through bf16 terms
+    assert matmul(lib.opsgnn_segment_matmul_workspace_bytes, 0, ref(size), **four) == 0 and size.value >= 6 * (2_000_000 * 8 + 2 * 64)
     assert matmul(rows, 16, 16, 16, 16, None, 0, None, **four) == -3
     assert matmul(lib.opsgnn_segment_matmul_workspace_bytes, 0, ref(size)) == 0 and size.value == 0
     assert matmul(fp8, None, None, None, None, None, None, None) == -2
@@ -1031,3 +1031,74 @@ def test_segment_matmul_one_gradient_at_a_time(cuda_device, dtype, turned, k, n)
     only_weight, = torch.autograd.grad(segment_matmul(src, ptr, w), w, grad)
     assert torch.equal(both[0], only_src) and torch.equal(both[1], only_weight)
     assert both[1].stride() == w.stride()
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", KINDS, ids=str)
+@pytest.mark.parametrize("rows,k,n,segments", [(3001, 201, 133, 3), (2500, 257, 130, 2), (2100, 130, 641, 1), (9000, 100, 77, 5)])
+def test_segment_matmul_large_odd_sizes(cuda_device, dtype, rows, k, n, segments):
+    """Sizes that are no whole vectors and large enough for the tensor cores, both layouts of the weight."""
+    from ops_gnn import segment_matmul
+
+    lengths = [rows // segments - 7 * e for e in range(segments)]
+    src, ptr, weight, grad = _matmul_inputs((lengths, 5, 2, k, n), dtype, 71)
+    want, size = _plain_matmul(src, ptr, weight), _plain_matmul(src.abs(), ptr, weight.abs())
+    back = weight.transpose(1, 2)
+    want_src, size_src = _plain_matmul(grad, ptr, back), _plain_matmul(grad.abs(), ptr, back.abs())
+    want_weight, size_weight = _plain_weight_grad(src, ptr, grad), _plain_weight_grad(src.abs(), ptr, grad.abs())
+    for turned in (False, True):
+        x = src.to(cuda_device).requires_grad_()
+        w = (back.contiguous() if turned else weight).to(cuda_device).requires_grad_()
+        out = segment_matmul(x, ptr.to(cuda_device), w.transpose(1, 2) if turned else w)
+        grad_src, grad_weight = torch.autograd.grad(out, (x, w), grad.to(cuda_device))
+        _within(out, want, size, k + 2, "out")
+        _within(grad_src, want_src, size_src, n + 2, "grad_src")
+        _within(grad_weight.transpose(1, 2) if turned else grad_weight, want_weight, size_weight, max(lengths) + 2, "grad_weight")
+
+
+@requires_gpu
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+@pytest.mark.parametrize("m,k,n", [(700, 304, 333), (513, 1040, 129), (900, 331, 250), (2000, 272, 131)])
+def test_segment_matmul_fp8_large_odd_sizes(cuda_device, m, k, n, out_dtype):
+    from ops_gnn import segment_matmul_fp8
+
+    args = _fp8_inputs([m // 2, 0, m - m // 2], 0, 0, k, n, 81, True)
+    args = (args[0], args[1] * 2.0 ** -9, args[2], args[3] * 2.0 ** -9, args[4])
+    a, b = _stands_for(args[0], args[1], 1), _stands_for(args[2], args[3], 128).transpose(1, 2)
+    got = segment_matmul_fp8(*[t.to(cuda_device) for t in args], out_dtype)
+    _within(got, _plain_matmul(a, args[4], b), _plain_matmul(a.abs(), args[4], b.abs()), k + 4, "fp8")
+
+
+@requires_gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp32", "fp8"])
+def test_stalled_wait_raises(cuda_device, kind):
+    """Waits without polls give up at once: the launch ends, the next call raises, and the one after it is right again."""
+    import ops_gnn
+
+    gen = _gen(91)
+    # large enough for every type to run on the kernels that wait (fp32: 2 * 1200 * 256 * 512 = 3.1e8 operations)
+    src, weight = torch.randn(1200, 256, generator=gen), torch.randn(2, 256, 512, generator=gen)
+    ptr = torch.tensor([0, 500, 1200], device=cuda_device)
+    if kind == "fp8":
+        operands = ops_gnn.quantize_fp8(src.to(cuda_device)) + ops_gnn.quantize_fp8(weight.transpose(1, 2).contiguous().to(cuda_device), 128)
+
+        def run():
+            return ops_gnn.segment_matmul_fp8(*operands, ptr)
+    else:
+        dtype = torch.bfloat16 if kind == "bf16" else torch.float32
+        operands = src.to(dtype).to(cuda_device), ptr, weight.to(dtype).to(cuda_device)
+
+        def run():
+            return ops_gnn.segment_matmul(*operands)
+    want = run()
+    ops_gnn._pybind.device_stall_count(cuda_device.index or 0, True)
+    try:
+        ops_gnn._pybind.set_wait_polls(0)
+        run()
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="timed out"):
+            run()
+    finally:
+        ops_gnn._pybind.set_wait_polls(-1)
+        ops_gnn._pybind.device_stall_count(cuda_device.index or 0, True)
+    assert torch.equal(run(), want)
