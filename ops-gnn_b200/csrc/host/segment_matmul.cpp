@@ -1,12 +1,25 @@
 // Launch planners of the segment products (16 / 32 bits with both gradients, 8 bits with block scales) and of quantize_fp8.
 // No counterpart in the reference.  The pointers are never read on the host: the kernels find their tiles on the device and
 // clamp what they read, so a call neither synchronises nor reads back and can be captured into a graph.
+#include <c10/cuda/CUDAException.h>
+#include <cuda_runtime_api.h>
 #include <pybind11/pybind11.h>
 
 #include "ops.h"
 
 namespace opsgnn {
 namespace {
+
+// A stall of an earlier launch raises here, but not while a graph is captured: the look allocates pinned memory on a device's
+// first use.
+void LookForStalls(const at::Tensor& t, const char* api)
+{
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    C10_CUDA_CHECK(cudaStreamIsCapturing(c10::cuda::getCurrentCUDAStream(t.device().index()).stream(), &capturing));
+    if (capturing == cudaStreamCaptureStatusNone) {
+        RaiseIfDeviceStalled(t, api);
+    }
+}
 
 // A matrix whose rows are runs of consecutive elements, at any row distance.
 at::Tensor RowMajor(const at::Tensor& t)
@@ -105,7 +118,7 @@ at::Tensor segment_matmul_forward(const at::Tensor& src, const at::Tensor& indpt
                 api, ": src must be [rows, width] and weight [segments, width, out] of one dtype on one GPU");
     CheckPointers(indptr, src, weight.size(0), api);
     c10::cuda::CUDAGuard guard(src.device());
-    RaiseIfDeviceStalled(src, api);
+    LookForStalls(src, api);
     at::Tensor rows = RowMajor(src), matrices = Matrices(weight);
     if (Wants(rows, matrices)) {
         rows = OnBoundaries(rows);
@@ -133,7 +146,7 @@ at::Tensor segment_matmul_weight_grad(const at::Tensor& src, const at::Tensor& i
     const int64_t segments = indptr.numel() - 1;
     CheckPointers(indptr, src, segments, api);
     c10::cuda::CUDAGuard guard(src.device());
-    RaiseIfDeviceStalled(src, api);
+    LookForStalls(src, api);
     at::Tensor rows = RowMajor(src), upstream = RowMajor(grad);
     if (rows.scalar_type() != at::kFloat && static_cast<double>(rows.numel()) * static_cast<double>(grad.size(1)) >= kWorthCopy) {
         rows = OnBoundaries(rows);
@@ -158,7 +171,7 @@ std::vector<at::Tensor> Gradients(const at::Tensor& src, const at::Tensor& indpt
 {
     const char* api = "segment_matmul backward";
     c10::cuda::CUDAGuard guard(src.device());
-    RaiseIfDeviceStalled(src, api);
+    LookForStalls(src, api);
     at::Tensor rows = RowMajor(src), matrices = Matrices(weight), upstream = RowMajor(grad);
     if (Wants(rows, matrices)) {
         rows = OnBoundaries(rows);
@@ -242,7 +255,7 @@ at::Tensor segment_matmul_fp8(const at::Tensor& src, const at::Tensor& src_scale
         TORCH_CHECK(segments == 1, api, ": without indptr there is one weight");
     }
     c10::cuda::CUDAGuard guard(src.device());
-    RaiseIfDeviceStalled(src, api);
+    LookForStalls(src, api);
     at::Tensor rows = RowMajor(src), matrices = weight.contiguous();
     if (Wants(rows, matrices)) {
         rows = OnBoundaries(rows);
