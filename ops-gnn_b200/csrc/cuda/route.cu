@@ -800,12 +800,13 @@ __global__ void __launch_bounds__(kWarps * 32) TopkBackwardKernel(RouteParams p,
 // One tile needs the last kernel only.  No atomics on global memory; shared counters are per warp and commute.
 // Bound by latency: three launches, and in the last a chain of counts, prefix and ranks.  1048576 pairs, 256 experts: 512 tiles
 // of eight warps 21.9 us, one tile per SM of 32 warps 17.9 us (24.5 with the scan inside the last kernel, where every block reads
-// all counts); 512 pairs, 128 experts in one tile: 5.0 us with eight warps, 3.8 with 32.
+// all counts); 512 pairs, 128 experts in one tile: 3.0 us with 16 warps, 3.7 with
+// 32.
 constexpr int kMaxBins = 4096;
 constexpr int kSortWarps = 32;
 
-// Warps of a block: as many tables of bins as shared memory holds.
-inline int SortWarps(int bins) { return bins <= 1500 ? kSortWarps : 8; }
+// Warps of a block: as many tables of bins as shared memory holds; a block on its own is done sooner with half as many.
+inline int SortWarps(int bins, int64_t tiles) { return bins > 1500 ? 8 : (tiles == 1 ? kSortWarps / 2 : kSortWarps); }
 
 template <class I> __device__ __forceinline__ int BinOf(const I* index, int64_t at, int64_t end, int experts)
 {
@@ -1187,7 +1188,7 @@ extern "C" int opsgnn_route_csr(const void* index, int index_type, int64_t count
     const int64_t tiles = route::SortTiles(count), tile = std::max<int64_t>(1, CeilDiv(count, tiles));
     int32_t* counts = tiles > 1 ? static_cast<int32_t*>(workspace) : nullptr;
     int32_t* totals = tiles > 1 ? counts + bins * tiles : nullptr;
-    const int warps = route::SortWarps(bins);
+    const int warps = route::SortWarps(bins, tiles);
     const int shared = warps * bins * 4;
     auto run = [&](auto tag) {
         using I = decltype(tag);

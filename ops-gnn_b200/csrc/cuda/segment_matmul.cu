@@ -36,7 +36,7 @@ bool Splits(const OpsgnnSegmentMatmulDesc& d, int what)
     return flops >= 2e8 || (what != OPSGNN_SEGMENT_MATMUL_FORWARD && d.rows >= 2048);
 }
 
-// Weight gradients of 16-bit types that may be summed in pieces.
+// 16-bit products, which may be summed in pieces.
 bool Pieces(const OpsgnnSegmentMatmulDesc& d)
 {
     return d.in_type != OPSGNN_F32 && d.rows > 0 && d.segments > 0 && d.width > 0 && d.out > 0;
@@ -57,7 +57,7 @@ int RunRows(const RowsProblem& p, void* workspace, cudaStream_t stream)
 {
     int ran = OPSGNN_ERR_UNSUPPORTED;
     if (p.in_type != OPSGNN_F32) {
-        ran = RunRowsTensor(p, stream);
+        ran = RunRowsTensor(p, workspace, stream);
     } else if (workspace != nullptr) {
         ran = RunRowsSplit(p, workspace, stream);
     }
@@ -94,14 +94,16 @@ extern "C" int opsgnn_segment_matmul_workspace_bytes(const OpsgnnSegmentMatmulDe
     const bool split = segmm::Splits(*desc, what);
     *bytes = 0;
     if (what == OPSGNN_SEGMENT_MATMUL_FORWARD) {
-        *bytes = split ? segmm::RowsSplitBytes(rows, segments, width, out) : 0;
+        *bytes = split ? segmm::RowsSplitBytes(rows, segments, width, out)
+                       : (segmm::Pieces(*desc) ? segmm::RowsPartialBytes(rows, segments, width, out) : 0);
     } else if (what == OPSGNN_SEGMENT_MATMUL_WEIGHT_GRAD) {
         *bytes = split ? segmm::OuterSplitBytes(rows, segments, width, out)
                        : (segmm::Pieces(*desc) ? segmm::OuterPartialBytes(rows, segments, width, out) : 0);
     } else if (what == OPSGNN_SEGMENT_MATMUL_GRADS) {
         *bytes = split ? segmm::GradsSplitBytes(rows, segments, width, out)
-                       : (segmm::Pieces(*desc) ? std::max(segmm::OuterPartialBytes(rows, segments, width, out),
-                                                          segmm::OuterPartialBytes(rows, segments, out, width))
+                       : (segmm::Pieces(*desc) ? std::max({segmm::RowsPartialBytes(rows, segments, out, width),
+                                                           segmm::OuterPartialBytes(rows, segments, width, out),
+                                                           segmm::OuterPartialBytes(rows, segments, out, width)})
                                                : 0);
     } else {
         return OPSGNN_ERR_INVALID;

@@ -37,7 +37,7 @@ int RunRowsSimple(const RowsProblem& p, cudaStream_t stream);
 int RunOuterSimple(const OuterProblem& p, cudaStream_t stream);
 // 16-bit types on the tensor cores (segment_matmul_tc.cu): widths and strides of whole 16-byte vectors, 16-byte aligned
 // bases.  OPSGNN_ERR_UNSUPPORTED, with nothing launched, for anything else.
-int RunRowsTensor(const RowsProblem& p, cudaStream_t stream);
+int RunRowsTensor(const RowsProblem& p, void* workspace, cudaStream_t stream);
 int RunOuterTensor(const OuterProblem& p, void* workspace, cudaStream_t stream);
 // 8-bit and fp32 operands on the tensor cores (segment_matmul_promoted.cu), under the same conditions; fp32 needs a workspace.
 int RunRowsFp8(const RowsProblem& p, cudaStream_t stream);
@@ -51,6 +51,7 @@ int64_t GradsSplitBytes(int64_t rows, int64_t segments, int64_t k, int64_t n);
 int RunGradsSplit(const RowsProblem& rows, const OuterProblem& outer, bool turned, void* workspace, cudaStream_t stream);
 // Outer form with few result tiles: rows per piece (0: one piece per segment), fp32 scratch for the pieces, and their sum.
 int64_t OuterChunk(int64_t rows, int64_t segments, int64_t k, int64_t n);
+int64_t RowsPartialBytes(int64_t rows, int64_t segments, int64_t k, int64_t n);  // the same for the rows form; null: in one piece
 int64_t OuterPartialBytes(int64_t rows, int64_t segments, int64_t k, int64_t n);
 int JoinPieces(const OuterProblem& p, int64_t chunk, const float* partial, cudaStream_t stream);
 

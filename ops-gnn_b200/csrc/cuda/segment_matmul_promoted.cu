@@ -652,6 +652,9 @@ int Launch(const CUtensorMap& a, const CUtensorMap& tail, const CUtensorMap& b, 
 // Bytes of the planes of lines of `width` values.
 int64_t PlaneBytes(int64_t lines, int64_t width) { return AlignUp(lines * PlaneWidth(width) * 3 * 2, 1024); }
 
+// Tiles of 128 columns in place of 256: where the wide ones leave half the SMs without a tile.
+bool Narrow128(int64_t down, int64_t n) { return n <= 128 || down * CeilDiv(n, 256) * 2 <= SmCount(); }
+
 bool RowsSplittable(const RowsProblem& p)
 {
     return p.in_type == OPSGNN_F32 && p.k >= 1 && p.ldo == p.n && (p.b_k == 1 || p.b_n == 1) && p.ptr.segments >= 1 &&
@@ -700,7 +703,8 @@ int RowsFromPlanes(const RowsProblem& p, const void* planes_a, const void* plane
     q.b_n = p.b_n;
     OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
     const int64_t inner = turned ? p.k : p.n, other = turned ? p.n : p.k, e = p.ptr.segments;
-    const bool narrow = p.n <= 128;
+    const int64_t down = p.ptr.rows / kRows + std::min(e, p.ptr.rows);
+    const bool narrow = Narrow128(down, p.n);
     q.whole_b = tc::WholeSlabs(p.n);
     const int64_t wide_a = PlaneWidth(p.k), wide_b = PlaneWidth(inner);
     q.vec = p.n % 4 == 0 && Aligned(p.out, 16);
@@ -711,11 +715,11 @@ int RowsFromPlanes(const RowsProblem& p, const void* planes_a, const void* plane
                  : tc::EncodeSlabs(&b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, planes_b, p.n, p.k, 3 * e, wide_b * 2, wide_b * p.k * 2, narrow ? 2 : 4))) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
-    const int64_t down = p.ptr.rows / kRows + e;
+    const int64_t tiles = down * CeilDiv(p.n, narrow ? 128 : 256);
     if (narrow) {
-        return turned ? Launch<false, float, 128, kRowsTurned>(a, tail, b, q, down, stream) : Launch<false, float, 128, kRowsWide>(a, tail, b, q, down, stream);
+        return turned ? Launch<false, float, 128, kRowsTurned>(a, tail, b, q, tiles, stream)
+                      : Launch<false, float, 128, kRowsWide>(a, tail, b, q, tiles, stream);
     }
-    const int64_t tiles = down * CeilDiv(p.n, 256);
     return turned ? Launch<false, float, 256, kRowsTurned>(a, tail, b, q, tiles, stream) : Launch<false, float, 256, kRowsWide>(a, tail, b, q, tiles, stream);
 }
 
@@ -827,13 +831,14 @@ int RunRowsFp8(const RowsProblem& p, cudaStream_t stream)
     q.k = p.k;
     OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
     q.vec = p.n % (16 / DtypeBytes(p.out_type)) == 0 && Aligned(p.out, 16);
-    const bool narrow = p.n <= 128;
+    const int64_t down = p.ptr.rows / kRows + std::min(p.ptr.segments, p.ptr.rows);
+    const bool narrow = Narrow128(down, p.n);
     CUtensorMap a, tail, b;
     if (!Map3(&a, true, p.a, p.k, p.ptr.rows, 1, p.lda, p.lda, kRows) || !Map3(&tail, true, p.a, p.k, p.ptr.rows, 1, p.lda, p.lda, kBoxRows) ||
         !Map3(&b, true, p.b, p.k, p.n, p.ptr.segments, p.b_n, p.b_segment, narrow ? 128 : 256)) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
-    const int64_t across = CeilDiv(p.n, narrow ? 128 : 256), tiles = (p.ptr.rows / kRows + p.ptr.segments) * across;
+    const int64_t tiles = down * CeilDiv(p.n, narrow ? 128 : 256);
     auto run = [&](auto tag) {
         using O = decltype(tag);
         return narrow ? Launch<true, O, 128, kRowsTurned>(a, tail, b, q, tiles, stream)

@@ -68,7 +68,7 @@ constexpr int kStagingBytes = 4 * 32 * 128;  // per epilogue warp 32 rows of 64 
 
 enum Form { kRowsWide, kRowsTurned, kOuter };  // weight's columns along memory; its reduced index along memory; grad_weight
 
-template <int BN> constexpr int Stages() { return BN == 256 ? 4 : 6; }
+template <int BN> constexpr int Stages() { return BN == 256 ? 4 : (BN == 128 ? 6 : 8); }
 template <int BN> constexpr int StageBytes() { return kRows * 128 + BN * 128; }
 template <int BN> constexpr int SharedBytes() { return 1024 + Stages<BN>() * StageBytes<BN>() + kStagingBytes + 256; }
 
@@ -78,13 +78,14 @@ struct Params {
     int64_t m, n, k;   // rows form: n columns, k reduced; outer form: m x n results per segment
     bool whole_a, whole_b;  // MN-major operands: all slabs in one load
     bool vec;               // rows of out start on 16-byte boundaries
-    int64_t chunk;     // outer form: rows per partial result; 0: a segment's rows in one piece
-    float* partial;    // [pieces][m][n]
+    int64_t chunk;     // of the reduced index per partial result; 0: all of it in one piece
+    int64_t pieces;    // rows form: pieces of the reduced index
+    float* partial;    // outer form [pieces][m][n], rows form [pieces][rows][n]
     WaitSettings wait;
 };
 
 struct Barriers {
-    uint64_t full[6], empty[6], done[2], free[2], drain;
+    uint64_t full[8], empty[8], done[2], free[2], drain;
     uint32_t tmem, stop;
 };
 
@@ -142,14 +143,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Rows, widths and tile numbers fit 32 bits (checked on the host); offsets in memory are formed in 64.
     const int n = static_cast<int>(p.n), m = static_cast<int>(p.m), width = static_cast<int>(p.k), chunk = static_cast<int>(p.chunk);
     const int across = (n + BN - 1) / BN;
-    const int down = FORM == kOuter ? (m + kRows - 1) / kRows : 1;
+    const int down = FORM == kOuter ? (m + kRows - 1) / kRows : 1, pieces = static_cast<int>(p.pieces);
     SegmentWalk<FORM == kOuter ? 0 : kRows, int> walk;
     if (warp != 2 && warp != 3 && (FORM != kOuter || chunk > 0)) {
         walk.Start(p.ptr, FORM == kOuter ? chunk : kRows);
     }
     // Tile t: its segment, first result row and column, and the range of the reduced index.
-    int segment = 0, row = 0, row_end = 0, column = 0, from = 0, depth = 0;
+    int segment = 0, row = 0, row_end = 0, column = 0, from = 0, depth = 0, piece = 0;
     auto find = [&](int t) {
+        if constexpr (FORM != kOuter) {
+            piece = t % pieces;
+            t /= pieces;
+        }
         column = t % across * BN;
         t /= across;
         if constexpr (FORM == kOuter) {
@@ -178,7 +183,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             segment = walk.segment;
             row = walk.row;
             row_end = walk.row_end;
-            depth = width;
+            from = piece * chunk;
+            depth = chunk > 0 ? min(chunk, width - from) : width;
             return true;
         }
     };
@@ -206,16 +212,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const int boxes = Boxes(row_end - row);
                         tc::BarExpect(&bar.full[s], boxes * kBoxRows * 128 + BN * 128);
                         if (boxes * kBoxRows == kRows) {
-                            tc::LoadTo(map_a, full, a, k, row);
+                            tc::LoadTo(map_a, full, a, from + k, row);
                         } else {
                             for (int i = 0; i < boxes; ++i) {
-                                tc::LoadTo(map_tail, full, a + i * kBoxRows * 128, k, row + i * kBoxRows);
+                                tc::LoadTo(map_tail, full, a + i * kBoxRows * 128, from + k, row + i * kBoxRows);
                             }
                         }
                         if constexpr (FORM == kRowsTurned) {
-                            tc::LoadTo(map_b, full, b, k, column, segment);
+                            tc::LoadTo(map_b, full, b, from + k, column, segment);
                         } else {
-                            tc::LoadSlabs(map_b, full, b, column, k, segment, BN / 64, p.whole_b);
+                            tc::LoadSlabs(map_b, full, b, column, from + k, segment, BN / 64, p.whole_b);
                         }
                     }
                 }
@@ -321,6 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc::FenceAfter();
             }
             T* to = out + (FORM == kOuter ? segment * p.m * p.n : 0);
+            float* sums = p.partial + (FORM == kOuter ? segment * p.m * p.n : piece * p.ptr.rows * p.n);
             const int first = row + quarter * 32;
 #pragma unroll 1
             for (int c = 0; c < BN; c += 64) {
@@ -334,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc::TmemLoad32(at, low);
                     tc::TmemLoad32(at + 32, high);
                     tc::TmemWait();
-                    if (FORM == kOuter && p.chunk > 0) {
+                    if (chunk > 0) {
                         // A piece of the sum, kept in fp32: 32 columns are 128 bytes.
 #pragma unroll
                         for (int side = 0; side < 2; ++side) {
@@ -346,8 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                             __syncwarp();
                             const int col = column + c + side * 32;
-                            tc::StoreStaged<128>(mine, p.partial + segment * p.m * p.n + first * p.n + col, p.n, row_end - first, n - col,
-                                                 n % 4 == 0);
+                            tc::StoreStaged<128>(mine, sums + first * p.n + col, p.n, row_end - first, n - col, n % 4 == 0);
                             __syncwarp();
                         }
                         continue;
@@ -383,9 +389,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         if constexpr (FORM != kOuter) {
-            // Rows of no segment.
+            // Rows of no segment (in pieces, the join writes them).
             const int64_t before = p.ptr.Raw(0), behind = p.ptr.Raw(p.ptr.segments);
-            for (int64_t r = blockIdx.x * 4 + quarter; r < before + (p.ptr.rows - behind); r += gridDim.x * 4) {
+            for (int64_t r = blockIdx.x * 4 + quarter; chunk == 0 && r < before + (p.ptr.rows - behind); r += gridDim.x * 4) {
                 const int64_t at = r < before ? r : behind + (r - before);
                 for (int c = lane; c < n; c += 32) {
                     out[at * p.n + c] = Narrow<T, float>(0.0f);
@@ -439,18 +445,78 @@ int Launch(const CUtensorMap& a, const CUtensorMap& tail, const CUtensorMap& b, 
     return LaunchStatus();
 }
 
-template <int FORM, class F> int ByType(int type, bool narrow, F&& f)
+// f(type tag, integral constant of a tile's columns)
+template <class F> int ByType(int type, int columns, F&& f)
 {
     using std::integral_constant;
-    if (type == OPSGNN_BF16) {
-        return narrow ? f(__nv_bfloat16(), integral_constant<int, 128>()) : f(__nv_bfloat16(), integral_constant<int, 256>());
+    auto by_columns = [&](auto tag) {
+        switch (columns) {
+            case 64:
+                return f(tag, integral_constant<int, 64>());
+            case 128:
+                return f(tag, integral_constant<int, 128>());
+            default:
+                return f(tag, integral_constant<int, 256>());
+        }
+    };
+    return type == OPSGNN_BF16 ? by_columns(__nv_bfloat16()) : by_columns(__half());
+}
+
+// Columns of a tile of the rows form: 256, which reads an operand least often, unless that leaves half the SMs without a tile
+// (`down`: most row tiles there can be).  2000 x 300 -> 300 in 5 segments: 16.8 us with 64 columns, 29.3 with 256.
+int TileColumns(int64_t down, int64_t n)
+{
+    int columns = n <= 64 ? 64 : (n <= 128 ? 128 : 256);
+    while (columns > 64 && down * CeilDiv(n, columns) * 2 <= SmCount()) {
+        columns /= 2;
     }
-    return narrow ? f(__half(), integral_constant<int, 128>()) : f(__half(), integral_constant<int, 256>());
+    return columns;
+}
+
+int64_t RowTiles(int64_t rows, int64_t segments) { return rows / kRows + std::min(segments, rows); }
+
+// Pieces of the reduced index of the rows form, summed apart and joined: where even narrow tiles leave half the SMs idle and the
+// sum is long.  One row x 2048 -> 2048 (32 tiles, four pieces): 16.6 us in one piece, 12.8 us in pieces; 16 rows in 4 segments,
+// 2048 -> 1024 (64 tiles, two pieces) 16.8 us either way, hence three pieces at least.
+int64_t RowPieces(int64_t rows, int64_t segments, int64_t k, int64_t n)
+{
+    const int64_t tiles = RowTiles(rows, segments) * CeilDiv(n, 64);
+    return tiles * 3 > SmCount() || k < 1536 ? 1 : std::min<int64_t>(SmCount() / std::max<int64_t>(tiles, 1), k / 512);
 }
 
 }  // namespace
 
-int RunRowsTensor(const RowsProblem& p, cudaStream_t stream)
+int64_t RowsPartialBytes(int64_t rows, int64_t segments, int64_t k, int64_t n)
+{
+    const int64_t pieces = RowPieces(rows, segments, k, n);
+    return pieces > 1 ? AlignUp(pieces * rows * n * 4, 256) : 0;
+}
+
+namespace {
+
+// out[r] <- the sum of the pieces of row r, in their order; 0 for a row of no segment.
+template <class T>
+__global__ void __launch_bounds__(256) JoinRowsKernel(SegmentPointers ptr, int64_t n, int64_t pieces, const float* __restrict__ partial,
+                                                      T* __restrict__ out)
+{
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x, size = ptr.rows * n;
+    if (i >= size) {
+        return;
+    }
+    const int64_t row = i / n;
+    float sum = 0.0f;
+    if (row >= ptr.Raw(0) && row < ptr.Raw(ptr.segments)) {
+#pragma unroll 4
+        for (int64_t c = 0; c < pieces; ++c) {
+            sum += __ldcs(partial + c * size + i);
+        }
+    }
+    out[i] = Narrow<T, float>(sum);
+}
+
+}  // namespace
+
+int RunRowsTensor(const RowsProblem& p, void* workspace, cudaStream_t stream)
 {
     const bool turned = p.b_k == 1 && p.b_n != 1;
     const int64_t inner = turned ? p.k : p.n, other = turned ? p.n : p.k, stride = turned ? p.b_n : p.b_k;
@@ -467,26 +533,41 @@ int RunRowsTensor(const RowsProblem& p, cudaStream_t stream)
     q.k = p.k;
     q.vec = p.n % 8 == 0 && Aligned(p.out, 16);
     OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
-    const bool narrow = p.n <= 128;
+    const int64_t down = RowTiles(p.ptr.rows, p.ptr.segments);
+    const int64_t pieces = workspace != nullptr ? RowPieces(p.ptr.rows, p.ptr.segments, p.k, p.n) : 1;
+    q.chunk = pieces > 1 ? AlignUp(CeilDiv(p.k, pieces), kDepth) : 0;
+    q.pieces = pieces > 1 ? CeilDiv(p.k, q.chunk) : 1;
+    q.partial = static_cast<float*>(workspace);
+    const int columns = TileColumns(down, p.n);
     q.whole_b = tc::WholeSlabs(p.n);
     CUtensorMap a, tail, b;
     const uint64_t sizes[3] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(other), static_cast<uint64_t>(p.ptr.segments)};
     const uint64_t strides[2] = {static_cast<uint64_t>(stride) * 2, static_cast<uint64_t>(p.b_segment) * 2};
-    const uint32_t box[3] = {64, narrow ? 128u : 256u, 1};
+    const uint32_t box[3] = {64, static_cast<uint32_t>(columns), 1};
     const CUtensorMapDataType type = TypeOf(p.in_type);
     if (!Map2(&a, p.in_type, p.a, p.k, p.ptr.rows, p.lda, kDepth, kRows) ||
         !Map2(&tail, p.in_type, p.a, p.k, p.ptr.rows, p.lda, kDepth, kBoxRows) ||
         !(turned ? tc::EncodeMap(&b, type, 3, p.b, sizes, strides, box)
-                 : tc::EncodeSlabs(&b, type, p.b, p.n, p.k, p.ptr.segments, stride * 2, p.b_segment * 2, narrow ? 2 : 4))) {
+                 : tc::EncodeSlabs(&b, type, p.b, p.n, p.k, p.ptr.segments, stride * 2, p.b_segment * 2, columns / 64))) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
     auto run = [&](auto tag, auto width) {
         using T = decltype(tag);
         constexpr int BN = decltype(width)::value;
-        const int64_t tiles = (p.ptr.rows / kRows + p.ptr.segments) * CeilDiv(p.n, BN);
+        const int64_t tiles = down * CeilDiv(p.n, BN) * q.pieces;
         return turned ? Launch<T, BN, kRowsTurned>(a, tail, b, q, tiles, stream) : Launch<T, BN, kRowsWide>(a, tail, b, q, tiles, stream);
     };
-    return ByType<0>(p.in_type, narrow, run);
+    const int status = ByType(p.in_type, columns, run);
+    if (status != OPSGNN_OK || q.pieces == 1) {
+        return status;
+    }
+    const unsigned grid = static_cast<unsigned>(CeilDiv(p.ptr.rows * p.n, 256));
+    if (p.in_type == OPSGNN_BF16) {
+        JoinRowsKernel<<<grid, 256, 0, stream>>>(p.ptr, p.n, q.pieces, q.partial, static_cast<__nv_bfloat16*>(p.out));
+    } else {
+        JoinRowsKernel<<<grid, 256, 0, stream>>>(p.ptr, p.n, q.pieces, q.partial, static_cast<__half*>(p.out));
+    }
+    return LaunchStatus();
 }
 
 namespace {
@@ -596,7 +677,7 @@ int RunOuterTensor(const OuterProblem& p, void* workspace, cudaStream_t stream)
         const int64_t results = q.chunk > 0 ? p.ptr.rows / q.chunk + p.ptr.segments : p.ptr.segments;
         return Launch<T, BN, kOuter>(a, a, b, q, results * CeilDiv(p.k, kRows) * CeilDiv(p.n, BN), stream);
     };
-    const int status = ByType<0>(p.type, narrow, run);
+    const int status = ByType(p.type, narrow ? 128 : 256, run);
     return status == OPSGNN_OK && q.chunk > 0 ? JoinPieces(p, q.chunk, q.partial, stream) : status;
 }
 

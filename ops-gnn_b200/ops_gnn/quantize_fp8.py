@@ -35,4 +35,4 @@ def quantize_fp8(src: torch.Tensor, block_rows: int = 1) -> Tuple[torch.Tensor, 
         raise ValueError(f"block_rows must be 1 or {BLOCK}, got {block_rows}")
     if src.device.type != "cuda":
         raise RuntimeError("quantize_fp8 requires CUDA tensors")
-    return _pybind.quantize_fp8(src.detach().contiguous(), block_rows)
+    return _pybind.quantize_fp8(src.contiguous(), block_rows)

@@ -12,6 +12,8 @@ MAX_EXPERTS, MAX_CHOSEN, MAX_GROUPS = 1024, 32, 32
 
 
 def _check_int(name: str, value, low: int, high: int) -> None:
+    if type(value) is int and low <= value <= high:
+        return
     if not isinstance(value, int) or isinstance(value, bool):
         raise TypeError(f"{name} must be an int, got {type(value).__name__}")
     if not low <= value <= high:

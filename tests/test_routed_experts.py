@@ -1102,3 +1102,26 @@ def test_stalled_wait_raises(cuda_device, kind):
         ops_gnn._pybind.set_wait_polls(-1)
         ops_gnn._pybind.device_stall_count(cuda_device.index or 0, True)
     assert torch.equal(run(), want)
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("lengths,k,n", [([1], 2048, 256), ([3, 0, 14], 1100, 65), ([130], 4096, 8), ([2, 2], 1536, 1024), ([1], 1025, 72)])
+def test_segment_matmul_few_rows_and_long_sums(cuda_device, dtype, lengths, k, n):
+    """Serving steps: the sum over the width is cut into pieces and joined; rows of no segment are 0."""
+    from ops_gnn import segment_matmul
+
+    src, ptr, weight, grad = _matmul_inputs((lengths, 2, 3, k, n), dtype, 101)
+    want, size = _plain_matmul(src, ptr, weight), _plain_matmul(src.abs(), ptr, weight.abs())
+    for turned in (False, True):
+        x = src.to(cuda_device).requires_grad_()
+        w = (weight.transpose(1, 2).contiguous() if turned else weight).to(cuda_device).requires_grad_()
+        out = segment_matmul(x, ptr.to(cuda_device), w.transpose(1, 2) if turned else w)
+        _within(out, want, size, k + 2, "out")
+        assert not out[:2].any() and not out[-3:].any()
+        assert torch.equal(out, segment_matmul(x, ptr.to(cuda_device), w.transpose(1, 2) if turned else w))
+        grad_src, grad_weight = torch.autograd.grad(out, (x, w), grad.to(cuda_device))
+        back = weight.transpose(1, 2)
+        _within(grad_src, _plain_matmul(grad, ptr, back), _plain_matmul(grad.abs(), ptr, back.abs()), n + 2, "grad_src")
+        _within(grad_weight.transpose(1, 2) if turned else grad_weight, _plain_weight_grad(src, ptr, grad),
+                _plain_weight_grad(src.abs(), ptr, grad.abs()), sum(lengths) + 2, "grad_weight")
