@@ -218,21 +218,24 @@ __device__ __forceinline__ void CloseGroups(const RouteParams& p, uint32_t (&key
     }
 }
 
-// One score in 64 bits; `inverse`: 1 / the softmax's sum.
-__device__ __forceinline__ double FineScore(const RouteParams& p, float l, float base, double inverse)
+// What the choice goes by, in 64 bits; `inverse`: 1 / the softmax's sum.
+template <bool BIASED> __device__ __forceinline__ double FineScore(const RouteParams& p, float l, float base, double inverse)
 {
     const double x = static_cast<double>(l);
+    if constexpr (!BIASED) {
+        return base == base ? x : static_cast<double>(NAN);  // scores order as the logits do
+    }
     return p.softmax ? exp(x - static_cast<double>(base)) * inverse : 1.0 / (1.0 + exp(-x));
 }
 
-// The choice with scores in 64 bits, for rows whose fp32 scores are too close to tell.  Lane i < k gets the i-th choice.  The
+// The choice in 64 bits, for rows whose packed keys are too close to tell.  Lane i < k gets the i-th choice.  The
 // keys live in shared memory (experts keys per warp), so that nothing of this weighs on the registers of the common path.
-template <class T>
+template <class T, bool BIASED>
 __device__ __noinline__ void ChooseFine(const RouteParams& p, const T* row, const float* bias, float base, uint64_t* keys, int& chosen)
 {
     const int lane = threadIdx.x & 31;
     double inverse = 1.0;
-    if (p.softmax) {
+    if (BIASED && p.softmax) {
         double part = 0.0;
 #pragma unroll 4
         for (int at = lane; at < p.experts; at += 32) {
@@ -245,7 +248,7 @@ __device__ __noinline__ void ChooseFine(const RouteParams& p, const T* row, cons
 #pragma unroll 4
     for (int at = lane; at < p.experts; at += 32) {
         const float l = Widen<float, T>(LoadNc(row + at));
-        double v = FineScore(p, l, base, inverse);
+        double v = FineScore<BIASED>(p, l, base, inverse);
         if (bias != nullptr) {
             v += static_cast<double>(__ldg(bias + at));
         }
@@ -306,13 +309,19 @@ __device__ __noinline__ void ChooseFine(const RouteParams& p, const T* row, cons
 
 // BIASED: the choice needs the scores themselves (a bias, or groups ranked by a sum of two); otherwise it compares logits.
 //
-// Logits of 16 bits and their expert's number fit one 32-bit key, all keys differ, and each step of the choice is one warp
-// maximum (redux) and a pop from the winning lane's sorted keys.  32-bit keys take a second step to find the winner's lane.
+// Every expert gets one 32-bit key that differs from all others: where it stands in the order, then its number, the lower first.
+// Each step of the choice is one warp maximum (redux) and a pop from the winning lane's sorted keys.  Logits of 16 bits fit
+// the key as they are.  Others are measured on a scale of 22 bits that reaches from the largest down to the smallest of the
+// lanes' largest values, below which no k <= 31 winners lie, and neighbours in the resulting order that are too close to tell
+// send the row to ChooseFine: closer than the scale's steps or, BIASED, than twice the error of the scores, unless they are
+// equal by their inputs.  (4099 x 256, bias, 8 groups: 17.4 us with 32-bit keys and a search for the winner's lane, 12.5 us;
+// about one row in 300 goes to ChooseFine.)
 //
-// BIASED scores are formed in fp32 first.  A sigmoid is off by at most 2^-22 (exp to 2 ulp at a slope of 1/4, an addition, a
-// division), a softmax by 2^-20 of its largest score, less the error of the sum, which all share; the bias adds 2^-24 of the
-// result.  Where two neighbours in the order, or a group let in and one left out, are closer than twice that and not equal by
-// their inputs, the row is chosen again in 64 bits: about one row in 300 at 256 experts.
+// BIASED scores are formed in fp32 with the fast exponential and division.  A sigmoid is off by at most 2^-22: its slope times
+// the exponential's 2 + 1.16 |x| steps, an addition, a division.  A softmax is off by 2^-21 of its largest score, and the sum's
+// error is shared; the bias adds 2^-24 of the result.
+constexpr float kScale = 4194000.0f;
+
 template <class T, int VPL, bool BIASED>
 __global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T* __restrict__ logits, const float* __restrict__ bias,
                                                           T* __restrict__ weight, int64_t* __restrict__ index, bool wide)
@@ -320,11 +329,12 @@ __global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T
     extern __shared__ __align__(16) unsigned char shared[];
     constexpr bool PACKED = sizeof(T) == 2 && !BIASED;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // The keys of a warp's row, needed across lanes only where groups are not whole lanes (64-bit ones in ChooseFine).
-    unsigned char* row_keys = shared + static_cast<size_t>(warp) * p.experts * (BIASED ? 8 : 4);
+    // The keys of a warp's row, needed across lanes only where groups are not whole lanes, and by ChooseFine.
+    unsigned char* row_keys = shared + static_cast<size_t>(warp) * p.experts * (PACKED ? 4 : 8);
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWarps + warp; r < p.rows; r += static_cast<int64_t>(gridDim.x) * kWarps) {
+        const T* row = logits + r * p.experts;
         float l[VPL];
-        LoadRow<T, VPL>(logits + r * p.experts, p.experts, wide, lane, l);
+        LoadRow<T, VPL>(row, p.experts, wide, lane, l);
         // A softmax over NaN or +inf has no finite value: the whole row is NaN, as torch.softmax has it.
         float top = -INFINITY;
         bool bad = false;
@@ -341,19 +351,19 @@ __global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T
             }
         }
 
+        // What the choice goes by, as order-preserving keys.
         uint32_t key[VPL];
-        float margin = 0.0f, whole_sum = 1.0f;
+        float margin = 0.0f;
         if constexpr (BIASED) {
             float c[VPL];
             if (p.softmax) {
                 float part = 0.0f;
 #pragma unroll
                 for (int j = 0; j < VPL; ++j) {
-                    c[j] = l[j] == -INFINITY ? 0.0f : expf(l[j] - top);
+                    c[j] = l[j] == -INFINITY ? 0.0f : __expf(l[j] - top);
                     part += c[j];
                 }
-                whole_sum = WarpSum(part);
-                const float inverse = 1.0f / whole_sum;
+                const float inverse = 1.0f / WarpSum(part);
 #pragma unroll
                 for (int j = 0; j < VPL; ++j) {
                     c[j] *= inverse;
@@ -362,7 +372,7 @@ __global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T
             } else {
 #pragma unroll
                 for (int j = 0; j < VPL; ++j) {
-                    c[j] = Sigmoid(l[j]);
+                    c[j] = __fdividef(1.0f, 1.0f + __expf(-l[j]));
                 }
                 margin = 0x1p-20f;
             }
@@ -401,50 +411,76 @@ __global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T
 
         bool sure = true;
         if (p.groups > 1) {
+            // (Packed keys rank a group by its best logit, ties to the lower group: the expert's number orders the same way.)
             float gap;
-            if constexpr (PACKED) {
-                // Rank by the logit alone, ties to the lower group: the expert's number inside the key orders the same way.
-                CloseGroups<VPL>(p, key, reinterpret_cast<uint32_t*>(row_keys), lane, gap);
-            } else {
-                CloseGroups<VPL>(p, key, reinterpret_cast<uint32_t*>(row_keys), lane, gap);
-                sure = !BIASED || gap > 2.0f * margin;
+            CloseGroups<VPL>(p, key, reinterpret_cast<uint32_t*>(row_keys), lane, gap);
+            sure = !BIASED || gap > 2.0f * margin;
+        }
+
+        const int steps = PACKED ? p.k : min(p.k + 3, 32);  // a few beyond the choice, to see that it is clear of them
+        float units = 0.0f;                                 // of the scale: what tells two neighbours apart
+        if constexpr (!PACKED) {
+            uint32_t mine = 0;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                mine = max(mine, key[j]);
+            }
+            const uint32_t high = __reduce_max_sync(kFull, mine);
+            uint32_t low = mine > kMasked ? mine : 0xffffffffu;
+            if (__popc(__ballot_sync(kFull, mine > kMasked)) <= steps) {  // too few lanes: the smallest value of all
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) {
+                    low = min(low, key[j] > kMasked ? key[j] : 0xffffffffu);
+                }
+            }
+            low = __reduce_min_sync(kFull, low);
+            const float floor = ValueOf(low), range = ValueOf(high) - floor;
+            const float scale = high > kMasked && range > 0.0f ? kScale / range : 0.0f;
+            units = margin * scale + 4.0f;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                const int at = lane * VPL + j;
+                // 0 closed, 1 masked or below the scale
+                // (a range too small or too large for its scale makes it infinite or 0, and then every pair is open)
+                const uint32_t place = key[j] >= low ? 2u + static_cast<uint32_t>(fminf((ValueOf(key[j]) - floor) * scale, kScale)) : 1u;
+                key[j] = key[j] == 0u ? 0u : (place << 10) | (1023u - static_cast<uint32_t>(at));
             }
         }
 
-        int chosen = 0;
-        float chosen_logit = -INFINITY;
-        if constexpr (PACKED) {
-            if constexpr (VPL <= 8) {
-                SortDown<VPL>(key);
+        if constexpr (VPL <= 8) {
+            SortDown<VPL>(key);
+        }
+        uint32_t head = key[0];
+        if constexpr (VPL > 8) {
+#pragma unroll
+            for (int j = 1; j < VPL; ++j) {
+                head = max(head, key[j]);
             }
-            uint32_t head = key[0];
-            if constexpr (VPL > 8) {
+        }
+        uint32_t mine = 0;
+        for (int i = 0; i < steps; ++i) {
+            const uint32_t winner = __reduce_max_sync(kFull, head);
+            mine = lane == i ? winner : mine;
+            if (head == winner) {
+                if constexpr (VPL <= 8) {
 #pragma unroll
-                for (int j = 1; j < VPL; ++j) {
-                    head = max(head, key[j]);
-                }
-            }
-            uint32_t mine = 0;
-            for (int i = 0; i < p.k; ++i) {
-                const uint32_t winner = __reduce_max_sync(kFull, head);
-                mine = lane == i ? winner : mine;
-                if (head == winner) {
-                    if constexpr (VPL <= 8) {
+                    for (int j = 0; j + 1 < VPL; ++j) {
+                        key[j] = key[j + 1];
+                    }
+                    key[VPL - 1] = 0;
+                    head = key[0];
+                } else {
+                    head = 0;
 #pragma unroll
-                        for (int j = 0; j + 1 < VPL; ++j) {
-                            key[j] = key[j + 1];
-                        }
-                        key[VPL - 1] = 0;
-                        head = key[0];
-                    } else {
-                        head = 0;
-#pragma unroll
-                        for (int j = 0; j < VPL; ++j) {
-                            head = max(head, key[j] < winner ? key[j] : 0u);
-                        }
+                    for (int j = 0; j < VPL; ++j) {
+                        head = max(head, key[j] < winner ? key[j] : 0u);
                     }
                 }
             }
+        }
+        int chosen = 0;
+        float chosen_logit = -INFINITY;
+        if constexpr (PACKED) {
             if (lane < p.k) {
                 chosen = static_cast<int>(0xffffu - (mine & 0xffffu));
                 uint32_t bits = mine >> 16;
@@ -455,71 +491,35 @@ __global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T
                     chosen_logit = __uint_as_float(bits << 16);
                 }
                 if (chosen_logit == -INFINITY) {  // the key of a masked expert is that of a NaN, too
-                    chosen_logit = Widen<float, T>(LoadNc(logits + r * p.experts + chosen));
+                    chosen_logit = Widen<float, T>(LoadNc(row + chosen));
                 }
             }
         } else {
-            uint32_t best = 0;
-            int where = 0;
-#pragma unroll
-            for (int j = 0; j < VPL; ++j) {
-                where = key[j] > best ? j : where;
-                best = key[j] > best ? key[j] : best;
-            }
-            uint32_t before = 0;
-            float before_value = 0.0f;
-            int before_at = 0;
-            // BIASED looks one step further: the first expert left out must be clear of the last one taken.
-            const int steps = BIASED && p.k < p.experts ? p.k + 1 : p.k;
-            for (int i = 0; sure && i < steps; ++i) {
-                const uint32_t winner = __reduce_max_sync(kFull, best);
-                if (winner == 0) {
-                    break;  // only the look-ahead can run out of experts
-                }
-                const int owner = __ffs(__ballot_sync(kFull, best == winner)) - 1;
-                float value = l[0];
-#pragma unroll
-                for (int j = 1; j < VPL; ++j) {
-                    value = where == j ? l[j] : value;
-                }
-                const int at = __shfl_sync(kFull, lane * VPL + where, owner);
-                value = __shfl_sync(kFull, value, owner);
-                if (lane == owner) {
-#pragma unroll
-                    for (int j = 0; j < VPL; ++j) {
-                        key[j] = j == where ? 0u : key[j];
-                    }
-                    best = 0;
-#pragma unroll
-                    for (int j = 0; j < VPL; ++j) {
-                        where = key[j] > best ? j : where;
-                        best = key[j] > best ? key[j] : best;
-                    }
-                }
-                if (lane == i) {
-                    chosen = at;
-                    chosen_logit = value;
-                }
-                if constexpr (BIASED) {
-                    if (i > 0 && !(ValueOf(before) - ValueOf(winner) > margin)) {
-                        // Equal by their inputs, or both masked: a tie in every precision.
-                        const bool tie = (before == kMasked && winner == kMasked) ||
-                                         (value == before_value && (bias == nullptr || __ldg(bias + at) == __ldg(bias + before_at)));
-                        sure = tie;
-                    }
-                    before = winner;
-                    before_value = value;
-                    before_at = at;
+            const uint32_t extra = __reduce_max_sync(kFull, head);  // the one after the last step
+            uint32_t next = __shfl_down_sync(kFull, mine, 1);
+            next = lane == steps - 1 ? extra : next;
+            chosen = lane < steps && mine != 0 ? static_cast<int>(1023u - (mine & 1023u)) : 0;
+            chosen_logit = lane < steps ? Widen<float, T>(LoadNc(row + chosen)) : 0.0f;
+            // A pair of neighbours is clear (far apart, or the second masked: those go by their numbers), a tie (equal by
+            // their inputs, the lower number first in every precision) or open.
+            const bool pair = lane < steps && mine != 0;
+            const bool clear = pair && ((next >> 10) <= 1u || static_cast<float>((mine >> 10) - (next >> 10)) > units);
+            bool open = pair && !clear;
+            if (__any_sync(kFull, open)) {
+                const int other = static_cast<int>(1023u - (next & 1023u));
+                if (open) {
+                    const bool same = chosen_logit == Widen<float, T>(LoadNc(row + other));
+                    open = !(same && (!BIASED || bias == nullptr || __ldg(bias + chosen) == __ldg(bias + other)));
                 }
             }
-            if constexpr (BIASED) {
-                if (!sure) {
-                    const T* row = logits + r * p.experts;
-                    ChooseFine<T>(p, row, bias, bad ? NAN : top, reinterpret_cast<uint64_t*>(row_keys), chosen);
-                    if (lane < p.k) {
-                        chosen_logit = Widen<float, T>(LoadNc(row + chosen));
-                    }
-                }
+            // All pairs within the choice are clear or ties; from its last one on, a clear pair comes before an open one.
+            const unsigned opens = __ballot_sync(kFull, open), clears = __ballot_sync(kFull, clear);
+            const unsigned behind = ~0u << (p.k - 1);
+            const unsigned first = (opens | clears) & behind;
+            sure = sure && (opens & ~behind) == 0 && (first & (0u - first) & clears) != 0;
+            if (!sure) {
+                ChooseFine<T, BIASED>(p, row, bias, bad ? NAN : top, reinterpret_cast<uint64_t*>(row_keys), chosen);
+                chosen_logit = lane < p.k ? Widen<float, T>(LoadNc(row + chosen)) : 0.0f;
             }
         }
 
@@ -534,8 +534,6 @@ __global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T
             s = taken && chosen_logit != -INFINITY ? expf(chosen_logit - base) : 0.0f;
             if (p.renormalize) {
                 total = WarpSum(s);
-            } else if (BIASED) {
-                total = whole_sum;
             } else {
                 float part = 0.0f;
 #pragma unroll
@@ -1060,7 +1058,8 @@ int RunTopk(const OpsgnnRouteDesc& d, const void* logits, const float* bias, voi
         }
     }
     const bool wide = Wide<T, VPL>(d.experts, logits, logits);
-    const size_t shared = biased || d.groups > 1 ? static_cast<size_t>(kWarps) * d.experts * (biased ? 8 : 4) : 0;
+    const bool packed = sizeof(T) == 2 && !biased;
+    const size_t shared = !packed || d.groups > 1 ? static_cast<size_t>(kWarps) * d.experts * (packed ? 4 : 8) : 0;
     if (biased) {
         TopkKernel<T, VPL, true><<<Grid(d.rows, 1), kWarps * 32, shared, stream>>>(p, in, bias, out, index, wide);
     } else {

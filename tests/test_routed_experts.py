@@ -1125,3 +1125,36 @@ def test_segment_matmul_few_rows_and_long_sums(cuda_device, dtype, lengths, k, n
         _within(grad_src, _plain_matmul(grad, ptr, back), _plain_matmul(grad.abs(), ptr, back.abs()), n + 2, "grad_src")
         _within(grad_weight.transpose(1, 2) if turned else grad_weight, _plain_weight_grad(src, ptr, grad),
                 _plain_weight_grad(src.abs(), ptr, grad.abs()), sum(lengths) + 2, "grad_weight")
+
+
+@requires_gpu
+@pytest.mark.parametrize("experts", [5, 40, 300])
+def test_topk_route_looks_beyond_ties(cuda_device, experts):
+    """The last choice ties with its neighbours by their inputs, and a better expert hides behind them within fp32 rounding."""
+    from ops_gnn import topk_route
+
+    logits = torch.full((2, experts), -20.0)
+    logits[1, experts - 1] = -19.999  # 2e-12 better beside a bias of 1
+    bias = torch.ones(experts, device=cuda_device)
+    for k in (1, 2, 3):
+        index = topk_route(logits.to(cuda_device), k, score="sigmoid", bias=bias)[1]
+        assert index.tolist() == [list(range(k)), [experts - 1] + list(range(k - 1))]
+
+
+@requires_gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("scale", [1e-30, 1e-3, 1e4, 1e38])
+def test_topk_route_fp32_logits_of_any_size(cuda_device, score, scale):
+    """The order of fp32 logits is theirs, however close or far apart; one row holds the lowest number as its mask."""
+    from ops_gnn import topk_route
+
+    x = torch.randn(50, 200, generator=_gen(111)) * scale
+    x[7, ::2] = torch.finfo(torch.float32).min
+    x[8] = torch.nextafter(x[8, :1].expand(200), torch.full((200,), math.inf))
+    x[8, 150] = x[9, 0]
+    x[9, 1:] = x[9, 0] + x[9, 1:] * 1e-7
+    _, index = topk_route(x.to(cuda_device), 9, score=score)
+    want = torch.sort(x.double(), dim=1, descending=True, stable=True).indices[:, :9]
+    if score == "softmax":  # 3.5 sigma times 1e38 is +inf, which makes a softmax NaN: all rank alike, lower numbers first
+        want[(x == math.inf).any(1)] = torch.arange(9)
+    assert torch.equal(index.cpu(), want)
