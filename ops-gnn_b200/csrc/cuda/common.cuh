@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <limits>
 #include <type_traits>
 
@@ -57,6 +58,19 @@ inline int SmCount()
         cached[device] = count;
     }
     return cached[device];
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory, once per device (`done`: one bit each, a static of the call site).
+template <class Kernel> inline int AllowShared(Kernel kernel, int bytes, std::atomic<uint64_t>& done)
+{
+    int device = 0;
+    OPSGNN_CUDA_TRY(cudaGetDevice(&device));
+    const uint64_t bit = device >= 0 && device < 64 ? uint64_t{1} << device : 0;
+    if ((done.load(std::memory_order_acquire) & bit) == 0) {
+        OPSGNN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        done.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    return OPSGNN_OK;
 }
 
 inline int64_t CeilDiv(int64_t a, int64_t b) { return (a + b - 1) / b; }

@@ -643,7 +643,8 @@ int Launch(const CUtensorMap& a, const CUtensorMap& tail, const CUtensorMap& b, 
         return OPSGNN_ERR_UNSUPPORTED;
     }
     constexpr int kShared = SharedBytes<BN>();
-    OPSGNN_CUDA_TRY(cudaFuncSetAttribute(PromotedKernel<F8, O, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
+    static std::atomic<uint64_t> allowed{0};
+    OPSGNN_CUDA_TRY(static_cast<cudaError_t>(AllowShared(PromotedKernel<F8, O, BN, FORM>, kShared, allowed)));
     const int grid = static_cast<int>(std::min<int64_t>(std::max<int64_t>(tiles, 1), SmCount()));
     PromotedKernel<F8, O, BN, FORM><<<grid, kThreads, kShared, stream>>>(a, tail, b, p);
     return LaunchStatus();

@@ -439,7 +439,8 @@ int Launch(const CUtensorMap& a, const CUtensorMap& tail, const CUtensorMap& b, 
         return OPSGNN_ERR_UNSUPPORTED;
     }
     constexpr int kShared = SharedBytes<BN>();
-    OPSGNN_CUDA_TRY(cudaFuncSetAttribute(TensorKernel<T, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
+    static std::atomic<uint64_t> allowed{0};
+    OPSGNN_CUDA_TRY(static_cast<cudaError_t>(AllowShared(TensorKernel<T, BN, FORM>, kShared, allowed)));
     const int grid = static_cast<int>(std::min<int64_t>(std::max<int64_t>(tiles, 1), SmCount()));
     TensorKernel<T, BN, FORM><<<grid, kThreads, kShared, stream>>>(a, tail, b, p);
     return LaunchStatus();
@@ -545,11 +546,15 @@ int RunRowsTensor(const RowsProblem& p, void* workspace, cudaStream_t stream)
     const uint64_t strides[2] = {static_cast<uint64_t>(stride) * 2, static_cast<uint64_t>(p.b_segment) * 2};
     const uint32_t box[3] = {64, static_cast<uint32_t>(columns), 1};
     const CUtensorMapDataType type = TypeOf(p.in_type);
-    if (!Map2(&a, p.in_type, p.a, p.k, p.ptr.rows, p.lda, kDepth, kRows) ||
+    // (with fewer rows than a full tile's last box reaches, every tile is short and the first map is never used)
+    if ((p.ptr.rows > kRows - kBoxRows && !Map2(&a, p.in_type, p.a, p.k, p.ptr.rows, p.lda, kDepth, kRows)) ||
         !Map2(&tail, p.in_type, p.a, p.k, p.ptr.rows, p.lda, kDepth, kBoxRows) ||
         !(turned ? tc::EncodeMap(&b, type, 3, p.b, sizes, strides, box)
                  : tc::EncodeSlabs(&b, type, p.b, p.n, p.k, p.ptr.segments, stride * 2, p.b_segment * 2, columns / 64))) {
         return OPSGNN_ERR_UNSUPPORTED;
+    }
+    if (p.ptr.rows <= kRows - kBoxRows) {
+        a = tail;
     }
     auto run = [&](auto tag, auto width) {
         using T = decltype(tag);
