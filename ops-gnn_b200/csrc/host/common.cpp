@@ -289,7 +289,7 @@ void RaiseIfDeviceStalled(const at::Tensor& on_device, const char* api)
     const int device = on_device.device().index();
     TORCH_CHECK(DeviceStallCount(device, false) == 0, api,
                 ": device wait timed out in an earlier launch on cuda:", device,
-                " (a bulk-copy wait of the reduce kernel ran out of polls; that launch's output is incomplete)");
+                " (a bounded wait of a kernel ran out of polls; that launch's output is incomplete)");
 }
 
 void RunCsrReduce(CsrReduceCall& call, const char* api)

@@ -71,7 +71,7 @@ def check_device_status(device=None) -> None:
     index = torch.cuda.current_device() if device is None else torch.device(device).index
     count = _pybind.device_stall_count(int(index or 0), True)
     if count:
-        raise RuntimeError(f"ops_gnn: device wait timed out on cuda:{index} (a bulk-copy wait of the reduce kernel ran "
+        raise RuntimeError(f"ops_gnn: device wait timed out on cuda:{index} (a bounded wait of a kernel ran "
                            "out of polls; the output of that launch is incomplete)")
 
 
