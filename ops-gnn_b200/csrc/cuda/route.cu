@@ -798,13 +798,14 @@ __global__ void __launch_bounds__(kWarps * 32) TopkBackwardKernel(RouteParams p,
 // One tile needs the last kernel only.  No atomics on global memory; shared counters are per warp and commute.
 // Bound by latency: three launches, and in the last a chain of counts, prefix and ranks.  1048576 pairs, 256 experts: 512 tiles
 // of eight warps 21.9 us, one tile per SM of 32 warps 17.9 us (24.5 with the scan inside the last kernel, where every block reads
-// all counts); 512 pairs, 128 experts in one tile: 3.0 us with 16 warps, 3.7 with
-// 32.
+// all counts; 19.6 with perm sorted in shared memory before it is written); 512 pairs, 128 experts in one tile: 3.0 us with 16
+// warps, 3.7 with 32.
 constexpr int kMaxBins = 4096;
 constexpr int kSortWarps = 32;
 
-// Warps of a block: as many tables of bins as shared memory holds; a block on its own is done sooner with half as many.
-inline int SortWarps(int bins, int64_t tiles) { return bins > 1500 ? 8 : (tiles == 1 ? kSortWarps / 2 : kSortWarps); }
+// Warps of a block: a table of bins each, which takes its time to clear and add up; a block on its own is done sooner with half
+// as many.  1048576 pairs, 1500 experts: 35 us with 32 warps, 26 us with 16; 4000 experts: 48 us with eight.
+inline int SortWarps(int bins, int64_t tiles) { return bins > 2000 ? 8 : (bins > 1000 || tiles == 1 ? kSortWarps / 2 : kSortWarps); }
 
 template <class I> __device__ __forceinline__ int BinOf(const I* index, int64_t at, int64_t end, int experts)
 {
@@ -989,8 +990,17 @@ __global__ void __launch_bounds__(1024)
     }
 }
 
-// Tiles: at most one per SM, of 1024 pairs or more.
-inline int64_t SortTiles(int64_t count) { return count <= 4096 ? 1 : std::min<int64_t>(SmCount(), CeilDiv(count, 1024)); }
+// Tiles: at most one per SM, of 1024 to 32768 pairs; of more pairs, 8192 each.  Long tiles write perm in so many far streams
+// that sectors leave the cache half written: 8388608 pairs, 256 experts: 171 us with one tile per SM, 124 us with 1024 tiles
+// (33554432: 1091 and 460), but 4194304 pairs 45 us with one tile per SM, 53 us with 512.
+inline int64_t SortTiles(int64_t count)
+{
+    if (count <= 4096) {
+        return 1;
+    }
+    const int64_t sms = SmCount();
+    return count > sms * 32768 ? CeilDiv(count, 8192) : std::min<int64_t>(sms, CeilDiv(count, 1024));
+}
 
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxChosen = 32;
@@ -1192,9 +1202,8 @@ extern "C" int opsgnn_route_csr(const void* index, int index_type, int64_t count
     auto run = [&](auto tag) {
         using I = decltype(tag);
         const I* in = static_cast<const I*>(index);
-        if (shared > 48 * 1024) {
-            OPSGNN_CUDA_TRY(cudaFuncSetAttribute(route::PlaceKernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
-        }
+        static std::atomic<uint64_t> allowed{0};
+        OPSGNN_CUDA_TRY(static_cast<cudaError_t>(AllowShared(route::PlaceKernel<I>, 8 * (route::kMaxBins + 1) * 4, allowed)));
         if (tiles > 1) {
             route::CountKernel<I><<<static_cast<unsigned>(tiles), 1024, bins * 4, AsStream(stream)>>>(in, count, static_cast<int>(experts),
                                                                                                     tile, counts);

@@ -19,8 +19,8 @@
 //
 // What bounds the 8-bit product: reading every block's sums out of TMEM.  128 x 256 sums are 128 KB at 128 bytes per cycle and
 // SM, twice the 512 cycles of the block's multiplication.  Measured, 18944 x 4096 -> 2048: 171 us (1.86 PFLOP/s); with the
-// sums left unread 130 us, with one sum over all of K 117 us, Sixteen
-// summing warps in place of eight (187 us) and pairs of blocks that halve the operand traffic (170 us) change nothing.
+// sums left unread 130 us, with one sum over all of K 117 us.  Sixteen summing warps in place of eight (187 us) and pairs of
+// blocks that halve the operand traffic (170 us) gain nothing.
 #include <algorithm>
 
 #include "segment_matmul.cuh"

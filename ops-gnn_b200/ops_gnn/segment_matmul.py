@@ -31,10 +31,13 @@ def segment_matmul(src: torch.Tensor, indptr: torch.Tensor, weight: torch.Tensor
     rows of ``src`` and either layout of ``weight`` (``weight.transpose(1, 2)`` of ``[E, N, K]``) are read in place, other
     layouts are copied first.  Differentiable in ``src`` and ``weight`` (second derivatives are not built).
 
+    Larger float32 products take scratch memory of about 1.5 times their operands while they run; their values below 2^-110
+    lose low bits.  Every sum is taken in a fixed order: the same call gives the same bits.
+
     The pointers stay on the device: nothing is read back, so the call can be captured into a graph and replayed with other
-    pointers.  Their order is not checked; a pointer outside ``[0, M]`` counts as the nearer end and a segment that would
-    end before it starts is empty.  Raises ``TypeError`` / ``ValueError`` for bad arguments and ``RuntimeError`` for tensors
-    that are not on a CUDA device.
+    pointers.  A pointer outside ``[0, M]`` counts as the nearer end.  Their order is not checked: where they descend, rows
+    and gradients of the segments concerned are unspecified, but nothing outside the tensors is read or written.  Raises
+    ``TypeError`` / ``ValueError`` for bad arguments and ``RuntimeError`` for tensors that are not on a CUDA device.
     """
     if not isinstance(src, torch.Tensor):
         raise TypeError(f"src must be a torch.Tensor, got {type(src).__name__}")

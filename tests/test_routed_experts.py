@@ -1158,3 +1158,20 @@ def test_topk_route_fp32_logits_of_any_size(cuda_device, score, scale):
     if score == "softmax":  # 3.5 sigma times 1e38 is +inf, which makes a softmax NaN: all rank alike, lower numbers first
         want[(x == math.inf).any(1)] = torch.arange(9)
     assert torch.equal(index.cpu(), want)
+
+
+@requires_gpu
+@pytest.mark.parametrize("count,experts", [(70001, 1500), (30000, 2500), (5000003, 40), (9000001, 1200)])
+def test_route_csr_many_tiles_and_experts(cuda_device, count, experts):
+    from ops_gnn import route_csr
+
+    index = torch.randint(-1, experts, (count,), generator=_gen(count))
+    indptr, perm, position = route_csr(index.to(cuda_device), experts)
+    label = torch.where(index >= 0, index, experts)
+    want = torch.sort(label, stable=True).indices
+    assert torch.equal(perm.cpu(), want)
+    counts = torch.bincount(label, minlength=experts + 1)[:experts]
+    assert torch.equal(indptr.cpu(), torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)]))
+    back = torch.empty_like(want)
+    back[want] = torch.arange(count)
+    assert torch.equal(position.cpu(), back)
