@@ -383,8 +383,8 @@ __global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T
                 if (bias != nullptr && at < p.experts) {
                     c[j] += __ldg(bias + at);
                 }
-                largest = fmaxf(largest, fabsf(c[j]));
                 c[j] = l[j] == -INFINITY ? -INFINITY : (bad ? NAN : c[j]);
+                largest = fmaxf(largest, c[j] == -INFINITY ? 0.0f : fabsf(c[j]));  // what is masked is not compared
                 key[j] = at < p.experts ? KeyOf(c[j]) : 0u;
             }
             margin += __uint_as_float(__reduce_max_sync(kFull, __float_as_uint(largest))) * 0x1p-22f;

@@ -16,7 +16,8 @@ def segment_matmul_fp8(src: torch.Tensor, src_scale: torch.Tensor, weight: torch
     rows ``indptr[e] <= r < indptr[e + 1]`` of each segment ``e``.
 
     ``src`` is ``[M, K]`` and ``weight`` ``[E, N, K]``, both float8_e4m3fn; the scales are float32, ``[M, ceil(K / 128)]`` and
-    ``[E, ceil(N / 128), ceil(K / 128)]``, any positive values (``quantize_fp8`` makes powers of two).  Without ``indptr``
+    ``[E, ceil(N / 128), ceil(K / 128)]``, any positive values (``quantize_fp8`` makes powers of two) whose products
+    are within float32's range (the two scales of a block are multiplied first).  Without ``indptr``
     it is one dense product with ``weight`` ``[N, K]`` and ``weight_scale`` ``[ceil(N / 128), ceil(K / 128)]``.  The result
     ``[M, N]`` is ``out_dtype`` (bfloat16, float16 or float32).  Products of a block of 128 are added up on the tensor cores,
     blocks in fp32 registers, so no sum is held in fewer than 32 bits.

@@ -1175,3 +1175,19 @@ def test_route_csr_many_tiles_and_experts(cuda_device, count, experts):
     back = torch.empty_like(want)
     back[want] = torch.arange(count)
     assert torch.equal(position.cpu(), back)
+
+
+@requires_gpu
+@pytest.mark.parametrize("case", [c for c in ROUTES if c[4]], ids=str)
+def test_topk_route_bias_closes_experts(cuda_device, case):
+    """A bias of -inf or of the lowest number puts experts behind all others; +inf puts one before them."""
+    from ops_gnn import topk_route
+
+    rows, experts, k, score, _, groups, kept, top, renormalize, dtype = case
+    logits, bias = _route_inputs(case, 9)
+    bias[1::3] = -math.inf
+    for special in (None, (4, torch.finfo(torch.float32).min), (experts - 1, math.inf)):
+        if special is not None:
+            bias[special[0]] = special[1]
+        weight, index = topk_route(logits.to(cuda_device), k, score, bias.to(cuda_device), groups, kept, top, renormalize)
+        _check_route(logits, bias, case, weight, index, f"{case} {special}")
