@@ -58,7 +58,7 @@ struct Params {
     bool whole_a, whole_b;  // MN-major operands: all slabs in one load
     bool vec;               // rows of out start on 16-byte boundaries
     int64_t chunk;     // outer form: rows per partial result; 0: a segment's rows in one piece
-    float* partial;    // [pieces][m][n]
+    float* partial;    // [slots][m][n]
     WaitSettings wait;
 };
 
@@ -155,11 +155,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (FORM == kOuter) {
             row = t % down * kRows;
             row_end = m;
-            segment = t / down;  // of the result to write: a segment or a piece
+            segment = t / down;  // in pieces: the piece, then its target
             if (chunk > 0) {
                 if (!walk.Seek(p.ptr, segment)) {
                     return false;
                 }
+                segment = PieceTarget(walk, chunk);
                 from = walk.row;
                 depth = min(walk.row_end - from, chunk);
                 return true;
@@ -380,8 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr int kMine = BN / 2;  // columns of this warp
         const int quarter = warp & 3, side = (warp - 4) >> 2;
         unsigned char* mine = staging + (warp - 4) * (32 * 128);
-        // a piece of a segment's sum (outer form in pieces; fp32 then) goes to `partial`
-        O* out = FORM == kOuter && p.chunk > 0 ? reinterpret_cast<O*>(p.partial) : static_cast<O*>(p.out);
+        O* out = static_cast<O*>(p.out);
         const int scale_blocks = F8 ? (width + 127) / 128 : 0, scale_bands = F8 ? (n + 127) / 128 : 0;
         uint32_t blocks = 0, turn = 0;
         bool going = true;
@@ -461,7 +461,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!going) {
                 break;
             }
-            O* to = out + (FORM == kOuter ? segment * p.m * p.n : 0);
+            O* to = out;
+            if constexpr (FORM == kOuter) {
+                // a piece of a longer sum (fp32 as the result) goes to `partial`
+                const bool in_piece = p.chunk > 0 && (segment & 1) == 0;
+                to = (in_piece ? reinterpret_cast<O*>(p.partial) : out) + (p.chunk > 0 ? segment >> 1 : segment) * p.m * p.n;
+            }
             constexpr int kLine = 128 / sizeof(O);       // columns in 128 bytes
             constexpr int kPerWord = 4 / sizeof(O);
             bool odd = false;

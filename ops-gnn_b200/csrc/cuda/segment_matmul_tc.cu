@@ -80,7 +80,7 @@ struct Params {
     bool vec;               // rows of out start on 16-byte boundaries
     int64_t chunk;     // of the reduced index per partial result; 0: all of it in one piece
     int64_t pieces;    // rows form: pieces of the reduced index
-    float* partial;    // outer form [pieces][m][n], rows form [pieces][rows][n]
+    float* partial;    // outer form [slots][m][n], rows form [pieces][rows][n]
     WaitSettings wait;
 };
 
@@ -160,11 +160,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (FORM == kOuter) {
             row = t % down * kRows;
             row_end = m;
-            segment = t / down;  // of the result to write: a segment or a piece
+            segment = t / down;  // in pieces: the piece, then its target
             if (chunk > 0) {
                 if (!walk.Seek(p.ptr, segment)) {
                     return false;
                 }
+                segment = PieceTarget(walk, chunk);
                 from = walk.row;
                 depth = min(walk.row_end - from, chunk);
                 return true;
@@ -326,8 +327,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 tc::FenceAfter();
             }
-            T* to = out + (FORM == kOuter ? segment * p.m * p.n : 0);
-            float* sums = p.partial + (FORM == kOuter ? segment * p.m * p.n : piece * p.ptr.rows * p.n);
+            const bool in_piece = chunk > 0 && (FORM != kOuter || (segment & 1) == 0);  // else a whole sum
+            const int64_t result = FORM == kOuter && chunk > 0 ? segment >> 1 : segment;
+            T* to = out + (FORM == kOuter ? result * p.m * p.n : 0);
+            float* sums = p.partial + (FORM == kOuter ? result * p.m * p.n : piece * p.ptr.rows * p.n);
             const int first = row + quarter * 32;
 #pragma unroll 1
             for (int c = 0; c < BN; c += 64) {
@@ -341,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc::TmemLoad32(at, low);
                     tc::TmemLoad32(at + 32, high);
                     tc::TmemWait();
-                    if (chunk > 0) {
+                    if (in_piece) {
                         // A piece of the sum, kept in fp32: 32 columns are 128 bytes.
 #pragma unroll
                         for (int side = 0; side < 2; ++side) {
@@ -577,30 +580,44 @@ int RunRowsTensor(const RowsProblem& p, void* workspace, cudaStream_t stream)
 
 namespace {
 
-// out[e][i] <- the sum of the pieces of segment e, in their order.  blockIdx.y: segment.
+// out[e][i] <- the sum of the pieces of segment e, in their order; 0 for an empty one.
 template <class T, int VEC>
-__global__ void __launch_bounds__(256) JoinKernel(SegmentPointers ptr, int64_t chunk, int64_t size, const float* __restrict__ partial,
+__global__ void __launch_bounds__(256) JoinKernel(SegmentPointers ptr, int chunk, int per, int64_t size, const float* __restrict__ partial,
                                                   T* __restrict__ out)
 {
-    const int64_t e = blockIdx.y;
-    SegmentWalk<0, int> walk;  // numbers the pieces as the kernel that made them did
-    walk.Start(ptr, static_cast<int>(chunk));
-    int before, pieces;
-    walk.Count(ptr, static_cast<int>(e), before, pieces);
+    // `per` segments at a time, a lane of every warp looks at one; those of one piece are done already.
+    const int lane = threadIdx.x & 31;
     const int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * VEC;
-    if (i >= size) {
-        return;
-    }
-    float sum[VEC] = {};
+    for (int64_t e0 = static_cast<int64_t>(blockIdx.y) * per; e0 < ptr.segments; e0 += static_cast<int64_t>(gridDim.y) * per) {
+        int begin = 0, pieces = 1;
+        if (lane < per && e0 + lane < ptr.segments) {
+            int64_t first, end;
+            ptr.Range<int64_t>(e0 + lane, first, end);
+            begin = static_cast<int>(first);
+            pieces = static_cast<int>((end - first + chunk - 1) / chunk);
+        }
+        unsigned left = __ballot_sync(0xffffffffu, pieces != 1);
+        while (left != 0) {
+            const int owner = __ffs(left) - 1;
+            left &= left - 1;
+            const int slot = PieceSlot(__shfl_sync(0xffffffffu, begin, owner), false, chunk);
+            const int count = __shfl_sync(0xffffffffu, pieces, owner);
+            if (i >= size) {
+                continue;
+            }
+            float sum[VEC] = {};
 #pragma unroll 8
-    for (int c = 0; c < pieces; ++c) {
-        const Pack<float, VEC> v = LoadPlain<float, VEC>(partial + static_cast<int64_t>(before + c) * size + i);
+            for (int c = 0; c < count; ++c) {
+                const int64_t at = slot + 2 * c + (c == count - 1 ? 1 : 0);
+                const Pack<float, VEC> v = LoadPlain<float, VEC>(partial + at * size + i);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            sum[j] += v.v[j];
+                for (int j = 0; j < VEC; ++j) {
+                    sum[j] += v.v[j];
+                }
+            }
+            StorePlain<T, VEC>(out + (e0 + owner) * size + i, Repack<T, float, VEC>(sum));
         }
     }
-    StorePlain<T, VEC>(out + e * size + i, Repack<T, float, VEC>(sum));
 }
 
 }  // namespace
@@ -608,25 +625,35 @@ __global__ void __launch_bounds__(256) JoinKernel(SegmentPointers ptr, int64_t c
 int64_t OuterChunk(int64_t rows, int64_t segments, int64_t k, int64_t n)
 {
     // A result tile is one block's sequential sum over a segment's rows.  With fewer tiles than SMs the rows are cut into
-    // pieces (200003 x 256 -> 256 in 13 segments, fp32: one piece each 1271 us, in pieces 313 us); with more tiles, or few rows,
-    // partial results would cost more than they give (32 segments of 2048 x 1024: 8 MB a piece; 4096 x 256 -> 256 in 32 segments,
-    // bf16: 10.5 us in one piece each, 22.9 us in pieces).  Two rounds of tiles over the SMs where a piece is a few tiles (bf16,
-    // the first case: 55.7 us, four rounds 65.6 us), four where it is many and two would leave the second round half empty
-    // (two segments, 32768 x 2048 -> 1024: 131 us, two rounds 148 us).  A segment's last piece is half full on average.
+    // pieces (200003 x 256 -> 256 in 13 segments, fp32: one piece each 1271 us, in pieces 303 us); with few rows, partial results
+    // would cost more than they give (4096 x 256 -> 256 in 32 segments, bf16: 10.5 us in one piece each, 22.9 us in pieces).  Two
+    // rounds of tiles over the SMs where a result is a few tiles (bf16, the first case: 51 us, four rounds 65.6 us), four where it
+    // is many and two would leave the second round half empty (two segments, 32768 x 2048 -> 1024: 131 us, two rounds 148 us).  A
+    // segment's last piece is half full on average.
     const int64_t tiles = CeilDiv(k, kRows) * CeilDiv(n, n <= 128 ? 128 : 256);
-    if (tiles * segments >= SmCount() || rows < 8192) {
+    if (rows < 8192) {
         return 0;
     }
-    const int64_t rounds = tiles * 8 <= SmCount() ? 2 : 4;
-    const int64_t pieces = std::max<int64_t>(1, SmCount() * rounds / tiles - segments / 2);
-    const int64_t chunk = std::max<int64_t>(256, AlignUp(CeilDiv(rows, pieces), kDepth));
-    return chunk >= rows ? 0 : chunk;
+    int64_t length = 0;
+    if (tiles * segments < SmCount()) {
+        const int64_t rounds = tiles * 8 <= SmCount() ? 2 : 4;
+        length = CeilDiv(rows, std::max<int64_t>(1, SmCount() * rounds / tiles - segments / 2));
+    } else if (tiles * 4 <= SmCount()) {
+        // Enough tiles for all SMs when segments are alike: only those of twice the mean length and more are cut, as one long
+        // segment would keep its few SMs busy alone.  bf16, whole against cut: 200003 x 256 -> 256 in 100 segments, half of the
+        // rows in one 561 and 61 us, lengths like 1 / i 269 and 74 us, lengths alike 52 and 56 us (finding the pieces, and the
+        // join's launch); 65536 x 64 -> 64 in 500 segments 143 and 32 us, 59 and 30 us, 13 and 22 us.  A result of more tiles
+        // keeps a quarter of the SMs busy by itself and is not cut: its partial results are large.
+        length = std::max(CeilDiv(rows * tiles, 2 * SmCount()), CeilDiv(2 * rows, segments));
+    }
+    const int64_t chunk = std::max<int64_t>(256, AlignUp(length, kDepth));
+    return length == 0 || chunk >= rows ? 0 : chunk;
 }
 
 int64_t OuterPartialBytes(int64_t rows, int64_t segments, int64_t k, int64_t n)
 {
     const int64_t chunk = OuterChunk(rows, segments, k, n);
-    return chunk > 0 ? AlignUp((rows / chunk + segments) * k * n * 4, 256) : 0;
+    return chunk > 0 ? AlignUp(PieceSlots(rows, chunk) * k * n * 4, 256) : 0;
 }
 
 int JoinPieces(const OuterProblem& p, int64_t chunk, const float* partial, cudaStream_t stream)
@@ -635,11 +662,14 @@ int JoinPieces(const OuterProblem& p, int64_t chunk, const float* partial, cudaS
     auto run = [&](auto tag) {
         using T = decltype(tag);
         const bool vec = size % 4 == 0 && Aligned(p.out, 16);
-        const dim3 grid(static_cast<unsigned>(CeilDiv(size, vec ? 1024 : 256)), static_cast<unsigned>(p.ptr.segments));
+        // Enough blocks for the machine; with many segments a block looks at up to 32 of them at once.
+        const int64_t across = CeilDiv(size, vec ? 1024 : 256), most = CeilDiv(static_cast<int64_t>(SmCount()) * 32, across);
+        const int per = static_cast<int>(std::min<int64_t>(32, CeilDiv(p.ptr.segments, most)));
+        const dim3 grid(static_cast<unsigned>(across), static_cast<unsigned>(std::min(CeilDiv(p.ptr.segments, per), 4 * most)));
         if (vec) {
-            JoinKernel<T, 4><<<grid, 256, 0, stream>>>(p.ptr, chunk, size, partial, static_cast<T*>(p.out));
+            JoinKernel<T, 4><<<grid, 256, 0, stream>>>(p.ptr, static_cast<int>(chunk), per, size, partial, static_cast<T*>(p.out));
         } else {
-            JoinKernel<T, 1><<<grid, 256, 0, stream>>>(p.ptr, chunk, size, partial, static_cast<T*>(p.out));
+            JoinKernel<T, 1><<<grid, 256, 0, stream>>>(p.ptr, static_cast<int>(chunk), per, size, partial, static_cast<T*>(p.out));
         }
         return LaunchStatus();
     };

@@ -1191,3 +1191,32 @@ def test_topk_route_bias_closes_experts(cuda_device, case):
             bias[special[0]] = special[1]
         weight, index = topk_route(logits.to(cuda_device), k, score, bias.to(cuda_device), groups, kept, top, renormalize)
         _check_route(logits, bias, case, weight, index, f"{case} {special}")
+
+
+def _uneven(segments, long, seed):
+    """Lengths of many short segments, some empty, with a few long ones between them."""
+    lengths = torch.randint(0, 60, (segments,), generator=_gen(seed))
+    lengths[torch.rand(segments, generator=_gen(seed + 1)) < 0.2] = 0
+    for place, length in long:
+        lengths[place] = length
+    return lengths.tolist()
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", KINDS, ids=str)
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("segments,long,k,n", [(150, [(0, 6000), (1, 700), (149, 2100)], 64, 40), (200, [(70, 9000), (71, 513), (72, 1200)], 17, 130),
+                                               (40, [(3, 8000), (9, 3000)], 264, 264), (2000, [(1000, 900), (1999, 4000)], 24, 16)])
+def test_segment_matmul_uneven_segments(cuda_device, dtype, turned, segments, long, k, n):
+    """Many segments: the weight gradients of the long ones are summed in pieces, those of the others are not."""
+    from ops_gnn import segment_matmul
+
+    lengths = _uneven(segments, long, segments)
+    src, ptr, weight, grad = _matmul_inputs((lengths, 5, 11, k, n), dtype, 71)
+    if turned:
+        weight = weight.transpose(1, 2).contiguous().transpose(1, 2)
+    x, w = src.to(cuda_device).requires_grad_(), weight.to(cuda_device).requires_grad_()
+    grads = torch.autograd.grad(segment_matmul(x, ptr.to(cuda_device), w), (x, w), grad.to(cuda_device))
+    back = weight.transpose(1, 2)
+    _within(grads[0], _plain_matmul(grad, ptr, back), _plain_matmul(grad.abs(), ptr, back.abs()), n + 2, "grad_src")
+    _within(grads[1], _plain_weight_grad(src, ptr, grad), _plain_weight_grad(src.abs(), ptr, grad.abs()), max(lengths) + 2, "grad_weight")
