@@ -50,64 +50,53 @@ template <int TILE, class I> struct SegmentWalk {
         base = 0;
         high = p.data != nullptr ? static_cast<I>(p.Raw(0)) : 0;
     }
-    // The pointer behind this lane's segment of the 32 from `first` on; 0 past the last.
-    __device__ __forceinline__ I Load(const SegmentPointers& p, I first) const
+    // This lane's segment of the 32 at hand, and the tiles of the 32 up to and with it.
+    __device__ __forceinline__ void Scan(const SegmentPointers& p, I& begin, I& end, I& inclusive) const
     {
-        const I at = first + (threadIdx.x & 31);
-        return at < static_cast<I>(p.segments) ? (p.data != nullptr ? static_cast<I>(p.Raw(static_cast<int64_t>(at) + 1)) : static_cast<I>(p.rows))
-                                               : 0;
+        const int lane = threadIdx.x & 31;
+        end = 0;
+        if (from + lane < static_cast<I>(p.segments)) {
+            end = p.data != nullptr ? static_cast<I>(p.Raw(static_cast<int64_t>(from) + lane + 1)) : static_cast<I>(p.rows);
+        }
+        // A pointer below an earlier one counts as that one: segments never overlap, and all tiles together are bounded.
+        end = end > high ? end : high;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const I up = __shfl_up_sync(0xffffffffu, end, d);
+            end = lane >= d && up > end ? up : end;
+        }
+        begin = __shfl_up_sync(0xffffffffu, end, 1);
+        begin = lane == 0 ? high : begin;
+        inclusive = (end - begin + Rows() - 1) / Rows();
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const I up = __shfl_up_sync(0xffffffffu, inclusive, d);
+            inclusive += lane >= d ? up : 0;
+        }
+    }
+    __device__ __forceinline__ void Next(I end, I inclusive)
+    {
+        base += __shfl_sync(0xffffffffu, inclusive, 31);
+        high = __shfl_sync(0xffffffffu, end, 31);
+        from += 32;
     }
     // False past the last tile.
     __device__ __forceinline__ bool Seek(const SegmentPointers& p, I t)
     {
-        const int lane = threadIdx.x & 31;
-        I next = Load(p, from);
         while (from < static_cast<I>(p.segments)) {
-            I end = next;
-            next = Load(p, from + 32);  // on its way while this one is looked at
-            // A pointer below an earlier one counts as that one: segments never overlap, and all tiles together are bounded.
-            end = end > high ? end : high;
-            I begin = __shfl_up_sync(0xffffffffu, end, 1);
-            begin = lane == 0 ? high : begin;
-            if (__any_sync(0xffffffffu, end < begin)) {
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const I up = __shfl_up_sync(0xffffffffu, end, d);
-                    end = lane >= d && up > end ? up : end;
-                }
-                begin = __shfl_up_sync(0xffffffffu, end, 1);
-                begin = lane == 0 ? high : begin;
-            }
-            // This lane's tiles, and those of the 32 up to and with it.
-            const I mine = (end - begin + Rows() - 1) / Rows();
-            if constexpr (sizeof(I) == 4) {  // past all of them at once
-                const I all = __reduce_add_sync(0xffffffffu, mine);
-                if (t >= base + all) {
-                    base += all;
-                    high = __shfl_sync(0xffffffffu, end, 31);
-                    from += 32;
-                    continue;
-                }
-            }
-            I inclusive = mine;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const I up = __shfl_up_sync(0xffffffffu, inclusive, d);
-                inclusive += lane >= d ? up : 0;
-            }
+            I begin, end, inclusive;
+            Scan(p, begin, end, inclusive);
             const unsigned there = __ballot_sync(0xffffffffu, t < base + inclusive);
             if (there != 0) {
                 const int owner = __ffs(there) - 1;
-                const I before = __shfl_sync(0xffffffffu, base + inclusive - mine, owner);
+                const I before = __shfl_sync(0xffffffffu, base + inclusive - (end - begin + Rows() - 1) / Rows(), owner);
                 row_end = __shfl_sync(0xffffffffu, end, owner);
                 begin_row = __shfl_sync(0xffffffffu, begin, owner);
                 row = begin_row + (t - before) * Rows();
                 segment = from + owner;
                 return true;
             }
-            base += __shfl_sync(0xffffffffu, inclusive, 31);
-            high = __shfl_sync(0xffffffffu, end, 31);
-            from += 32;
+            Next(end, inclusive);
         }
         return false;
     }
