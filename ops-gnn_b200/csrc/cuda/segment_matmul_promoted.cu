@@ -348,14 +348,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-            if (!going) {  // let what was issued end before TMEM is freed
-                if (lane == 0) {
-                    tc::Commit(&bar.drain);
-                    for (uint32_t i = 0; i < (1u << 15) && !tc::BarTry(&bar.drain, 0); ++i) {
-                    }
-                }
-                __syncwarp();
-            }
         } else if (warp == 3) {
             // The tiles, looked up for the summing warps, whose registers hold nothing but sums.
             uint32_t turn = 0;
@@ -529,16 +521,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     __syncwarp();
-    if (warp == 0 && lane == 0 && bar.stop != 0) {
-        // Copies in flight must land before the block's shared memory is given up.
-        for (int s = 0; s < kStages; ++s) {
-            for (uint32_t i = 0; bar.fills[s] > 0 && i < (1u << 15) && !tc::BarTry(&bar.full[s], (bar.fills[s] - 1) & 1); ++i) {
-            }
-        }
-    }
-    __syncwarp();
     tc::FenceBefore();
     __syncthreads();
+    // As in segment_matmul_tc.cu: `stop` is final here, and what is in flight ends before shared memory and TMEM are given up.
+    if (bar.stop != 0) {
+        if (warp == 0 && lane == 0) {
+            for (int s = 0; s < kStages; ++s) {
+                for (uint32_t i = 0; bar.fills[s] > 0 && i < (1u << 15) && !tc::BarTry(&bar.full[s], (bar.fills[s] - 1) & 1); ++i) {
+                }
+            }
+        } else if (warp == 1 && lane == 0) {
+            tc::Commit(&bar.drain);
+            for (uint32_t i = 0; i < (1u << 15) && !tc::BarTry(&bar.drain, 0); ++i) {
+            }
+        }
+        __syncwarp();
+        __syncthreads();
+    }
     if (warp == 2) {
         tc::FenceAfter();
         tc::TmemFree(tmem);

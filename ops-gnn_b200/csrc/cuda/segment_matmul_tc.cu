@@ -304,14 +304,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             ++tiles;
         }
-        if (!going) {  // let what was issued end before TMEM is freed
-            if (lane == 0) {
-                tc::Commit(&bar.drain);
-                for (uint32_t i = 0; i < (1u << 15) && !tc::BarTry(&bar.drain, 0); ++i) {
-                }
-            }
-            __syncwarp();
-        }
     } else if (warp >= 4) {
         const int quarter = warp - 4;
         unsigned char* mine = staging + quarter * (32 * 128);
@@ -403,16 +395,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     __syncwarp();
-    if (warp == 0 && lane == 0 && bar.stop != 0) {
-        // Copies in flight must land before the block's shared memory is given up.
-        for (uint32_t f = filled > kStages ? filled - kStages : 0; f < filled; ++f) {
-            for (uint32_t i = 0; i < (1u << 15) && !tc::BarTry(&bar.full[f % kStages], (f / kStages) & 1); ++i) {
-            }
-        }
-    }
-    __syncwarp();
     tc::FenceBefore();
     __syncthreads();
+    // Past this barrier no wait of the block is left, so `stop` is final: a wait that ran out after a warp had issued its last
+    // work is seen here, too.  What is in flight must end before the block's shared memory and TMEM are given up.
+    if (bar.stop != 0) {
+        if (warp == 0 && lane == 0) {
+            for (uint32_t f = filled > kStages ? filled - kStages : 0; f < filled; ++f) {
+                for (uint32_t i = 0; i < (1u << 15) && !tc::BarTry(&bar.full[f % kStages], (f / kStages) & 1); ++i) {
+                }
+            }
+        } else if (warp == 1 && lane == 0) {
+            tc::Commit(&bar.drain);
+            for (uint32_t i = 0; i < (1u << 15) && !tc::BarTry(&bar.drain, 0); ++i) {
+            }
+        }
+        __syncwarp();
+        __syncthreads();
+    }
     if (warp == 2) {
         tc::FenceAfter();
         tc::TmemFree(tmem);

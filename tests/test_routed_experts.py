@@ -1220,3 +1220,53 @@ def test_segment_matmul_uneven_segments(cuda_device, dtype, turned, segments, lo
     back = weight.transpose(1, 2)
     _within(grads[0], _plain_matmul(grad, ptr, back), _plain_matmul(grad.abs(), ptr, back.abs()), n + 2, "grad_src")
     _within(grads[1], _plain_weight_grad(src, ptr, grad), _plain_weight_grad(src.abs(), ptr, grad.abs()), max(lengths) + 2, "grad_weight")
+
+
+@pytest.mark.parametrize("source", ["segment_matmul_tc.cu", "segment_matmul_promoted.cu"])
+def test_kernels_that_give_up_drain_after_the_last_wait(source):
+    """A wait may run out in any warp, up to the last one of the block.  So the flag that says so is read behind a barrier that
+    follows every wait, and what is in flight (loads, matrix products) ends between it and the release of tensor memory.  When a
+    wait runs out in mid flight cannot be arranged from outside, so the order is read from the source."""
+    import pathlib
+
+    path = pathlib.Path(__file__).resolve().parent.parent / "ops-gnn_b200" / "csrc" / "cuda" / source
+    text = path.read_text()
+    last_wait = max(text.rfind("wait.Warp("), text.rfind("wait(&bar"))
+    final = text.index("bar.stop != 0")
+    release = text.index("TmemFree(", final)
+    assert last_wait < final and "__syncthreads();" in text[last_wait:final]
+    for drained in ("BarTry(&bar.full", "tc::Commit(&bar.drain)", "BarTry(&bar.drain"):
+        at = text.index(drained, final)
+        assert at < release and text.count(drained) == 1
+        assert "__syncthreads();" in text[at:release]
+
+
+@requires_gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+def test_waits_of_a_single_poll(cuda_device, kind):
+    """One poll for each wait: the launch ends, complete or given up anywhere within; either way the next one is right."""
+    import ops_gnn
+
+    gen = _gen(93)
+    dtype = torch.bfloat16 if kind == "bf16" else torch.float32
+    src = torch.randn(3000, 512, generator=gen).to(dtype).to(cuda_device).requires_grad_()
+    weight = torch.randn(3, 512, 512, generator=gen).to(dtype).to(cuda_device).requires_grad_()
+    grad = torch.randn(3000, 512, generator=gen).to(dtype).to(cuda_device)
+    ptr = torch.tensor([0, 700, 701, 3000], device=cuda_device)
+
+    def run():
+        out = ops_gnn.segment_matmul(src, ptr, weight)
+        return (out.detach(),) + torch.autograd.grad(out, (src, weight), grad)
+
+    want = run()
+    device = cuda_device.index or 0
+    try:
+        ops_gnn._pybind.set_wait_polls(1)
+        for _ in range(3):
+            ops_gnn._pybind.device_stall_count(device, True)
+            ops_gnn._pybind.segment_matmul_forward(src.detach(), ptr, weight.detach())
+            torch.cuda.synchronize()
+    finally:
+        ops_gnn._pybind.set_wait_polls(-1)
+        ops_gnn._pybind.device_stall_count(device, True)
+    assert all(torch.equal(a, b) for a, b in zip(run(), want))
