@@ -8,9 +8,11 @@
 //     a b = a1 b1 + (a1 b2 + a2 b1) + (a1 b3 + a2 b2 + a3 b1) + terms below 2^-24 of |a b|, which are left out.
 // The six products are exact; 64 values of the reduced index are summed in TMEM, a1 b1 last, so that only the last four
 // instructions add at full magnitude, then the sum moves to registers, which round to nearest.  Six bf16 products cost
-// 1/6 of the bf16 rate, four times what fp32 multiply-adds reach.  An infinity or NaN among the operands breaks the split
-// (inf - inf): a result that is not finite is computed again from the fp32 operands, one multiply-add at a time.  Values below
-// 2^-110 lose low bits, as their third term lies below the smallest bf16.
+// 1/6 of the bf16 rate, four times what fp32 multiply-adds reach.  Values below 2^-110 lose low bits, as their third term lies
+// below the smallest bf16.  An infinity, a number that rounds to one in bf16 or a sum that overflows breaks the split
+// (inf - inf, inf * 0): where the largest magnitudes of the operands, noted as the terms are made, leave one of these possible,
+// results that are not finite are computed again from the fp32 operands, after the block's last tile and with nobody waiting
+// (Repair).  Where they do not, such a result stems from a NaN and is right.
 //
 // Layout as in segment_matmul_tc.cu (one persistent block per SM: a loading warp, a multiplying warp), with eight summing
 // warps, each 32 rows x half the columns of a tile, whose sums need BN / 2 registers a thread.  The first four warps hand
@@ -24,6 +26,7 @@
 #include <algorithm>
 
 #include "segment_matmul.cuh"
+#include "segment_tile.cuh"
 #include "tensor_core.cuh"
 
 namespace opsgnn {
@@ -55,6 +58,9 @@ struct Params {
     const float* b;
     int64_t lda, ldb;                // outer form: ldb = row stride of b
     int64_t b_segment, b_k, b_n;
+    const float* a_tops;             // fp32: largest magnitudes of parts of the operands (NaN left out)
+    const float* b_tops;
+    int a_parts, b_parts;
     bool whole_a, whole_b;  // MN-major operands: all slabs in one load
     bool vec;               // rows of out start on 16-byte boundaries
     int64_t chunk;     // outer form: rows per partial result; 0: a segment's rows in one piece
@@ -65,9 +71,10 @@ struct Params {
 struct Barriers {
     uint64_t full[kStages], empty[kStages], done[2], free[2], drain;
     uint64_t told[2], taken[2];
-    int32_t tile[2][6];          // for the summing warps: segment, row, row_end, column, from, depth
+    int32_t tile[2][5];          // for the summing warps: segment, row, row_end, column, depth
     uint32_t fills[kStages];  // loads asked for, per stage (loading warp)
     uint32_t tmem, stop;
+    uint32_t odd;             // summing warps: 1 results that are not finite, 2 a wait that ran out
 };
 
 // Loads of kBoxRows rows that cover the first `rows` of a block's rows.
@@ -101,10 +108,170 @@ template <int N> __device__ __forceinline__ void Add(float (&sum)[N], int at, co
     }
 }
 
+// A tile: its segment, first result row and column, and the range of the reduced index.
+struct Tile {
+    int segment = 0, row = 0, row_end = 0, column = 0, from = 0, depth = 0;
+};
+template <int FORM> using Walk = SegmentWalk<FORM == kOuter ? 0 : kRows, int>;
+
+template <int FORM> __device__ __forceinline__ void StartWalk(const Params& p, Walk<FORM>& walk)
+{
+    if (FORM != kOuter || p.chunk > 0) {
+        walk.Start(p.ptr, FORM == kOuter ? static_cast<int>(p.chunk) : kRows);
+    }
+}
+
+// Tile t of `across` columns and `down` rows of tiles, by a whole warp, with ascending t; false past the last one.  Rows, widths and
+// tile numbers fit 32 bits (checked on the host); offsets in memory are formed in 64.
+template <int BN, int FORM>
+__device__ __forceinline__ bool FindTile(const Params& p, Walk<FORM>& walk, int t, int across, int down, int width, int m, int chunk, Tile& tile)
+{
+    tile.column = t % across * BN;
+    t /= across;
+    if constexpr (FORM == kOuter) {
+        tile.row = t % down * kRows;
+        tile.row_end = m;
+        tile.segment = t / down;  // in pieces: the piece, then its target
+        if (chunk > 0) {
+            if (!walk.Seek(p.ptr, tile.segment)) {
+                return false;
+            }
+            tile.segment = PieceTarget(walk, chunk);
+            tile.from = walk.row;
+            tile.depth = min(walk.row_end - tile.from, chunk);
+            return true;
+        }
+        if (tile.segment >= p.ptr.segments) {
+            return false;
+        }
+        int end;
+        p.ptr.Range<int>(tile.segment, tile.from, end);
+        tile.depth = end - tile.from;
+        return true;
+    } else {
+        if (!walk.Seek(p.ptr, t)) {
+            return false;
+        }
+        tile.segment = walk.segment;
+        tile.row = walk.row;
+        tile.row_end = walk.row_end;
+        tile.depth = width;
+        return true;
+    }
+}
+
+// Where the results of a tile go.  Outer form: a piece of a longer sum (fp32 as the result) goes to `partial`.
+template <class O, int FORM> __device__ __forceinline__ O* ResultsOf(const Params& p, int segment)
+{
+    O* to = static_cast<O*>(p.out);
+    if constexpr (FORM == kOuter) {
+        const bool in_piece = p.chunk > 0 && (segment & 1) == 0;
+        to = (in_piece ? reinterpret_cast<O*>(p.partial) : to) + (p.chunk > 0 ? segment >> 1 : segment) * p.m * p.n;
+    }
+    return to;
+}
+
+// Barriers of the summing warps alone.
+struct SumSync {
+    __device__ __forceinline__ void operator()() const { asm volatile("bar.sync 1, %0;" ::"n"(32 * kSumWarps) : "memory"); }
+};
+__device__ __forceinline__ bool AnySum(bool mine)
+{
+    uint32_t any;
+    asm volatile(
+        "{\n"
+        ".reg .pred p, q;\n"
+        "setp.ne.u32 p, %1, 0;\n"
+        "bar.red.or.pred q, 1, %2, p;\n"
+        "selp.u32 %0, 1, 0, q;\n"
+        "}\n"
+        : "=r"(any)
+        : "r"(static_cast<uint32_t>(mine)), "n"(32 * kSumWarps)
+        : "memory");
+    return any != 0;
+}
+
+// fp32, after a block's last tile: its results that are not finite, again from the operands as given, by the eight summing warps
+// (thread: of these).  A function of its own, so that nothing of it weighs on the registers of the summing loop.  No wait
+// depends on it, and it takes at most what the multiply-add kernel takes for the tiles concerned.  65536 x 512 -> 512 in four
+// segments, forward and both gradients: 653 us; with a row of NaN 651 us, with one infinity 2993 us.
+template <int BN, int FORM> __device__ __noinline__ void Repair(const Params& p, unsigned char* scratch, int thread)
+{
+    float a_top = 0.0f, b_top = 0.0f;
+    for (int i = thread; i < p.a_parts; i += 32 * kSumWarps) {
+        a_top = fmaxf(a_top, p.a_tops[i]);
+    }
+    for (int i = thread; i < p.b_parts; i += 32 * kSumWarps) {
+        b_top = fmaxf(b_top, p.b_tops[i]);
+    }
+    float* shared_tops = reinterpret_cast<float*>(scratch);
+    for (int d = 16; d > 0; d >>= 1) {
+        a_top = fmaxf(a_top, __shfl_xor_sync(0xffffffffu, a_top, d));
+        b_top = fmaxf(b_top, __shfl_xor_sync(0xffffffffu, b_top, d));
+    }
+    if ((thread & 31) == 0) {
+        shared_tops[thread >> 5] = a_top;
+        shared_tops[kSumWarps + (thread >> 5)] = b_top;
+    }
+    SumSync()();
+    for (int w = 0; w < kSumWarps; ++w) {
+        a_top = fmaxf(a_top, shared_tops[w]);
+        b_top = fmaxf(b_top, shared_tops[kSumWarps + w]);
+    }
+    SumSync()();
+    // The largest bf16 is 2^128 - 2^120.  The products of all terms add up to less than 2^127 where this bound is below 2^126.
+    const float largest = __uint_as_float(0x7f7f0000u);
+    const float terms = static_cast<float>(FORM == kOuter ? p.ptr.rows : p.k);
+    if (a_top <= largest && b_top <= largest && a_top * b_top * terms < 0x1p126f) {
+        return;
+    }
+    tile::Operands& shared = *reinterpret_cast<tile::Operands*>(scratch);
+    const int n = static_cast<int>(p.n), m = static_cast<int>(p.m), width = static_cast<int>(p.k), chunk = static_cast<int>(p.chunk);
+    const int across = (n + BN - 1) / BN, down = (m + kRows - 1) / kRows, below = thread / 16 * 4, right = thread % 16 * 4;
+    Walk<FORM> walk;
+    StartWalk<FORM>(p, walk);
+    Tile at;
+    for (int t = blockIdx.x; FindTile<BN, FORM>(p, walk, t, across, down, width, m, chunk, at); t += gridDim.x) {
+        float* to = ResultsOf<float, FORM>(p, at.segment);
+        for (int part = 0; part < kRows / tile::kSize * (BN / tile::kSize); ++part) {
+            const int64_t r0 = at.row + part / (BN / tile::kSize) * tile::kSize, c0 = at.column + part % (BN / tile::kSize) * tile::kSize;
+            uint32_t odd = 0;  // which of the thread's 4 x 4 results
+            for (int i = 0; i < 16; ++i) {
+                const int64_t r = r0 + below + i / 4, c = c0 + right + i % 4;
+                if (r < at.row_end && c < n && !(fabsf(to[r * n + c]) < INFINITY)) {
+                    odd |= 1u << i;
+                }
+            }
+            if (!AnySum(odd != 0)) {
+                continue;
+            }
+            float sum[4][4] = {};
+            if constexpr (FORM == kOuter) {
+                tile::Multiply(
+                    shared, thread, SumSync(), [&](int r, int64_t d) { return r0 + r < p.m ? p.a[(at.from + d) * p.lda + r0 + r] : 0.0f; },
+                    [&](int64_t d, int c) { return c0 + c < n ? p.b[(at.from + d) * p.ldb + c0 + c] : 0.0f; }, false, false, at.depth,
+                    sum);
+            } else {
+                const float* matrix = p.b + at.segment * p.b_segment;
+                tile::Multiply(
+                    shared, thread, SumSync(), [&](int r, int64_t d) { return r0 + r < at.row_end ? p.a[(r0 + r) * p.lda + d] : 0.0f; },
+                    [&](int64_t d, int c) { return c0 + c < n ? matrix[d * p.b_k + (c0 + c) * p.b_n] : 0.0f; }, true, p.b_k == 1,
+                    at.depth, sum);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if ((odd >> i) & 1u) {
+                    to[(r0 + below + i / 4) * n + c0 + right + i % 4] = sum[i / 4][i % 4];
+                }
+            }
+        }
+    }
+}
+
 template <bool F8, class O, int BN, int FORM>
 __global__ void __launch_bounds__(kThreads, 1)
     PromotedKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_tail,
-                   const __grid_constant__ CUtensorMap map_b, const Params p)
+                   const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Params p)
 {
     constexpr int kStage = StageBytes<BN>();
     constexpr int kDepth = F8 ? 128 : 64;  // values of the reduced index in one 128-byte row
@@ -128,6 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc::BarInit(&bar.drain, 1);
         bar.stop = 0;
+        bar.odd = 0;
         tc::BarInitFence();
     }
     if (warp == 2) {
@@ -139,50 +307,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = bar.tmem;
     const tc::Waiter wait{&bar.stop, p.wait};
 
-    // Rows, widths and tile numbers fit 32 bits (checked on the host); offsets in memory are formed in 64.
     const int n = static_cast<int>(p.n), m = static_cast<int>(p.m), width = static_cast<int>(p.k), chunk = static_cast<int>(p.chunk);
-    const int across = (n + BN - 1) / BN;
-    const int down = FORM == kOuter ? (m + kRows - 1) / kRows : 1;
-    SegmentWalk<FORM == kOuter ? 0 : kRows, int> walk;
-    if (warp != 2 && warp < 4 && (FORM != kOuter || chunk > 0)) {
-        walk.Start(p.ptr, FORM == kOuter ? chunk : kRows);
+    const int across = (n + BN - 1) / BN, down = (m + kRows - 1) / kRows;
+    Walk<FORM> walk;
+    if (warp != 2 && warp < 4) {
+        StartWalk<FORM>(p, walk);
     }
-    // Tile t: its segment, first result row and column, and the range of the reduced index.
-    int segment = 0, row = 0, row_end = 0, column = 0, from = 0, depth = 0;
-    auto find = [&](int t) {
-        column = t % across * BN;
-        t /= across;
-        if constexpr (FORM == kOuter) {
-            row = t % down * kRows;
-            row_end = m;
-            segment = t / down;  // in pieces: the piece, then its target
-            if (chunk > 0) {
-                if (!walk.Seek(p.ptr, segment)) {
-                    return false;
-                }
-                segment = PieceTarget(walk, chunk);
-                from = walk.row;
-                depth = min(walk.row_end - from, chunk);
-                return true;
-            }
-            if (segment >= p.ptr.segments) {
-                return false;
-            }
-            int end;
-            p.ptr.Range<int>(segment, from, end);
-            depth = end - from;
-            return true;
-        } else {
-            if (!walk.Seek(p.ptr, t)) {
-                return false;
-            }
-            segment = walk.segment;
-            row = walk.row;
-            row_end = walk.row_end;
-            depth = width;
-            return true;
-        }
-    };
+    Tile at;
+    const int &segment = at.segment, &row = at.row, &row_end = at.row_end, &column = at.column, &from = at.from, &depth = at.depth;
+    auto find = [&](int t) { return FindTile<BN, FORM>(p, walk, t, across, down, width, m, chunk, at); };
 
     // 8 bits: the stages are a ring.  fp32: stages 0 and 1 take turns with the first terms of both operands, stage 2 holds the
     // second, stage 3 the third; every term is loaded once per 64 values of the reduced index and used in up to three products
@@ -361,8 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tile[1] = row;
                     tile[2] = row_end;
                     tile[3] = column;
-                    tile[4] = from;
-                    tile[5] = depth;
+                    tile[4] = depth;
                     tc::BarArrive(&bar.told[turn & 1]);
                 }
                 __syncwarp();
@@ -373,7 +505,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr int kMine = BN / 2;  // columns of this warp
         const int quarter = warp & 3, side = (warp - 4) >> 2;
         unsigned char* mine = staging + (warp - 4) * (32 * 128);
-        O* out = static_cast<O*>(p.out);
         const int scale_blocks = F8 ? (width + 127) / 128 : 0, scale_bands = F8 ? (n + 127) / 128 : 0;
         uint32_t blocks = 0, turn = 0;
         bool going = true;
@@ -383,8 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 break;
             }
             const volatile int32_t* tile = bar.tile[turn & 1];
-            const int segment = tile[0], row = tile[1], row_end = tile[2], column = tile[3], depth = tile[5];
-            [[maybe_unused]] const int from = tile[4];
+            const int segment = tile[0], row = tile[1], row_end = tile[2], column = tile[3], depth = tile[4];
             __syncwarp();
             if (lane == 0) {
                 tc::BarArrive(&bar.taken[turn & 1]);
@@ -453,15 +583,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!going) {
                 break;
             }
-            O* to = out;
-            if constexpr (FORM == kOuter) {
-                // a piece of a longer sum (fp32 as the result) goes to `partial`
-                const bool in_piece = p.chunk > 0 && (segment & 1) == 0;
-                to = (in_piece ? reinterpret_cast<O*>(p.partial) : out) + (p.chunk > 0 ? segment >> 1 : segment) * p.m * p.n;
-            }
+            O* to = ResultsOf<O, FORM>(p, segment);
             constexpr int kLine = 128 / sizeof(O);       // columns in 128 bytes
             constexpr int kPerWord = 4 / sizeof(O);
-            bool odd = false;
 #pragma unroll
             for (int c = 0; c < kMine; c += kLine) {
                 if (col0 + c < n) {
@@ -480,36 +604,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             if constexpr (!F8) {
+                bool odd = false;
 #pragma unroll
                 for (int i = 0; i < kMine; ++i) {
                     odd |= !(fabsf(sum[i]) < INFINITY);
                 }
-                if (__any_sync(0xffffffffu, odd)) {
-                    // Results that are not finite, from the operands as given: the row of a lane, column by column.
-                    for (int i = lane; i < 32 * kMine; i += 32) {
-                        const int64_t r = r0 + i / kMine, c = col0 + i % kMine;
-                        if (r >= row_end || c >= p.n) {
-                            continue;
-                        }
-                        float* place = reinterpret_cast<float*>(to) + r * p.n + c;
-                        if (fabsf(*place) < INFINITY) {
-                            continue;
-                        }
-                        const float* x = FORM == kOuter ? p.a + static_cast<int64_t>(from) * p.lda + r : p.a + r * p.lda;
-                        const float* y = FORM == kOuter ? p.b + static_cast<int64_t>(from) * p.ldb + c : p.b + segment * p.b_segment + c * p.b_n;
-                        const int64_t dx = FORM == kOuter ? p.lda : 1, dy = FORM == kOuter ? p.ldb : p.b_k;
-                        float v = 0.0f;
-                        for (int64_t d = 0; d < depth && v == v; ++d) {  // NaN stays NaN
-                            v = fmaf(__ldg(x + d * dx), __ldg(y + d * dy), v);
-                        }
-                        *place = v;
-                    }
+                if (odd && r0 + lane < row_end) {  // what lies past the segment's rows is not a result
+                    atomicOr(&bar.odd, 1u);
                 }
-                __syncwarp();
+            }
+        }
+        if constexpr (!F8) {
+            if (!going) {
+                atomicOr(&bar.odd, 2u);
+            }
+            SumSync()();
+            if (bar.odd == 1) {
+                Repair<BN, FORM>(p, staging, threadIdx.x - 128);
             }
         }
         if constexpr (FORM != kOuter) {
             // Rows of no segment.
+            O* out = static_cast<O*>(p.out);
             const int64_t before = p.ptr.data != nullptr ? p.ptr.Raw(0) : 0;
             const int64_t behind = p.ptr.data != nullptr ? p.ptr.Raw(p.ptr.segments) : p.ptr.rows;
             for (int64_t r = blockIdx.x * kSumWarps + warp - 4; r < before + (p.ptr.rows - behind); r += gridDim.x * kSumWarps) {
@@ -567,11 +683,15 @@ __host__ __device__ inline int64_t PlaneWidth(int64_t width) { return (width + 7
 
 // planes[3][matrices * rows][PlaneWidth(width)] <- the three bf16 terms of src[matrices][rows][width], any strides and alignment
 // (`vec`: every row starts on a 16-byte boundary).  What lies past `width` in a plane is not read.  FLAT: src is one contiguous
-// run of vectors and width a multiple of 8.  Bound by memory: 200003 x 256 reads 205 MB and writes 307 MB.
+// run of vectors and width a multiple of 8.  tops[block] <- the largest magnitude that a block has seen, NaN left out.
+// Bound by memory: 200003 x 256 reads 205 MB and writes 307 MB.
 template <bool FLAT>
 __global__ void __launch_bounds__(256) SplitKernel(const float* __restrict__ src, int64_t matrices, int64_t rows, int64_t width,
-                                                   int64_t matrix_stride, int64_t row_stride, bool vec, __nv_bfloat16* __restrict__ planes)
+                                                   int64_t matrix_stride, int64_t row_stride, bool vec, __nv_bfloat16* __restrict__ planes,
+                float* __restrict__ tops)
 {
+    __shared__ uint32_t shared_top[256 / 32];
+    float top = 0.0f;
     const int64_t vectors = PlaneWidth(width) / 4, total = matrices * rows * vectors, plane = total * 4;
     const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += 2 * stride) {
@@ -603,6 +723,7 @@ __global__ void __launch_bounds__(256) SplitKernel(const float* __restrict__ src
             if (at < total) {
                 uint2 words[3];
                 SplitFour(v[u], words);
+                top = fmaxf(fmaxf(top, fmaxf(fabsf(v[u].x), fabsf(v[u].y))), fmaxf(fabsf(v[u].z), fabsf(v[u].w)));
 #pragma unroll
                 for (int j = 0; j < 3; ++j) {
                     *reinterpret_cast<uint2*>(planes + j * plane + at * 4) = words[j];
@@ -610,19 +731,44 @@ __global__ void __launch_bounds__(256) SplitKernel(const float* __restrict__ src
             }
         }
     }
+    const uint32_t warp_top = __reduce_max_sync(0xffffffffu, __float_as_uint(top));  // magnitudes order as their bits do
+    if ((threadIdx.x & 31) == 0) {
+        shared_top[threadIdx.x >> 5] = warp_top;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint32_t all = 0;
+        for (int w = 0; w < 256 / 32; ++w) {
+            all = max(all, shared_top[w]);
+        }
+        tops[blockIdx.x] = __uint_as_float(all);
+    }
+}
+
+// The planes of an operand, and behind them the largest magnitudes of its parts.
+int64_t PlanesOnly(int64_t lines, int64_t width) { return AlignUp(lines * PlaneWidth(width) * 3 * 2, 1024); }
+int64_t MostParts() { return static_cast<int64_t>(SmCount()) * 32; }
+int64_t PlaneBytes(int64_t lines, int64_t width) { return PlanesOnly(lines, width) + AlignUp(MostParts() * 4, 1024); }
+int Parts(int64_t lines, int64_t width)
+{
+    return static_cast<int>(std::min<int64_t>(CeilDiv(lines * (PlaneWidth(width) / 4), 512), MostParts()));
+}
+const float* TopsOf(const void* planes, int64_t lines, int64_t width)
+{
+    return reinterpret_cast<const float*>(static_cast<const char*>(planes) + PlanesOnly(lines, width));
 }
 
 int Split(const float* src, int64_t matrices, int64_t rows, int64_t width, int64_t matrix_stride, int64_t row_stride, void* planes,
           cudaStream_t stream)
 {
-    const int64_t total = matrices * rows * (PlaneWidth(width) / 4);
-    const int grid = static_cast<int>(std::min<int64_t>(CeilDiv(total, 512), static_cast<int64_t>(SmCount()) * 32));
+    const int grid = Parts(matrices * rows, width);
     __nv_bfloat16* to = static_cast<__nv_bfloat16*>(planes);
+    float* tops = const_cast<float*>(TopsOf(planes, matrices * rows, width));
     const bool vec = Aligned(src, 16) && row_stride % 4 == 0 && (matrices == 1 || matrix_stride % 4 == 0);
     if (vec && width % 8 == 0 && row_stride == width && (matrices == 1 || matrix_stride == rows * width)) {
-        SplitKernel<true><<<grid, 256, 0, stream>>>(src, matrices, rows, width, matrix_stride, row_stride, vec, to);
+        SplitKernel<true><<<grid, 256, 0, stream>>>(src, matrices, rows, width, matrix_stride, row_stride, vec, to, tops);
     } else {
-        SplitKernel<false><<<grid, 256, 0, stream>>>(src, matrices, rows, width, matrix_stride, row_stride, vec, to);
+        SplitKernel<false><<<grid, 256, 0, stream>>>(src, matrices, rows, width, matrix_stride, row_stride, vec, to, tops);
     }
     return LaunchStatus();
 }
@@ -653,9 +799,6 @@ int Launch(const CUtensorMap& a, const CUtensorMap& tail, const CUtensorMap& b, 
     PromotedKernel<F8, O, BN, FORM><<<grid, kThreads, kShared, stream>>>(a, tail, b, p);
     return LaunchStatus();
 }
-
-// Bytes of the planes of lines of `width` values.
-int64_t PlaneBytes(int64_t lines, int64_t width) { return AlignUp(lines * PlaneWidth(width) * 3 * 2, 1024); }
 
 // Tiles of 128 columns in place of 256: where the wide ones leave half the SMs without a tile.
 bool Narrow128(int64_t down, int64_t n) { return n <= 128 || down * CeilDiv(n, 256) * 2 <= SmCount(); }
@@ -706,6 +849,10 @@ int RowsFromPlanes(const RowsProblem& p, const void* planes_a, const void* plane
     q.b_segment = p.b_segment;
     q.b_k = p.b_k;
     q.b_n = p.b_n;
+    q.a_tops = TopsOf(planes_a, p.ptr.rows, p.k);
+    q.a_parts = Parts(p.ptr.rows, p.k);
+    q.b_tops = TopsOf(planes_b, p.ptr.segments * (turned ? p.n : p.k), turned ? p.k : p.n);
+    q.b_parts = Parts(p.ptr.segments * (turned ? p.n : p.k), turned ? p.k : p.n);
     OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
     const int64_t inner = turned ? p.k : p.n, other = turned ? p.n : p.k, e = p.ptr.segments;
     const int64_t down = p.ptr.rows / kRows + std::min(e, p.ptr.rows);
@@ -741,6 +888,10 @@ int OuterFromPlanes(const OuterProblem& p, const void* planes_a, const void* pla
     q.b = static_cast<const float*>(p.b);
     q.lda = p.lda;
     q.ldb = p.ldb;
+    q.a_tops = TopsOf(planes_a, p.ptr.rows, p.k);
+    q.a_parts = Parts(p.ptr.rows, p.k);
+    q.b_tops = TopsOf(planes_b, p.ptr.rows, p.n);
+    q.b_parts = Parts(p.ptr.rows, p.n);
     OPSGNN_CUDA_TRY(static_cast<cudaError_t>(CurrentWaitSettings(&q.wait)));
     q.whole_a = tc::WholeSlabs(p.k);
     q.whole_b = tc::WholeSlabs(p.n);

@@ -1,20 +1,17 @@
-// Segment products for every type, size, stride and alignment: tiles of 64 x 64 in shared memory, 4 x 4 results per thread,
-// fp32 multiply-adds.  Sums of more than kChunk terms are added up in chunks, which bounds the growth of the rounding error
-// with the length of the sum.
+// Segment products for every type, size, stride and alignment: tiles of 64 x 64 in shared memory (segment_tile.cuh).
 #include <cuda_fp8.h>
 
 #include <algorithm>
 
 #include "segment_matmul.cuh"
+#include "segment_tile.cuh"
 
 namespace opsgnn {
 namespace segmm {
 namespace {
 
-constexpr int kTile = 64;
-constexpr int kDepth = 16;
-constexpr int kChunk = 128;
-constexpr int kThreads = 256;
+constexpr int kTile = tile::kSize;
+constexpr int kThreads = tile::kThreads;
 
 template <class T> __device__ __forceinline__ float ValueOf(const T* p) { return Widen<float, T>(LoadNc(p)); }
 template <> __device__ __forceinline__ float ValueOf<__nv_fp8_e4m3>(const __nv_fp8_e4m3* p)
@@ -22,53 +19,13 @@ template <> __device__ __forceinline__ float ValueOf<__nv_fp8_e4m3>(const __nv_f
     return static_cast<float>(*p);
 }
 
-// One 64 x 64 tile: total[i][j] += sum over d < depth of a(row, d) * b(d, col).  fa(row, d) and fb(d, col) give values and 0
-// outside; a_fast / b_fast say which index runs along memory, so that neighbouring threads read neighbouring addresses.
-template <class FA, class FB>
-__device__ __forceinline__ void Multiply(FA&& fa, FB&& fb, bool a_depth_fast, bool b_depth_fast, int64_t depth, float (&total)[4][4])
-{
-    __shared__ float sa[kDepth][kTile + 4], sb[kDepth][kTile + 4];
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    float part[4][4] = {};
-    for (int64_t d0 = 0; d0 < depth; d0 += kDepth) {
-#pragma unroll
-        for (int i = 0; i < kTile * kDepth / kThreads; ++i) {
-            const int at = i * kThreads + threadIdx.x;
-            const int da = a_depth_fast ? at % kDepth : at / kTile, ra = a_depth_fast ? at / kDepth : at % kTile;
-            sa[da][ra] = d0 + da < depth ? fa(ra, d0 + da) : 0.0f;
-            const int db = b_depth_fast ? at % kDepth : at / kTile, cb = b_depth_fast ? at / kDepth : at % kTile;
-            sb[db][cb] = d0 + db < depth ? fb(d0 + db, cb) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int d = 0; d < kDepth; ++d) {
-            const float4 x = *reinterpret_cast<const float4*>(&sa[d][ty * 4]);
-            const float4 y = *reinterpret_cast<const float4*>(&sb[d][tx * 4]);
-            const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    part[i][j] = fmaf(xs[i], ys[j], part[i][j]);
-                }
-            }
-        }
-        __syncthreads();
-        if ((d0 + kDepth) % kChunk == 0 || d0 + kDepth >= depth) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    total[i][j] += part[i][j];
-                    part[i][j] = 0.0f;
-                }
-            }
-        }
-    }
-}
+struct BlockSync {
+    __device__ __forceinline__ void operator()() const { __syncthreads(); }
+};
 
 template <class T, class O> __global__ void __launch_bounds__(kThreads) RowsKernel(RowsProblem p)
 {
+    __shared__ tile::Operands shared;
     const T* a = static_cast<const T*>(p.a);
     const T* b = static_cast<const T*>(p.b);
     O* out = static_cast<O*>(p.out);
@@ -89,9 +46,11 @@ template <class T, class O> __global__ void __launch_bounds__(kThreads) RowsKern
                               ? p.b_scale + (walk.segment * ((p.n + 127) / 128) + col0 / 128) * blocks
                               : nullptr;
         auto multiply = [&](int64_t from, int64_t depth, float (&sum)[4][4]) {
-            Multiply([&](int r, int64_t d) { return row + r < row_end ? ValueOf(a + (row + r) * p.lda + from + d) : 0.0f; },
-                     [&](int64_t d, int c) { return col0 + c < p.n ? ValueOf(matrix + (from + d) * p.b_k + (col0 + c) * p.b_n) : 0.0f; },
-                     true, p.b_k == 1, depth, sum);
+            tile::Multiply(
+                shared, threadIdx.x, BlockSync(),
+                [&](int r, int64_t d) { return row + r < row_end ? ValueOf(a + (row + r) * p.lda + from + d) : 0.0f; },
+                [&](int64_t d, int c) { return col0 + c < p.n ? ValueOf(matrix + (from + d) * p.b_k + (col0 + c) * p.b_n) : 0.0f; }, true,
+                p.b_k == 1, depth, sum);
         };
         if (bs == nullptr) {
             multiply(0, p.k, total);
@@ -136,6 +95,7 @@ template <class T, class O> __global__ void __launch_bounds__(kThreads) RowsKern
 
 template <class T> __global__ void __launch_bounds__(kThreads) OuterKernel(OuterProblem p)
 {
+    __shared__ tile::Operands shared;
     const T* a = static_cast<const T*>(p.a);
     const T* b = static_cast<const T*>(p.b);
     T* out = static_cast<T*>(p.out);
@@ -146,9 +106,10 @@ template <class T> __global__ void __launch_bounds__(kThreads) OuterKernel(Outer
         int64_t begin, end;
         p.ptr.Range<int64_t>(e, begin, end);
         float total[4][4] = {};
-        Multiply([&](int r, int64_t d) { return k0 + r < p.k ? ValueOf(a + (begin + d) * p.lda + k0 + r) : 0.0f; },
-                 [&](int64_t d, int c) { return n0 + c < p.n ? ValueOf(b + (begin + d) * p.ldb + n0 + c) : 0.0f; }, false, false,
-                 end - begin, total);
+        tile::Multiply(
+            shared, threadIdx.x, BlockSync(), [&](int r, int64_t d) { return k0 + r < p.k ? ValueOf(a + (begin + d) * p.lda + k0 + r) : 0.0f; },
+            [&](int64_t d, int c) { return n0 + c < p.n ? ValueOf(b + (begin + d) * p.ldb + n0 + c) : 0.0f; }, false, false, end - begin,
+            total);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll

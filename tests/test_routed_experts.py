@@ -1270,3 +1270,87 @@ def test_waits_of_a_single_poll(cuda_device, kind):
         ops_gnn._pybind.set_wait_polls(-1)
         ops_gnn._pybind.device_stall_count(device, True)
     assert all(torch.equal(a, b) for a, b in zip(run(), want))
+
+
+def _matches(actual, product, a, b, terms, what):
+    """product(a, b) in 64 bits: NaN and infinities where it has them when rounded to the type, finite results within the bound of
+    _within.
+
+    Left out: results whose finite terms' magnitudes add up to 2^127 or more, unless all terms are finite and have one sign.  A sum
+    in fp32 of some of the terms may pass 2^128, as an infinity of either sign, before the others bring the total back or an
+    infinity of the other sign joins it, so such a result depends on the order of the sum.  Terms of one sign only grow, and smaller
+    magnitudes never get there, in any order."""
+    expected, magnitude = product(a, b), product(a.abs(), b.abs())
+    a0, b0 = [torch.where(torch.isfinite(t), t, torch.zeros_like(t)) for t in (a, b)]
+    size = product(a0.abs(), b0.abs())
+    open_ = (size >= 2.0 ** 127) & ~(torch.isfinite(magnitude) & (expected.abs() >= magnitude * (1 - 1e-12)))
+    got, want = actual.detach().cpu(), expected.to(actual.dtype)
+    assert not open_.all()
+    got, want, expected, magnitude = [t[~open_] for t in (got, want, expected, magnitude)]
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what + ": NaN"
+    assert torch.equal(got[torch.isinf(got)], want[torch.isinf(got)]) and torch.equal(torch.isinf(got), torch.isinf(want)), what + ": infinities"
+    fine = torch.isfinite(want)
+    _within(got[fine], expected[fine], magnitude[fine], terms, what)
+
+
+@requires_gpu
+@pytest.mark.parametrize("kind", ["nan", "infinite", "above bf16", "overflow"])
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("lengths,k,n", [([700, 0, 1000, 403], 264, 200), ([6000, 30, 4500], 72, 264), ([5000, 4000], 40, 520), ([3, 2500], 130, 264)])
+def test_segment_matmul_special_values_in_fp32_terms(cuda_device, lengths, k, n, turned, kind):
+    """fp32 products large enough for the sums of bf16 terms (2e8 operations, 2048 rows for gradients), in one piece and in
+    pieces: NaN, infinities, numbers that round to an infinity in bf16 and sums that overflow."""
+    from ops_gnn import segment_matmul
+
+    assert 2 * sum(lengths) * k * n >= 1.5e8 and sum(lengths) >= 2048
+    src, ptr, weight, grad = _matmul_inputs((lengths, 3, 5, k, n), torch.float32, 121)
+    last, middle = sum(lengths) + 2, 3 + lengths[0] // 2  # the last row of the last segment, one within the first
+    if kind == "nan":
+        src[last, 3], grad[middle, n - 1] = math.nan, math.nan
+    elif kind == "infinite":
+        src[last, 3], src[middle, 5], grad[middle, n - 1] = math.inf, -math.inf, math.inf
+        weight[0, 5, 2], weight[-1, 7, 9] = 0.0, math.inf
+        src[middle + 1, 5] = math.inf  # and minus infinity in the same column: NaN in its weight gradient
+    elif kind == "above bf16":  # times small numbers only
+        src[last, 3], weight[-1, 3], grad[last] = 3.398e38, weight[-1, 3] * 1e-30, grad[last] * 1e-30
+        grad[middle, 4], weight[0, :, 4], src[middle] = -3.398e38, weight[0, :, 4] * 1e-30, src[middle] * 1e-30
+    else:
+        src[last], weight[-1], grad[middle] = 1e38, weight[-1].abs() * 1e38, 2e38
+        src[middle] = src[middle].abs() + 1
+    back = weight.transpose(1, 2)
+    x = src.to(cuda_device).requires_grad_()
+    w = (back.contiguous() if turned else weight).to(cuda_device).requires_grad_()
+    out = segment_matmul(x, ptr.to(cuda_device), w.transpose(1, 2) if turned else w)
+    grad_src, grad_weight = torch.autograd.grad(out, (x, w), grad.to(cuda_device))
+    _matches(out, lambda a, b: _plain_matmul(a, ptr, b), src, weight, k + 2, "out")
+    _matches(grad_src, lambda a, b: _plain_matmul(a, ptr, b), grad, back, n + 2, "grad_src")
+    _matches(grad_weight.transpose(1, 2) if turned else grad_weight, lambda a, b: _plain_weight_grad(a, ptr, b), src, grad,
+             max(lengths) + 2, "grad_weight")
+
+
+@requires_gpu
+def test_segment_matmul_fp32_with_a_row_of_nan_takes_no_longer(cuda_device):
+    """One row of NaN makes a whole weight gradient NaN; nothing is summed again for it."""
+    from ops_gnn import segment_matmul
+
+    src, ptr, weight, grad = [t.to(cuda_device) for t in _matmul_inputs(([2000, 6000, 192], 0, 0, 512, 512), torch.float32, 131)]
+    dirty = src.clone()
+    dirty[-200] = math.nan
+
+    def step(values):
+        x, w = values.requires_grad_(), weight.requires_grad_()
+        times = []
+        for _ in range(8):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            out = segment_matmul(x, ptr, w)
+            grads = torch.autograd.grad(out, (x, w), grad)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times[2:]), grads[1]
+
+    clean, _ = step(src)
+    slow, grad_weight = step(dirty)
+    assert torch.isnan(grad_weight[1]).all() and torch.isfinite(grad_weight[0]).all() and torch.isfinite(grad_weight[2]).all()
+    assert slow <= 2 * clean, (slow, clean)
