@@ -72,7 +72,8 @@ template <class T> __device__ __forceinline__ T WarpSum(T v)
     return v;
 }
 
-// The same over teams of LANES neighbouring lanes (the whole warp calls).
+// The same over teams of LANES neighbouring lanes.  The whole warp calls, never from a branch that one team's row takes and
+// another's does not: a lane that stays out leaves the others waiting.
 template <int LANES> __device__ __forceinline__ float TeamMax(float v)
 {
 #pragma unroll
@@ -755,7 +756,8 @@ __global__ void __launch_bounds__(kWarps * 32) TopkBackwardKernel(RouteParams p,
             if (p.renormalize) {
                 const float sum = TeamSum<LANES>(s);
                 const float w = sum == 0.0f ? 0.0f : s / sum;
-                v = sum == 0.0f ? 0.0f : (u - TeamSum<LANES>(u * w)) / sum;
+                const float mean = TeamSum<LANES>(u * w);  // by every lane, also where the row's sum is 0 and its neighbours' are not
+                v = sum == 0.0f ? 0.0f : (u - mean) / sum;
             }
             value = v * s * (1.0f - s);
         }

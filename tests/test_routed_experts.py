@@ -1354,3 +1354,36 @@ def test_segment_matmul_fp32_with_a_row_of_nan_takes_no_longer(cuda_device):
     slow, grad_weight = step(dirty)
     assert torch.isnan(grad_weight[1]).all() and torch.isfinite(grad_weight[0]).all() and torch.isfinite(grad_weight[2]).all()
     assert slow <= 2 * clean, (slow, clean)
+
+
+def test_teams_sum_outside_of_branches():
+    """Sums over a team of lanes are warp-wide shuffles: a condition in front of one that differs from row to row keeps lanes away
+    from it.  So none stands behind the ? of a condition, but for those of the call's own choices, alike in all rows."""
+    import pathlib
+    import re
+
+    source = pathlib.Path(__file__).resolve().parent.parent / "ops-gnn_b200" / "csrc" / "cuda" / "route.cu"
+    guarded = re.findall(r"([\w.:]+(?: (?:==|!=|<=|>=|<|>) [\w.]+)?) \?[^;]*?(?:Team|Warp)(?:Sum|Max)", source.read_text())
+    assert set(guarded) <= {"p.renormalize", "p.softmax"}, guarded
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", KINDS, ids=str)
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("experts,k", [(40, 4), (33, 3), (200, 8), (96, 12), (1000, 2)])
+def test_topk_route_gradient_beside_masked_rows(cuda_device, dtype, score, renormalize, experts, k):
+    """Rows that the mask leaves nothing of have no gradient, and their neighbours keep theirs to the bit."""
+    from ops_gnn import topk_route
+
+    x = (torch.randn(23, experts, generator=_gen(151)) * 2).to(dtype)
+    grad = torch.randn(23, k, generator=_gen(152)).to(dtype).to(cuda_device)
+    plain = x.to(cuda_device).requires_grad_()
+    want, = torch.autograd.grad(topk_route(plain, k, score, renormalize=renormalize)[0], plain, grad)
+    masked = [0, 2, 5, 6, 15, 22]
+    x[masked] = -math.inf
+    leaf = x.to(cuda_device).requires_grad_()
+    weight, _ = topk_route(leaf, k, score, renormalize=renormalize)
+    got, = torch.autograd.grad(weight, leaf, grad)
+    want[masked] = 0
+    assert not weight[masked].any() and torch.equal(got, want)
