@@ -12,7 +12,8 @@
 // Backward (u = grad * scale, sums over the chosen i):
 //     softmax, renormalized:  dl_i = w_i (u_i - sum u w)                     with w the softmax over the chosen logits
 //     softmax:                dl_j = s_j ([j chosen] u_j - sum u s)          for every expert j
-//     sigmoid:                dl_i = v_i s_i (1 - s_i),  v = u or (u - sum u w) / sum s when renormalized
+//     sigmoid, renormalized:  dl_i = w_i (1 - s_i) (u_i - sum u w)           with w = s / sum s
+//     sigmoid:                dl_i = u_i s_i (1 - s_i)
 // and 0 for every expert that has no term.
 //
 // route_csr is a stable counting sort of the pairs by expert; see there.
@@ -752,14 +753,14 @@ __global__ void __launch_bounds__(kWarps * 32) TopkBackwardKernel(RouteParams p,
             }
         } else {
             const float s = at < 0 ? 0.0f : Sigmoid(x);
-            float v = u;
+            value = u * s * (1.0f - s);
             if (p.renormalize) {
+                // (s / sum first: dividing by the sum alone overflows where scores are near the smallest number)
                 const float sum = TeamSum<LANES>(s);
                 const float w = sum == 0.0f ? 0.0f : s / sum;
                 const float mean = TeamSum<LANES>(u * w);  // by every lane, also where the row's sum is 0 and its neighbours' are not
-                v = sum == 0.0f ? 0.0f : (u - mean) / sum;
+                value = w * (1.0f - s) * (u - mean);
             }
-            value = v * s * (1.0f - s);
         }
         // The whole row first, the chosen experts over it: same warp, ordered by the barrier.
         const bool dense = p.softmax && !p.renormalize;

@@ -1387,3 +1387,30 @@ def test_topk_route_gradient_beside_masked_rows(cuda_device, dtype, score, renor
     got, = torch.autograd.grad(weight, leaf, grad)
     want[masked] = 0
     assert not weight[masked].any() and torch.equal(got, want)
+
+
+@requires_gpu
+@pytest.mark.parametrize("experts,k", [(16, 2), (40, 12)])
+def test_topk_route_gradient_of_tiny_scores(cuda_device, experts, k):
+    """Sigmoid scores near the smallest number of fp32, whose sum no gradient can be divided by: their shares of it are ordinary.
+
+    A score of 3e-39 has steps of 2^-149, 4.7e-7 of its value or 4 * 2^-23: three of them (score, sum, share) make 12 steps more
+    than the bound of ordinary scores counts."""
+    from ops_gnn import topk_route
+
+    gen = _gen(161)
+    x = -88.2 + 0.4 * torch.rand(30, experts, generator=gen)
+    x[7] = -math.inf
+    grad = torch.randn(30, k, generator=gen) * 20
+    leaf = x.to(cuda_device).requires_grad_()
+    weight, index = topk_route(leaf, k, "sigmoid")
+    got, = torch.autograd.grad(weight, leaf, grad.to(cuda_device))
+    chosen = index.cpu()
+    s = torch.sigmoid(x.double())
+    picked = s.gather(1, chosen)
+    share = picked / picked.sum(1, keepdim=True).clamp(min=1e-300)
+    u = grad.double()
+    want = torch.zeros_like(s).scatter_(1, chosen, share * (1 - picked) * (u - (u * share).sum(1, keepdim=True)))
+    size = torch.zeros_like(s).scatter_(1, chosen, share * (u.abs() + (u.abs() * share).sum(1, keepdim=True)))
+    _within(got, want, size, 4 * experts + 64 + 12, "gradient")
+    _within(weight, share, share, experts + 16 + 12, "weight")
