@@ -442,6 +442,14 @@ OPSGNN_API int opsgnn_topk_route(const OpsgnnRouteDesc* desc, const void* logits
 OPSGNN_API int opsgnn_topk_route_backward(const OpsgnnRouteDesc* desc, const void* logits, const int64_t* index,
                                           const void* grad_weight, void* grad_logits, void* stream);
 
+/* The same pair for a forward pass that is differentiated later: undefined[T] (bytes, may be NULL in either) gets 1 for a row whose
+ * softmax has no value (NaN or +inf among its logits), else 0, which spares the backward pass of renormalised weights
+ * reading all logits to find such rows, whose gradient is NaN. */
+OPSGNN_API int opsgnn_topk_route_recorded(const OpsgnnRouteDesc* desc, const void* logits, const float* bias, void* weight,
+                                          int64_t* index, uint8_t* undefined, void* stream);
+OPSGNN_API int opsgnn_topk_route_backward_recorded(const OpsgnnRouteDesc* desc, const void* logits, const int64_t* index,
+                                                   const uint8_t* undefined, const void* grad_weight, void* grad_logits, void* stream);
+
 /* The CSR structure of `count` labels: indptr[experts + 1], perm[count] (the labels' positions in stable order of their
  * experts) and position[count] (perm's inverse).  Labels outside [0, experts) come last, behind indptr[experts].
  * experts <= 4096, count < 2^31. */

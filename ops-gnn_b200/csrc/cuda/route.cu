@@ -14,7 +14,7 @@
 //     softmax:                dl_j = s_j ([j chosen] u_j - sum u s)          for every expert j
 //     sigmoid, renormalized:  dl_i = w_i (1 - s_i) (u_i - sum u w)           with w = s / sum s
 //     sigmoid:                dl_i = u_i s_i (1 - s_i)
-// and 0 for every expert that has no term.
+// and 0 for every expert that has no term.  Under softmax a row with a NaN or +inf has weights of NaN, and so its whole gradient is.
 //
 // route_csr is a stable counting sort of the pairs by expert; see there.
 #include <algorithm>
@@ -32,6 +32,7 @@ struct RouteParams {
     int32_t experts, k, groups, kept_groups, group_top;
     int32_t softmax, renormalize;
     float scale;
+    uint8_t* undefined;  // may be null; forward writes, backward reads 1 for a row whose softmax has no value
 };
 
 // Order-preserving keys; 0 is below every number and marks what cannot be chosen any more.  NaN ranks with -inf.
@@ -548,6 +549,9 @@ __global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T
             s = taken ? Sigmoid(chosen_logit) : 0.0f;
             total = p.renormalize ? WarpSum(s) : 1.0f;
         }
+        if (p.undefined != nullptr && lane == 0) {
+            p.undefined[r] = bad ? 1 : 0;
+        }
         if (taken) {
             const float w = bad ? NAN : (total == 0.0f ? 0.0f : s / total * p.scale);
             weight[r * p.k + lane] = Narrow<T, float>(w);
@@ -686,6 +690,9 @@ __global__ void __launch_bounds__(kWarps * 32) TopkTeamKernel(RouteParams p, con
             s = taken ? Sigmoid(x) : 0.0f;
             total = p.renormalize ? TeamSum<8>(s) : 1.0f;
         }
+        if (p.undefined != nullptr && member == 0 && real) {
+            p.undefined[r] = bad ? 1 : 0;
+        }
         if (taken && real) {
             const float w = bad ? NAN : (total == 0.0f ? 0.0f : s / total * p.scale);
             weight[r * p.k + member] = Narrow<T, float>(w);
@@ -709,6 +716,7 @@ __global__ void __launch_bounds__(kWarps * 32) TopkBackwardKernel(RouteParams p,
         const int64_t r = real ? r0 + lane / LANES : r0;
         const T* row = logits + r * p.experts;
         T* out = grad_logits + r * p.experts;
+        const bool undefined = p.undefined != nullptr && __ldg(p.undefined + r) != 0;
         int64_t at = -1;
         float u = 0.0f, x = -INFINITY;
         if (member < p.k) {
@@ -730,7 +738,8 @@ __global__ void __launch_bounds__(kWarps * 32) TopkBackwardKernel(RouteParams p,
                 const float e = at < 0 || (x == -INFINITY && top == -INFINITY) ? 0.0f : expf(x - top);
                 const float sum = TeamSum<LANES>(e);
                 const float w = sum == 0.0f ? 0.0f : e / sum;
-                value = w * (u - TeamSum<LANES>(u * w));
+                const float mean = TeamSum<LANES>(u * w);
+                value = w * (u - mean);
             } else {
                 LoadRow<T, VPL>(row, p.experts, wide, member, l);
                 top = -INFINITY;
@@ -787,6 +796,31 @@ __global__ void __launch_bounds__(kWarps * 32) TopkBackwardKernel(RouteParams p,
         __syncwarp();
         if (real && at >= 0) {
             out[at] = Narrow<T, float>(value);
+        }
+        // A row without a softmax: the chosen experts of renormalised weights do not show it.
+        if (__any_sync(kFull, undefined)) {
+            __syncwarp();
+            for (int j = undefined && real ? member : p.experts; j < p.experts; j += LANES) {
+                out[j] = Narrow<T, float>(NAN);
+            }
+        }
+    }
+}
+
+// The same for a backward pass that was not told which rows these are: NaN for the gradient of every row with a NaN or +inf.
+template <class T>
+__global__ void __launch_bounds__(kWarps * 32) UndefinedRowsKernel(RouteParams p, const T* __restrict__ logits, T* __restrict__ grad_logits)
+{
+    const int lane = threadIdx.x & 31;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); r < p.rows; r += static_cast<int64_t>(gridDim.x) * kWarps) {
+        bool odd = false;
+        for (int j = lane; j < p.experts; j += 32) {
+            odd |= !(Widen<float, T>(LoadNc(logits + r * p.experts + j)) < INFINITY);
+        }
+        if (__any_sync(kFull, odd)) {
+            for (int j = lane; j < p.experts; j += 32) {
+                grad_logits[r * p.experts + j] = Narrow<T, float>(NAN);
+            }
         }
     }
 }
@@ -1029,9 +1063,10 @@ int CheckRoute(const OpsgnnRouteDesc* d)
     return OPSGNN_OK;
 }
 
-RouteParams ParamsOf(const OpsgnnRouteDesc& d)
+RouteParams ParamsOf(const OpsgnnRouteDesc& d, uint8_t* undefined)
 {
     RouteParams p;
+    p.undefined = undefined;
     p.rows = d.rows;
     p.experts = static_cast<int32_t>(d.experts);
     p.k = static_cast<int32_t>(d.k);
@@ -1057,9 +1092,10 @@ template <class T, int VPL> bool Wide(int64_t experts, const void* a, const void
 }
 
 template <class T, int VPL>
-int RunTopk(const OpsgnnRouteDesc& d, const void* logits, const float* bias, void* weight, int64_t* index, cudaStream_t stream)
+int RunTopk(const OpsgnnRouteDesc& d, const void* logits, const float* bias, void* weight, int64_t* index, uint8_t* undefined,
+            cudaStream_t stream)
 {
-    const RouteParams p = ParamsOf(d);
+    const RouteParams p = ParamsOf(d, undefined);
     const bool biased = bias != nullptr || (d.groups > 1 && d.group_top == 2);
     const T* in = static_cast<const T*>(logits);
     T* out = static_cast<T*>(weight);
@@ -1082,22 +1118,29 @@ int RunTopk(const OpsgnnRouteDesc& d, const void* logits, const float* bias, voi
 }
 
 template <class T, int VPL>
-int RunTopkBackward(const OpsgnnRouteDesc& d, const void* logits, const int64_t* index, const void* grad, void* grad_logits,
-                    cudaStream_t stream)
+int RunTopkBackward(const OpsgnnRouteDesc& d, const void* logits, const int64_t* index, const uint8_t* undefined, const void* grad,
+                    void* grad_logits, cudaStream_t stream)
 {
+    const RouteParams p = ParamsOf(d, const_cast<uint8_t*>(undefined));
     const T* in = static_cast<const T*>(logits);
     const T* g = static_cast<const T*>(grad);
     T* out = static_cast<T*>(grad_logits);
+    auto launched = [&]() {
+        if (p.softmax && p.renormalize && undefined == nullptr) {
+            UndefinedRowsKernel<T><<<Grid(d.rows, 1), kWarps * 32, 0, stream>>>(p, in, out);
+        }
+        return LaunchStatus();
+    };
     if constexpr (VPL <= 8) {
         if (d.k <= 8) {
-            TopkBackwardKernel<T, 4 * VPL, 8><<<Grid(d.rows, 4), kWarps * 32, 0, stream>>>(ParamsOf(d), in, index, g, out,
+            TopkBackwardKernel<T, 4 * VPL, 8><<<Grid(d.rows, 4), kWarps * 32, 0, stream>>>(p, in, index, g, out,
                                                                                            Wide<T, 4 * VPL>(d.experts, in, out));
-            return LaunchStatus();
+            return launched();
         }
     }
-    TopkBackwardKernel<T, VPL, 32><<<Grid(d.rows, 1), kWarps * 32, 0, stream>>>(ParamsOf(d), in, index, g, out,
+    TopkBackwardKernel<T, VPL, 32><<<Grid(d.rows, 1), kWarps * 32, 0, stream>>>(p, in, index, g, out,
                                                                               Wide<T, VPL>(d.experts, in, out));
-    return LaunchStatus();
+    return launched();
 }
 
 // f(type tag, integral constant VPL): experts a lane of a warp holds, a power of two.
@@ -1137,8 +1180,8 @@ template <class F> int Dispatch(const OpsgnnRouteDesc& d, F&& f)
 
 using namespace opsgnn;
 
-extern "C" int opsgnn_topk_route(const OpsgnnRouteDesc* desc, const void* logits, const float* bias, void* weight, int64_t* index,
-                                 void* stream)
+extern "C" int opsgnn_topk_route_recorded(const OpsgnnRouteDesc* desc, const void* logits, const float* bias, void* weight,
+                                          int64_t* index, uint8_t* undefined, void* stream)
 {
     const int status = route::CheckRoute(desc);
     if (status != OPSGNN_OK || desc->rows == 0) {
@@ -1148,12 +1191,18 @@ extern "C" int opsgnn_topk_route(const OpsgnnRouteDesc* desc, const void* logits
         return OPSGNN_ERR_INVALID;
     }
     return route::Dispatch(*desc, [&](auto tag, auto vpl) {
-        return route::RunTopk<decltype(tag), decltype(vpl)::value>(*desc, logits, bias, weight, index, AsStream(stream));
+        return route::RunTopk<decltype(tag), decltype(vpl)::value>(*desc, logits, bias, weight, index, undefined, AsStream(stream));
     });
 }
 
-extern "C" int opsgnn_topk_route_backward(const OpsgnnRouteDesc* desc, const void* logits, const int64_t* index, const void* grad_weight,
-                                          void* grad_logits, void* stream)
+extern "C" int opsgnn_topk_route(const OpsgnnRouteDesc* desc, const void* logits, const float* bias, void* weight, int64_t* index,
+                                 void* stream)
+{
+    return opsgnn_topk_route_recorded(desc, logits, bias, weight, index, nullptr, stream);
+}
+
+extern "C" int opsgnn_topk_route_backward_recorded(const OpsgnnRouteDesc* desc, const void* logits, const int64_t* index,
+                                                   const uint8_t* undefined, const void* grad_weight, void* grad_logits, void* stream)
 {
     const int status = route::CheckRoute(desc);
     if (status != OPSGNN_OK || desc->rows == 0) {
@@ -1163,9 +1212,15 @@ extern "C" int opsgnn_topk_route_backward(const OpsgnnRouteDesc* desc, const voi
         return OPSGNN_ERR_INVALID;
     }
     return route::Dispatch(*desc, [&](auto tag, auto vpl) {
-        return route::RunTopkBackward<decltype(tag), decltype(vpl)::value>(*desc, logits, index, grad_weight, grad_logits,
+        return route::RunTopkBackward<decltype(tag), decltype(vpl)::value>(*desc, logits, index, undefined, grad_weight, grad_logits,
                                                                            AsStream(stream));
     });
+}
+
+extern "C" int opsgnn_topk_route_backward(const OpsgnnRouteDesc* desc, const void* logits, const int64_t* index, const void* grad_weight,
+                                          void* grad_logits, void* stream)
+{
+    return opsgnn_topk_route_backward_recorded(desc, logits, index, nullptr, grad_weight, grad_logits, stream);
 }
 
 extern "C" int opsgnn_route_csr_workspace_bytes(int64_t count, int64_t experts, int64_t* bytes)

@@ -27,9 +27,12 @@ OpsgnnRouteDesc RouteDescOf(const at::Tensor& logits, int64_t k, int64_t score, 
 
 }  // namespace
 
-std::tuple<at::Tensor, at::Tensor> topk_route_forward(const at::Tensor& logits, const std::optional<at::Tensor>& bias, int64_t k,
-                                                      int64_t score, int64_t groups, int64_t kept_groups, int64_t group_top,
-                                                      bool renormalize, double scale)
+namespace {
+
+// `undefined`: bytes, one per row, for the backward pass; may be null.
+std::tuple<at::Tensor, at::Tensor> Forward(const at::Tensor& logits, const std::optional<at::Tensor>& bias, int64_t k, int64_t score,
+                                           int64_t groups, int64_t kept_groups, int64_t group_top, bool renormalize, double scale,
+                                           at::Tensor* undefined)
 {
     const char* api = "topk_route";
     const OpsgnnRouteDesc desc = RouteDescOf(logits, k, score, groups, kept_groups, group_top, renormalize, scale, api);
@@ -41,14 +44,18 @@ std::tuple<at::Tensor, at::Tensor> topk_route_forward(const at::Tensor& logits, 
     c10::cuda::CUDAGuard guard(logits.device());
     at::Tensor weight = at::empty({desc.rows, k}, logits.options());
     at::Tensor index = at::empty({desc.rows, k}, logits.options().dtype(at::kLong));
-    CheckStatus(opsgnn_topk_route(&desc, logits.const_data_ptr(), bias ? bias->const_data_ptr<float>() : nullptr, weight.data_ptr(),
-                                  index.data_ptr<int64_t>(), CurrentStream(logits)),
+    if (undefined != nullptr) {
+        *undefined = at::empty({desc.rows}, logits.options().dtype(at::kByte));
+    }
+    CheckStatus(opsgnn_topk_route_recorded(&desc, logits.const_data_ptr(), bias ? bias->const_data_ptr<float>() : nullptr,
+                                           weight.data_ptr(), index.data_ptr<int64_t>(),
+                                           undefined != nullptr ? undefined->data_ptr<uint8_t>() : nullptr, CurrentStream(logits)),
                 api);
     return {weight, index};
 }
 
-at::Tensor topk_route_backward(const at::Tensor& logits, const at::Tensor& index, const at::Tensor& grad_weight, int64_t score,
-                               bool renormalize, double scale)
+at::Tensor Backward(const at::Tensor& logits, const at::Tensor& index, const at::Tensor& undefined, const at::Tensor& grad_weight,
+                    int64_t score, bool renormalize, double scale)
 {
     const char* api = "topk_route backward";
     const OpsgnnRouteDesc desc = RouteDescOf(logits, index.size(-1), score, 1, 1, 1, renormalize, scale, api);
@@ -58,10 +65,26 @@ at::Tensor topk_route_backward(const at::Tensor& logits, const at::Tensor& index
                 api, ": index and grad_weight must be contiguous [rows, k] tensors on the GPU of logits");
     c10::cuda::CUDAGuard guard(logits.device());
     at::Tensor grad_logits = at::empty_like(logits);
-    CheckStatus(opsgnn_topk_route_backward(&desc, logits.const_data_ptr(), index.const_data_ptr<int64_t>(), grad_weight.const_data_ptr(),
-                                           grad_logits.data_ptr(), CurrentStream(logits)),
+    CheckStatus(opsgnn_topk_route_backward_recorded(&desc, logits.const_data_ptr(), index.const_data_ptr<int64_t>(),
+                                                    undefined.defined() ? undefined.const_data_ptr<uint8_t>() : nullptr,
+                                                    grad_weight.const_data_ptr(), grad_logits.data_ptr(), CurrentStream(logits)),
                 api);
     return grad_logits;
+}
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor> topk_route_forward(const at::Tensor& logits, const std::optional<at::Tensor>& bias, int64_t k,
+                                                      int64_t score, int64_t groups, int64_t kept_groups, int64_t group_top,
+                                                      bool renormalize, double scale)
+{
+    return Forward(logits, bias, k, score, groups, kept_groups, group_top, renormalize, scale, nullptr);
+}
+
+at::Tensor topk_route_backward(const at::Tensor& logits, const at::Tensor& index, const at::Tensor& grad_weight, int64_t score,
+                               bool renormalize, double scale)
+{
+    return Backward(logits, index, at::Tensor(), grad_weight, score, renormalize, scale);
 }
 
 namespace {
@@ -73,8 +96,11 @@ public:
                                                   const std::optional<at::Tensor>& bias, int64_t k, int64_t score, int64_t groups,
                                                   int64_t kept_groups, int64_t group_top, bool renormalize, double scale)
     {
-        auto [weight, index] = topk_route_forward(logits, bias, k, score, groups, kept_groups, group_top, renormalize, scale);
-        ctx->save_for_backward({logits, index});
+        at::Tensor undefined;
+        const bool marks = score == OPSGNN_ROUTE_SOFTMAX && renormalize;
+        auto [weight, index] =
+            Forward(logits, bias, k, score, groups, kept_groups, group_top, renormalize, scale, marks ? &undefined : nullptr);
+        ctx->save_for_backward({logits, index, undefined});
         ctx->saved_data["score"] = score;
         ctx->saved_data["renormalize"] = renormalize;
         ctx->saved_data["scale"] = scale;
@@ -88,9 +114,9 @@ public:
         if (grads[0].defined()) {
             PlannerScope scope;
             const auto saved = ctx->get_saved_variables();
-            const at::Tensor grad = topk_route_backward(saved[0].detach(), saved[1], grads[0].detach().contiguous(),
-                                                        ctx->saved_data["score"].toInt(), ctx->saved_data["renormalize"].toBool(),
-                                                        ctx->saved_data["scale"].toDouble());
+            const at::Tensor grad = Backward(saved[0].detach(), saved[1], saved[2], grads[0].detach().contiguous(),
+                                             ctx->saved_data["score"].toInt(), ctx->saved_data["renormalize"].toBool(),
+                                             ctx->saved_data["scale"].toDouble());
             out[0] = OnceDifferentiable({grad}, "topk_route")[0];
         }
         return out;

@@ -35,7 +35,8 @@ EXPORTS = (
     "opsgnn_index_longest_run",
     "opsgnn_scatter_workspace_bytes", "opsgnn_scatter",
     "opsgnn_grouped_workspace_bytes", "opsgnn_grouped_forward", "opsgnn_grouped_forward_permuted", "opsgnn_grouped_backward",
-    "opsgnn_topk_route", "opsgnn_topk_route_backward", "opsgnn_route_csr_workspace_bytes", "opsgnn_route_csr",
+    "opsgnn_topk_route", "opsgnn_topk_route_backward", "opsgnn_topk_route_recorded", "opsgnn_topk_route_backward_recorded",
+    "opsgnn_route_csr_workspace_bytes", "opsgnn_route_csr",
     "opsgnn_segment_matmul_workspace_bytes", "opsgnn_segment_matmul", "opsgnn_segment_matmul_weight_grad", "opsgnn_segment_matmul_grads",
     "opsgnn_segment_matmul_fp8", "opsgnn_quantize_fp8",
 )
@@ -143,6 +144,8 @@ _PROTOTYPES = {
                                         c_void_p, c_int64, c_void_p]),
     "opsgnn_topk_route": (c_int, [POINTER(RouteDesc), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "opsgnn_topk_route_backward": (c_int, [POINTER(RouteDesc), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "opsgnn_topk_route_recorded": (c_int, [POINTER(RouteDesc), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "opsgnn_topk_route_backward_recorded": (c_int, [POINTER(RouteDesc), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "opsgnn_route_csr_workspace_bytes": (c_int, [c_int64, c_int64, POINTER(c_int64)]),
     "opsgnn_route_csr": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "opsgnn_segment_matmul_workspace_bytes": (c_int, [POINTER(SegmentMatmulDesc), c_int, POINTER(c_int64)]),

@@ -34,7 +34,7 @@ def topk_route(logits: torch.Tensor, k: int, score: str = "softmax", bias: Optio
 
     An expert whose logit is ``-inf`` is masked: it comes after every other of the open groups and weighs 0; a row of
     nothing else has weights 0.  A NaN ranks with the masked ones and shows as NaN weights; under softmax a NaN or ``+inf``
-    makes the whole row NaN, as with ``torch.softmax``.  The choice does not depend on how scores round: it compares the
+    makes the whole row NaN, as with ``torch.softmax``, and its gradient.  The choice does not depend on how scores round: it compares the
     logits where the scores order as they do, and scores in 64 bits where a bias or a sum of two decides.
 
     float16, float32 and bfloat16 on a CUDA device; at most 1024 experts, 32 chosen, 32 groups.  Raises ``TypeError`` /

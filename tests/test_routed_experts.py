@@ -1414,3 +1414,31 @@ def test_topk_route_gradient_of_tiny_scores(cuda_device, experts, k):
     size = torch.zeros_like(s).scatter_(1, chosen, share * (u.abs() + (u.abs() * share).sum(1, keepdim=True)))
     _within(got, want, size, 4 * experts + 64 + 12, "gradient")
     _within(weight, share, share, experts + 16 + 12, "weight")
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", KINDS, ids=str)
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("experts,k", [(40, 4), (33, 3), (200, 8), (256, 12), (1000, 2)])
+def test_topk_route_gradient_of_a_row_without_a_softmax(cuda_device, dtype, renormalize, experts, k):
+    """A NaN or +inf anywhere in a row makes its softmax NaN: the weights, and the gradient of every logit.  Other rows keep theirs."""
+    from ops_gnn import _pybind, topk_route
+
+    x = (torch.randn(9, experts, generator=_gen(141)) * 2).to(dtype)
+    grad = torch.randn(9, k, generator=_gen(142)).to(dtype).to(cuda_device)
+    plain = x.to(cuda_device).requires_grad_()
+    want, = torch.autograd.grad(topk_route(plain, k, renormalize=renormalize)[0], plain, grad)
+    low = x.argmin(1)  # not among the chosen
+    x[1, low[1]], x[3, low[3]], x[6, 0] = math.nan, math.inf, math.nan
+    x[6, 1] = -math.inf
+    leaf = x.to(cuda_device).requires_grad_()
+    weight, index = topk_route(leaf, k, renormalize=renormalize)
+    got, = torch.autograd.grad(weight, leaf, grad)
+    for r in range(9):
+        if r in (1, 3, 6):
+            assert torch.isnan(weight[r]).all() and torch.isnan(got[r]).all(), r
+        else:
+            assert torch.equal(got[r], want[r]), r
+    # without the forward pass's note of such rows
+    alone = _pybind.topk_route_backward(leaf.detach(), index, grad, 0, renormalize, 1.0)
+    assert torch.equal(torch.isnan(alone), torch.isnan(got)) and torch.equal(torch.nan_to_num(alone), torch.nan_to_num(got))
