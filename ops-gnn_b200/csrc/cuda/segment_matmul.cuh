@@ -32,6 +32,10 @@ struct OuterProblem {
     int32_t type;
 };
 
+// The stride of a dimension as a tensor map takes it: nothing steps over the stride of a single element, so there any run of whole
+// 16-byte vectors that holds `extent` values will do.
+inline int64_t StrideOf(int64_t stride, int64_t count, int64_t extent, int64_t vec) { return count > 1 ? stride : AlignUp(extent, vec); }
+
 // Any type, size, stride and alignment (segment_matmul_simple.cu).
 int RunRowsSimple(const RowsProblem& p, cudaStream_t stream);
 int RunOuterSimple(const OuterProblem& p, cudaStream_t stream);

@@ -972,10 +972,12 @@ int RunGradsSplit(const RowsProblem& rows, const OuterProblem& outer, bool turne
 
 int RunRowsFp8(const RowsProblem& p, cudaStream_t stream)
 {
-    if (p.in_type != OPSGNN_F8E4M3 || p.k < 1 || p.ptr.segments < 1 || p.b_k != 1 || p.lda % 16 != 0 || p.b_n % 16 != 0 ||
-        p.b_segment % 16 != 0 || p.b_segment < 1 || p.b_n < p.k || p.ldo != p.n || !Aligned(p.a, 16) ||
+    const int64_t lda = StrideOf(p.lda, p.ptr.rows, p.k, 16), stride = StrideOf(p.b_n, p.n, p.k, 16);
+    const int64_t segment_stride = StrideOf(p.b_segment, p.ptr.segments, stride * p.n, 16);
+    if (p.in_type != OPSGNN_F8E4M3 || p.k < 1 || p.ptr.segments < 1 || p.b_k != 1 || lda % 16 != 0 || stride % 16 != 0 ||
+        segment_stride % 16 != 0 || segment_stride < 1 || stride < p.k || p.ldo != p.n || !Aligned(p.a, 16) ||
         !Aligned(p.b, 16) || !Fits(p.ptr.rows) || !Fits(p.k) || !Fits(p.n) || !Fits(p.ptr.segments) ||
-        p.lda >= (INT64_C(1) << 39) || p.b_segment >= (INT64_C(1) << 39)) {
+        lda >= (INT64_C(1) << 39) || segment_stride >= (INT64_C(1) << 39)) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
     Params q{};
@@ -990,8 +992,8 @@ int RunRowsFp8(const RowsProblem& p, cudaStream_t stream)
     const int64_t down = p.ptr.rows / kRows + std::min(p.ptr.segments, p.ptr.rows);
     const bool narrow = Narrow128(down, p.n);
     CUtensorMap a, tail, b;
-    if (!Map3(&a, true, p.a, p.k, p.ptr.rows, 1, p.lda, p.lda, kRows) || !Map3(&tail, true, p.a, p.k, p.ptr.rows, 1, p.lda, p.lda, kBoxRows) ||
-        !Map3(&b, true, p.b, p.k, p.n, p.ptr.segments, p.b_n, p.b_segment, narrow ? 128 : 256)) {
+    if (!Map3(&a, true, p.a, p.k, p.ptr.rows, 1, lda, lda, kRows) || !Map3(&tail, true, p.a, p.k, p.ptr.rows, 1, lda, lda, kBoxRows) ||
+        !Map3(&b, true, p.b, p.k, p.n, p.ptr.segments, stride, segment_stride, narrow ? 128 : 256)) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
     const int64_t tiles = down * CeilDiv(p.n, narrow ? 128 : 256);

@@ -523,11 +523,13 @@ __global__ void __launch_bounds__(256) JoinRowsKernel(SegmentPointers ptr, int64
 int RunRowsTensor(const RowsProblem& p, void* workspace, cudaStream_t stream)
 {
     const bool turned = p.b_k == 1 && p.b_n != 1;
-    const int64_t inner = turned ? p.k : p.n, other = turned ? p.n : p.k, stride = turned ? p.b_n : p.b_k;
+    const int64_t inner = turned ? p.k : p.n, other = turned ? p.n : p.k;
+    const int64_t stride = StrideOf(turned ? p.b_n : p.b_k, other, inner, 8), lda = StrideOf(p.lda, p.ptr.rows, p.k, 8);
+    const int64_t segment_stride = StrideOf(p.b_segment, p.ptr.segments, stride * other, 8);
     if ((p.in_type != OPSGNN_BF16 && p.in_type != OPSGNN_F16) || p.out_type != p.in_type || p.k < 1 || p.ptr.data == nullptr ||
         p.ptr.segments < 1 || p.ldo != p.n || (!turned && p.b_n != 1) || stride < inner ||
-        p.b_segment % 8 != 0 || p.b_segment >= (INT64_C(1) << 38) || p.b_segment < 1 || p.ptr.segments >= (INT64_C(1) << 31) ||
-        !Loadable(p.a, p.lda, std::max(p.k, p.ptr.rows)) || !Loadable(p.b, stride, std::max(inner, other))) {
+        segment_stride % 8 != 0 || segment_stride >= (INT64_C(1) << 38) || segment_stride < 1 || p.ptr.segments >= (INT64_C(1) << 31) ||
+        !Loadable(p.a, lda, std::max(p.k, p.ptr.rows)) || !Loadable(p.b, stride, std::max(inner, other))) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
     Params q{};
@@ -546,14 +548,14 @@ int RunRowsTensor(const RowsProblem& p, void* workspace, cudaStream_t stream)
     q.whole_b = tc::WholeSlabs(p.n);
     CUtensorMap a, tail, b;
     const uint64_t sizes[3] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(other), static_cast<uint64_t>(p.ptr.segments)};
-    const uint64_t strides[2] = {static_cast<uint64_t>(stride) * 2, static_cast<uint64_t>(p.b_segment) * 2};
+    const uint64_t strides[2] = {static_cast<uint64_t>(stride) * 2, static_cast<uint64_t>(segment_stride) * 2};
     const uint32_t box[3] = {64, static_cast<uint32_t>(columns), 1};
     const CUtensorMapDataType type = TypeOf(p.in_type);
     // (with fewer rows than a full tile's last box reaches, every tile is short and the first map is never used)
-    if ((p.ptr.rows > kRows - kBoxRows && !Map2(&a, p.in_type, p.a, p.k, p.ptr.rows, p.lda, kDepth, kRows)) ||
-        !Map2(&tail, p.in_type, p.a, p.k, p.ptr.rows, p.lda, kDepth, kBoxRows) ||
+    if ((p.ptr.rows > kRows - kBoxRows && !Map2(&a, p.in_type, p.a, p.k, p.ptr.rows, lda, kDepth, kRows)) ||
+        !Map2(&tail, p.in_type, p.a, p.k, p.ptr.rows, lda, kDepth, kBoxRows) ||
         !(turned ? tc::EncodeMap(&b, type, 3, p.b, sizes, strides, box)
-                 : tc::EncodeSlabs(&b, type, p.b, p.n, p.k, p.ptr.segments, stride * 2, p.b_segment * 2, columns / 64))) {
+                 : tc::EncodeSlabs(&b, type, p.b, p.n, p.k, p.ptr.segments, stride * 2, segment_stride * 2, columns / 64))) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
     if (p.ptr.rows <= kRows - kBoxRows) {
@@ -685,8 +687,9 @@ int JoinPieces(const OuterProblem& p, int64_t chunk, const float* partial, cudaS
 
 int RunOuterTensor(const OuterProblem& p, void* workspace, cudaStream_t stream)
 {
+    const int64_t lda = StrideOf(p.lda, p.ptr.rows, p.k, 8), ldb = StrideOf(p.ldb, p.ptr.rows, p.n, 8);
     if ((p.type != OPSGNN_BF16 && p.type != OPSGNN_F16) || p.ptr.rows < 1 ||
-        !Loadable(p.a, p.lda, std::max(p.k, p.ptr.rows)) || !Loadable(p.b, p.ldb, std::max(p.n, p.ptr.rows))) {
+        !Loadable(p.a, lda, std::max(p.k, p.ptr.rows)) || !Loadable(p.b, ldb, std::max(p.n, p.ptr.rows))) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
     Params q{};
@@ -702,8 +705,8 @@ int RunOuterTensor(const OuterProblem& p, void* workspace, cudaStream_t stream)
     q.whole_a = tc::WholeSlabs(p.k);
     q.whole_b = tc::WholeSlabs(p.n);
     CUtensorMap a, b;
-    if (!tc::EncodeSlabs(&a, TypeOf(p.type), p.a, p.k, p.ptr.rows, 1, p.lda * 2, 16, kRows / 64) ||
-        !tc::EncodeSlabs(&b, TypeOf(p.type), p.b, p.n, p.ptr.rows, 1, p.ldb * 2, 16, narrow ? 2 : 4)) {
+    if (!tc::EncodeSlabs(&a, TypeOf(p.type), p.a, p.k, p.ptr.rows, 1, lda * 2, 16, kRows / 64) ||
+        !tc::EncodeSlabs(&b, TypeOf(p.type), p.b, p.n, p.ptr.rows, 1, ldb * 2, 16, narrow ? 2 : 4)) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
     auto run = [&](auto tag, auto width) {

@@ -1442,3 +1442,56 @@ def test_topk_route_gradient_of_a_row_without_a_softmax(cuda_device, dtype, reno
     # without the forward pass's note of such rows
     alone = _pybind.topk_route_backward(leaf.detach(), index, grad, 0, renormalize, 1.0)
     assert torch.equal(torch.isnan(alone), torch.isnan(got)) and torch.equal(torch.nan_to_num(alone), torch.nan_to_num(got))
+
+
+def _waits(run, device):
+    """Whether a call runs on the kernels that wait for their loads (the tensor cores'): without polls these report a stall."""
+    from ops_gnn import _pybind
+
+    index = device.index or 0
+    torch.cuda.synchronize()
+    _pybind.device_stall_count(index, True)
+    try:
+        _pybind.set_wait_polls(0)
+        run()
+        torch.cuda.synchronize()
+        return _pybind.device_stall_count(index, True) > 0
+    finally:
+        _pybind.set_wait_polls(-1)
+        _pybind.device_stall_count(index, True)
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("rows,k,n,segments", [(2100, 130, 641, 1), (3000, 257, 131, 1), (1, 2049, 25000, 1), (2100, 130, 641, 3), (2000, 25001, 1, 1)])
+def test_segment_matmul_odd_sizes_reach_the_tensor_cores(cuda_device, dtype, turned, rows, k, n, segments):
+    """Large products of odd sizes run on the tensor cores, also where a dimension has one element: nothing steps over its stride."""
+    from ops_gnn import segment_matmul
+
+    lengths = [rows] if segments == 1 else [rows - 1200, 0, 1200]
+    src, ptr, weight, grad = _matmul_inputs((lengths, 0, 0, k, n), dtype, 171)
+    back = weight.transpose(1, 2)
+    x, p, g = src.to(cuda_device).requires_grad_(), ptr.to(cuda_device), grad.to(cuda_device)
+    w = (back.contiguous() if turned else weight).to(cuda_device)
+    call = (lambda a: segment_matmul(a, p, w.transpose(1, 2) if turned else w))
+    out = call(x)
+    grad_src, = torch.autograd.grad(out, x, g)
+    _within(out, _plain_matmul(src, ptr, weight), _plain_matmul(src.abs(), ptr, weight.abs()), k + 2, "out")
+    _within(grad_src, _plain_matmul(grad, ptr, back), _plain_matmul(grad.abs(), ptr, back.abs()), n + 2, "grad_src")
+    assert _waits(lambda: call(x.detach()), cuda_device), "forward"
+    out = call(x)
+    assert _waits(lambda: torch.autograd.grad(out, x, g), cuda_device), "grad_src"
+
+
+@requires_gpu
+@pytest.mark.parametrize("m,k,n", [(1, 2049, 25000), (700, 331, 333), (2000, 25001, 1)])
+def test_segment_matmul_fp8_odd_sizes_reach_the_tensor_cores(cuda_device, m, k, n):
+    from ops_gnn import segment_matmul_fp8
+
+    src, src_scale, weight, weight_scale, ptr = [t.to(cuda_device) for t in _fp8_inputs([m], 0, 0, k, n, 181)]
+    for call in (lambda: segment_matmul_fp8(src, src_scale, weight, weight_scale, ptr, torch.float32),
+                 lambda: segment_matmul_fp8(src, src_scale, weight[0], weight_scale[0], out_dtype=torch.float32)):
+        a, b = _stands_for(src.cpu(), src_scale.cpu(), 1), _stands_for(weight.cpu(), weight_scale.cpu(), 128)[0]
+        _within(call(), a @ b.t(), a.abs() @ b.abs().t(), k + 4, "fp8")
+        assert _waits(call, cuda_device)
