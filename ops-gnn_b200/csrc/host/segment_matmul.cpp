@@ -44,13 +44,27 @@ at::Tensor Matrices(const at::Tensor& t)
 }
 
 // The tensor cores' loads want rows on 16-byte boundaries.  A product of this many multiply-adds or more is worth a copy of an
-// operand that has them elsewhere; smaller ones run as they are, on the kernel for any layout.
+// operand that has them elsewhere; smaller ones run as they are, on the kernel for any layout.  bf16 forward, as it is and with both
+// operands copied: 32768 x 33 -> 33 (3.6e7) 16 and 25 us, 4096 x 101 -> 77 in 20 segments (3.2e7) 16 and 16 us, 256 x 333 -> 501
+// (4.3e7) 28 and 17 us; 2100 x 130 -> 641 (1.7e8) 48 and 27 us.
 constexpr double kWorthCopy = 5e7;
 
-bool Wants(const at::Tensor& rows, const at::Tensor& matrices)
+bool Wants(const at::Tensor& rows, int64_t width, int64_t out)
 {
     return rows.scalar_type() != at::kFloat &&
-           static_cast<double>(rows.size(0)) * static_cast<double>(matrices.size(1)) * static_cast<double>(matrices.size(2)) >= kWorthCopy;
+           static_cast<double>(rows.size(0)) * static_cast<double>(width) * static_cast<double>(out) >= kWorthCopy;
+}
+bool Wants(const at::Tensor& rows, const at::Tensor& matrices) { return Wants(rows, matrices.size(1), matrices.size(2)); }
+
+// A weight gradient on the kernel for any layout is one block's sum over all rows of a segment, 70 ns a row, however few the
+// columns, so there the copies also pay for long segments.  How long these are the host does not know: the mean tells where lengths
+// are alike, and from so many rows on one long segment would cost more than the copies.  bf16 33 -> 33, as it is and with copies:
+// 512 rows in one segment 38 and 18 us, 64 rows 7 and 14 us; 1024 rows in 8 segments 11 and 15 us, 4096 rows 38 and 18 us; 32768
+// rows in 64 segments 38 and 22 us, in 500 segments 18 and 49 us, in one 2238 and 41 us.
+bool WantsWeightGrad(const at::Tensor& rows, int64_t segments, int64_t width, int64_t out)
+{
+    const int64_t m = rows.size(0);
+    return Wants(rows, width, out) || (rows.scalar_type() != at::kFloat && ((m >= 256 && m >= 128 * segments) || m >= 16384));
 }
 
 // t itself, or a copy with rows (the last dimension or, `turned`, the one before it) on 16-byte boundaries.
@@ -148,7 +162,7 @@ at::Tensor segment_matmul_weight_grad(const at::Tensor& src, const at::Tensor& i
     c10::cuda::CUDAGuard guard(src.device());
     LookForStalls(src, api);
     at::Tensor rows = RowMajor(src), upstream = RowMajor(grad);
-    if (rows.scalar_type() != at::kFloat && static_cast<double>(rows.numel()) * static_cast<double>(grad.size(1)) >= kWorthCopy) {
+    if (WantsWeightGrad(rows, segments, src.size(1), grad.size(1))) {
         rows = OnBoundaries(rows);
         upstream = OnBoundaries(upstream);
     }
@@ -174,8 +188,10 @@ std::vector<at::Tensor> Gradients(const at::Tensor& src, const at::Tensor& indpt
     LookForStalls(src, api);
     at::Tensor rows = RowMajor(src), matrices = Matrices(weight), upstream = RowMajor(grad);
     if (Wants(rows, matrices)) {
-        rows = OnBoundaries(rows);
         matrices = OnBoundaries(matrices, Turned(matrices));
+    }
+    if (WantsWeightGrad(rows, weight.size(0), weight.size(1), weight.size(2))) {
+        rows = OnBoundaries(rows);
         upstream = OnBoundaries(upstream);
     }
     const bool turned = weight.stride(1) == 1 && weight.stride(2) != 1;

@@ -1495,3 +1495,26 @@ def test_segment_matmul_fp8_odd_sizes_reach_the_tensor_cores(cuda_device, m, k, 
         a, b = _stands_for(src.cpu(), src_scale.cpu(), 1), _stands_for(weight.cpu(), weight_scale.cpu(), 128)[0]
         _within(call(), a @ b.t(), a.abs() @ b.abs().t(), k + 4, "fp8")
         assert _waits(call, cuda_device)
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("lengths,k,n", [([9001], 15, 15), ([300], 33, 33), ([700, 0, 1400], 7, 21), ([3] * 400 + [17000], 15, 9)])
+def test_segment_matmul_weight_gradient_of_long_narrow_segments(cuda_device, dtype, lengths, k, n):
+    """Few columns, none of them whole vectors, and long segments: the weight gradient does not run as one block's sum per segment,
+    alone or together with the gradient of src."""
+    from ops_gnn import segment_matmul
+
+    src, ptr, weight, grad = _matmul_inputs((lengths, 1, 2, k, n), dtype, 191)
+    x, w = src.to(cuda_device).requires_grad_(), weight.to(cuda_device).requires_grad_()
+    p, g = ptr.to(cuda_device), grad.to(cuda_device)
+    want, size = _plain_weight_grad(src, ptr, grad), _plain_weight_grad(src.abs(), ptr, grad.abs())
+    only, = torch.autograd.grad(segment_matmul(x.detach(), p, w), w, g)
+    grad_src, both = torch.autograd.grad(segment_matmul(x, p, w), (x, w), g)
+    _within(only, want, size, max(lengths) + 2, "grad_weight")
+    assert torch.equal(only, both)
+    back = weight.transpose(1, 2)
+    _within(grad_src, _plain_matmul(grad, ptr, back), _plain_matmul(grad.abs(), ptr, back.abs()), n + 2, "grad_src")
+    for leaves in ((w,), (x, w)):
+        out = segment_matmul(x if len(leaves) == 2 else x.detach(), p, w)
+        assert _waits(lambda: torch.autograd.grad(out, leaves, g), cuda_device)
