@@ -528,7 +528,7 @@ int RunRowsTensor(const RowsProblem& p, void* workspace, cudaStream_t stream)
     const int64_t segment_stride = StrideOf(p.b_segment, p.ptr.segments, stride * other, 8);
     if ((p.in_type != OPSGNN_BF16 && p.in_type != OPSGNN_F16) || p.out_type != p.in_type || p.k < 1 || p.ptr.data == nullptr ||
         p.ptr.segments < 1 || p.ldo != p.n || (!turned && p.b_n != 1) || stride < inner ||
-        segment_stride % 8 != 0 || segment_stride >= (INT64_C(1) << 38) || segment_stride < 1 || p.ptr.segments >= (INT64_C(1) << 31) ||
+        segment_stride % 8 != 0 || segment_stride >= (INT64_C(1) << 38) || segment_stride < 1 || p.ptr.segments >= (INT64_C(1) << 30) ||
         !Loadable(p.a, lda, std::max(p.k, p.ptr.rows)) || !Loadable(p.b, stride, std::max(inner, other))) {
         return OPSGNN_ERR_UNSUPPORTED;
     }
@@ -633,7 +633,7 @@ int64_t OuterChunk(int64_t rows, int64_t segments, int64_t k, int64_t n)
     // is many and two would leave the second round half empty (two segments, 32768 x 2048 -> 1024: 131 us, two rounds 148 us).  A
     // segment's last piece is half full on average.
     const int64_t tiles = CeilDiv(k, kRows) * CeilDiv(n, n <= 128 ? 128 : 256);
-    if (rows < 8192) {
+    if (rows < 8192 || segments >= (INT64_C(1) << 30)) {  // (twice a segment's number has to fit 32 bits)
         return 0;
     }
     int64_t length = 0;

@@ -1518,3 +1518,15 @@ def test_segment_matmul_weight_gradient_of_long_narrow_segments(cuda_device, dty
     for leaves in ((w,), (x, w)):
         out = segment_matmul(x if len(leaves) == 2 else x.detach(), p, w)
         assert _waits(lambda: torch.autograd.grad(out, leaves, g), cuda_device)
+
+
+def test_weight_gradients_of_very_many_segments_are_not_cut():
+    """Where a piece goes is told by twice its segment's number and one, in 32 bits."""
+    from ops_gnn import _cabi
+
+    lib, size = _cabi.load(), ctypes.c_int64()
+    for kind in (_cabi.BF16, _cabi.F16):
+        for segments, cut in ((1000, True), (2 ** 30 - 1, True), (2 ** 30, False), (2 ** 31 - 600, False)):
+            desc = _cabi.SegmentMatmulDesc(2 ** 20, segments, 8, 8, 8, 64, 8, 1, _cabi.I64, kind, kind)
+            assert lib.opsgnn_segment_matmul_workspace_bytes(ctypes.byref(desc), 1, ctypes.byref(size)) == 0
+            assert (size.value > 0) == cut
