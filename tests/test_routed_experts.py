@@ -1530,3 +1530,30 @@ def test_weight_gradients_of_very_many_segments_are_not_cut():
             desc = _cabi.SegmentMatmulDesc(2 ** 20, segments, 8, 8, 8, 64, 8, 1, _cabi.I64, kind, kind)
             assert lib.opsgnn_segment_matmul_workspace_bytes(ctypes.byref(desc), 1, ctypes.byref(size)) == 0
             assert (size.value > 0) == cut
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", KINDS, ids=str)
+@pytest.mark.parametrize("lengths,k,n", [([9000, 0, 70, 1, 300, 3000], 64, 40), ([4000, 300, 0, 1, 4001, 2], 264, 264), ([8192], 16, 16), ([0, 8500, 0], 128, 24),
+                                         ([600] * 15, 8, 136)])
+def test_segment_matmul_few_results_of_many_rows_in_pieces(cuda_device, dtype, lengths, k, n):
+    """Weight gradients of fewer tiles than SMs: pieces of long segments, empty and one-row segments between them, and segments
+    that end and start within one piece's length of rows, which is what two slots for each are for."""
+    from ops_gnn import _cabi, segment_matmul
+
+    src, ptr, weight, grad = _matmul_inputs((lengths, 3, 9, k, n), dtype, 201)
+    if dtype != torch.float32:
+        size, kind = ctypes.c_int64(), _cabi.BF16 if dtype == torch.bfloat16 else _cabi.F16
+        desc = _cabi.SegmentMatmulDesc(src.size(0), len(lengths), k, n, k, k * n, n, 1, _cabi.I64, kind, kind)
+        assert _cabi.load().opsgnn_segment_matmul_workspace_bytes(ctypes.byref(desc), 1, ctypes.byref(size)) == 0
+        assert size.value > 0, "not in pieces any more: longer segments, please"
+    w = weight.to(cuda_device).requires_grad_()
+    x = src.to(cuda_device)
+    p, g = ptr.to(cuda_device), grad.to(cuda_device)
+    first, = torch.autograd.grad(segment_matmul(x, p, w), w, g)
+    again, = torch.autograd.grad(segment_matmul(x, p, w), w, g)
+    assert torch.equal(first, again)
+    _within(first, _plain_weight_grad(src, ptr, grad), _plain_weight_grad(src.abs(), ptr, grad.abs()), max(lengths) + 2, "grad_weight")
+    turned = weight.transpose(1, 2).contiguous().to(cuda_device).requires_grad_()
+    other, = torch.autograd.grad(segment_matmul(x, p, turned.transpose(1, 2)), turned, g)
+    _within(other.transpose(1, 2), _plain_weight_grad(src, ptr, grad), _plain_weight_grad(src.abs(), ptr, grad.abs()), max(lengths) + 2, "turned")
