@@ -1557,3 +1557,50 @@ def test_segment_matmul_few_results_of_many_rows_in_pieces(cuda_device, dtype, l
     turned = weight.transpose(1, 2).contiguous().to(cuda_device).requires_grad_()
     other, = torch.autograd.grad(segment_matmul(x, p, turned.transpose(1, 2)), turned, g)
     _within(other.transpose(1, 2), _plain_weight_grad(src, ptr, grad), _plain_weight_grad(src.abs(), ptr, grad.abs()), max(lengths) + 2, "turned")
+
+
+@requires_gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups,kept,top", [(1, 1, 2), (8, 3, 2), (8, 4, 1)])
+@pytest.mark.parametrize("mask", [-1e4, -1e9, torch.finfo(torch.float32).min, 1e6])
+def test_topk_route_biases_of_any_size(cuda_device, score, groups, kept, top, mask):
+    """Some biases as large as masks are, the others so close that fp32 does not tell their sums with the scores apart."""
+    from ops_gnn import topk_route
+
+    gen = _gen(211)
+    rows, experts, k = 150, 80, 6
+    logits = torch.randint(-2, 3, (rows, experts), generator=gen).float() * 0.25
+    bias = torch.randint(0, 3, (experts,), generator=gen).float() * 2.0 ** -24 + 0.5
+    for few in (slice(1, None, 5), slice(20, 30)):  # some of each group, one whole group of eight
+        some = bias.clone()
+        some[few] = mask
+        weight, index = topk_route(logits.to(cuda_device), k, score, some.to(cuda_device), groups, kept, top)
+        assert torch.equal(index.cpu(), _plain_choice(logits, k, score, some, groups, kept, 1 if groups == 1 else top))
+
+
+@requires_gpu
+@pytest.mark.parametrize("groups,kept", [(1, 1), (8, 4)])
+def test_topk_route_with_a_finite_mask_in_the_bias_takes_no_longer(cuda_device, groups, kept):
+    """The error of a masked expert's score is as large as its mask, and has no part in choosing among the others."""
+    from ops_gnn import topk_route
+
+    gen = torch.Generator(device=cuda_device).manual_seed(221)
+    logits = torch.randn(65536, 256, generator=gen, device=cuda_device)
+    bias = torch.randn(256, generator=gen, device=cuda_device) * 0.05
+    masked = bias.clone()
+    masked[::5] = -1e9
+
+    def best(b):
+        times = []
+        for _ in range(8):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            for _ in range(8):
+                topk_route(logits, 8, "sigmoid", b, groups, kept)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times[2:])
+
+    plain, other = best(bias), best(masked)
+    assert other <= 1.5 * plain, (other, plain)
