@@ -49,21 +49,12 @@ __device__ __forceinline__ uint64_t KeyOf(double v)
     return (u >> 63) ? ~u : (u | 0x8000000000000000ULL);
 }
 
-__device__ __forceinline__ uint32_t WarpMax(uint32_t v) { return __reduce_max_sync(kFull, v); }
 __device__ __forceinline__ uint64_t WarpMax(uint64_t v)
 {
     const uint32_t hi = static_cast<uint32_t>(v >> 32);
     const uint32_t top = __reduce_max_sync(kFull, hi);
     const uint32_t lo = __reduce_max_sync(kFull, hi == top ? static_cast<uint32_t>(v) : 0u);
     return (static_cast<uint64_t>(top) << 32) | lo;
-}
-__device__ __forceinline__ float WarpMax(float v)
-{
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        v = fmaxf(v, __shfl_xor_sync(kFull, v, d));
-    }
-    return v;
 }
 template <class T> __device__ __forceinline__ T WarpSum(T v)
 {

@@ -449,19 +449,17 @@ int Launch(const CUtensorMap& a, const CUtensorMap& tail, const CUtensorMap& b, 
     return LaunchStatus();
 }
 
-// f(type tag, integral constant of a tile's columns)
-template <class F> int ByType(int type, int columns, F&& f)
+// f(type tag, integral constant of a tile's columns); the outer form has no tiles of 64.
+template <int FORM, class F> int ByType(int type, int columns, F&& f)
 {
     using std::integral_constant;
     auto by_columns = [&](auto tag) {
-        switch (columns) {
-            case 64:
+        if constexpr (FORM != kOuter) {
+            if (columns == 64) {
                 return f(tag, integral_constant<int, 64>());
-            case 128:
-                return f(tag, integral_constant<int, 128>());
-            default:
-                return f(tag, integral_constant<int, 256>());
+            }
         }
+        return columns == 128 ? f(tag, integral_constant<int, 128>()) : f(tag, integral_constant<int, 256>());
     };
     return type == OPSGNN_BF16 ? by_columns(__nv_bfloat16()) : by_columns(__half());
 }
@@ -567,7 +565,7 @@ int RunRowsTensor(const RowsProblem& p, void* workspace, cudaStream_t stream)
         const int64_t tiles = down * CeilDiv(p.n, BN) * q.pieces;
         return turned ? Launch<T, BN, kRowsTurned>(a, tail, b, q, tiles, stream) : Launch<T, BN, kRowsWide>(a, tail, b, q, tiles, stream);
     };
-    const int status = ByType(p.in_type, columns, run);
+    const int status = ByType<kRowsWide>(p.in_type, columns, run);
     if (status != OPSGNN_OK || q.pieces == 1) {
         return status;
     }
@@ -715,7 +713,7 @@ int RunOuterTensor(const OuterProblem& p, void* workspace, cudaStream_t stream)
         const int64_t results = q.chunk > 0 ? p.ptr.rows / q.chunk + p.ptr.segments : p.ptr.segments;
         return Launch<T, BN, kOuter>(a, a, b, q, results * CeilDiv(p.k, kRows) * CeilDiv(p.n, BN), stream);
     };
-    const int status = ByType(p.type, narrow ? 128 : 256, run);
+    const int status = ByType<kOuter>(p.type, narrow ? 128 : 256, run);
     return status == OPSGNN_OK && q.chunk > 0 ? JoinPieces(p, q.chunk, q.partial, stream) : status;
 }
 
