@@ -26,7 +26,9 @@ int CheckDesc(const OpsgnnSegmentMatmulDesc* d, bool eight_bits)
 // fp32 products that go through bf16 terms on the tensor cores.  Making the terms costs launches and passes over the operands,
 // which small products do not earn back: forward 4096 x 128 -> 128 (134 MFLOP) 13.1 us against 11.2 us on the simple kernel,
 // 16384 x 101 -> 77 (255 MFLOP) 20.8 against 27.4 us, 32768 x 501 -> 333 157 against 586 us.  The simple weight gradient also
-// grows with the rows a block sums alone: 1000 x 128 -> 128 12.2 us in terms against 11.7 us, 4096 x 64 -> 64 20.1 against 38.7.
+// grows with the rows a block sums alone, a segment's: 1024 x 128 -> 128 in 8 segments 12.5 us in terms against 12.0 us, in one 32 against
+// 76; 2000 rows in 8 segments 16 against 21, 4096 x 64 -> 64 20.1 against 38.7.  (Below 2048 rows one long segment could gain, but a
+// gradient of src computed alone would no longer have the bits of one computed together with the weight's.)
 bool Splits(const OpsgnnSegmentMatmulDesc& d, int what)
 {
     if (d.in_type != OPSGNN_F32 || d.rows <= 0 || d.segments <= 0 || d.width <= 0 || d.out <= 0) {

@@ -228,10 +228,28 @@ template <int BN, int FORM> __device__ __noinline__ void Repair(const Params& p,
     tile::Operands& shared = *reinterpret_cast<tile::Operands*>(scratch);
     const int n = static_cast<int>(p.n), m = static_cast<int>(p.m), width = static_cast<int>(p.k), chunk = static_cast<int>(p.chunk);
     const int across = (n + BN - 1) / BN, down = (m + kRows - 1) / kRows, below = thread / 16 * 4, right = thread % 16 * 4;
+    // One warp finds the tiles for all eight, whose barriers have to agree.
     Walk<FORM> walk;
-    StartWalk<FORM>(p, walk);
+    if (thread < 32) {
+        StartWalk<FORM>(p, walk);
+    }
     Tile at;
-    for (int t = blockIdx.x; FindTile<BN, FORM>(p, walk, t, across, down, width, m, chunk, at); t += gridDim.x) {
+    Tile* told = reinterpret_cast<Tile*>(scratch + sizeof(tile::Operands));
+    for (int t = blockIdx.x;; t += gridDim.x) {
+        if (thread < 32) {
+            if (!FindTile<BN, FORM>(p, walk, t, across, down, width, m, chunk, at)) {
+                at.segment = -1;
+            }
+            if (thread == 0) {
+                *told = at;
+            }
+        }
+        SumSync()();
+        at = *told;
+        SumSync()();
+        if (at.segment < 0) {
+            break;
+        }
         float* to = ResultsOf<float, FORM>(p, at.segment);
         for (int part = 0; part < kRows / tile::kSize * (BN / tile::kSize); ++part) {
             const int64_t r0 = at.row + part / (BN / tile::kSize) * tile::kSize, c0 = at.column + part % (BN / tile::kSize) * tile::kSize;
