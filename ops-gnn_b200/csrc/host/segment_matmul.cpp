@@ -67,17 +67,24 @@ bool WantsWeightGrad(const at::Tensor& rows, int64_t segments, int64_t width, in
     return Wants(rows, width, out) || (rows.scalar_type() != at::kFloat && ((m >= 256 && m >= 128 * segments) || m >= 16384));
 }
 
-// t itself, or a copy with rows (the last dimension or, `turned`, the one before it) on 16-byte boundaries.
-at::Tensor OnBoundaries(const at::Tensor& t, bool turned = false)
+// Rows (the last dimension or, `turned`, the one before it) on 16-byte boundaries?
+bool IsOnBoundaries(const at::Tensor& t, bool turned = false)
 {
     const int64_t vec = 16 / t.element_size(), inner = turned ? t.dim() - 2 : t.dim() - 1;
     bool fine = reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
     for (int64_t d = 0; d < t.dim(); ++d) {
         fine = fine && (d == inner || t.size(d) <= 1 || t.stride(d) % vec == 0);
     }
-    if (fine) {
+    return fine;
+}
+
+// t itself, or a copy with rows on 16-byte boundaries.
+at::Tensor OnBoundaries(const at::Tensor& t, bool turned = false)
+{
+    if (IsOnBoundaries(t, turned)) {
         return t;
     }
+    const int64_t vec = 16 / t.element_size();
     at::Tensor from = turned ? t.transpose(-1, -2) : t;
     auto shape = from.sizes().vec();
     const int64_t width = shape.back();
@@ -188,10 +195,8 @@ std::vector<at::Tensor> Gradients(const at::Tensor& src, const at::Tensor& indpt
     LookForStalls(src, api);
     at::Tensor rows = RowMajor(src), matrices = Matrices(weight), upstream = RowMajor(grad);
     if (Wants(rows, matrices)) {
-        matrices = OnBoundaries(matrices, Turned(matrices));
-    }
-    if (WantsWeightGrad(rows, weight.size(0), weight.size(1), weight.size(2))) {
         rows = OnBoundaries(rows);
+        matrices = OnBoundaries(matrices, Turned(matrices));
         upstream = OnBoundaries(upstream);
     }
     const bool turned = weight.stride(1) == 1 && weight.stride(2) != 1;
@@ -223,14 +228,21 @@ public:
     {
         PlannerScope scope;
         const auto saved = ctx->get_saved_variables();
-        const at::Tensor src = saved[0].detach(), indptr = saved[1], weight = saved[2].detach(), grad = grads[0].detach();
         const bool of_src = ctx->needs_input_grad(0), of_weight = ctx->needs_input_grad(2);
+        const at::Tensor indptr = saved[1], weight = saved[2].detach(), grad = RowMajor(grads[0].detach());
+        const at::Tensor src = of_weight ? RowMajor(saved[0].detach()) : saved[0].detach();
+        // Together, unless only the weight's wants copies: the gradient of src has the bits that it has alone.
+        const bool together = of_src && of_weight &&
+                              (Wants(src, weight) == WantsWeightGrad(src, weight.size(0), weight.size(1), weight.size(2)) ||
+                               (IsOnBoundaries(src) && IsOnBoundaries(grad)));
         std::vector<at::Tensor> out(2);
-        if (of_src && of_weight) {
+        if (together) {
             out = Gradients(src, indptr, weight, grad);
-        } else if (of_src) {
+        }
+        if (of_src && !together) {
             out[0] = segment_matmul_forward(grad, indptr, weight.transpose(1, 2));
-        } else if (of_weight) {  // in the layout of the weight
+        }
+        if (of_weight && !together) {  // in the layout of the weight
             out[1] = weight.stride(1) == 1 && weight.stride(2) != 1 ? segment_matmul_weight_grad(grad, indptr, src).transpose(1, 2)
                                                                     : segment_matmul_weight_grad(src, indptr, grad);
         }

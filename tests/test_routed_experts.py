@@ -1604,3 +1604,22 @@ def test_topk_route_with_a_finite_mask_in_the_bias_takes_no_longer(cuda_device, 
 
     plain, other = best(bias), best(masked)
     assert other <= 1.5 * plain, (other, plain)
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("lengths,k,n", [([9000], 16, 15), ([300, 500], 15, 16), ([600], 264, 15), ([3000, 17000], 7, 24)])
+def test_segment_matmul_gradients_alone_and_together(cuda_device, dtype, turned, lengths, k, n):
+    """The gradient of src has the same bits alone and beside the weight's, also where only the latter's operands are copied."""
+    from ops_gnn import segment_matmul
+
+    src, ptr, weight, grad = [t.to(cuda_device) for t in _matmul_inputs((lengths, 1, 2, k, n), dtype, 231)]
+    if turned:
+        weight = weight.transpose(1, 2).contiguous().transpose(1, 2)
+    x, w = src.clone().requires_grad_(), weight.detach().requires_grad_()
+    both = torch.autograd.grad(segment_matmul(x, ptr, w), (x, w), grad)
+    only_src, = torch.autograd.grad(segment_matmul(x, ptr, weight), x, grad)
+    only_weight, = torch.autograd.grad(segment_matmul(src, ptr, w), w, grad)
+    assert torch.equal(both[0], only_src) and torch.equal(both[1], only_weight)
+    assert both[1].stride() == w.stride()
