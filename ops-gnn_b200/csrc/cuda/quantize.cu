@@ -168,7 +168,8 @@ __global__ void __launch_bounds__(256) RowKernel(const T* __restrict__ src, int6
     }
 }
 
-// The same for any width and alignment, a block of 128 per warp.
+// The same for any width and alignment, a block of 128 per warp: single loads and one-byte stores, 2.3 times as long (16381 x 4095
+// bf16 85 us, fp32 83 us, against 37 us for 16381 x 4096 bf16).
 template <class T>
 __global__ void __launch_bounds__(256) RowScalarKernel(const T* __restrict__ src, int64_t blocks, int64_t width, int64_t across,
                                                        uint8_t* __restrict__ values, float* __restrict__ scales)
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(256) RowScalarKernel(const T* __restrict__ src
 }
 
 // One scale per tile of 128 x 128: a thread block per tile, the tile stays in registers (as loaded) between the maximum and
-// the conversion.
+// the conversion.  VEC 1: any width and alignment (64 x 1024 x 2047 bf16 197 us, x 2048 in vectors 70 us).
 constexpr int kTileThreads = 256;
 
 template <class T, int VEC>

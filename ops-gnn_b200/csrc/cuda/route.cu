@@ -311,7 +311,7 @@ __device__ __noinline__ void ChooseFine(const RouteParams& p, const T* row, cons
 // the key as they are.  Others are measured on a scale of 22 bits that reaches from the largest down to the smallest of the
 // lanes' largest values, below which no k <= 31 winners lie, and neighbours in the resulting order that are too close to tell
 // send the row to ChooseFine: closer than the scale's steps or, BIASED, than twice the error of the scores, unless they are
-// equal by their inputs.  (4099 x 256, bias, 8 groups: 17.4 us with 32-bit keys and a search for the winner's lane, 12.5 us;
+// equal by their inputs.  (4099 x 256, bias, 8 groups: 17.4 us with 32-bit keys and a search for the winner's lane, 13.4 us;
 // about one row in 300 goes to ChooseFine.)
 //
 // BIASED scores are formed in fp32 with the fast exponential and division.  A sigmoid is off by at most 2^-22: its slope times
@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(kWarps * 32) TopkKernel(RouteParams p, const T
 // VPL packed keys eight at a time and merges the lists (of two sorted lists of eight, the eight largest are the pairwise
 // maxima of one with the other reversed, a bitonic list), three more merges with its neighbours leave the row's eight largest in
 // every lane; lane i then owns the i-th choice.  Per row a quarter of the instructions of the one-row-per-warp form, which
-// is bound by them: 131072 x 128, k 8: 56 -> 21 us.
+// is bound by them: 131072 x 128, k 8: 56 -> 31 us.
 constexpr int kList = 8;
 
 __device__ __forceinline__ void Exchange(uint32_t& a, uint32_t& b)

@@ -32,7 +32,8 @@ def segment_matmul(src: torch.Tensor, indptr: torch.Tensor, weight: torch.Tensor
     layouts are copied first.  Differentiable in ``src`` and ``weight`` (second derivatives are not built).
 
     Larger float32 products take scratch memory of about 1.5 times their operands while they run; their values below 2^-110
-    lose low bits.  Every sum is taken in a fixed order: the same call gives the same bits.
+    lose low bits, and an infinity or a value above 3.389e38 among the operands makes them several times slower (a NaN does not).
+    16-bit operands whose rows are off 16-byte boundaries are copied onto them where that pays.  Every sum is taken in a fixed order: the same call gives the same bits.
 
     The pointers stay on the device: nothing is read back, so the call can be captured into a graph and replayed with other
     pointers.  A pointer outside ``[0, M]`` counts as the nearer end.  Their order is not checked: where they descend, rows
