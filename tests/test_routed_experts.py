@@ -1623,3 +1623,111 @@ def test_segment_matmul_gradients_alone_and_together(cuda_device, dtype, turned,
     only_weight, = torch.autograd.grad(segment_matmul(src, ptr, w), w, grad)
     assert torch.equal(both[0], only_src) and torch.equal(both[1], only_weight)
     assert both[1].stride() == w.stride()
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_training_step_in_a_graph(cuda_device, dtype):
+    """Choice, dispatch, products and all gradients, captured once and replayed on other inputs: the bits of eager passes."""
+    import ops_gnn
+
+    tokens, width, hidden, experts, k = 1100, 64, 72, 12, 2
+    gen = _gen(241)
+    weight = (torch.randn(experts, width, hidden, generator=gen) / 8).to(dtype).to(cuda_device)
+
+    def inputs(seed):
+        g = _gen(seed)
+        logits = torch.randn(tokens, experts, generator=g)
+        logits[5] = -math.inf
+        return [torch.randn(tokens, width, generator=g).to(dtype).to(cuda_device), logits.to(dtype).to(cuda_device),
+                torch.randn(tokens, hidden, generator=g).to(dtype).to(cuda_device)]
+
+    def step(x, logits, upstream):
+        leaves = [t.detach().requires_grad_() for t in (x, logits, weight)]
+        chosen, index = ops_gnn.topk_route(leaves[1], k)
+        indptr, perm, position = ops_gnn.route_csr(index, experts)
+        y = ops_gnn.segment_matmul(leaves[0][perm // k], indptr, leaves[2])
+        out = (y[position.view(-1)].view(tokens, k, hidden) * chosen.unsqueeze(-1)).sum(1)
+        return (out.detach(),) + torch.autograd.grad(out, leaves[1:], upstream)
+
+    static = inputs(1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(*static)
+    for seed in (2, 3):
+        fresh = inputs(seed)
+        for buffer, value in zip(static, fresh):
+            buffer.copy_(value)
+        graph.replay()
+        want = step(*fresh)
+        assert all(torch.equal(a, b) for a, b in zip(captured, want)), seed
+    del graph
+
+
+@requires_gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp32", "fp8"])
+def test_products_past_32_bit_offsets(cuda_device, kind):
+    """More than 2^31 values in src and in the result, the last segment past both: rows at the ends and at the 2^31st value."""
+    import ops_gnn
+
+    rows, k, n, segments = 4_200_000, 520, 520, 3
+    assert rows * k > 2 ** 31
+    if torch.cuda.get_device_properties(cuda_device).total_memory < 120 * 2 ** 30:
+        pytest.skip("needs a GPU of 120 GiB")
+    gen = torch.Generator(device=cuda_device).manual_seed(251)
+    dtype = torch.float32 if kind == "fp32" else torch.bfloat16
+    src = torch.empty(rows, k, dtype=dtype, device=cuda_device)
+    for part in src.split(500_000):
+        part.normal_(generator=gen)
+    weight = torch.randn(segments, k, n, generator=gen, device=cuda_device).to(dtype)
+    ptr = torch.tensor([0, 4_000_000, 4_199_000, rows - 1], device=cuda_device)
+    edge = 2 ** 31 // k
+    look = torch.tensor([0, 1, edge - 1, edge, edge + 1, 3_999_999, 4_000_000, 4_198_999, 4_199_000, rows - 2], device=cuda_device)
+    which = torch.bucketize(look, ptr[1:], right=True)
+    if kind == "fp8":
+        values, scale = ops_gnn.quantize_fp8(src)
+        w8, w8_scale = ops_gnn.quantize_fp8(weight.transpose(1, 2).contiguous(), 128)
+        out = ops_gnn.segment_matmul_fp8(values, scale, w8, w8_scale, ptr)
+        part, part_scale = ops_gnn.quantize_fp8(src[look])
+        assert torch.equal(part.view(torch.uint8), values.view(torch.uint8)[look]) and torch.equal(part_scale, scale[look])
+        a, b = _stands_for(part.cpu(), part_scale.cpu(), 1), _stands_for(w8.cpu(), w8_scale.cpu(), 128).transpose(1, 2)
+    else:
+        out = ops_gnn.segment_matmul(src, ptr, weight)
+        a, b = src[look].cpu().double(), weight.cpu().double()
+    want = torch.stack([a[i] @ b[int(e)] for i, e in enumerate(which)])
+    size = torch.stack([a[i].abs() @ b[int(e)].abs() for i, e in enumerate(which)])
+    _within(out[look], want, size, k + 4, "out")
+    assert not out[-1].any()
+    if kind == "fp8":
+        return
+    # The weight gradient of the last segment, which lies past the 2^31st value of both.
+    grad_weight = ops_gnn._pybind.segment_matmul_weight_grad(src, ptr, out)
+    x, g = src[4_199_000:rows - 1].cpu(), out[4_199_000:rows - 1].cpu()
+    last = torch.tensor([0, x.size(0)])
+    _within(grad_weight[2:], _plain_weight_grad(x, last, g), _plain_weight_grad(x.abs(), last, g.abs()), x.size(0) + 2, "grad_weight")
+
+
+@requires_gpu
+def test_topk_route_past_32_bit_offsets(cuda_device):
+    from ops_gnn import topk_route
+
+    rows, experts = 2_100_001, 1024
+    assert rows * experts > 2 ** 31
+    gen = torch.Generator(device=cuda_device).manual_seed(261)
+    logits = torch.empty(rows, experts, dtype=torch.bfloat16, device=cuda_device)
+    for part in logits.split(300_000):
+        part.normal_(generator=gen)
+    leaf = logits.requires_grad_()
+    weight, index = topk_route(leaf, 4)
+    grad, = torch.autograd.grad(weight, leaf, weight.detach())
+    tail = logits.detach()[-3:].clone().requires_grad_()
+    tail_weight, tail_index = topk_route(tail, 4)
+    tail_grad, = torch.autograd.grad(tail_weight, tail, tail_weight.detach())
+    assert torch.equal(weight[-3:], tail_weight) and torch.equal(index[-3:], tail_index) and torch.equal(grad[-3:], tail_grad)
+    assert torch.equal(index[-3:].cpu(), _plain_choice(tail.detach().cpu(), 4, "softmax", None, 1, 1, 1))
