@@ -36,7 +36,8 @@ def segment_matmul(src: torch.Tensor, indptr: torch.Tensor, weight: torch.Tensor
     16-bit operands whose rows are off 16-byte boundaries are copied onto them where that pays.  Every sum is taken in a fixed order: the same call gives the same bits.
 
     The pointers stay on the device: nothing is read back, so the call can be captured into a graph and replayed with other
-    pointers.  A pointer outside ``[0, M]`` counts as the nearer end.  Their order is not checked: where they descend, rows
+    pointers.  (A backward pass is captured together with its forward pass, on leaves that no other living autograd graph uses:
+    torch joins the streams of all of a leaf's uses.)  A pointer outside ``[0, M]`` counts as the nearer end.  Their order is not checked: where they descend, rows
     and gradients of the segments concerned are unspecified, but nothing outside the tensors is read or written.  Raises
     ``TypeError`` / ``ValueError`` for bad arguments and ``RuntimeError`` for tensors that are not on a CUDA device.
     """

@@ -37,6 +37,9 @@ def topk_route(logits: torch.Tensor, k: int, score: str = "softmax", bias: Optio
     makes the whole row NaN, as with ``torch.softmax``, and its gradient.  The choice does not depend on how scores round: it compares the
     logits where the scores order as they do, and scores in 64 bits where a bias or a sum of two decides.
 
+    The call can be captured into a graph; a backward pass together with its forward pass, on leaves that no other living
+    autograd graph uses.
+
     float16, float32 and bfloat16 on a CUDA device; at most 1024 experts, 32 chosen, 32 groups.  Raises ``TypeError`` /
     ``ValueError`` for bad arguments and ``RuntimeError`` for tensors that are not on a CUDA device.
     """
